@@ -563,6 +563,137 @@ vsk_status vsk_kmeans(vsk_ctx *ctx, const float *x, int64_t n, int32_t d,
                       int32_t max_iter, float tolerance, float *out_centroids,
                       int32_t *out_assign, vsk_kmeans_result *result);
 
+/* ---- key-value cache and attention ----------------------------------------
+ * The step after retrieval: a language model answers over what was found
+ * (LLM/RAG is the reference's application layer; its one attention kernel is
+ * scaled_dot_product_attention_optimized, Core/ML/Shaders/
+ * OptimizedMLShaders.metal:523).  The cache is a store of vectors in pages of
+ * device memory that the caller owns; these calls give new tokens their
+ * rotary positions, write them, keep the pages, and attend.
+ *
+ * Unlike the search calls, every call of this section takes device memory
+ * only and is queued on `stream` (a hipStream_t, NULL: the default stream): it
+ * returns without waiting, since a decoder makes dozens a token, and can be
+ * captured into a graph.  It allocates nothing.  Buffers stay the caller's
+ * until the stream has passed the call.  With profiling on, it waits.
+ *
+ * What device memory holds (page ids, lengths, offsets, slots) is held to its
+ * buffers by the kernels: a value out of range reads or writes nothing
+ * outside them, but what is computed from it is unspecified.  Strides are in
+ * elements, the innermost dimension is dense. */
+#define VSK_DTYPE_F32 0
+#define VSK_DTYPE_F16 1
+#define VSK_DTYPE_BF16 2
+#define VSK_MAX_HEAD_DIM 256 /* largest head of the attention and the cache */
+
+/* Rotary positions.  Pair i of the first 2 * pairs values of a head turns by
+ * position * inv_freq[i] radians and is multiplied by amplitude; the values
+ * after them pass through.  The phase is kept exactly, as a 64-bit fraction
+ * of a turn, at any int32 position. */
+#define VSK_ROTARY_HALF 0        /* pairs (i, i + pairs)    */
+#define VSK_ROTARY_INTERLEAVED 1 /* pairs (2 i, 2 i + 1)    */
+typedef struct vsk_rotary vsk_rotary;
+vsk_status vsk_rotary_create(vsk_ctx *ctx, const double *inv_freq, int32_t pairs,
+                             int32_t layout, double amplitude, vsk_rotary **out);
+vsk_status vsk_rotary_free(vsk_ctx *ctx, vsk_rotary *rotary);
+/* Heads of one tensor, tokens x heads x d: src may equal dst. */
+typedef struct {
+  const void *src;
+  void *dst;
+  int64_t src_row, src_head, dst_row, dst_head;
+  int32_t heads;
+} vsk_head_rows;
+/* Rotates n_tensors (1 to 3) tensors of `tokens` tokens with heads of d
+ * values by positions[tokens] (int32, device); inverse turns the other way
+ * (with the same amplitude): the gradient of the rotation. */
+vsk_status vsk_rotary_apply(vsk_ctx *ctx, void *stream, const vsk_rotary *rotary,
+                            int32_t dtype, int32_t d, int64_t tokens,
+                            const int32_t *positions, int32_t inverse,
+                            const vsk_head_rows *tensors, int32_t n_tensors);
+
+/* A paged cache, as the caller holds it: k and v are layers x pages x
+ * page_size x kv_heads x head_dim (any strides over a dense head);
+ * table[slot * table_stride + i] is the page of tokens i * page_size on of
+ * the sequence in that slot (-1: none), lengths[slot] its tokens; refs[page]
+ * counts the sequences that hold a page (0: free).  page_size is a power of
+ * two of at least 16.  refs, status and scratch serve the page calls only.
+ * status (4 ints): [0] pages that were missing in the last vsk_kv_reserve or
+ * vsk_kv_fork, [1] pages in use and [2] pages moved by the last
+ * vsk_kv_compact.  scratch: vsk_kv_scratch_ints() ints. */
+typedef struct {
+  void *k, *v;
+  int64_t k_layer, k_page, k_row, k_head;
+  int64_t v_layer, v_page, v_row, v_head;
+  int32_t *table, *lengths, *refs, *status, *scratch;
+  int64_t table_stride;
+  int32_t dtype, layers, pages, page_size, kv_heads, head_dim, slots, width;
+} vsk_kv;
+int64_t vsk_kv_scratch_ints(int32_t pages, int32_t slots);
+/* Grows the n sequences in slots seqs[] (distinct) by counts[] tokens: takes
+ * the lowest free pages, in the sequences' order, and sets the lengths.  With
+ * too few free pages, or past the table's width, a sequence grows only as far
+ * as its pages reach. */
+vsk_status vsk_kv_reserve(vsk_ctx *ctx, void *stream, const vsk_kv *kv, const int32_t *seqs,
+                          const int32_t *counts, int32_t n);
+/* What the sequences in slots children[] (distinct, none of them a parent)
+ * held is released; child i becomes a branch of parents[i]: it shares the
+ * whole pages and gets a copy of the rows of a last page that is not full, in
+ * the lowest free page.  A child for which none is left keeps the whole pages
+ * only. */
+vsk_status vsk_kv_fork(vsk_ctx *ctx, void *stream, const vsk_kv *kv, const int32_t *parents,
+                       const int32_t *children, int32_t n);
+/* Releases the sequences' pages: lengths 0, table rows -1. */
+vsk_status vsk_kv_free(vsk_ctx *ctx, void *stream, const vsk_kv *kv, const int32_t *seqs,
+                       int32_t n);
+/* With m pages in use, moves those numbered m and above, in order, to the
+ * free pages below m and renames them in every table row. */
+vsk_status vsk_kv_compact(vsk_ctx *ctx, void *stream, const vsk_kv *kv);
+/* Copies page src[i] to page dst[i] in every layer; no page may be written
+ * twice or be both read and written.  Ids outside the pool are skipped. */
+vsk_status vsk_kv_copy(vsk_ctx *ctx, void *stream, const vsk_kv *kv, const int32_t *src,
+                       const int32_t *dst, int32_t n);
+
+/* The new tokens of n sequences: sequence i (slot seqs[i], or i without
+ * seqs) has rows starts[i] .. starts[i + 1] of q, k and v (starts NULL: row i
+ * alone), which are the last tokens of its length.  max_new bounds the new
+ * tokens of a sequence: rows past it are not treated. */
+typedef struct {
+  const int32_t *starts, *seqs;
+  int32_t n, max_new;
+  int64_t tokens; /* rows in all */
+} vsk_new_tokens;
+/* Writes k and v (dst unused) to their places in layer's pages; rotary (may
+ * be NULL) turns k, and q (may be NULL) to q->dst, by the tokens' positions. */
+vsk_status vsk_kv_append(vsk_ctx *ctx, void *stream, const vsk_kv *kv, int32_t layer,
+                         const vsk_new_tokens *news, const vsk_head_rows *k,
+                         const vsk_head_rows *v, const vsk_rotary *rotary,
+                         const vsk_head_rows *q);
+/* Attention of the new tokens: out = sum_j w_j v_j / sum_j w_j, w_j =
+ * exp(scale * q . k_j), over the keys j at or before the token's position
+ * with (window 0, or position - j < window, or j < sinks).  A token that sees
+ * no key gets zeros (and lse -inf).  q.src is read, q.dst written; q.heads a
+ * multiple of kv_heads, consecutive heads share a key head.  lse (may be
+ * NULL): tokens x heads, log of the sum.  max_length: the longest length, for
+ * the division of the work only (0: what the table holds).  Masked places of
+ * the cache may hold anything, infinities and NaN included.
+ * kv for dense keys and values: table NULL, page_size 0, `pages` rows of k
+ * and v (k_row, k_head, v_row, v_head apart) and k_starts[n + 1] their
+ * sequences' offsets; else k_starts is unused.
+ * workspace: at least vsk_attention_workspace() bytes, 16-byte aligned. */
+typedef struct {
+  vsk_head_rows q;
+  float *lse;
+  const int32_t *k_starts;
+  void *workspace;
+  int64_t workspace_bytes;
+  float scale;
+  int32_t window, sinks, max_length;
+} vsk_attention_args;
+int64_t vsk_attention_workspace(vsk_ctx *ctx, const vsk_kv *kv, const vsk_new_tokens *news,
+                                const vsk_attention_args *args);
+vsk_status vsk_attention(vsk_ctx *ctx, void *stream, const vsk_kv *kv, int32_t layer,
+                         const vsk_new_tokens *news, const vsk_attention_args *args);
+
 #ifdef __cplusplus
 }
 #endif

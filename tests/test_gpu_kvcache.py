@@ -1,0 +1,665 @@
+"""Key-value cache, rotary positions and attention against their definitions
+in 64 bits.
+
+Tolerances, derived here and used by every case.  With u the unit roundoff of
+the output's type (2^-8 bf16, 2^-11 f16, 2^-24 f32):
+
+* a rotated value: one rounding u of the result, fp32 products and a sine and
+  cosine that are off by at most 2^-18 (16-bit types) or 2^-22: |err| <=
+  u |y| + 2^-17 (|a| + |b|) A, or + 2^-21 (...) for f32;
+* an attention output: the score of fp32 products is off by at most
+  e = 2^-24 (d + 8) scale max sum |q k|, a weight by a factor within
+  e + 2^-21, the sum of L weights by 2^-24 (L + 16); 16-bit types may round
+  each weight once (u); so |err| <= u |o| + max |v| (2 (e + 2^-21 +
+  2^-24 (L + 16)) + (16-bit) u), and the errors are independent, so their
+  2-norm is at most u (16-bit) of the result's."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+U = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11, torch.float32: 2.0 ** -24}
+BF, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+DEV = "cuda:0"
+
+
+def ints(x):
+    return torch.tensor(list(x), dtype=torch.int32, device=DEV)
+
+
+def normal(g, *shape, dtype=F32):
+    return torch.randn(*shape, generator=g, dtype=torch.float32).to(dtype).to(DEV)
+
+
+def gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+# ------------------------------------------------------------------ definitions
+
+def rotated(x, positions, inv, amplitude, layout, sign=1.0):
+    """x (tokens x heads x d) turned, in 64 bits on the CPU."""
+    y = x.detach().cpu().double().clone()
+    r = 2 * len(inv)
+    angle = positions.cpu().double()[:, None] * torch.from_numpy(inv)
+    c, s = torch.cos(angle)[:, None] * amplitude, sign * torch.sin(angle)[:, None] * amplitude
+    i = (slice(0, r // 2), slice(r // 2, r)) if layout == "half" else (slice(0, r, 2), slice(1, r, 2))
+    a, b = y[..., i[0]].clone(), y[..., i[1]].clone()
+    y[..., i[0]], y[..., i[1]] = a * c - b * s, a * s + b * c
+    return y
+
+
+def attended(q, k, v, scale, window, sinks):
+    """One sequence: q (T x H x d) the last tokens of k, v (L x Hkv x d), in 64
+    bits on the CPU.  Only what a row sees enters its sums.  Returns the
+    outputs, the logarithms of the sums, and the tolerance of each output."""
+    t, heads, d = q.shape
+    dtype = q.dtype
+    q, k, v = (x.detach().cpu().double() for x in (q, k, v))
+    length, kv = k.shape[0], k.shape[1]
+    out = torch.zeros(t, heads, d, dtype=torch.float64)
+    lse = torch.full((t, heads), -math.inf, dtype=torch.float64)
+    tol = torch.zeros(t, heads, d, dtype=torch.float64)
+    j = torch.arange(length)
+    u = U[dtype]
+    for i in range(t):
+        pos = length - t + i
+        see = j <= pos
+        if window:
+            see &= (pos - j < window) | (j < sinks)
+        if not see.any():
+            continue
+        for h in range(heads):
+            kk, vv = k[see, h // (heads // kv)], v[see, h // (heads // kv)]
+            s = kk @ q[i, h] * scale
+            lse[i, h] = torch.logsumexp(s, 0)
+            out[i, h] = torch.softmax(s, 0) @ vv
+            e = 2.0 ** -24 * (d + 8) * scale * float((kk.abs() @ q[i, h].abs()).max())
+            w = 2 * (e + 2.0 ** -21 + 2.0 ** -24 * (length + 16)) + (u if u > 2.0 ** -20 else 0)
+            tol[i, h] = u * out[i, h].abs() + float(vv.abs().max()) * w
+    return out, lse, tol
+
+
+def check(got, want, tol):
+    got = got.detach().cpu().double()
+    fine = torch.isfinite(want)
+    assert torch.equal(torch.isfinite(got), fine)
+    err = (got - want).abs()[fine]
+    assert bool((err <= tol[fine]).all()), float((err - tol[fine]).max())
+
+
+def check_norm(got, want, dtype):
+    if dtype != F32 and float(want.norm()) > 0:
+        assert float((got.cpu().double() - want).norm()) <= U[dtype] * float(want.norm())
+
+
+# ------------------------------------------------------------------------ rotary
+
+@pytest.mark.parametrize("dtype", [BF, F16, F32])
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("d,r,tokens,heads,kv", [(128, 128, 7, 8, 2), (80, 32, 33, 5, 5),
+                                                 (96, 48, 1, 3, 1), (64, 40, 300, 2, 1),
+                                                 (37, 10, 5, 3, 3), (256, 256, 2, 1, 1),
+                                                 (2, 2, 9, 1, 1)])
+def test_rotary(ctx, dtype, layout, d, r, tokens, heads, kv):
+    from vectorstorekit_amd import RotaryEmbedding
+
+    g = gen(d + r)
+    rope = RotaryEmbedding(ctx, d, rotary_dim=r, layout=layout)
+    q, k = normal(g, tokens, heads, d, dtype=dtype), normal(g, tokens, kv, d, dtype=dtype)
+    pos = torch.randint(-5000, 1 << 20, (tokens,), generator=g, dtype=torch.int32).to(DEV)
+    pos[0] = 2 ** 31 - 1
+    for inverse in (False, True):
+        for x, y in zip((q, k), rope.apply(q, k, positions=pos, inverse=inverse)):
+            want = rotated(x, pos, rope.inv_freq, 1.0, layout, -1.0 if inverse else 1.0)
+            size = x.cpu().double().abs().amax(-1, keepdim=True)
+            e = 2.0 ** -21 if dtype == F32 else 2.0 ** -17
+            check(y, want, U[dtype] * want.abs() + 2 * e * size)
+            assert torch.equal(y[..., r:], x[..., r:])
+    back = rope.apply(q, positions=pos)
+    assert torch.equal(back, rope.apply(q, k, positions=pos)[0])
+    z = q.clone()
+    assert rope.apply(z, positions=pos, inplace=True) is z and torch.equal(z, back)
+    rope.free()
+
+
+@pytest.mark.parametrize("scaling", [{"type": "linear", "factor": 4.0},
+                                     {"type": "ntk", "factor": 8.0},
+                                     {"type": "yarn", "factor": 8.0, "original_length": 4096},
+                                     {"type": "yarn", "factor": 2.0, "original_length": 512,
+                                      "beta_fast": 16, "beta_slow": 2, "attention_factor": 1.5}])
+def test_rotary_scaled(ctx, scaling):
+    from vectorstorekit_amd import RotaryEmbedding
+
+    rope = RotaryEmbedding(ctx, 64, scaling=scaling, base=5000.0)
+    inv = np.array([5000.0 ** (-2 * i / 64) for i in range(32)])
+    amplitude, f = 1.0, scaling["factor"]
+    if scaling["type"] == "linear":
+        inv = inv / f
+    elif scaling["type"] == "ntk":
+        # the slowest pair is divided by f, the fastest stays
+        ntk = [5000.0 ** (-2 * i / 64) * f ** (-2 * i / 62) for i in range(32)]
+        inv = np.array(ntk)
+        assert abs(inv[-1] * f / 5000.0 ** (-62 / 64) - 1) < 1e-12 and inv[0] == 1
+    else:
+        n, fast, slow = scaling["original_length"], scaling.get("beta_fast", 32), scaling.get("beta_slow", 1)
+        turns = n * inv / (2 * math.pi)
+        at = [64 * math.log(n / (2 * math.pi * b)) / (2 * math.log(5000.0)) for b in (fast, slow)]
+        low, high = max(math.floor(at[0]), 0), min(math.ceil(at[1]), 63)
+        ramp = np.clip((np.arange(32) - low) / (high - low), 0, 1)
+        assert np.all(ramp[turns > fast * 1.5] == 0) and np.all(ramp[turns < slow / 1.5] == 1)
+        inv = inv * (1 - ramp) + inv / f * ramp
+        amplitude = scaling.get("attention_factor", 0.1 * math.log(f) + 1)
+    np.testing.assert_allclose(rope.inv_freq, inv, rtol=1e-12)
+    x = normal(gen(1), 50, 2, 64)
+    pos = ints(range(0, 50 * 997, 997))
+    want = rotated(x, pos, inv, amplitude, "half")
+    check(rope.apply(x, positions=pos), want, 2.0 ** -24 * want.abs()
+          + 2.0 ** -20 * x.cpu().double().abs().amax(-1, keepdim=True) * amplitude)
+
+
+def test_rotary_strides_and_gradient(ctx):
+    """Sliced inputs, and the inverse as the gradient: <R x, y> = <x, R' y>,
+    the formula's, and the differences of the (linear) forward."""
+    from vectorstorekit_amd import RotaryEmbedding
+
+    g = gen(2)
+    rope = RotaryEmbedding(ctx, 48, rotary_dim=32, layout="interleaved",
+                           scaling={"type": "yarn", "factor": 4.0, "original_length": 1024})
+    packed = normal(g, 21, 3, 6, 48)  # q, k, v of one projection
+    q, k = packed[:, 0], packed[:, 1, :2]
+    pos = ints(range(40, 61))
+    a, b = rope.apply(q, k, positions=pos)
+    assert torch.equal(a, rope.apply(q.contiguous(), positions=pos))
+    assert torch.equal(b, rope.apply(k.contiguous(), positions=pos))
+    t = q.transpose(1, 2).contiguous().transpose(1, 2)  # heads not dense
+    assert torch.equal(a, rope.apply(t, positions=pos))
+    y = normal(g, 21, 6, 48)
+    grad = rope.apply(y, positions=pos, inverse=True)
+    want = rotated(y, pos, rope.inv_freq, rope.amplitude, "interleaved", -1.0)
+    check(grad, want, 2.0 ** -24 * want.abs()
+          + 2.0 ** -20 * y.cpu().double().abs().amax(-1, keepdim=True) * rope.amplitude)
+    e = normal(g, 21, 6, 48)
+    h = 0.5
+    up, down = (rope.apply((q + f * e).contiguous(), positions=pos) for f in (h, -h))
+    slope = float(((up - down).double() * y.double()).sum()) / (2 * h)
+    # the sums of 21 * 6 * 48 products, each off by 2^-20 of its size
+    size = float((e.double().abs() * y.double().abs()).sum()) * 4
+    assert abs(slope - float((e.double() * grad.double()).sum())) <= 2.0 ** -20 * size
+
+
+# ---------------------------------------------------------------------- the cache
+
+def filled(ctx, lengths, page, kv, d, dtype, *, layers=1, order="nhd", seed=0, width=None,
+           poison=True):
+    """A cache whose sequences hold pages from all over the pool; what no
+    sequence holds (page tails, free pages) is NaN.  Also each sequence's keys
+    and values, layers x L x kv x d."""
+    from vectorstorekit_amd import PagedKVCache
+
+    g = gen(seed)
+    used = [-(-x // page) for x in lengths]
+    pages = sum(used) + 3
+    width = width or max(max(used), 1)
+    ids = torch.randperm(pages, generator=g).tolist()
+    shape = (layers, pages, page, kv, d)
+    k, v = (torch.full(shape, math.nan if poison else 0.0, dtype=dtype) for _ in range(2))
+    table = torch.full((len(lengths), width), -1, dtype=torch.int32)
+    seqs, at = [], 0
+    for s, x in enumerate(lengths):
+        kk, vv = (torch.randn(layers, x, kv, d, generator=g).to(dtype) for _ in range(2))
+        for i in range(used[s]):
+            p = ids[at]
+            at += 1
+            table[s, i] = p
+            n = min(page, x - i * page)
+            k[:, p, :n], v[:, p, :n] = kk[:, i * page:i * page + n], vv[:, i * page:i * page + n]
+        seqs.append((kk, vv))
+    k, v = k.to(DEV), v.to(DEV)
+    if order == "hnd":  # heads outside the page's rows
+        k, v = (x.transpose(2, 3).contiguous().transpose(2, 3) for x in (k, v))
+    refs = torch.zeros(pages, dtype=torch.int32)
+    refs[table[table >= 0].long()] = 1
+    cache = PagedKVCache.over(ctx, k, v, table.to(DEV), ints(lengths), refs.to(DEV))
+    return cache, seqs
+
+
+TOKEN = [
+    # lengths, page, heads, kv, d, window, sinks
+    ([1], 16, 8, 8, 64, None, 0),
+    ([0, 1, 15, 16, 17, 33], 16, 8, 2, 128, None, 0),
+    ([777], 16, 32, 8, 128, None, 0),
+    ([2050, 3, 0, 129], 64, 4, 1, 128, 100, 4),
+    ([1500], 32, 12, 12, 96, 64, 0),
+    ([300, 299], 128, 20, 5, 80, 1, 1),
+    ([5000, 31], 16, 9, 3, 64, 333, 40),
+    ([260], 32, 8, 1, 256, None, 0),
+    ([200], 16, 34, 2, 128, 50, 2),   # 17 heads a group: two row tiles
+    ([90, 64], 16, 3, 1, 36, 20, 3),  # heads that take no 16-byte loads in 16 bits
+    ([70], 16, 2, 2, 1, None, 0),
+    ([65], 16, 2, 1, 255, 9, 0),
+]
+
+
+@pytest.mark.parametrize("dtype", [BF, F16, F32])
+@pytest.mark.parametrize("lengths,page,heads,kv,d,window,sinks", TOKEN)
+def test_token_attention(ctx, dtype, lengths, page, heads, kv, d, window, sinks):
+    cache, seqs = filled(ctx, lengths, page, kv, d, dtype, layers=2, seed=d + heads)
+    q = normal(gen(5), len(lengths), heads, d, dtype=dtype)
+    scale = d ** -0.5
+    for layer in (0, 1):
+        out, lse = cache.attend(q, layer=layer, window=window, sinks=sinks, return_lse=True)
+        want = [attended(q[i:i + 1], kk[layer], vv[layer], scale, window, sinks)
+                for i, (kk, vv) in enumerate(seqs)]
+        o, l, t = (torch.cat(x) for x in zip(*want))
+        check(out, o, t)
+        check_norm(out, o, dtype)
+        check(lse, l, 2.0 ** -16 * (1 + l.abs()))
+    # a bound of the lengths only divides the work, wrong ones included
+    for bound in (1, 200, 10 ** 6):
+        again = cache.attend(q, layer=1, window=window, sinks=sinks, max_length=bound)
+        check(again, o, t)
+
+
+def test_token_long_split(ctx):
+    """A length that many parts share, and slots out of order."""
+    cache, seqs = filled(ctx, [40, 70001, 5], 64, 2, 128, BF, seed=3)
+    q = normal(gen(6), 2, 8, 128, dtype=BF)
+    out, lse = cache.attend(q, seqs=[1, 0], scale=0.2, return_lse=True)
+    for i, s in enumerate((1, 0)):
+        o, l, t = attended(q[i:i + 1], seqs[s][0][0], seqs[s][1][0], 0.2, None, 0)
+        check(out[i:i + 1], o, t)
+        check(lse[i:i + 1], l, 2.0 ** -16 * (1 + l.abs()))
+
+
+@pytest.mark.parametrize("dtype", [BF, F16, F32])
+@pytest.mark.parametrize("order", ["nhd", "hnd"])
+@pytest.mark.parametrize("news,lengths,page,heads,kv,d,window,sinks", [
+    ([3, 1, 0, 17], [3, 90, 12, 40], 16, 4, 2, 64, None, 0),
+    ([70, 130], [200, 130], 32, 8, 2, 128, 33, 4),
+    ([5], [900], 64, 16, 2, 128, 200, 7),
+    ([300], [300], 64, 2, 1, 96, 64, 0),
+    ([65, 64, 63], [65, 100, 63], 16, 6, 6, 80, 16, 16),
+    ([40, 9], [64, 20], 16, 4, 1, 256, None, 0),
+    ([33], [50], 16, 3, 3, 20, 11, 1),
+])
+def test_prompt_attention(ctx, dtype, order, news, lengths, page, heads, kv, d, window, sinks):
+    """Several new tokens a sequence over the cache, ragged."""
+    cache, seqs = filled(ctx, lengths, page, kv, d, dtype, order=order, seed=d + 1)
+    starts = [0] + list(np.cumsum(news))
+    q = normal(gen(7), starts[-1], heads, d, dtype=dtype)
+    out, lse = cache.attend(q, starts=starts, max_new=max(news), window=window, sinks=sinks,
+                            return_lse=True)
+    for i, (kk, vv) in enumerate(seqs):
+        a, b = starts[i], starts[i + 1]
+        o, l, t = attended(q[a:b], kk[0], vv[0], d ** -0.5, window, sinks)
+        check(out[a:b], o, t)
+        check_norm(out[a:b], o, dtype)
+        check(lse[a:b], l, 2.0 ** -16 * (1 + l.abs()))
+
+
+@pytest.mark.parametrize("dtype", [BF, F16, F32])
+@pytest.mark.parametrize("lengths,heads,kv,d,window,sinks", [
+    ([1], 2, 2, 64, 1, 0),
+    ([333], 4, 4, 64, 128, 4),
+    ([0, 257, 64, 1], 8, 2, 128, 100, 4),
+    ([520, 31], 3, 1, 96, 64, 130),
+    ([190], 4, 1, 256, 32, 0),
+    ([130], 2, 2, 128, None, 0),
+    ([75, 20], 5, 5, 40, 30, 2),
+    ([66], 2, 1, 33, 12, 5),
+])
+def test_window_attention(ctx, dtype, lengths, heads, kv, d, window, sinks):
+    from vectorstorekit_amd import window_attention
+
+    g = gen(d)
+    starts = [0] + list(np.cumsum(lengths))
+    packed = normal(g, starts[-1], heads + 2 * kv, d, dtype=dtype)  # one projection's output
+    q, k, v = packed[:, :heads], packed[:, heads:heads + kv], packed[:, heads + kv:]
+    out, lse = window_attention(ctx, q, k, v, starts=starts, max_length=max(lengths),
+                                window=window, sinks=sinks, return_lse=True)
+    dense = window_attention(ctx, q.contiguous(), k.contiguous(), v.contiguous(),
+                             starts=ints(starts), window=window, sinks=sinks)
+    for i in range(len(lengths)):
+        a, b = starts[i], starts[i + 1]
+        o, l, t = attended(q[a:b], k[a:b], v[a:b], d ** -0.5, window, sinks)
+        check(out[a:b], o, t)
+        check(dense[a:b], o, t)
+        check_norm(out[a:b], o, dtype)
+        check(lse[a:b], l, 2.0 ** -16 * (1 + l.abs()))
+
+
+def test_queries_before_the_keys(ctx):
+    """More queries than keys: the first ones stand before every key, see
+    nothing and get zeros."""
+    from vectorstorekit_amd import window_attention
+
+    g = gen(8)
+    q, k, v = (normal(g, n, 2, 64, dtype=BF) for n in (40, 25, 25))
+    out, lse = window_attention(ctx, q, k, v, starts=[0, 30, 40], k_starts=[0, 25, 25],
+                                return_lse=True)
+    assert not out[:5].any() and not out[30:].any()
+    assert bool(torch.isneginf(lse[:5]).all()) and bool(torch.isneginf(lse[30:]).all())
+    o, _, t = attended(q[5:30], k, v, 64 ** -0.5, None, 0)
+    check(out[5:30], o, t)
+
+
+@pytest.mark.parametrize("dtype", [BF, F16, F32])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("heads,kv,d,n", [(4, 2, 128, 150), (2, 2, 64, 400), (4, 1, 256, 70)])
+def test_masked_places_do_not_reach_sums(ctx, dtype, bad, heads, kv, d, n):
+    """A key or value that is not finite reaches the rows that see it and no
+    others: the masked product 0 * NaN is not taken."""
+    from vectorstorekit_amd import window_attention
+
+    g = gen(9)
+    q, k, v = (normal(g, n, h, d, dtype=dtype) for h in (heads, kv, kv))
+    at, window, sinks = n - 45, 20, 3
+    for x, j in ((k, at), (v, at), (v, 1)):
+        y = [t.clone() for t in (k, v)]
+        (y[0] if x is k else y[1])[j, 0, d // 2] = bad
+        out = window_attention(ctx, q, *y, starts=[0, n], window=window, sinks=sinks)
+        rows = torch.arange(n)
+        see = (rows >= j) & ((rows - j < window) | (j < sinks))
+        clean, _, t = attended(q, k, v, d ** -0.5, window, sinks)
+        first = slice(0, heads // kv)  # the heads of key head 0
+        hidden = torch.ones(n, heads, dtype=torch.bool)
+        hidden[see, first] = False
+        got = out.cpu().double()
+        assert bool(torch.isfinite(got[hidden]).all())
+        assert bool(((got - clean).abs() <= t)[hidden].all())
+        if x is v:
+            col = got[see][:, first, d // 2]
+            assert not bool(torch.isfinite(col).any())
+            rest = torch.ones(d, dtype=torch.bool)
+            rest[d // 2] = False
+            assert bool(torch.isfinite(got[see][:, first][..., rest]).all())
+        elif math.isnan(bad):
+            assert bool(torch.isnan(got[see][:, first]).all())
+
+
+def test_large_scores(ctx):
+    """Scores far apart: the running maximum carries the sums."""
+    cache, seqs = filled(ctx, [500], 16, 1, 64, F32, seed=4)
+    cache.k.mul_(30.0)
+    kk = seqs[0][0] * 30.0
+    q = normal(gen(10), 1, 2, 64) * 30.0
+    out = cache.attend(q)
+    o, _, t = attended(q, kk[0], seqs[0][1][0], 0.125, None, 0)
+    check(out, o, t)
+
+
+@pytest.mark.parametrize("dtype,d,r,layout", [(BF, 128, 128, "half"), (F16, 96, 48, "interleaved"),
+                                              (F32, 37, 10, "half")])
+@pytest.mark.parametrize("order", ["nhd", "hnd"])
+def test_append(ctx, dtype, d, r, layout, order):
+    """The new tokens' rows land in their places, turned; no other row of the
+    pool changes."""
+    from vectorstorekit_amd import RotaryEmbedding
+
+    lengths, news, page, kv, heads = [40, 7, 16, 100], [40, 1, 0, 33], 16, 2, 6
+    cache, _ = filled(ctx, lengths, page, kv, d, dtype, layers=2, order=order, seed=d,
+                      poison=False)
+    rope = RotaryEmbedding(ctx, d, rotary_dim=r, layout=layout)
+    starts = [0] + list(np.cumsum(news))
+    g = gen(11)
+    q, k, v = (normal(g, starts[-1], h, d, dtype=dtype) for h in (heads, kv, kv))
+    want_k, want_v = cache.k.cpu().clone(), cache.v.cpu().clone()
+    table = cache.table.cpu()
+    pos = torch.cat([torch.arange(L - n, L) for L, n in zip(lengths, news)]).to(torch.int32).to(DEV)
+    turned_q, turned_k = rope.apply(q, k, positions=pos)
+    out = cache.append(k, v, starts=starts, max_new=40, layer=1, rotary=rope, q=q)
+    assert torch.equal(out, turned_q)
+    t = 0
+    for s, (length, n) in enumerate(zip(lengths, news)):
+        for p in range(length - n, length):
+            want_k[1, table[s, p // page], p % page] = turned_k[t].cpu()
+            want_v[1, table[s, p // page], p % page] = v[t].cpu()
+            t += 1
+    assert torch.equal(cache.k.cpu(), want_k) and torch.equal(cache.v.cpu(), want_v)
+    # one token each, slots out of order, as it is
+    k1, v1 = normal(g, 2, kv, d, dtype=dtype), normal(g, 2, kv, d, dtype=dtype)
+    assert cache.append(k1, v1, seqs=[3, 0]) is None
+    for i, s in enumerate((3, 0)):
+        p = lengths[s] - 1
+        want_k[0, table[s, p // page], p % page] = k1[i].cpu()
+        want_v[0, table[s, p // page], p % page] = v1[i].cpu()
+    assert torch.equal(cache.k.cpu(), want_k) and torch.equal(cache.v.cpu(), want_v)
+
+
+# ---------------------------------------------------------------------- the pages
+
+class Model:
+    """The page keeping on the host: lists and a loop."""
+
+    def __init__(self, cache):
+        self.page, self.width = cache.page_size, cache.width
+        self.k, self.v = cache.k.cpu().clone(), cache.v.cpu().clone()
+        self.table = cache.table.cpu().tolist()
+        self.lengths, self.refs = cache.lengths.cpu().tolist(), cache.refs.cpu().tolist()
+
+    def take(self, left):
+        return next((i for i, r in enumerate(self.refs) if r == 0), None) if left else None
+
+    def free(self, seqs):
+        for s in seqs:
+            for i, p in enumerate(self.table[s]):
+                if p >= 0:
+                    self.refs[p] -= 1
+                self.table[s][i] = -1
+            self.lengths[s] = 0
+
+    def reserve(self, seqs, counts):
+        missing = 0
+        for s, n in zip(seqs, counts):
+            old, to = self.lengths[s], self.lengths[s] + n
+            for i in range(-(-old // self.page), -(-to // self.page)):
+                p = self.take(i < self.width)
+                if p is None:
+                    missing += 1
+                    to = min(to, i * self.page)
+                else:
+                    self.table[s][i], self.refs[p] = p, 1
+            self.lengths[s] = to
+        return missing
+
+    def fork(self, parents, children):
+        missing = 0
+        self.free(children)
+        for f, c in zip(parents, children):
+            for i in range(self.lengths[f] // self.page):
+                self.table[c][i] = self.table[f][i]
+                self.refs[self.table[f][i]] += 1
+        for f, c in zip(parents, children):
+            full, fill = divmod(self.lengths[f], self.page)
+            self.lengths[c] = full * self.page
+            if fill:
+                p = self.take(True)
+                if p is None:
+                    missing += 1
+                    continue
+                self.table[c][full], self.refs[p] = p, 1
+                for x in (self.k, self.v):
+                    x[:, p, :fill] = x[:, self.table[f][full], :fill]
+                self.lengths[c] += fill
+        return missing
+
+    def compact(self):
+        live = sum(r > 0 for r in self.refs)
+        holes = [i for i in range(live) if self.refs[i] == 0]
+        movers = [i for i in range(live, len(self.refs)) if self.refs[i] > 0]
+        for to, at in zip(holes, movers):
+            for x in (self.k, self.v):
+                x[:, to] = x[:, at]
+            self.refs[to], self.refs[at] = self.refs[at], 0
+        new = dict(zip(movers, holes))
+        self.table = [[new.get(p, p) for p in row] for row in self.table]
+        return live
+
+    def same(self, cache):
+        assert cache.table.cpu().tolist() == self.table
+        assert cache.lengths.cpu().tolist() == self.lengths
+        assert cache.refs.cpu().tolist() == self.refs
+        assert torch.equal(cache.k.cpu(), self.k) and torch.equal(cache.v.cpu(), self.v)
+
+
+@pytest.mark.parametrize("dtype,kv,d,order", [(BF, 2, 64, "nhd"), (F16, 3, 5, "nhd"),
+                                              (F32, 2, 32, "hnd"), (F16, 2, 3, "hnd")])
+@pytest.mark.parametrize("pages", [40, 5000])
+def test_pages(ctx, dtype, kv, d, order, pages):
+    """A program's life: sequences grow, branch, end and the pool is packed,
+    step by step as on the host; with 40 pages it runs out of them."""
+    from vectorstorekit_amd import PagedKVCache
+
+    page, slots, width, layers = 16, 8, 9, 2
+    g = gen(pages + d)
+    shape = (layers, pages, page, kv, d)
+    k, v = (torch.randn(shape, generator=g).to(dtype).to(DEV) for _ in range(2))
+    if order == "hnd":
+        k, v = (x.transpose(2, 3).contiguous().transpose(2, 3) for x in (k, v))
+    refs = torch.zeros(pages, dtype=torch.int32)
+    if pages > 100:  # most of a large pool is held by others
+        refs[torch.randperm(pages, generator=g)[: pages - 60]] = 1
+    cache = PagedKVCache.over(ctx, k, v, torch.full((slots, width), -1, dtype=torch.int32,
+                                                    device=DEV),
+                              torch.zeros(slots, dtype=torch.int32, device=DEV), refs.to(DEV))
+    m = Model(cache)
+    rng = np.random.default_rng(pages)
+    short = 0
+    for step in range(40):
+        what = rng.integers(0, 5)
+        if what <= 1:
+            seqs = rng.permutation(slots)[: rng.integers(1, slots + 1)].tolist()
+            counts = rng.integers(0, 50, len(seqs)).tolist()
+            missing = m.reserve(seqs, counts)
+            cache.reserve(seqs, counts)
+            assert cache.missing() == missing
+            short += missing
+        elif what == 2:
+            order_ = rng.permutation(slots).tolist()
+            n = int(rng.integers(1, slots // 2 + 1))
+            children = order_[:n]
+            parents = [order_[n + int(rng.integers(0, slots - n))] for _ in range(n)]
+            missing = m.fork(parents, children)
+            cache.fork(parents, children)
+            assert cache.missing() == missing
+            short += missing
+        elif what == 3:
+            seqs = rng.permutation(slots)[: rng.integers(0, 3)].tolist()
+            m.free(seqs)
+            cache.free(seqs)
+        else:
+            assert int(cache.compact()) == m.compact()
+        m.same(cache)
+    assert short > 0 or pages > 100
+
+
+def test_copy_pages(ctx):
+    cache, _ = filled(ctx, [100], 32, 2, 40, F16, layers=3, seed=1, poison=False)
+    k, v = cache.k.cpu().clone(), cache.v.cpu().clone()
+    cache.copy_pages([0, 2], [5, 4])
+    for x in (k, v):
+        x[:, [5, 4]] = x[:, [0, 2]]
+    assert torch.equal(cache.k.cpu(), k) and torch.equal(cache.v.cpu(), v)
+
+
+# ------------------------------------------------------------- streams and graphs
+
+def test_other_stream_and_graph(ctx):
+    """A decoding step on a stream of its own, captured and replayed with new
+    inputs: each replay equals the eager calls."""
+    from vectorstorekit_amd import RotaryEmbedding
+
+    cache, _ = filled(ctx, [700, 33], 32, 2, 64, BF, seed=12, poison=False)
+    rope = RotaryEmbedding(ctx, 64)
+    q, k, v = (torch.zeros(2, h, 64, dtype=BF, device=DEV) for h in (4, 2, 2))
+
+    def step():
+        turned = cache.append(k, v, rotary=rope, q=q)
+        return cache.attend(turned, window=300, sinks=4)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    for i in range(4):
+        g = gen(20 + i)
+        for x in (q, k, v):
+            x.copy_(torch.randn(x.shape, generator=g).to(BF))
+        graph.replay()
+        got = held.clone()
+        eager = step()
+        torch.cuda.synchronize()
+        assert torch.equal(got, eager)
+
+
+# ------------------------------------------------------------------------ refusals
+
+def test_refusals(ctx):
+    from vectorstorekit_amd import PagedKVCache, RotaryEmbedding, VSKError, window_attention
+
+    def refused(kind, f, *a, **k):
+        with pytest.raises(VSKError) as e:
+            f(*a, **k)
+        assert e.value.kind == kind, e.value
+
+    bad = "invalidArgument"
+    for args in ({"layout": "spiral"}, {"rotary_dim": 7}, {"rotary_dim": 80}, {"base": 0.0},
+                 {"scaling": {"type": "linear"}}, {"scaling": {"type": "who", "factor": 2}},
+                 {"scaling": {"type": "yarn", "factor": 2}},
+                 {"scaling": {"type": "ntk", "factor": 2, "more": 1}}):
+        refused(bad, RotaryEmbedding, ctx, 64, **args)
+    rope = RotaryEmbedding(ctx, 64)
+    x = torch.zeros(3, 2, 64, device=DEV)
+    pos = ints([0, 1, 2])
+    refused("dimensionMismatch", rope.apply, x[..., :32], positions=pos)
+    refused("dimensionMismatch", rope.apply, x, positions=pos[:2])
+    refused(bad, rope.apply, x, positions=pos.long())
+    refused(bad, rope.apply, x.cpu(), positions=pos)
+    refused("unsupportedOperation", rope.apply, x.double(), positions=pos)
+    assert rope.apply(x[:0], positions=pos[:0]).shape == (0, 2, 64)
+
+    cache, _ = filled(ctx, [20, 4], 16, 2, 64, F32, poison=False)
+    k, v, t, n = cache.k, cache.v, cache.table, cache.lengths
+    refused("unsupportedOperation", PagedKVCache.over, ctx, k[:, :, :8], v[:, :, :8], t, n)
+    refused("dimensionMismatch", PagedKVCache.over, ctx, k, v[:, :, :, :1], t, n)
+    refused("dimensionMismatch", PagedKVCache.over, ctx, k, v, t, n[:1])
+    refused(bad, PagedKVCache.over, ctx, k, v, t.long(), n)
+    refused("unsupportedOperation", PagedKVCache.over(ctx, k, v, t, n).compact)
+    refused("unsupportedOperation", PagedKVCache, ctx, pages=4, page_size=24, kv_heads=1,
+            head_dim=8, slots=1, width=1)
+    q = torch.zeros(2, 4, 64, device=DEV)
+    refused("dimensionMismatch", cache.attend, q[:, :3])
+    refused("dimensionMismatch", cache.attend, q[..., :32])
+    refused(bad, cache.attend, q.half())
+    refused(bad, cache.attend, torch.zeros(3, 4, 64, device=DEV))  # more than the slots
+    refused(bad, cache.attend, q, scale=0.0)
+    refused(bad, cache.attend, q, scale=math.inf)
+    refused(bad, cache.attend, q, window=0)
+    refused(bad, cache.attend, q, sinks=-1)
+    refused(bad, cache.attend, q, layer=1)
+    refused("dimensionMismatch", cache.attend, q, seqs=[0])
+    refused("dimensionMismatch", cache.append, x[:2], x[:2, :1])
+    refused("dimensionMismatch", cache.append, x[:2], x[:1])
+    refused("dimensionMismatch", cache.append, x[:2], x[:2], rotary=RotaryEmbedding(ctx, 32))
+    refused(bad, cache.fork, [0], [0])
+    refused(bad, cache.fork, [0, 0], [1, 1])
+    refused(bad, cache.fork, [0], [2])
+    refused("dimensionMismatch", cache.reserve, [0, 1], [1])
+    refused("dimensionMismatch", window_attention, ctx, x, x[:, :, :32], x, starts=[0, 3])
+    refused("dimensionMismatch", window_attention, ctx, x, x[:2], x[:2], starts=[0, 3])
+    refused("dimensionMismatch", window_attention, ctx, x, x, x, starts=[0, 3], k_starts=[0])
+    refused(bad, window_attention, ctx, x, x.half(), x, starts=[0, 3])
+    big = torch.zeros(1, 1, 320, device=DEV)
+    refused("unsupportedOperation", window_attention, ctx, big, big, big, starts=[0, 1])
+    assert cache.attend(q[:0]).shape == (0, 4, 64)
+    # nothing was lost on the way
+    assert int(cache.lengths[0]) == 20 and cache.missing() == 0

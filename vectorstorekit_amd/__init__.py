@@ -31,3 +31,14 @@ from .quantization import (  # noqa: F401,E402
     ScalarQuantizer,
     SQ8Database,
 )
+
+# the cache and its attention work on torch tensors; torch is imported with them
+_KVCACHE = ("PagedKVCache", "RotaryEmbedding", "window_attention")
+
+
+def __getattr__(name):
+    if name in _KVCACHE:
+        from . import kvcache
+
+        return getattr(kvcache, name)
+    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")

@@ -82,6 +82,34 @@ class vsk_config(ctypes.Structure):
     _fields_ = [("kernel", c_int32), ("enable_profiling", c_int32), ("max_tile_bytes", c_int64)]
 
 
+class vsk_head_rows(ctypes.Structure):
+    _fields_ = [("src", c_void_p), ("dst", c_void_p), ("src_row", c_int64), ("src_head", c_int64),
+                ("dst_row", c_int64), ("dst_head", c_int64), ("heads", c_int32)]
+
+
+class vsk_kv(ctypes.Structure):
+    _fields_ = [("k", c_void_p), ("v", c_void_p),
+                ("k_layer", c_int64), ("k_page", c_int64), ("k_row", c_int64),
+                ("k_head", c_int64), ("v_layer", c_int64), ("v_page", c_int64),
+                ("v_row", c_int64), ("v_head", c_int64),
+                ("table", c_void_p), ("lengths", c_void_p), ("refs", c_void_p),
+                ("status", c_void_p), ("scratch", c_void_p), ("table_stride", c_int64),
+                ("dtype", c_int32), ("layers", c_int32), ("pages", c_int32),
+                ("page_size", c_int32), ("kv_heads", c_int32), ("head_dim", c_int32),
+                ("slots", c_int32), ("width", c_int32)]
+
+
+class vsk_new_tokens(ctypes.Structure):
+    _fields_ = [("starts", c_void_p), ("seqs", c_void_p), ("n", c_int32), ("max_new", c_int32),
+                ("tokens", c_int64)]
+
+
+class vsk_attention_args(ctypes.Structure):
+    _fields_ = [("q", vsk_head_rows), ("lse", c_void_p), ("k_starts", c_void_p),
+                ("workspace", c_void_p), ("workspace_bytes", c_int64), ("scale", c_float),
+                ("window", c_int32), ("sinks", c_int32), ("max_length", c_int32)]
+
+
 KERNEL_AUTO, KERNEL_EXACT, KERNEL_SCREEN, KERNEL_BF16X3, KERNEL_FP32 = 0, 1, 2, 3, 4
 
 P = c_void_p  # every buffer argument is passed as a raw address
@@ -164,6 +192,18 @@ SIGNATURES = {
     "vsk_bin_free": (c_int32, [P, P]),
     "vsk_bin_search": (c_int32, [P, P, P, c_int64, c_int32, P, P]),
     "vsk_bin_distances": (c_int32, [P, P, P, c_int64, P]),
+    "vsk_rotary_create": (c_int32, [P, P, c_int32, c_int32, c_double, PP]),
+    "vsk_rotary_free": (c_int32, [P, P]),
+    "vsk_rotary_apply": (c_int32, [P, P, P, c_int32, c_int32, c_int64, P, c_int32, P, c_int32]),
+    "vsk_kv_scratch_ints": (c_int64, [c_int32, c_int32]),
+    "vsk_kv_reserve": (c_int32, [P, P, P, P, P, c_int32]),
+    "vsk_kv_fork": (c_int32, [P, P, P, P, P, c_int32]),
+    "vsk_kv_free": (c_int32, [P, P, P, P, c_int32]),
+    "vsk_kv_compact": (c_int32, [P, P, P]),
+    "vsk_kv_copy": (c_int32, [P, P, P, P, P, c_int32]),
+    "vsk_kv_append": (c_int32, [P, P, P, c_int32, P, P, P, P, P]),
+    "vsk_attention_workspace": (c_int64, [P, P, P, P]),
+    "vsk_attention": (c_int32, [P, P, P, c_int32, P, P]),
 }
 
 _lib = None

@@ -1,0 +1,177 @@
+// attention.hip -- the attention entry points: checks, the division of the
+// work, and the choice of kernel.
+#include <cmath>
+
+#include "attn.hpp"
+#include "vsk_api.hpp"
+
+namespace vsk {
+
+namespace {
+
+int32_t padded_head(int32_t d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
+
+// How a call's work is divided.
+struct Plan {
+  int32_t tiles, splits, chunk;
+  bool split_keys;
+};
+
+Plan plan_of(const vsk_ctx *ctx, const vsk_kv *kv, const vsk_new_tokens *news,
+             const vsk_attention_args *args) {
+  Plan p;
+  const int64_t group = args->q.heads / kv->kv_heads;
+  const int64_t max_new = news->starts ? news->max_new : 1;
+  p.tiles = (int32_t)ceil_div(max_new * group, 16);
+  const int64_t blocks = (int64_t)news->n * kv->kv_heads * p.tiles;
+  const int32_t key_tile = kv->dtype == VSK_DTYPE_F32 ? 16 : 32;
+  p.splits = 1;
+  p.chunk = 1 << 30;
+  // row tiles enough to fill the device: a wave each
+  p.split_keys = blocks < 8 * (int64_t)ctx->cu_count || p.tiles < 4;
+  if (!p.split_keys) return p;
+  int64_t keys = kv->table ? (int64_t)kv->width * kv->page_size : kv->pages;
+  if (args->max_length > 0 && args->max_length < keys) keys = args->max_length;
+  if (args->window > 0) {
+    const int64_t seen = (int64_t)args->window + args->sinks + ceil_div(16, group) + 2 * key_tile;
+    if (seen < keys) keys = seen;
+  }
+  // parts of at least a tile for each of the four waves, as many as keep every
+  // compute unit supplied with blocks
+  const int64_t tiles = ceil_div(keys, key_tile);
+  const int64_t target = ceil_div(8 * (int64_t)ctx->cu_count, blocks);
+  int64_t chunk = ceil_div(ceil_div(tiles, target), 4) * 4;
+  p.chunk = (int32_t)(chunk < 4 ? 4 : chunk);
+  p.splits = (int32_t)ceil_div(tiles, p.chunk);
+  if (p.splits < 1) p.splits = 1;
+  return p;
+}
+
+int64_t workspace_of(const Plan &p, const vsk_kv *kv, const vsk_new_tokens *news,
+                     const vsk_attention_args *args) {
+  if (p.splits == 1) return 0;
+  return (int64_t)sizeof(float) * p.splits * news->tokens * args->q.heads *
+         (padded_head(kv->head_dim) + 2);
+}
+
+void check_shapes(const vsk_kv *kv, const vsk_new_tokens *news, const vsk_attention_args *args) {
+  VSK_REQUIRE(kv && news && args, VSK_ERR_INVALID_ARGUMENT, "null argument");
+  VSK_REQUIRE(kv->dtype >= VSK_DTYPE_F32 && kv->dtype <= VSK_DTYPE_BF16, VSK_ERR_UNSUPPORTED,
+              "unknown data type");
+  VSK_REQUIRE(kv->kv_heads >= 1 && args->q.heads >= 1 && args->q.heads % kv->kv_heads == 0,
+              VSK_ERR_DIMENSION_MISMATCH, "query heads must be a multiple of the key heads");
+  VSK_REQUIRE(kv->head_dim >= 1 && kv->head_dim <= VSK_MAX_HEAD_DIM, VSK_ERR_UNSUPPORTED,
+              "a head holds between 1 and 256 values");
+  VSK_REQUIRE(news->n >= 0 && news->max_new >= 0 && news->tokens >= 0 && kv->pages >= 0 &&
+                  args->window >= 0 && args->sinks >= 0 && args->max_length >= 0,
+              VSK_ERR_INVALID_ARGUMENT, "negative counts");
+  VSK_REQUIRE((int64_t)news->max_new * args->q.heads <= 0x3FFFFFFFll, VSK_ERR_INVALID_BUFFER_SIZE,
+              "too many query rows in one sequence");
+}
+
+template <class P> bool aligned_to(const P *p, int64_t bytes) {
+  return ((uintptr_t)p % bytes) == 0;
+}
+
+}  // namespace
+
+}  // namespace vsk
+
+using namespace vsk;
+
+extern "C" {
+
+int64_t vsk_attention_workspace(vsk_ctx *ctx, const vsk_kv *kv, const vsk_new_tokens *news,
+                                const vsk_attention_args *args) {
+  if (!ctx || !kv || !news || !args || kv->kv_heads < 1 || args->q.heads < 1 || news->n < 1 ||
+      args->q.heads % kv->kv_heads || news->max_new < 0 || news->tokens < 1)
+    return 0;
+  return workspace_of(plan_of(ctx, kv, news, args), kv, news, args);
+}
+
+vsk_status vsk_attention(vsk_ctx *ctx, void *stream, const vsk_kv *kv, int32_t layer,
+                         const vsk_new_tokens *news, const vsk_attention_args *args) {
+  VSK_API_BEGIN(ctx);
+  check_shapes(kv, news, args);
+  VSK_REQUIRE(std::isfinite(args->scale) && args->scale > 0, VSK_ERR_INVALID_ARGUMENT,
+              "scale must be positive and finite");
+  check_news(news);
+  if (news->n == 0 || news->tokens == 0 || news->max_new == 0) return VSK_OK;
+  const bool paged = kv->table != nullptr;
+  if (paged) {
+    check_kv(kv);
+    VSK_REQUIRE(layer >= 0 && layer < kv->layers, VSK_ERR_INVALID_ARGUMENT, "no such layer");
+    VSK_REQUIRE(news->seqs || news->n <= kv->slots, VSK_ERR_INVALID_ARGUMENT,
+                "more sequences than the cache has slots");
+  } else {
+    VSK_REQUIRE(kv->page_size == 0 && layer == 0, VSK_ERR_INVALID_ARGUMENT,
+                "dense keys have no pages or layers");
+    VSK_REQUIRE(args->k_starts && is_device_ptr(args->k_starts), VSK_ERR_INVALID_ARGUMENT,
+                "dense keys need k_starts in device memory");
+    VSK_REQUIRE(kv->k_row >= 0 && kv->v_row >= 0 && kv->k_row <= (1 << 26) &&
+                    kv->v_row <= (1 << 26),
+                VSK_ERR_INVALID_BUFFER_SIZE, "a row stride of more than 2^26 elements");
+    VSK_REQUIRE(kv->k && kv->v && is_device_ptr(kv->k) && is_device_ptr(kv->v),
+                VSK_ERR_INVALID_ARGUMENT, "keys and values must be device memory");
+  }
+  VSK_REQUIRE(news->starts || news->tokens >= news->n, VSK_ERR_DIMENSION_MISMATCH,
+              "fewer rows than sequences");
+  VSK_REQUIRE(args->q.src && args->q.dst && is_device_ptr(args->q.src) &&
+                  is_device_ptr(args->q.dst) && (!args->lse || is_device_ptr(args->lse)),
+              VSK_ERR_INVALID_ARGUMENT, "queries and outputs must be device memory");
+  const Plan p = plan_of(ctx, kv, news, args);
+  const int64_t need = workspace_of(p, kv, news, args);
+  VSK_REQUIRE(need == 0 || (args->workspace && args->workspace_bytes >= need &&
+                            aligned_to(args->workspace, 16) && is_device_ptr(args->workspace)),
+              VSK_ERR_INVALID_BUFFER_SIZE,
+              "the workspace must be " + std::to_string(need) + " bytes of device memory");
+  const int64_t size = kv->dtype == VSK_DTYPE_F32 ? 4 : 2;
+  AttnArgs a{};
+  a.q = args->q.src;
+  a.out = args->q.dst;
+  a.lse = args->lse;
+  a.q_row = args->q.src_row, a.q_head = args->q.src_head;
+  a.o_row = args->q.dst_row, a.o_head = args->q.dst_head;
+  a.k = static_cast<const char *>(kv->k) + (paged ? layer * kv->k_layer * size : 0);
+  a.v = static_cast<const char *>(kv->v) + (paged ? layer * kv->v_layer * size : 0);
+  a.k_row = kv->k_row, a.k_head = kv->k_head, a.v_row = kv->v_row, a.v_head = kv->v_head;
+  a.starts = news->starts;
+  a.seqs = news->seqs;
+  if (paged) {
+    a.k_page = kv->k_page, a.v_page = kv->v_page;
+    a.table = kv->table, a.lengths = kv->lengths, a.table_stride = kv->table_stride;
+    a.pages = kv->pages, a.slots = kv->slots, a.width = kv->width;
+    a.page_shift = __builtin_ctz((unsigned)kv->page_size);
+  } else {
+    a.k_starts = args->k_starts;
+    a.k_rows = kv->pages;
+  }
+  a.tokens = news->tokens;
+  a.n = news->n;
+  a.heads = args->q.heads;
+  a.kv_heads = kv->kv_heads;
+  a.group = a.heads / a.kv_heads;
+  a.d = kv->head_dim;
+  a.window = args->window;
+  a.sinks = args->sinks;
+  a.max_new = news->starts ? news->max_new : 1;
+  a.tiles = p.tiles, a.splits = p.splits, a.chunk = p.chunk;
+  a.scale_log2 = args->scale * 1.4426950408889634f;
+  if (need) {
+    a.part_o = static_cast<float *>(args->workspace);
+    a.part_ml = a.part_o + (int64_t)p.splits * a.tokens * a.heads * padded_head(a.d);
+  }
+  // 16-byte loads, and stores of four values
+  const int64_t w = 16 / size;
+  bool al = a.d % w == 0 && aligned_to(a.q, 16) && aligned_to(a.k, 16) && aligned_to(a.v, 16) &&
+            a.q_row % w == 0 && a.q_head % w == 0 && a.k_row % w == 0 && a.k_head % w == 0 &&
+            a.v_row % w == 0 && a.v_head % w == 0 && a.k_page % w == 0 && a.v_page % w == 0 &&
+            aligned_to(a.out, 4 * size) && a.o_row % 4 == 0 && a.o_head % 4 == 0;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  launch_attn_rows(ctx, st, a, kv->dtype, al, p.split_keys);
+  launch_attn_join(ctx, st, a, kv->dtype, al);
+  finish_queued(ctx, st);
+  VSK_API_END(ctx);
+}
+
+}  // extern "C"

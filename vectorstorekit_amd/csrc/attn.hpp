@@ -1,0 +1,181 @@
+// attn.hpp -- what the attention kernels share: the operands of one call, the
+// keys that a tile of query rows sees, and the 16- and 32-bit element types.
+//
+// A sequence's new tokens are its last ones: of T new tokens over a length L
+// (the new ones included), token t stands at position L - T + t and sees key
+// j when j <= its position and (no window, or position - j < window, or
+// j < sinks).  The query heads of one key head are packed into rows, row =
+// token * group + head within the group, so that keys and values are read
+// once for all of them.
+#pragma once
+
+#include "vsk_core.hpp"
+
+namespace vsk {
+
+typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
+typedef __attribute__((ext_vector_type(4))) __bf16 bf16x4;
+typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
+typedef __attribute__((ext_vector_type(4))) _Float16 f16x4;
+typedef __attribute__((ext_vector_type(4))) float f32x4;
+typedef __attribute__((ext_vector_type(16))) float f32x16;
+typedef __attribute__((ext_vector_type(4))) uint32_t u32x4;
+typedef __attribute__((ext_vector_type(2))) uint32_t u32x2;
+
+// The operands of a call, by value to every kernel.  Strides in elements.
+struct AttnArgs {
+  const void *q, *k, *v;
+  void *out;
+  float *lse;  // tokens x heads, or null
+  int64_t q_row, q_head, o_row, o_head;
+  int64_t k_page, k_row, k_head, v_page, v_row, v_head;
+  const int32_t *table;    // slots x width page ids; null: dense rows
+  const int32_t *lengths;  // per slot (paged)
+  const int32_t *starts;   // n + 1 offsets of the sequences' tokens, or null: one each
+  const int32_t *k_starts; // n + 1 offsets of the sequences' keys (dense)
+  const int32_t *seqs;     // slot of each sequence, or null
+  int64_t table_stride;
+  int64_t tokens, k_rows;
+  int32_t n, heads, kv_heads, group, d;
+  int32_t pages, page_shift, slots, width;
+  int32_t window, sinks;  // window <= 0: none
+  int32_t max_new;
+  int32_t tiles;        // row tiles of a sequence's max_new tokens
+  int32_t splits;       // parts a tile's keys may be split into
+  int32_t chunk;        // key tiles of a part
+  float scale_log2;     // scale * log2(e)
+  float *part_o;        // splits x tokens x heads x d
+  float *part_ml;       // splits x tokens x heads x 2: maximum (log2), sum
+};
+
+// One sequence of the call.
+struct AttnSeq {
+  int64_t token0, key0;  // its first row in q; its first dense key
+  int32_t slot, T, L;    // new tokens, keys
+};
+
+__device__ inline AttnSeq attn_seq(const AttnArgs &a, int32_t b) {
+  AttnSeq s;
+  s.slot = a.seqs ? a.seqs[b] : b;
+  if (a.starts) {
+    int32_t t0 = a.starts[b], t1 = a.starts[b + 1];
+    t0 = t0 < 0 ? 0 : t0;
+    if (t1 > a.tokens) t1 = (int32_t)a.tokens;
+    s.token0 = t0;
+    s.T = t1 > t0 ? t1 - t0 : 0;
+  } else {
+    s.token0 = b;
+    s.T = 1;
+  }
+  s.key0 = 0;
+  // every index below is taken from device memory, so each is held to its
+  // buffer here: a slot, length or offset out of range reads no foreign memory
+  if (a.table) {
+    if ((uint32_t)s.slot >= (uint32_t)a.slots) {
+      s.slot = 0;
+      s.L = 0;
+    } else {
+      const int64_t most = (int64_t)a.width << a.page_shift;
+      const int32_t l = a.lengths[s.slot];
+      s.L = l < 0 ? 0 : l > most ? (int32_t)most : l;
+    }
+  } else {
+    int64_t k0 = a.k_starts[b], k1 = a.k_starts[b + 1];
+    k0 = k0 < 0 ? 0 : k0;
+    if (k1 > a.k_rows) k1 = a.k_rows;
+    s.key0 = k0;
+    s.L = k1 > k0 ? (int32_t)(k1 - k0) : 0;
+  }
+  return s;
+}
+
+// The keys that query positions q0 .. q1 see between them, in tiles of KT
+// keys: the sinks' tiles from 0, then the tiles from lo on.
+template <int KT> struct AttnSpan {
+  int32_t lo, hi, sink_tiles, tiles;
+  __device__ int32_t base(int32_t t) const {
+    return t < sink_tiles ? KT * t : lo + KT * (t - sink_tiles);
+  }
+};
+template <int KT>
+__device__ inline AttnSpan<KT> attn_span(const AttnArgs &a, int32_t q0, int32_t q1) {
+  AttnSpan<KT> s;
+  s.hi = q1 + 1 > 0 ? q1 + 1 : 0;
+  s.lo = 0;
+  s.sink_tiles = 0;
+  if (a.window > 0) {
+    const int64_t first = (int64_t)q0 - a.window + 1;
+    if (first > 0) {
+      const int32_t lo = (int32_t)first & ~(KT - 1);
+      const int32_t st = a.sinks / KT + (a.sinks % KT != 0);
+      if ((int64_t)st * KT < lo) {
+        s.lo = lo;
+        s.sink_tiles = st;
+      }
+    }
+  }
+  s.tiles = s.sink_tiles + (s.hi > s.lo ? (s.hi - s.lo + KT - 1) / KT : 0);
+  return s;
+}
+
+// Parts of `tiles` key tiles: part s holds tiles s * chunk on, the last part
+// all that is left (a length over the caller's bound only makes it longer).
+__device__ inline int32_t attn_parts(const AttnArgs &a, int32_t tiles) {
+  const int32_t p = (tiles + a.chunk - 1) / a.chunk;
+  return p < 1 ? 1 : p > a.splits ? a.splits : p;
+}
+
+__device__ inline bool attn_sees(const AttnArgs &a, int32_t pos, int32_t j) {
+  return j <= pos && (a.window <= 0 || pos - j < a.window || j < a.sinks);
+}
+
+// Base (in elements) of the 16 keys from j16 on (a multiple of 16; pages hold
+// a multiple of 16) and how many of the 16 rows may be read.  The keys from L
+// on read row L - 1: they are masked, and their memory may not exist.
+struct AttnRows {
+  int64_t k, v;
+  int32_t last;
+};
+__device__ inline AttnRows attn_rows(const AttnArgs &a, const AttnSeq &s, int32_t h, int32_t j16) {
+  AttnRows r;
+  const int32_t tail = (s.L - 1) & ~15;
+  const int32_t j = j16 < tail ? j16 : tail;
+  r.last = s.L - 1 - j < 15 ? s.L - 1 - j : 15;
+  if (a.table) {
+    int32_t page = a.table[s.slot * a.table_stride + (j >> a.page_shift)];
+    page = page < 0 ? 0 : page >= a.pages ? a.pages - 1 : page;
+    const int32_t in = j & ((1 << a.page_shift) - 1);
+    r.k = page * a.k_page + in * a.k_row + h * a.k_head;
+    r.v = page * a.v_page + in * a.v_row + h * a.v_head;
+  } else {
+    r.k = (s.key0 + j) * a.k_row + h * a.k_head;
+    r.v = (s.key0 + j) * a.v_row + h * a.v_head;
+  }
+  return r;
+}
+
+__device__ inline float attn_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ inline float xor16_32_max(float x) {
+  x = fmaxf(x, __shfl_xor(x, 16));
+  return fmaxf(x, __shfl_xor(x, 32));
+}
+__device__ inline float xor16_32_sum(float x) {
+  x += __shfl_xor(x, 16);
+  return x + __shfl_xor(x, 32);
+}
+
+// what the entry points check of a cache and of a call's tokens (kvcache.hip)
+void check_kv(const vsk_kv *kv);
+void check_news(const vsk_new_tokens *news);
+// the end of a call that is queued: nothing, or, with profiling on, a wait for
+// the stream and the timers' results
+void finish_queued(vsk_ctx *ctx, hipStream_t stream);
+
+// launches (attn_rows.hip); t: a VSK_DTYPE; aligned: every pointer and
+// stride takes 16-byte loads (8-byte stores)
+void launch_attn_rows(vsk_ctx *ctx, hipStream_t stream, const AttnArgs &a, int32_t t,
+                      bool aligned, bool split_keys);
+void launch_attn_join(vsk_ctx *ctx, hipStream_t stream, const AttnArgs &a, int32_t t,
+                      bool aligned);
+
+}  // namespace vsk

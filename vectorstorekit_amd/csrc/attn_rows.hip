@@ -1,0 +1,590 @@
+// attn_rows.hip -- attention over 16 query rows a wave, keys and values from
+// memory straight into registers: one new token over a long cache, few new
+// tokens, and 32-bit prompts.
+//
+// S^T = K Q^T and O^T = V^T P^T on the matrix cores, 16 rows (columns of the
+// transposed products) at a time.  In the products' layout a lane owns one
+// query row (lane % 16) and, of every 16 keys, the four 4 * (lane / 16) on:
+// its scores, its running maximum and sum and its outputs belong to that row,
+// so the softmax needs two exchanges a tile (the maximum) and the rescaling
+// none.  The keys of a product may come in any order as long as both operands
+// agree on it: P stays in the registers that S^T was computed in, and a lane
+// loads V's rows for just those keys, 16 bytes of each, and turns the 8 x 8
+// block of 16-bit values around with byte permutes.  No shared memory is
+// touched before the waves' results are joined.
+//
+// One new token reads K and V once and does 4 * 16 * d operations a key for
+// up to 16 heads: far under what the matrix cores do in the time the bytes
+// take, so a group's heads ride along at no cost, and P goes in as a sum of
+// two 16-bit values (its rounding would be as large as the output's).
+#include "attn.hpp"
+#include "vsk_api.hpp"
+
+namespace vsk {
+
+namespace {
+
+// What a type's 32-bit words hold: E elements; 16 bytes hold 4 * E.
+template <class T> struct Elem;
+template <> struct Elem<float> {
+  static constexpr int E = 1;
+  static constexpr uint32_t EXP = 0x7F800000u;  // an infinity's or NaN's exponent
+};
+template <> struct Elem<__bf16> {
+  typedef bf16x8 V8;
+  static constexpr int E = 2;
+  static constexpr uint32_t EXP = 0x7F80u;
+  static __device__ f32x4 mfma(u32x4 a, V8 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(V8, a), b, c, 0, 0, 0);
+  }
+};
+template <> struct Elem<_Float16> {
+  typedef f16x8 V8;
+  static constexpr int E = 2;
+  static constexpr uint32_t EXP = 0x7C00u;
+  static __device__ f32x4 mfma(u32x4 a, V8 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(V8, a), b, c, 0, 0, 0);
+  }
+};
+template <class T> __device__ inline bool not_finite(uint32_t w) {
+  constexpr uint32_t X = Elem<T>::EXP;
+  if constexpr (sizeof(T) == 4) return (w & X) == X;
+  return (w & X) == X || ((w >> 16) & X) == X;
+}
+
+// W words (16 or 8 bytes) of a row from element e on, zero from element d on
+template <class T, int W, bool ALIGNED>
+__device__ inline void load_row(const T *row, int32_t e, int32_t d, uint32_t (&x)[W]) {
+  if constexpr (ALIGNED) {
+    typedef __attribute__((ext_vector_type(W))) uint32_t VW;
+    VW v = {};
+    if (e < d) v = *reinterpret_cast<const VW *>(row + e);
+#pragma unroll
+    for (int i = 0; i < W; ++i) x[i] = v[i];
+  } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < W; ++i) x[i] = e + i < d ? __builtin_bit_cast(uint32_t, row[e + i]) : 0u;
+  } else {
+    const uint16_t *h = reinterpret_cast<const uint16_t *>(row);
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      x[i] = e + 2 * i < d ? h[e + 2 * i] : 0u;
+      if (e + 2 * i + 1 < d) x[i] |= (uint32_t)h[e + 2 * i + 1] << 16;
+    }
+  }
+}
+
+constexpr int ROWS = 16;  // query rows of a wave
+// 16-key tiles of a step: the k of a 16-bit product is 32 keys
+template <class T> constexpr int SUBS = sizeof(T) == 4 ? 1 : 2;
+
+// The wave's 16 rows over key tiles.  VW: elements of V that a lane takes of a
+// row, 16 lanes a block; NB blocks.
+template <class T, int VW, int NB, bool ALIGNED> struct RowTile {
+  static constexpr int DV = 16 * VW * NB;
+  static constexpr bool F32 = sizeof(T) == 4;
+  static constexpr int E = Elem<T>::E;
+  static constexpr int KE = 4 * E;          // elements of 16 bytes
+  static constexpr int KS = DV / (4 * KE);  // 16-byte loads a lane makes of a key row
+  static constexpr int U = SUBS<T>;
+  static constexpr int KT = 16 * U;
+  static constexpr int WV = VW / E;         // words a lane takes of a row's block
+  const AttnArgs &a;
+  const AttnSeq &s;
+  const int32_t h, n, g;
+  int32_t pos;  // position of this lane's row, -1 if there is none
+  uint32_t q[KS][4];
+  f32x4 acc[NB][VW];
+  float m = -INFINITY, l = 0.f;
+
+  __device__ RowTile(const AttnArgs &a_, const AttnSeq &s_, int32_t h_, int lane)
+      : a(a_), s(s_), h(h_), n(lane & 15), g(lane >> 4) {}
+
+  __device__ void begin(int32_t row) {
+    const int32_t t = row / a.group;
+    const bool real = t < s.T && t < a.max_new;
+    pos = real ? s.L - s.T + t : -1;
+    const T *src = static_cast<const T *>(a.q) +
+                   (real ? (s.token0 + t) * a.q_row + (h * a.group + row % a.group) * a.q_head : 0);
+#pragma unroll
+    for (int i = 0; i < KS; ++i)
+      load_row<T, 4, ALIGNED>(src, (4 * i + g) * KE, real ? a.d : 0, q[i]);
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int t2 = 0; t2 < VW; ++t2) acc[b][t2] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+
+  // acc += V^T P^T; p[u][i] belongs to key 16 u + 4 g + i and v[u][i] is that
+  // key's row
+  __device__ void weigh(const float (&p)[U][4], const uint32_t (&v)[U][4][NB][WV]) {
+    if constexpr (F32) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+          for (int t = 0; t < VW; ++t)
+            acc[b][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                __builtin_bit_cast(float, v[0][i][b][t]), p[0][i], acc[b][t], 0, 0, 0);
+    } else {
+      typename Elem<T>::V8 hi, lo;
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          hi[4 * u + i] = (T)p[u][i];
+          lo[4 * u + i] = (T)(p[u][i] - (float)hi[4 * u + i]);
+        }
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int t = 0; t < VW; ++t) {
+          // element t of eight rows: the low or high halves of their words
+          constexpr uint32_t LOW = 0x05040100u, HIGH = 0x07060302u;
+          u32x4 x;
+#pragma unroll
+          for (int y = 0; y < 4; ++y)
+            x[y] = __builtin_amdgcn_perm(v[y >> 1][2 * (y & 1) + 1][b][t / 2],
+                                         v[y >> 1][2 * (y & 1)][b][t / 2], t & 1 ? HIGH : LOW);
+          acc[b][t] = Elem<T>::mfma(x, hi, acc[b][t]);
+          acc[b][t] = Elem<T>::mfma(x, lo, acc[b][t]);
+        }
+    }
+  }
+
+  // q_lo, q_hi: the smallest and largest position of the tile's rows
+  __device__ void step(int32_t kb, int32_t q_lo, int32_t q_hi) {
+    uint32_t k[U][KS][4], v[U][4][NB][WV];
+    AttnRows r[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      r[u] = attn_rows(a, s, h, kb + 16 * u);
+      const T *row = static_cast<const T *>(a.k) + r[u].k +
+                     (n < r[u].last ? n : r[u].last) * (int32_t)a.k_row;
+#pragma unroll
+      for (int i = 0; i < KS; ++i) load_row<T, 4, ALIGNED>(row, (4 * i + g) * KE, a.d, k[u][i]);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const T *row = v_row(r[u], 4 * g + i);
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+          load_row<T, WV, ALIGNED>(row, (16 * b + n) * VW, a.d, v[u][i][b]);
+      }
+    f32x4 sc[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      sc[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < KS; ++i) {
+        if constexpr (F32) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            sc[u] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, k[u][i][e]),
+                                                         __builtin_bit_cast(float, q[i][e]), sc[u],
+                                                         0, 0, 0);
+        } else {
+          const u32x4 x = {k[u][i][0], k[u][i][1], k[u][i][2], k[u][i][3]};
+          const u32x4 y = {q[i][0], q[i][1], q[i][2], q[i][3]};
+          sc[u] = Elem<T>::mfma(x, __builtin_bit_cast(typename Elem<T>::V8, y), sc[u]);
+        }
+      }
+    }
+    // every row sees every key of most tiles
+    const bool whole = kb + KT - 1 <= q_lo &&
+                       (a.window <= 0 || q_hi - kb < a.window || kb + KT <= a.sinks);
+    if (!whole) {
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (!attn_sees(a, pos, kb + 16 * u + 4 * g + i)) sc[u][i] = -INFINITY;
+    }
+    float top = fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3]));
+    if constexpr (U == 2)
+      top = fmaxf(top, fmaxf(fmaxf(sc[1][0], sc[1][1]), fmaxf(sc[1][2], sc[1][3])));
+    top = fmaxf(m, xor16_32_max(top) * a.scale_log2);
+    const float use = top == -INFINITY ? 0.f : top;
+    const float fade = attn_exp2(m - use);
+    m = top;
+    l *= fade;
+    float p[U][4];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        p[u][i] = attn_exp2(fmaf(sc[u][i], a.scale_log2, -use));
+        l += p[u][i];
+      }
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int t = 0; t < VW; ++t) acc[b][t] *= fade;
+    if (!whole && edge(r, kb, q_lo, q_hi, p, v)) return;
+    weigh(p, v);
+  }
+  __device__ const T *v_row(const AttnRows &r, int32_t at) const {
+    return static_cast<const T *>(a.v) + r.v + (at < r.last ? at : r.last) * (int32_t)a.v_row;
+  }
+
+  // A tile that not every row sees whole: what a masked place holds (memory
+  // never written, for one) must not reach a sum, and 0 * NaN is NaN.  Rows of
+  // V that no query row sees are cleared; if one that some rows see and some
+  // do not is not finite, its keys go one at a time and each row takes only
+  // those it sees (returns true).
+  __device__ bool edge(const AttnRows (&r)[U], int32_t kb, int32_t q_lo, int32_t q_hi,
+                       const float (&p)[U][4], uint32_t (&v)[U][4][NB][WV]) {
+    bool odd = false;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int32_t j = kb + 16 * u + 4 * g + i;
+        // (seen by some row: the last row's side of the diagonal and the
+        // first row's side of the window)
+        const bool seen = j <= q_hi && (a.window <= 0 || q_lo - j < a.window || j < a.sinks);
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+          for (int t = 0; t < WV; ++t) {
+            v[u][i][b][t] = seen ? v[u][i][b][t] : 0u;
+            odd |= not_finite<T>(v[u][i][b][t]);
+          }
+      }
+    if (q_lo == q_hi || !__any(odd)) return false;
+    one_by_one(r, kb, p);
+    return true;
+  }
+  __device__ void one_by_one(const AttnRows (&r)[U], int32_t kb, const float (&p)[U][4]) {
+#pragma unroll 1
+    for (int32_t j = 0; j < KT; ++j) {
+      const int32_t at = j & 15;
+      float w = 0.f;
+      AttnRows rr = r[0];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (u == j >> 4) rr = r[u];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w = 16 * u + i == (j & ~12) ? p[u][i] : w;
+      }
+      w = __shfl(w, n + 16 * (at >> 2));
+      if (!attn_sees(a, pos, kb + j)) continue;
+      const T *row = v_row(rr, at);
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int y = 0; y < 4; ++y)
+#pragma unroll
+          for (int t = 0; t < VW; ++t) {
+            const int32_t e = (16 * b + 4 * g + y) * VW + t;
+            if (e < a.d) acc[b][t][y] = fmaf(w, (float)row[e], acc[b][t][y]);
+          }
+    }
+  }
+};
+
+// waves a SIMD, by the registers that the loads of a step take
+template <class T> constexpr int row_waves(int elems) {
+  return elems * (int)sizeof(T) < 16 ? 4 : elems * (int)sizeof(T) <= 16 ? 3 : elems * (int)sizeof(T) <= 32 ? 2 : 1;
+}
+
+template <class T> __device__ inline void store4(T *dst, const float (&x)[4], int32_t left) {
+  if (left >= 4) {
+    typedef __attribute__((ext_vector_type(4))) T V4;
+    V4 y;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) y[i] = (T)x[i];
+    *reinterpret_cast<V4 *>(dst) = y;
+  }
+}
+
+// One block: a row tile of one sequence and key head, over one part of its
+// keys that the four waves share (KSPLIT), or four row tiles, a wave each.
+template <class T, int VW, int NB, bool KSPLIT, bool ALIGNED>
+__global__ __launch_bounds__(256, row_waves<T>(VW * NB)) void
+k_attn_rows(const AttnArgs a) {
+  typedef RowTile<T, VW, NB, ALIGNED> Tile;
+  constexpr int DV = Tile::DV;
+  const int lane = threadIdx.x & 63;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  // key heads fastest: neighbouring blocks read neighbouring parts of a page
+  uint32_t at = blockIdx.x;
+  const int32_t h = at % a.kv_heads;
+  at /= a.kv_heads;
+  const int32_t groups = KSPLIT ? a.tiles : (a.tiles + 3) / 4;
+  // (the last tiles see the most keys: they go first)
+  const int32_t tg = groups - 1 - (int32_t)(at % groups);
+  at /= groups;
+  const int32_t part = at % a.splits;
+  const AttnSeq s = attn_seq(a, at / a.splits);
+  const int32_t tile = KSPLIT ? tg : 4 * tg + w;
+  const int32_t row0 = tile * ROWS;
+  const int32_t T_used = s.T < a.max_new ? s.T : a.max_new;
+  const int32_t rows_all = T_used * a.group;
+  const bool have = row0 < rows_all;
+  if (KSPLIT ? !have : 4 * tg * ROWS >= rows_all) return;
+  const int32_t rows = !have ? 0 : rows_all - row0 < ROWS ? rows_all - row0 : ROWS;
+  const int32_t t_lo = row0 / a.group, t_hi = (row0 + rows - 1) / a.group;
+  const int32_t q_lo = s.L - s.T + t_lo, q_hi = s.L - s.T + t_hi;
+  const auto span = attn_span<Tile::KT>(a, q_lo, have ? q_hi : -1);
+  const int32_t parts = attn_parts(a, span.tiles);
+  if (part >= parts) return;
+  const int32_t first = part * a.chunk;
+  const int32_t end = part == parts - 1 ? span.tiles : first + a.chunk;
+
+  Tile tl(a, s, h, lane);
+  tl.begin(have ? row0 + tl.n : 0x3fffffff);
+  if (have)
+    for (int32_t t = KSPLIT ? first + w : first; t < end; t += KSPLIT ? 4 : 1)
+      tl.step(span.base(t), q_lo, q_hi);
+  tl.l = xor16_32_sum(tl.l);
+
+  const bool partial = parts > 1;
+  const int64_t row_of = (int64_t)part * a.tokens * a.heads;
+  if constexpr (!KSPLIT) {
+    if (tl.n < rows) {
+      const int32_t r = row0 + tl.n;
+      const int64_t token = s.token0 + r / a.group;
+      const int32_t head = h * a.group + r % a.group;
+      const float inv = tl.l > 0.f || tl.l != tl.l ? 1.f / tl.l : 0.f;
+      T *dst = static_cast<T *>(a.out) + token * a.o_row + head * a.o_head;
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int32_t e = 16 * VW * b + VW * (4 * tl.g + i);
+#pragma unroll
+          for (int t0 = 0; t0 < VW; t0 += 4) {
+            float x[4];
+#pragma unroll
+            for (int t = 0; t < 4; ++t) x[t] = tl.acc[b][t0 + t][i] * inv;
+            if constexpr (ALIGNED)
+              store4<T>(dst + e + t0, x, a.d - e - t0);
+            else
+#pragma unroll
+              for (int t = 0; t < 4; ++t)
+                if (e + t0 + t < a.d) dst[e + t0 + t] = (T)x[t];
+          }
+        }
+      if (a.lse && tl.g == 0)
+        a.lse[token * a.heads + head] =
+            tl.l > 0.f ? (tl.m + __log2f(tl.l)) * 0.6931471805599453f
+                       : tl.l != tl.l ? tl.l : -INFINITY;
+    }
+  } else {
+    __shared__ __attribute__((aligned(16))) float so[4][ROWS][DV + 4];
+    __shared__ float sm[4][ROWS], sl[4][ROWS];
+    if (tl.g == 0) sm[w][tl.n] = tl.m, sl[w][tl.n] = tl.l;
+    __syncthreads();
+    float top = -INFINITY, sum = 0.f;
+#pragma unroll
+    for (int x = 0; x < 4; ++x) top = fmaxf(top, sm[x][tl.n]);
+    const float use = top == -INFINITY ? 0.f : top;
+#pragma unroll
+    for (int x = 0; x < 4; ++x) sum += sl[x][tl.n] * attn_exp2(sm[x][tl.n] - use);
+    // rows of a part: the sums as they are; of the whole: the quotient
+    float f = attn_exp2(tl.m - use);
+    if (!partial) f *= sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+    if (tl.n < rows) {
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int t = 0; t < VW; t += 4) {
+            f32x4 x;
+#pragma unroll
+            for (int y = 0; y < 4; ++y) x[y] = tl.acc[b][t + y][i] * f;
+            *reinterpret_cast<f32x4 *>(
+                &so[w][tl.n][16 * VW * b + VW * (4 * tl.g + i) + t]) = x;
+          }
+      if (w == 0 && tl.g == 0) {
+        const int32_t r = row0 + tl.n;
+        const int64_t row = (s.token0 + r / a.group) * a.heads + h * a.group + r % a.group;
+        if (partial) {
+          a.part_ml[2 * (row_of + row)] = top;
+          a.part_ml[2 * (row_of + row) + 1] = sum;
+        } else if (a.lse) {
+          a.lse[row] = sum > 0.f ? (top + __log2f(sum)) * 0.6931471805599453f
+                                 : sum != sum ? sum : -INFINITY;
+        }
+      }
+    }
+    __syncthreads();
+    for (int32_t x = threadIdx.x; x < rows * (DV / 4); x += 256) {
+      const int32_t rr = x / (DV / 4), e = 4 * (x % (DV / 4));
+      if (e >= a.d) continue;
+      f32x4 y = *reinterpret_cast<f32x4 *>(&so[0][rr][e]);
+#pragma unroll
+      for (int z = 1; z < 4; ++z) y += *reinterpret_cast<f32x4 *>(&so[z][rr][e]);
+      const int32_t r = row0 + rr;
+      const int64_t token = s.token0 + r / a.group;
+      const int32_t head = h * a.group + r % a.group;
+      if (partial) {
+        float *dst = a.part_o + (row_of + token * a.heads + head) * DV + e;
+        *reinterpret_cast<f32x4 *>(dst) = y;
+      } else {
+        T *dst = static_cast<T *>(a.out) + token * a.o_row + head * a.o_head + e;
+        const float z[4] = {y[0], y[1], y[2], y[3]};
+        if constexpr (ALIGNED)
+          store4<T>(dst, z, a.d - e);
+        else
+#pragma unroll
+          for (int t = 0; t < 4; ++t)
+            if (e + t < a.d) dst[t] = (T)z[t];
+      }
+    }
+  }
+}
+
+// Joins the parts of one output row: sum of the parts' values and sums, each
+// times 2^(its maximum - the largest).  A block a row; the threads take four
+// values each of several parts at a time.
+template <class T, int DV, int RT, int KTILE, bool ALIGNED>
+__global__ __launch_bounds__(256) void k_attn_join(const AttnArgs a) {
+  constexpr int LANES = DV / 4, WAYS = 256 / LANES;
+  __shared__ __attribute__((aligned(16))) float so[WAYS][DV];
+  __shared__ float ss[WAYS];
+  const uint32_t per = (uint32_t)a.max_new * a.heads;
+  const AttnSeq s = attn_seq(a, blockIdx.x / per);
+  const int32_t x = blockIdx.x % per, t = x / a.heads, head = x % a.heads;
+  if (t >= s.T) return;
+  // the parts of the row tile that computed this row
+  const int32_t h = head / a.group, row = t * a.group + head - h * a.group;
+  const int32_t row0 = row / RT * RT;
+  const int32_t all = (s.T < a.max_new ? s.T : a.max_new) * a.group;
+  const int32_t last = row0 + RT < all ? row0 + RT - 1 : all - 1;
+  const int32_t p0 = s.L - s.T;
+  const AttnSpan<KTILE> span = attn_span<KTILE>(a, p0 + row0 / a.group, p0 + last / a.group);
+  const int32_t parts = attn_parts(a, span.tiles);
+  if (parts == 1) return;  // written by the row tile itself
+  const int64_t stride = a.tokens * a.heads;
+  const int64_t at = (s.token0 + t) * a.heads + head;
+  float top = -INFINITY;
+  for (int32_t i = threadIdx.x & 63; i < parts; i += 64)
+    top = fmaxf(top, a.part_ml[2 * (i * stride + at)]);
+  for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+  const float use = top == -INFINITY ? 0.f : top;
+  const int e = 4 * (threadIdx.x % LANES), way = threadIdx.x / LANES;
+  f32x4 o = {0.f, 0.f, 0.f, 0.f};
+  float sum = 0.f;
+#pragma unroll 4
+  for (int32_t i = way; i < parts; i += WAYS) {
+    const int64_t r = i * stride + at;
+    const float f = attn_exp2(a.part_ml[2 * r] - use);
+    sum += f * a.part_ml[2 * r + 1];
+    if (e < a.d) o += f * *reinterpret_cast<const f32x4 *>(a.part_o + r * DV + e);
+  }
+  *reinterpret_cast<f32x4 *>(&so[way][e]) = o;
+  if (threadIdx.x % LANES == 0) ss[way] = sum;
+  __syncthreads();
+  if (way) return;
+#pragma unroll
+  for (int i = 1; i < WAYS; ++i) {
+    o += *reinterpret_cast<f32x4 *>(&so[i][e]);
+    sum += ss[i];
+  }
+  const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+  if (threadIdx.x == 0 && a.lse)
+    a.lse[at] = sum > 0.f ? (top + __log2f(sum)) * 0.6931471805599453f
+                          : sum != sum ? sum : -INFINITY;
+  if (e >= a.d) return;
+  T *dst = static_cast<T *>(a.out) + (s.token0 + t) * a.o_row + head * a.o_head + e;
+  const float z[4] = {o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
+  if constexpr (ALIGNED)
+    store4<T>(dst, z, a.d - e);
+  else
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (e + i < a.d) dst[i] = (T)z[i];
+}
+
+template <class T, int VW, int NB>
+void rows_of(hipStream_t st, const AttnArgs &a, bool aligned, bool split, unsigned grid) {
+  if (split) {
+    if (aligned)
+      k_attn_rows<T, VW, NB, true, true><<<grid, 256, 0, st>>>(a);
+    else
+      k_attn_rows<T, VW, NB, true, false><<<grid, 256, 0, st>>>(a);
+  } else {
+    if (aligned)
+      k_attn_rows<T, VW, NB, false, true><<<grid, 256, 0, st>>>(a);
+    else
+      k_attn_rows<T, VW, NB, false, false><<<grid, 256, 0, st>>>(a);
+  }
+}
+
+}  // namespace
+
+void launch_attn_rows(vsk_ctx *ctx, hipStream_t st, const AttnArgs &a, int32_t t, bool aligned,
+                      bool split) {
+  const int64_t groups = split ? a.tiles : (a.tiles + 3) / 4;
+  const int64_t grid = (int64_t)a.n * a.splits * groups * a.kv_heads;
+  VSK_REQUIRE(grid <= 0x7FFFFFFFll, VSK_ERR_INVALID_BUFFER_SIZE, "too many query rows in one call");
+  const unsigned g = (unsigned)grid;
+  KernelTimer kt(ctx, "attn_rows", (double)a.tokens * a.heads, st);
+  if (t == VSK_DTYPE_F32) {
+    if (a.d <= 64)
+      rows_of<float, 4, 1>(st, a, aligned, split, g);
+    else if (a.d <= 128)
+      rows_of<float, 4, 2>(st, a, aligned, split, g);
+    else
+      rows_of<float, 4, 4>(st, a, aligned, split, g);
+  } else if (t == VSK_DTYPE_F16) {
+    if (a.d <= 64)
+      rows_of<_Float16, 4, 1>(st, a, aligned, split, g);
+    else if (a.d <= 128)
+      rows_of<_Float16, 8, 1>(st, a, aligned, split, g);
+    else
+      rows_of<_Float16, 8, 2>(st, a, aligned, split, g);
+  } else {
+    if (a.d <= 64)
+      rows_of<__bf16, 4, 1>(st, a, aligned, split, g);
+    else if (a.d <= 128)
+      rows_of<__bf16, 8, 1>(st, a, aligned, split, g);
+    else
+      rows_of<__bf16, 8, 2>(st, a, aligned, split, g);
+  }
+  check_launch("attn_rows");
+}
+
+namespace {
+template <class T, int RT, int KTILE>
+void join_of(hipStream_t st, const AttnArgs &a, bool aligned, unsigned g) {
+  if (a.d <= 64) {
+    if (aligned)
+      k_attn_join<T, 64, RT, KTILE, true><<<g, 256, 0, st>>>(a);
+    else
+      k_attn_join<T, 64, RT, KTILE, false><<<g, 256, 0, st>>>(a);
+  } else if (a.d <= 128) {
+    if (aligned)
+      k_attn_join<T, 128, RT, KTILE, true><<<g, 256, 0, st>>>(a);
+    else
+      k_attn_join<T, 128, RT, KTILE, false><<<g, 256, 0, st>>>(a);
+  } else {
+    if (aligned)
+      k_attn_join<T, 256, RT, KTILE, true><<<g, 256, 0, st>>>(a);
+    else
+      k_attn_join<T, 256, RT, KTILE, false><<<g, 256, 0, st>>>(a);
+  }
+}
+}  // namespace
+
+void launch_attn_join(vsk_ctx *ctx, hipStream_t st, const AttnArgs &a, int32_t t, bool aligned) {
+  if (a.splits == 1) return;
+  const int64_t grid = (int64_t)a.n * a.max_new * a.heads;
+  VSK_REQUIRE(grid <= 0x7FFFFFFFll, VSK_ERR_INVALID_BUFFER_SIZE, "too many query rows in one call");
+  KernelTimer kt(ctx, "attn_join", (double)grid, st);
+  if (t == VSK_DTYPE_F32)
+    join_of<float, ROWS, 16 * SUBS<float>>(st, a, aligned, (unsigned)grid);
+  else if (t == VSK_DTYPE_F16)
+    join_of<_Float16, ROWS, 16 * SUBS<_Float16>>(st, a, aligned, (unsigned)grid);
+  else
+    join_of<__bf16, ROWS, 16 * SUBS<__bf16>>(st, a, aligned, (unsigned)grid);
+  check_launch("attn_join");
+}
+
+}  // namespace vsk

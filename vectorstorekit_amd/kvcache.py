@@ -1,0 +1,495 @@
+"""Key-value cache, rotary positions and attention: what a language model that
+answers over retrieved vectors calls next to the search.
+
+* ``RotaryEmbedding`` -- rotary positions (half or interleaved pairs, part of
+  the head, scaled for longer contexts);
+* ``PagedKVCache`` -- pages of keys and values resident in HBM, their tables
+  and reference counts; ``append``, ``attend``, ``reserve``, ``fork``,
+  ``free``, ``compact``, ``copy_pages``;
+* ``window_attention`` -- causal attention over keys and values as the
+  projections left them, through a sliding window with sinks.
+
+Tensors are torch tensors on the context's GPU.  Unlike the search calls,
+these are queued on torch's current stream and do not wait: a decoder makes
+dozens a token.  They allocate through torch, so a captured graph may hold
+them.  The reference keeps its language-model layer on the application's side
+(LLM/, Core/ML/Shaders/OptimizedMLShaders.metal:523); there is no CPU
+fallback.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+
+import numpy as np
+import torch
+
+from . import _lib
+from ._lib import VSKError
+from .engine import Context
+
+_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+
+
+def _stream(device) -> int:
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+def _tensor(x, name, dtype=None, dims=None):
+    if not isinstance(x, torch.Tensor) or not x.is_cuda:
+        raise VSKError(-2, f"{name} must be a tensor on the GPU")
+    if dtype is not None and x.dtype != dtype:
+        raise VSKError(-2, f"{name} is {x.dtype}, not {dtype}")
+    if dims is not None and x.dim() != dims:
+        raise VSKError(-4, f"{name} must have {dims} dimensions, not {x.dim()}")
+    return x
+
+
+def _dense_heads(x, name):
+    """x itself, or a copy whose innermost dimension is dense."""
+    return x if x.stride(-1) == 1 or x.shape[-1] == 1 else x.contiguous()
+
+
+def _ints(x, name, device):
+    """A dense int32 vector on the device; a host sequence is copied there."""
+    if isinstance(x, torch.Tensor):
+        _tensor(x, name, torch.int32, 1)
+        return x if x.is_contiguous() else x.contiguous()
+    a = np.asarray(x)
+    if a.ndim != 1 or (a.size and a.dtype.kind not in "iu"):
+        raise VSKError(-2, f"{name} must be a vector of whole numbers")
+    return torch.from_numpy(a.astype(np.int32)).to(device)
+
+
+def _rows(src, dst):
+    r = _lib.vsk_head_rows()
+    r.src, r.src_row, r.src_head = src.data_ptr(), src.stride(0), src.stride(1)
+    if dst is not None:
+        r.dst, r.dst_row, r.dst_head = dst.data_ptr(), dst.stride(0), dst.stride(1)
+    r.heads = src.shape[1]
+    return r
+
+
+class RotaryEmbedding:
+    """Rotary positions (``vsk_rotary_*``).
+
+    ``layout``: "half" turns the pairs (i, i + rotary_dim / 2), "interleaved"
+    the pairs (2 i, 2 i + 1), of the first ``rotary_dim`` values of a head
+    (default: all); the others pass through.  Pair i turns by position *
+    base^(-2 i / rotary_dim) radians, changed by ``scaling`` for contexts
+    longer than those trained on:
+
+    * ``{"type": "linear", "factor": f}``: positions divided by f;
+    * ``{"type": "ntk", "factor": f}``: base * f^(r / (r - 2)), which leaves
+      the fastest pair as it is and divides the slowest one's by f;
+    * ``{"type": "yarn", "factor": f, "original_length": n}``: pairs that turn
+      more than ``beta_fast`` (32) times over n positions stay, those under
+      ``beta_slow`` (1) are divided by f, those between are blended, and the
+      rotated values are multiplied by ``attention_factor``
+      (0.1 ln f + 1)."""
+
+    LAYOUTS = {"half": 0, "interleaved": 1}
+
+    def __init__(self, ctx: Context, head_dim: int, rotary_dim: int | None = None,
+                 base: float = 10000.0, layout: str = "half", scaling: dict | None = None):
+        r = head_dim if rotary_dim is None else int(rotary_dim)
+        if layout not in self.LAYOUTS:
+            raise VSKError(-2, f"unknown rotary layout {layout!r}")
+        if r < 2 or r % 2 or r > head_dim:
+            raise VSKError(-2, "rotary_dim must be even, at least 2 and at most head_dim")
+        if not base > 0:
+            raise VSKError(-2, "base must be positive")
+        self.ctx, self.head_dim, self.rotary_dim, self.layout = ctx, int(head_dim), r, layout
+        self.inv_freq, self.amplitude = self.frequencies(r, base, scaling)
+        f = np.ascontiguousarray(self.inv_freq, np.float64)
+        h = ctypes.c_void_p()
+        ctx.check(ctx.lib.vsk_rotary_create(ctx.handle, f.ctypes.data, r // 2,
+                                            self.LAYOUTS[layout], self.amplitude,
+                                            ctypes.byref(h)))
+        self.handle = h
+
+    @staticmethod
+    def frequencies(rotary_dim: int, base: float = 10000.0, scaling: dict | None = None):
+        """(radians a position for each pair, factor on the rotated values)."""
+        r = rotary_dim
+        i = np.arange(r // 2, dtype=np.float64)
+        inv = float(base) ** (-2.0 * i / r)
+        if not scaling:
+            return inv, 1.0
+        s = dict(scaling)
+        kind, f = s.pop("type", None), float(s.pop("factor", 0))
+        if not f >= 1:
+            raise VSKError(-2, "scaling needs a factor of at least 1")
+        amplitude = 1.0
+        if kind == "linear":
+            inv = inv / f
+        elif kind == "ntk":
+            if r < 4:
+                raise VSKError(-2, "ntk scaling needs two pairs at least")
+            inv = (base * f ** (r / (r - 2.0))) ** (-2.0 * i / r)
+        elif kind == "yarn":
+            n = float(s.pop("original_length", 0))
+            fast, slow = float(s.pop("beta_fast", 32.0)), float(s.pop("beta_slow", 1.0))
+            if not n > 0 or not fast > slow > 0 or not base > 1:
+                raise VSKError(-2, "yarn scaling needs original_length, beta_fast > beta_slow > 0 "
+                               "and a base over 1")
+
+            def pair(turns):  # the pair that turns so often over n positions
+                return r * math.log(n / (2 * math.pi * turns)) / (2 * math.log(base))
+
+            low = max(math.floor(pair(fast)), 0)
+            high = min(math.ceil(pair(slow)), r - 1)
+            ramp = np.clip((i - low) / max(high - low, 1e-3), 0.0, 1.0)
+            inv = inv * (1 - ramp) + inv / f * ramp
+            amplitude = float(s.pop("attention_factor", 0.1 * math.log(f) + 1.0))
+        else:
+            raise VSKError(-2, f"unknown scaling {kind!r}")
+        if s:
+            raise VSKError(-2, f"unknown scaling options {sorted(s)}")
+        return inv, amplitude
+
+    def free(self):
+        if getattr(self, "handle", None):
+            self.ctx.lib.vsk_rotary_free(self.ctx.handle, self.handle)
+            self.handle = None
+
+    def __del__(self):
+        try:
+            self.free()
+        except Exception:
+            pass
+
+    def apply(self, q, k=None, *, positions, inverse: bool = False, inplace: bool = False):
+        """q (and k), tokens x heads x head_dim, turned by positions (int32,
+        one a token): new tensors, or the given ones with ``inplace``.
+        ``inverse`` turns back (with the same factor): the gradient of
+        ``apply``, and, with positions p - p', a cached key's move from p to
+        p'."""
+        tensors = [x for x in (q, k) if x is not None]
+        for x, name in zip(tensors, ("q", "k")):
+            _tensor(x, name, q.dtype, 3)
+            if x.shape[2] != self.head_dim or x.shape[0] != q.shape[0]:
+                raise VSKError(-4, f"{name} is {tuple(x.shape)}: head_dim is {self.head_dim}, "
+                               f"tokens are {q.shape[0]}")
+        if q.dtype not in _TYPES:
+            raise VSKError(-8, f"{q.dtype} is not supported")
+        _tensor(positions, "positions", torch.int32, 1)
+        if positions.shape[0] != q.shape[0]:
+            raise VSKError(-4, f"{positions.shape[0]} positions for {q.shape[0]} tokens")
+        positions = positions.contiguous()
+        if inplace:
+            if any(x.stride(-1) != 1 for x in tensors):
+                raise VSKError(-2, "inplace needs dense heads")
+            outs = tensors
+        else:
+            tensors = [_dense_heads(x, "q") for x in tensors]
+            outs = [torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in tensors]
+        if q.shape[0] and all(x.shape[1] for x in tensors):
+            rows = (_lib.vsk_head_rows * len(tensors))(*map(_rows, tensors, outs))
+            self.ctx.check(self.ctx.lib.vsk_rotary_apply(
+                self.ctx.handle, _stream(q.device), self.handle, _TYPES[q.dtype], self.head_dim,
+                q.shape[0], positions.data_ptr(), 1 if inverse else 0, rows, len(tensors)))
+        return outs[0] if k is None else tuple(outs)
+
+
+def _attend(ctx, kv, layer, q, news, k_starts, scale, window, sinks, max_length, out, lse):
+    """The checked call of vsk_attention."""
+    head_dim = q.shape[2]
+    a = _lib.vsk_attention_args()
+    a.scale = head_dim ** -0.5 if scale is None else float(scale)
+    if window is not None and window < 1:
+        raise VSKError(-2, "window must be at least 1 (None: no window)")
+    if sinks < 0:
+        raise VSKError(-2, "sinks must not be negative")
+    a.window, a.sinks = int(window or 0), int(sinks)
+    a.max_length = int(max_length or 0)
+    a.q = _rows(q, out)
+    a.lse = lse.data_ptr() if lse is not None else None
+    a.k_starts = k_starts
+    need = ctx.lib.vsk_attention_workspace(ctx.handle, kv, ctypes.byref(news), ctypes.byref(a))
+    if need:
+        work = torch.empty(need, dtype=torch.uint8, device=q.device)
+        a.workspace, a.workspace_bytes = work.data_ptr(), need
+    ctx.check(ctx.lib.vsk_attention(ctx.handle, _stream(q.device), kv, layer, ctypes.byref(news),
+                                    ctypes.byref(a)))
+
+
+def _outputs(q, return_lse):
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    lse = None
+    if return_lse:
+        lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
+    return out, lse
+
+
+class PagedKVCache:
+    """Keys and values of many sequences in pages of ``page_size`` tokens (a
+    power of two, at least 16).
+
+    ``k``, ``v``: layers x pages x page_size x kv_heads x head_dim;
+    ``table`` (int32, slots x width): the pages of the sequence in each slot,
+    -1 where there is none; ``lengths`` (int32, slots); ``refs`` (int32,
+    pages): how many sequences hold a page.  A page that is full may be
+    shared; one that is not belongs to one sequence.
+
+    A step of a decoder: ``reserve`` makes room for the new tokens, then each
+    layer calls ``append`` with their keys and values and ``attend`` with
+    their queries.  New tokens are always a sequence's last ones."""
+
+    def __init__(self, ctx: Context, *, pages: int, page_size: int, kv_heads: int, head_dim: int,
+                 slots: int, width: int, layers: int = 1, dtype=torch.bfloat16):
+        for name, x in (("pages", pages), ("kv_heads", kv_heads), ("head_dim", head_dim),
+                        ("slots", slots), ("width", width), ("layers", layers)):
+            if x < 1:
+                raise VSKError(-2, f"{name} must be positive")
+        dev = torch.device("cuda", ctx.device)
+        shape = (layers, pages, page_size, kv_heads, head_dim)
+        if dtype not in _TYPES:
+            raise VSKError(-8, f"{dtype} is not supported")
+        k, v = (torch.empty(shape, dtype=dtype, device=dev) for _ in range(2))
+        table = torch.full((slots, width), -1, dtype=torch.int32, device=dev)
+        self._hold(ctx, k, v, table, torch.zeros(slots, dtype=torch.int32, device=dev),
+                   torch.zeros(pages, dtype=torch.int32, device=dev))
+
+    @classmethod
+    def over(cls, ctx: Context, k, v, table, lengths, refs=None) -> "PagedKVCache":
+        """A cache over tensors that the caller holds (k and v may lack the
+        layers' dimension, and may have any strides over dense heads).
+        Without ``refs`` there is no page keeping, only ``append`` and
+        ``attend``."""
+        self = cls.__new__(cls)
+        self._hold(ctx, k, v, table, lengths, refs)
+        return self
+
+    def _hold(self, ctx, k, v, table, lengths, refs):
+        for x, name in ((k, "k"), (v, "v")):
+            _tensor(x, name)
+            if x.dim() not in (4, 5):
+                raise VSKError(-4, f"{name} must be (layers x) pages x page_size x kv_heads x "
+                               "head_dim")
+            if x.dtype not in _TYPES:
+                raise VSKError(-8, f"{x.dtype} is not supported")
+            if x.stride(-1) != 1 and x.shape[-1] != 1:
+                raise VSKError(-2, f"the heads of {name} must be dense")
+        if k.shape != v.shape or k.dtype != v.dtype:
+            raise VSKError(-4, "k and v differ in shape or type")
+        _tensor(table, "table", torch.int32, 2)
+        _tensor(lengths, "lengths", torch.int32, 1)
+        if table.shape[0] != lengths.shape[0] or table.stride(1) != 1 and table.shape[1] != 1:
+            raise VSKError(-4, "table must be slots x width, dense rows, lengths of slots")
+        if lengths.stride(0) != 1 and lengths.shape[0] != 1:
+            raise VSKError(-2, "lengths must be dense")
+        k5, v5 = (x if x.dim() == 5 else x[None] for x in (k, v))
+        layers, pages, page_size, kv_heads, head_dim = k5.shape
+        if page_size < 16 or page_size & (page_size - 1):
+            raise VSKError(-8, "page_size must be a power of two of at least 16")
+        self.ctx, self.k, self.v = ctx, k, v
+        self.table, self.lengths, self.refs = table, lengths, refs
+        self.layers, self.pages, self.page_size = layers, pages, page_size
+        self.kv_heads, self.head_dim, self.dtype = kv_heads, head_dim, k.dtype
+        self.slots, self.width = table.shape
+        self.device = k.device
+        kv = _lib.vsk_kv()
+        kv.k, kv.v = k.data_ptr(), v.data_ptr()
+        kv.k_layer, kv.k_page, kv.k_row, kv.k_head = k5.stride()[:4]
+        kv.v_layer, kv.v_page, kv.v_row, kv.v_head = v5.stride()[:4]
+        kv.table, kv.lengths = table.data_ptr(), lengths.data_ptr()
+        kv.table_stride = table.stride(0)
+        kv.dtype, kv.layers, kv.pages, kv.page_size = _TYPES[k.dtype], layers, pages, page_size
+        kv.kv_heads, kv.head_dim, kv.slots, kv.width = kv_heads, head_dim, self.slots, self.width
+        if refs is not None:
+            _tensor(refs, "refs", torch.int32, 1)
+            if refs.shape[0] != pages or refs.stride(0) != 1 and pages != 1:
+                raise VSKError(-4, "refs must be a dense vector of a count a page")
+            self.status = torch.zeros(4, dtype=torch.int32, device=k.device)
+            self._scratch = torch.empty(ctx.lib.vsk_kv_scratch_ints(pages, self.slots),
+                                        dtype=torch.int32, device=k.device)
+            kv.refs, kv.status = refs.data_ptr(), self.status.data_ptr()
+            kv.scratch = self._scratch.data_ptr()
+        self._kv = kv
+        self._ref = ctypes.byref(kv)
+
+    # -- new tokens -----------------------------------------------------------
+    def _news(self, x, starts, seqs, max_new):
+        """vsk_new_tokens of the rows of x and what must outlive the call."""
+        n = _lib.vsk_new_tokens()
+        n.tokens = x.shape[0]
+        keep = []
+        if starts is None:
+            n.n, n.max_new = x.shape[0], 1
+        else:
+            s = _ints(starts, "starts", self.device)
+            keep.append(s)
+            if s.shape[0] < 1:
+                raise VSKError(-4, "starts holds an offset a sequence and the end")
+            n.starts, n.n = s.data_ptr(), s.shape[0] - 1
+            n.max_new = x.shape[0] if max_new is None else min(int(max_new), x.shape[0])
+            if n.max_new < 0:
+                raise VSKError(-2, "max_new must not be negative")
+        if seqs is not None:
+            q = _ints(seqs, "seqs", self.device)
+            keep.append(q)
+            if q.shape[0] != n.n:
+                raise VSKError(-4, f"{q.shape[0]} slots for {n.n} sequences")
+            n.seqs = q.data_ptr()
+        elif n.n > self.slots:
+            raise VSKError(-2, f"{n.n} sequences, {self.slots} slots")
+        return n, keep
+
+    def _heads(self, x, name, heads=None):
+        _tensor(x, name, self.dtype, 3)
+        if x.shape[2] != self.head_dim or heads is not None and x.shape[1] != heads:
+            raise VSKError(-4, f"{name} is {tuple(x.shape)}: heads of {self.head_dim} are wanted"
+                           + (f", {heads} of them" if heads is not None else ""))
+        return _dense_heads(x, name)
+
+    def append(self, k, v, *, starts=None, seqs=None, max_new=None, layer: int = 0,
+               rotary: RotaryEmbedding | None = None, q=None):
+        """Writes the new tokens' keys and values (tokens x kv_heads x
+        head_dim) to their places.  Sequence i, in slot ``seqs[i]`` (default:
+        i), has the rows ``starts[i] .. starts[i + 1]`` (default: row i), at
+        most ``max_new``; they are the last of its length.  ``rotary`` turns
+        the keys by their positions, and ``q``, returned turned, with them."""
+        k, v = self._heads(k, "k", self.kv_heads), self._heads(v, "v", self.kv_heads)
+        if v.shape[0] != k.shape[0]:
+            raise VSKError(-4, f"{k.shape[0]} keys, {v.shape[0]} values")
+        if rotary is not None and rotary.head_dim != self.head_dim:
+            raise VSKError(-4, f"rotary is for heads of {rotary.head_dim}")
+        news, keep = self._news(k, starts, seqs, max_new)
+        out, qr = None, None
+        if q is not None:
+            q = self._heads(q, "q")
+            if q.shape[0] != k.shape[0]:
+                raise VSKError(-4, f"{k.shape[0]} keys, {q.shape[0]} queries")
+            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            qr = ctypes.byref(_rows(q, out))
+        if k.shape[0]:
+            self.ctx.check(self.ctx.lib.vsk_kv_append(
+                self.ctx.handle, _stream(self.device), self._ref, layer, ctypes.byref(news),
+                ctypes.byref(_rows(k, None)), ctypes.byref(_rows(v, None)),
+                rotary.handle if rotary is not None else None, qr))
+        return out
+
+    def attend(self, q, *, starts=None, seqs=None, max_new=None, layer: int = 0,
+               scale: float | None = None, window: int | None = None, sinks: int = 0,
+               max_length: int | None = None, return_lse: bool = False):
+        """Attention of the new tokens' queries (tokens x heads x head_dim;
+        consecutive heads share a key head) over their sequences in the
+        cache, laid out as in ``append``.  A token sees the keys up to its own
+        position, with a ``window`` only the last ``window`` of them and the
+        first ``sinks``.  ``scale`` defaults to head_dim^-0.5; ``max_length``
+        bounds the lengths, to divide the work by (default: the table's
+        width).  Returns the outputs, with ``return_lse`` also the logarithm
+        of each row's sum (-inf, and zeros, where a row sees nothing)."""
+        q = self._heads(q, "q")
+        if q.shape[1] % self.kv_heads or not q.shape[1]:
+            raise VSKError(-4, f"{q.shape[1]} query heads over {self.kv_heads} key heads")
+        news, keep = self._news(q, starts, seqs, max_new)
+        out, lse = _outputs(q, return_lse)
+        _attend(self.ctx, self._ref, layer, q, news, None, scale, window, sinks, max_length, out,
+                lse)
+        return (out, lse) if return_lse else out
+
+    # -- pages ------------------------------------------------------------------
+    def _keeping(self):
+        if self.refs is None:
+            raise VSKError(-8, "a cache without refs keeps no pages")
+
+    def reserve(self, seqs, counts):
+        """Grows the sequences in these slots by these numbers of tokens,
+        taking the lowest free pages; ``missing()`` tells of a shortage."""
+        self._keeping()
+        s, c = _ints(seqs, "seqs", self.device), _ints(counts, "counts", self.device)
+        if s.shape != c.shape:
+            raise VSKError(-4, f"{s.shape[0]} slots, {c.shape[0]} counts")
+        self.ctx.check(self.ctx.lib.vsk_kv_reserve(self.ctx.handle, _stream(self.device),
+                                                   self._ref, s.data_ptr(), c.data_ptr(),
+                                                   s.shape[0]))
+
+    def fork(self, parents, children):
+        """The sequences in slots ``children`` become branches of those in
+        ``parents``: whole pages are shared, a last page that is not full is
+        copied.  What the children held is released."""
+        self._keeping()
+        for x, name in ((parents, "parents"), (children, "children")):
+            if not isinstance(x, torch.Tensor):
+                a = np.asarray(x)
+                if a.size and (a.min() < 0 or a.max() >= self.slots):
+                    raise VSKError(-2, f"{name} outside the {self.slots} slots")
+        if not isinstance(parents, torch.Tensor) and not isinstance(children, torch.Tensor):
+            c = list(children)
+            if len(set(c)) != len(c) or set(c) & set(parents):
+                raise VSKError(-2, "children must be distinct and none of them a parent")
+        p, c = _ints(parents, "parents", self.device), _ints(children, "children", self.device)
+        if p.shape != c.shape:
+            raise VSKError(-4, f"{p.shape[0]} parents, {c.shape[0]} children")
+        self.ctx.check(self.ctx.lib.vsk_kv_fork(self.ctx.handle, _stream(self.device), self._ref,
+                                                p.data_ptr(), c.data_ptr(), p.shape[0]))
+
+    def free(self, seqs):
+        """Releases the pages of the sequences in these slots."""
+        self._keeping()
+        s = _ints(seqs, "seqs", self.device)
+        self.ctx.check(self.ctx.lib.vsk_kv_free(self.ctx.handle, _stream(self.device), self._ref,
+                                                s.data_ptr(), s.shape[0]))
+
+    def compact(self):
+        """Moves the pages in use to the low end of the pool, as few as that
+        takes; returns their number (an int32 tensor, the cache's own)."""
+        self._keeping()
+        self.ctx.check(self.ctx.lib.vsk_kv_compact(self.ctx.handle, _stream(self.device),
+                                                   self._ref))
+        return self.status[1]
+
+    def copy_pages(self, src, dst):
+        """Copies pages ``src`` to pages ``dst`` in every layer."""
+        self._keeping()
+        s, d = _ints(src, "src", self.device), _ints(dst, "dst", self.device)
+        if s.shape != d.shape:
+            raise VSKError(-4, f"{s.shape[0]} sources, {d.shape[0]} destinations")
+        self.ctx.check(self.ctx.lib.vsk_kv_copy(self.ctx.handle, _stream(self.device), self._ref,
+                                                s.data_ptr(), d.data_ptr(), s.shape[0]))
+
+    def missing(self) -> int:
+        """Pages that the last ``reserve`` or ``fork`` found none for (waits
+        for the stream)."""
+        self._keeping()
+        return int(self.status[0])
+
+
+def window_attention(ctx: Context, q, k, v, *, starts, k_starts=None, max_length: int | None = None,
+                     scale: float | None = None, window: int | None = None, sinks: int = 0,
+                     return_lse: bool = False):
+    """Causal attention of ragged sequences over dense keys and values: q is
+    tokens x heads x head_dim, sequence i its rows ``starts[i] ..
+    starts[i + 1]``; k and v are rows x kv_heads x head_dim with the offsets
+    ``k_starts`` (default: ``starts``), the queries standing at the keys' end.
+    ``max_length`` bounds the sequences' queries (default: all rows); window,
+    sinks, scale and return_lse as in ``PagedKVCache.attend``."""
+    for x, name in ((q, "q"), (k, "k"), (v, "v")):
+        _tensor(x, name, q.dtype if isinstance(q, torch.Tensor) else None, 3)
+    if q.dtype not in _TYPES:
+        raise VSKError(-8, f"{q.dtype} is not supported")
+    if k.shape != v.shape or q.shape[2] != k.shape[2]:
+        raise VSKError(-4, f"q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}")
+    if not q.shape[1] or not k.shape[1] or q.shape[1] % k.shape[1]:
+        raise VSKError(-4, f"{q.shape[1]} query heads over {k.shape[1]} key heads")
+    if not k.shape[0] and q.shape[0]:
+        raise VSKError(-3, "no keys")
+    q, k, v = (_dense_heads(x, "q") for x in (q, k, v))
+    s = _ints(starts, "starts", q.device)
+    ks = s if k_starts is None else _ints(k_starts, "k_starts", q.device)
+    if s.shape[0] < 1 or ks.shape != s.shape:
+        raise VSKError(-4, "starts and k_starts hold an offset a sequence and the end")
+    if k_starts is None and k.shape[0] != q.shape[0]:
+        raise VSKError(-4, f"{q.shape[0]} queries, {k.shape[0]} keys: k_starts is wanted")
+    kv, news = _lib.vsk_kv(), _lib.vsk_new_tokens()
+    kv.k, kv.v, kv.dtype = k.data_ptr(), v.data_ptr(), _TYPES[q.dtype]
+    kv.k_row, kv.k_head, kv.v_row, kv.v_head = k.stride(0), k.stride(1), v.stride(0), v.stride(1)
+    kv.pages, kv.kv_heads, kv.head_dim, kv.layers = k.shape[0], k.shape[1], k.shape[2], 1
+    news.starts, news.n, news.tokens = s.data_ptr(), s.shape[0] - 1, q.shape[0]
+    news.max_new = q.shape[0] if max_length is None else min(int(max_length), q.shape[0])
+    out, lse = _outputs(q, return_lse)
+    _attend(ctx, ctypes.byref(kv), 0, q, news, ks.data_ptr(), scale, window, sinks,
+            max_length if k_starts is None else None, out, lse)
+    return (out, lse) if return_lse else out
