@@ -14,34 +14,64 @@ int32_t padded_head(int32_t d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
 // How a call's work is divided.
 struct Plan {
   int32_t tiles, splits, chunk;
-  bool split_keys;
+  bool split_keys;  // attn_rows: the waves of a block share a row tile's keys
+  int32_t waves;    // > 0: attn_tile, so many waves a block
 };
+
+// 16-byte loads of every operand, and stores of four values.
+bool aligned_operands(const vsk_kv *kv, const vsk_attention_args *args) {
+  const int64_t size = kv->dtype == VSK_DTYPE_F32 ? 4 : 2, w = 16 / size;
+  const vsk_head_rows &q = args->q;
+  auto at = [](const void *p, int64_t bytes) { return (uintptr_t)p % bytes == 0; };
+  bool ok = kv->head_dim % w == 0 && at(q.src, 16) && at(kv->k, 16) && at(kv->v, 16) &&
+            q.src_row % w == 0 && q.src_head % w == 0 && kv->k_row % w == 0 &&
+            kv->k_head % w == 0 && kv->v_row % w == 0 && kv->v_head % w == 0 &&
+            at(q.dst, 4 * size) && q.dst_row % 4 == 0 && q.dst_head % 4 == 0;
+  if (kv->table)
+    ok = ok && kv->k_layer % w == 0 && kv->v_layer % w == 0 && kv->k_page % w == 0 &&
+         kv->v_page % w == 0;
+  return ok;
+}
 
 Plan plan_of(const vsk_ctx *ctx, const vsk_kv *kv, const vsk_new_tokens *news,
              const vsk_attention_args *args) {
   Plan p;
   const int64_t group = args->q.heads / kv->kv_heads;
   const int64_t max_new = news->starts ? news->max_new : 1;
-  p.tiles = (int32_t)ceil_div(max_new * group, 16);
-  const int64_t blocks = (int64_t)news->n * kv->kv_heads * p.tiles;
-  const int32_t key_tile = kv->dtype == VSK_DTYPE_F32 ? 16 : 32;
+  const int64_t rows = max_new * group, pairs = (int64_t)news->n * kv->kv_heads;
   p.splits = 1;
   p.chunk = 1 << 30;
-  // row tiles enough to fill the device: a wave each
-  p.split_keys = blocks < 8 * (int64_t)ctx->cu_count || p.tiles < 4;
-  if (!p.split_keys) return p;
+  p.waves = 0;
+  p.split_keys = true;
+  int64_t row_tile = 16, key_tile = kv->dtype == VSK_DTYPE_F32 ? 16 : 32, per = 4;
+  int64_t want = 8 * (int64_t)ctx->cu_count;
+  if (kv->dtype != VSK_DTYPE_F32 && rows >= 64 && aligned_operands(kv, args)) {
+    p.waves = kv->head_dim > 128 || pairs * ceil_div(rows, 256) < ctx->cu_count ? 4 : 8;
+    row_tile = 32 * p.waves;
+    key_tile = 64;
+    per = 2;
+    want = ctx->cu_count;
+  }
+  p.tiles = (int32_t)ceil_div(rows, row_tile);
+  const int64_t blocks = pairs * p.tiles;
+  if (p.waves == 0) {
+    // row tiles enough to fill the device: a wave each
+    p.split_keys = blocks < want || p.tiles < 4;
+    if (!p.split_keys) return p;
+  }
   int64_t keys = kv->table ? (int64_t)kv->width * kv->page_size : kv->pages;
   if (args->max_length > 0 && args->max_length < keys) keys = args->max_length;
   if (args->window > 0) {
-    const int64_t seen = (int64_t)args->window + args->sinks + ceil_div(16, group) + 2 * key_tile;
+    const int64_t seen = (int64_t)args->window + args->sinks + ceil_div(row_tile, group) +
+                         2 * key_tile;
     if (seen < keys) keys = seen;
   }
-  // parts of at least a tile for each of the four waves, as many as keep every
-  // compute unit supplied with blocks
+  // parts as many as keep every compute unit supplied with blocks, of at least
+  // a tile for each of the four waves that share them (two tiles)
   const int64_t tiles = ceil_div(keys, key_tile);
-  const int64_t target = ceil_div(8 * (int64_t)ctx->cu_count, blocks);
-  int64_t chunk = ceil_div(ceil_div(tiles, target), 4) * 4;
-  p.chunk = (int32_t)(chunk < 4 ? 4 : chunk);
+  const int64_t target = ceil_div(want, blocks);
+  const int64_t chunk = ceil_div(ceil_div(tiles, target), per) * per;
+  p.chunk = (int32_t)(chunk < per ? per : chunk);
   p.splits = (int32_t)ceil_div(tiles, p.chunk);
   if (p.splits < 1) p.splits = 1;
   return p;
@@ -161,15 +191,13 @@ vsk_status vsk_attention(vsk_ctx *ctx, void *stream, const vsk_kv *kv, int32_t l
     a.part_o = static_cast<float *>(args->workspace);
     a.part_ml = a.part_o + (int64_t)p.splits * a.tokens * a.heads * padded_head(a.d);
   }
-  // 16-byte loads, and stores of four values
-  const int64_t w = 16 / size;
-  bool al = a.d % w == 0 && aligned_to(a.q, 16) && aligned_to(a.k, 16) && aligned_to(a.v, 16) &&
-            a.q_row % w == 0 && a.q_head % w == 0 && a.k_row % w == 0 && a.k_head % w == 0 &&
-            a.v_row % w == 0 && a.v_head % w == 0 && a.k_page % w == 0 && a.v_page % w == 0 &&
-            aligned_to(a.out, 4 * size) && a.o_row % 4 == 0 && a.o_head % 4 == 0;
+  const bool al = aligned_operands(kv, args);
   hipStream_t st = static_cast<hipStream_t>(stream);
-  launch_attn_rows(ctx, st, a, kv->dtype, al, p.split_keys);
-  launch_attn_join(ctx, st, a, kv->dtype, al);
+  if (p.waves)
+    launch_attn_tile(ctx, st, a, kv->dtype, p.waves);
+  else
+    launch_attn_rows(ctx, st, a, kv->dtype, al, p.split_keys);
+  launch_attn_join(ctx, st, a, kv->dtype, al, p.waves ? 32 * p.waves : 16);
   finish_queued(ctx, st);
   VSK_API_END(ctx);
 }

@@ -171,11 +171,16 @@ void check_news(const vsk_new_tokens *news);
 // the stream and the timers' results
 void finish_queued(vsk_ctx *ctx, hipStream_t stream);
 
-// launches (attn_rows.hip); t: a VSK_DTYPE; aligned: every pointer and
+// launches; attn_rows.hip; t: a VSK_DTYPE; aligned: every pointer and
 // stride takes 16-byte loads (8-byte stores)
 void launch_attn_rows(vsk_ctx *ctx, hipStream_t stream, const AttnArgs &a, int32_t t,
                       bool aligned, bool split_keys);
+// attn_tile.hip: 16-bit types, aligned; waves: 8 or 4 a workgroup
+void launch_attn_tile(vsk_ctx *ctx, hipStream_t stream, const AttnArgs &a, int32_t t,
+                      int32_t waves);
+// joins the parts that row tiles of `rows` rows left: 16 (launch_attn_rows),
+// or 32 a wave (launch_attn_tile)
 void launch_attn_join(vsk_ctx *ctx, hipStream_t stream, const AttnArgs &a, int32_t t,
-                      bool aligned);
+                      bool aligned, int32_t rows);
 
 }  // namespace vsk

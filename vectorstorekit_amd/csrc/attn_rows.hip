@@ -443,8 +443,8 @@ k_attn_rows(const AttnArgs a) {
 // Joins the parts of one output row: sum of the parts' values and sums, each
 // times 2^(its maximum - the largest).  A block a row; the threads take four
 // values each of several parts at a time.
-template <class T, int DV, int RT, int KTILE, bool ALIGNED>
-__global__ __launch_bounds__(256) void k_attn_join(const AttnArgs a) {
+template <class T, int DV, int KTILE, bool ALIGNED>
+__global__ __launch_bounds__(256) void k_attn_join(const AttnArgs a, const int32_t RT) {
   constexpr int LANES = DV / 4, WAYS = 256 / LANES;
   __shared__ __attribute__((aligned(16))) float so[WAYS][DV];
   __shared__ float ss[WAYS];
@@ -552,38 +552,46 @@ void launch_attn_rows(vsk_ctx *ctx, hipStream_t st, const AttnArgs &a, int32_t t
 }
 
 namespace {
-template <class T, int RT, int KTILE>
-void join_of(hipStream_t st, const AttnArgs &a, bool aligned, unsigned g) {
+template <class T, int KTILE>
+void join_of(hipStream_t st, const AttnArgs &a, bool aligned, int32_t rows, unsigned g) {
   if (a.d <= 64) {
     if (aligned)
-      k_attn_join<T, 64, RT, KTILE, true><<<g, 256, 0, st>>>(a);
+      k_attn_join<T, 64, KTILE, true><<<g, 256, 0, st>>>(a, rows);
     else
-      k_attn_join<T, 64, RT, KTILE, false><<<g, 256, 0, st>>>(a);
+      k_attn_join<T, 64, KTILE, false><<<g, 256, 0, st>>>(a, rows);
   } else if (a.d <= 128) {
     if (aligned)
-      k_attn_join<T, 128, RT, KTILE, true><<<g, 256, 0, st>>>(a);
+      k_attn_join<T, 128, KTILE, true><<<g, 256, 0, st>>>(a, rows);
     else
-      k_attn_join<T, 128, RT, KTILE, false><<<g, 256, 0, st>>>(a);
+      k_attn_join<T, 128, KTILE, false><<<g, 256, 0, st>>>(a, rows);
   } else {
     if (aligned)
-      k_attn_join<T, 256, RT, KTILE, true><<<g, 256, 0, st>>>(a);
+      k_attn_join<T, 256, KTILE, true><<<g, 256, 0, st>>>(a, rows);
     else
-      k_attn_join<T, 256, RT, KTILE, false><<<g, 256, 0, st>>>(a);
+      k_attn_join<T, 256, KTILE, false><<<g, 256, 0, st>>>(a, rows);
   }
+}
+template <class T>
+void join_rows(hipStream_t st, const AttnArgs &a, bool aligned, int32_t rows, unsigned g) {
+  if (rows == ROWS)
+    join_of<T, 16 * SUBS<T>>(st, a, aligned, rows, g);
+  else
+    join_of<T, 64>(st, a, aligned, rows, g);
 }
 }  // namespace
 
-void launch_attn_join(vsk_ctx *ctx, hipStream_t st, const AttnArgs &a, int32_t t, bool aligned) {
+void launch_attn_join(vsk_ctx *ctx, hipStream_t st, const AttnArgs &a, int32_t t, bool aligned,
+                      int32_t rows) {
   if (a.splits == 1) return;
   const int64_t grid = (int64_t)a.n * a.max_new * a.heads;
   VSK_REQUIRE(grid <= 0x7FFFFFFFll, VSK_ERR_INVALID_BUFFER_SIZE, "too many query rows in one call");
   KernelTimer kt(ctx, "attn_join", (double)grid, st);
   if (t == VSK_DTYPE_F32)
-    join_of<float, ROWS, 16 * SUBS<float>>(st, a, aligned, (unsigned)grid);
+    join_of<float, 16 * SUBS<float>>(st, a, aligned, rows, (unsigned)grid);
   else if (t == VSK_DTYPE_F16)
-    join_of<_Float16, ROWS, 16 * SUBS<_Float16>>(st, a, aligned, (unsigned)grid);
+    join_rows<_Float16>(st, a, aligned, rows, (unsigned)grid);
   else
-    join_of<__bf16, ROWS, 16 * SUBS<__bf16>>(st, a, aligned, (unsigned)grid);
+    join_rows<__bf16>(st, a, aligned, rows, (unsigned)grid);
   check_launch("attn_join");
 }
 
