@@ -48,7 +48,7 @@ Plan plan_of(const vsk_ctx *ctx, const vsk_kv *kv, const vsk_new_tokens *news,
   if (kv->dtype != VSK_DTYPE_F32 && rows >= 64 && aligned_operands(kv, args)) {
     p.waves = kv->head_dim > 128 || pairs * ceil_div(rows, 256) < ctx->cu_count ? 4 : 8;
     row_tile = 32 * p.waves;
-    key_tile = 64;
+    key_tile = attn_tile_keys(kv->head_dim);
     per = 2;
     want = ctx->cu_count;
   }

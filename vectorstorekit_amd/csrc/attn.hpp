@@ -136,32 +136,65 @@ struct AttnRows {
   int64_t k, v;
   int32_t last;
 };
-__device__ inline AttnRows attn_rows(const AttnArgs &a, const AttnSeq &s, int32_t h, int32_t j16) {
-  AttnRows r;
+__device__ inline int32_t attn_row16(const AttnSeq &s, int32_t j16) {
   const int32_t tail = (s.L - 1) & ~15;
-  const int32_t j = j16 < tail ? j16 : tail;
+  return j16 < tail ? j16 : tail;
+}
+// the page that holds them, as the table has it (dense: 0).  The index is
+// hidden from the compiler, which would turn the value into a scalar, and wait
+// for it, at once: it is asked for a step before it is used.
+__device__ inline int32_t attn_page(const AttnArgs &a, const AttnSeq &s, int32_t j16) {
+  if (!a.table) return 0;
+  int32_t i = attn_row16(s, j16) >> a.page_shift;
+  asm volatile("" : "+v"(i));
+  return a.table[s.slot * a.table_stride + i];
+}
+__device__ inline AttnRows attn_rows(const AttnArgs &a, const AttnSeq &s, int32_t h, int32_t j16,
+                                     int32_t page) {
+  AttnRows r;
+  page = __builtin_amdgcn_readfirstlane(page);
+  page = page < 0 ? 0 : page >= a.pages && a.table ? a.pages - 1 : page;
+  const int32_t j = attn_row16(s, j16);
   r.last = s.L - 1 - j < 15 ? s.L - 1 - j : 15;
-  if (a.table) {
-    int32_t page = a.table[s.slot * a.table_stride + (j >> a.page_shift)];
-    page = page < 0 ? 0 : page >= a.pages ? a.pages - 1 : page;
-    const int32_t in = j & ((1 << a.page_shift) - 1);
-    r.k = page * a.k_page + in * a.k_row + h * a.k_head;
-    r.v = page * a.v_page + in * a.v_row + h * a.v_head;
-  } else {
-    r.k = (s.key0 + j) * a.k_row + h * a.k_head;
-    r.v = (s.key0 + j) * a.v_row + h * a.v_head;
-  }
+  const int64_t in = a.table ? j & ((1 << a.page_shift) - 1) : s.key0 + j;
+  r.k = page * a.k_page + in * a.k_row + h * a.k_head;
+  r.v = page * a.v_page + in * a.v_row + h * a.v_head;
   return r;
 }
 
 __device__ inline float attn_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
+// Exchanges between lanes 16 and 32 apart on the vector unit: of x twice, the
+// swap of the odd rows (the upper half) of the one with the even rows (the
+// lower half) of the other leaves each pair's two values in the two results.
+__device__ inline void pair32(float x, float *lo, float *hi) {
+  const uint32_t u = __float_as_uint(x);
+  const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  *lo = __uint_as_float(r[0]), *hi = __uint_as_float(r[1]);
+}
+__device__ inline void pair16(float x, float *lo, float *hi) {
+  const uint32_t u = __float_as_uint(x);
+  const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  *lo = __uint_as_float(r[0]), *hi = __uint_as_float(r[1]);
+}
+__device__ inline float xor32_max(float x) {
+  float a, b;
+  pair32(x, &a, &b);
+  return fmaxf(a, b);
+}
+__device__ inline float xor32_sum(float x) {
+  float a, b;
+  pair32(x, &a, &b);
+  return a + b;
+}
 __device__ inline float xor16_32_max(float x) {
-  x = fmaxf(x, __shfl_xor(x, 16));
-  return fmaxf(x, __shfl_xor(x, 32));
+  float a, b;
+  pair16(x, &a, &b);
+  return xor32_max(fmaxf(a, b));
 }
 __device__ inline float xor16_32_sum(float x) {
-  x += __shfl_xor(x, 16);
-  return x + __shfl_xor(x, 32);
+  float a, b;
+  pair16(x, &a, &b);
+  return xor32_sum(a + b);
 }
 
 // what the entry points check of a cache and of a call's tokens (kvcache.hip)
@@ -175,6 +208,8 @@ void finish_queued(vsk_ctx *ctx, hipStream_t stream);
 // stride takes 16-byte loads (8-byte stores)
 void launch_attn_rows(vsk_ctx *ctx, hipStream_t stream, const AttnArgs &a, int32_t t,
                       bool aligned, bool split_keys);
+// keys of a tile of attn_tile.hip, by the (padded) head
+constexpr int attn_tile_keys(int d) { return d > 128 ? 32 : 64; }
 // attn_tile.hip: 16-bit types, aligned; waves: 8 or 4 a workgroup
 void launch_attn_tile(vsk_ctx *ctx, hipStream_t stream, const AttnArgs &a, int32_t t,
                       int32_t waves);

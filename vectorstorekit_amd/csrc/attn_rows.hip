@@ -159,7 +159,7 @@ template <class T, int VW, int NB, bool ALIGNED> struct RowTile {
     AttnRows r[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      r[u] = attn_rows(a, s, h, kb + 16 * u);
+      r[u] = attn_rows(a, s, h, kb + 16 * u, attn_page(a, s, kb + 16 * u));
       const T *row = static_cast<const T *>(a.k) + r[u].k +
                      (n < r[u].last ? n : r[u].last) * (int32_t)a.k_row;
 #pragma unroll
@@ -552,31 +552,26 @@ void launch_attn_rows(vsk_ctx *ctx, hipStream_t st, const AttnArgs &a, int32_t t
 }
 
 namespace {
-template <class T, int KTILE>
-void join_of(hipStream_t st, const AttnArgs &a, bool aligned, int32_t rows, unsigned g) {
-  if (a.d <= 64) {
+template <class T, int DV>
+void join_head(hipStream_t st, const AttnArgs &a, bool aligned, int32_t rows, unsigned g) {
+  constexpr int KR = 16 * SUBS<T>, KB = attn_tile_keys(DV);
+  if (rows == ROWS) {
     if (aligned)
-      k_attn_join<T, 64, KTILE, true><<<g, 256, 0, st>>>(a, rows);
+      k_attn_join<T, DV, KR, true><<<g, 256, 0, st>>>(a, rows);
     else
-      k_attn_join<T, 64, KTILE, false><<<g, 256, 0, st>>>(a, rows);
-  } else if (a.d <= 128) {
-    if (aligned)
-      k_attn_join<T, 128, KTILE, true><<<g, 256, 0, st>>>(a, rows);
-    else
-      k_attn_join<T, 128, KTILE, false><<<g, 256, 0, st>>>(a, rows);
-  } else {
-    if (aligned)
-      k_attn_join<T, 256, KTILE, true><<<g, 256, 0, st>>>(a, rows);
-    else
-      k_attn_join<T, 256, KTILE, false><<<g, 256, 0, st>>>(a, rows);
+      k_attn_join<T, DV, KR, false><<<g, 256, 0, st>>>(a, rows);
+  } else if constexpr (sizeof(T) == 2) {  // (tiles are for 16-bit, aligned operands)
+    k_attn_join<T, DV, KB, true><<<g, 256, 0, st>>>(a, rows);
   }
 }
 template <class T>
-void join_rows(hipStream_t st, const AttnArgs &a, bool aligned, int32_t rows, unsigned g) {
-  if (rows == ROWS)
-    join_of<T, 16 * SUBS<T>>(st, a, aligned, rows, g);
+void join_of(hipStream_t st, const AttnArgs &a, bool aligned, int32_t rows, unsigned g) {
+  if (a.d <= 64)
+    join_head<T, 64>(st, a, aligned, rows, g);
+  else if (a.d <= 128)
+    join_head<T, 128>(st, a, aligned, rows, g);
   else
-    join_of<T, 64>(st, a, aligned, rows, g);
+    join_head<T, 256>(st, a, aligned, rows, g);
 }
 }  // namespace
 
@@ -587,11 +582,11 @@ void launch_attn_join(vsk_ctx *ctx, hipStream_t st, const AttnArgs &a, int32_t t
   VSK_REQUIRE(grid <= 0x7FFFFFFFll, VSK_ERR_INVALID_BUFFER_SIZE, "too many query rows in one call");
   KernelTimer kt(ctx, "attn_join", (double)grid, st);
   if (t == VSK_DTYPE_F32)
-    join_of<float, 16 * SUBS<float>>(st, a, aligned, rows, (unsigned)grid);
+    join_of<float>(st, a, aligned, rows, (unsigned)grid);
   else if (t == VSK_DTYPE_F16)
-    join_rows<_Float16>(st, a, aligned, rows, (unsigned)grid);
+    join_of<_Float16>(st, a, aligned, rows, (unsigned)grid);
   else
-    join_rows<__bf16>(st, a, aligned, rows, (unsigned)grid);
+    join_of<__bf16>(st, a, aligned, rows, (unsigned)grid);
   check_launch("attn_join");
 }
 

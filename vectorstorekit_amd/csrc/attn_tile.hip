@@ -21,10 +21,10 @@ namespace vsk {
 
 namespace {
 
-constexpr int KT = 64;  // keys of a tile
 
 typedef __attribute__((ext_vector_type(4))) short i16x4;
-typedef __attribute__((address_space(3))) char lds_char;
+#define lds_as __attribute__((address_space(3)))
+typedef lds_as char lds_char;
 
 template <class T> struct Mm;
 template <> struct Mm<__bf16> {
@@ -53,34 +53,54 @@ template <int CH> __device__ inline int v_swizzle(int row) {
   return CH >= 16 ? 4 * x + 2 * (x >> 1) : 2 * x;
 }
 
-// 16 bytes a lane from src to dst + 16 * lane (dst the same in every lane).
-// Written as assembly because the compiler makes every read of LDS after the
-// builtin wait for it: here a tile's copies fly while the last tile is
-// computed with, and one wait before the barrier covers them.  (M0 holds the
-// destination of such loads; nothing else in these kernels uses it.)
-__device__ inline void load_to_lds(const void *src, const void *dst) {
-  const uint32_t at = __builtin_amdgcn_readfirstlane(
-      (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void *)dst);
+// 16 bytes a lane from base + off to dst + 16 * lane (base and dst the same in
+// every lane).  Written as assembly because the compiler makes every read of
+// LDS after the builtin wait for it: here a tile's copies fly while the last
+// tile is computed with, and one wait before the barrier covers them.  (M0
+// holds the destination of such loads; nothing else in these kernels uses it.)
+__device__ inline void load_to_lds(uint64_t base, uint32_t off, const lds_char *dst) {
+  const uint32_t at = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)dst);
   asm volatile(
       "s_mov_b32 m0, %0\n\t"
       "s_nop 0\n\t"
-      "global_load_lds_dwordx4 %1, off"
+      "global_load_lds_dwordx4 %1, %2"
       :
-      : "s"(at), "v"(src)
+      : "s"(at), "v"(off), "s"(base)
       : "memory");
 }
 
-template <class T, int DP, int NW>
-__global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void k_attn_tile(const AttnArgs a) {
+__device__ inline uint64_t lane_of(uint32_t lo, uint32_t hi, int i) {
+  return (uint64_t)(uint32_t)__builtin_amdgcn_readlane(hi, i) << 32 |
+         (uint32_t)__builtin_amdgcn_readlane(lo, i);
+}
+
+// (fmaxf would first quiet each product, an instruction a value: the maximum
+// here passes over NaN without it)
+__device__ inline float max3(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+
+// RW: row tiles (of 32) of a wave.
+template <class T, int DP, int NW, int RW>
+__global__ __launch_bounds__(64 * NW, 2) void k_attn_tile(const AttnArgs a) {
   typedef typename Mm<T>::V8 V8;
+  constexpr int KT = attn_tile_keys(DP), U = KT / 32;
   constexpr int CH = DP / 8;         // 16-byte pieces of a row
   constexpr int ROWB = 2 * DP;       // bytes of a row
   constexpr int TILEB = KT * ROWB;   // bytes of a tile
   constexpr int RPI = 64 / CH;       // rows that one load of a wave brings
   constexpr int MINE = KT / NW;      // rows of a tile that a wave brings
+  constexpr int LD = MINE / RPI;     // loads that takes
   constexpr int KS = DP / 16, DT = DP / 32;
-  __shared__ __attribute__((aligned(1024))) char kbuf[2][TILEB];
-  __shared__ __attribute__((aligned(1024))) char vbuf[2][TILEB];
+  constexpr int ROWS = 32 * RW * NW; // query rows of the block
+  // tile i's keys in kbuf[i % 3], two tiles ahead of their products, its
+  // values in vbuf[i % 2], one ahead
+  __shared__ __attribute__((aligned(1024))) char keys_lds[3 * TILEB];
+  __shared__ __attribute__((aligned(1024))) char values_lds[2 * TILEB];
+  lds_char *const kbuf = (lds_char *)keys_lds;
+  lds_char *const vbuf = (lds_char *)values_lds;
 
   const int lane = threadIdx.x & 63, h2 = lane >> 5, n = lane & 31;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -91,11 +111,11 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void k_attn_tile(const 
   at /= a.tiles;
   const int32_t part = at % a.splits;
   const AttnSeq s = attn_seq(a, at / a.splits);
-  const int32_t row0 = tile * 32 * NW;
+  const int32_t row0 = tile * ROWS;
   const int32_t T_used = s.T < a.max_new ? s.T : a.max_new;
   const int32_t rows_all = T_used * a.group;
   if (row0 >= rows_all) return;
-  const int32_t last = row0 + 32 * NW < rows_all ? row0 + 32 * NW - 1 : rows_all - 1;
+  const int32_t last = row0 + ROWS < rows_all ? row0 + ROWS - 1 : rows_all - 1;
   const int32_t p0 = s.L - s.T;
   const AttnSpan<KT> span = attn_span<KT>(a, p0 + row0 / a.group, p0 + last / a.group);
   const int32_t parts = attn_parts(a, span.tiles);
@@ -104,225 +124,436 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void k_attn_tile(const 
   const int32_t end = part == parts - 1 ? span.tiles : first + a.chunk;
 
   // this wave's rows and what they see
-  const int32_t w0 = row0 + 32 * w, w1 = w0 + 31 < last ? w0 + 31 : last;
+  const int32_t w0 = row0 + 32 * RW * w, w1 = w0 + 32 * RW - 1 < last ? w0 + 32 * RW - 1 : last;
   const bool have = w0 <= last;
   const int32_t q_lo = p0 + w0 / a.group, q_hi = have ? p0 + w1 / a.group : -1;
-  const int32_t row = w0 + n;
-  const bool real = row <= last;
-  const int32_t t = row / a.group, head = h * a.group + row - t * a.group;
-  const int32_t pos = real ? p0 + t : -1;
-
-  V8 q[KS];
-  {
+  int32_t pos[RW];
+  V8 q[RW][KS];
+#pragma unroll
+  for (int r = 0; r < RW; ++r) {
+    const int32_t row = w0 + 32 * r + n, t = row / a.group, head = h * a.group + row - t * a.group;
+    const bool real = row <= last;
+    pos[r] = real ? p0 + t : -1;
     const T *src = static_cast<const T *>(a.q) + (real ? (s.token0 + t) * a.q_row + head * a.q_head : 0);
 #pragma unroll
     for (int i = 0; i < KS; ++i) {
-      q[i] = V8{};
-      if (real && 16 * i + 8 * h2 < a.d) q[i] = *reinterpret_cast<const V8 *>(src + 16 * i + 8 * h2);
+      q[r][i] = V8{};
+      if (real && 16 * i + 8 * h2 < a.d)
+        q[r][i] = *reinterpret_cast<const V8 *>(src + 16 * i + 8 * h2);
     }
   }
   if (a.d < DP) {
     // pieces past the head are never loaded: they stay zero
-    u32x4 *z = reinterpret_cast<u32x4 *>(kbuf), *y = reinterpret_cast<u32x4 *>(vbuf);
-    for (int i = threadIdx.x; i < 2 * TILEB / 16; i += 64 * NW) z[i] = y[i] = u32x4{0, 0, 0, 0};
+    u32x4 *z = reinterpret_cast<u32x4 *>(keys_lds), *y = reinterpret_cast<u32x4 *>(values_lds);
+    for (int i = threadIdx.x; i < 3 * TILEB / 16; i += 64 * NW) z[i] = u32x4{0, 0, 0, 0};
+    for (int i = threadIdx.x; i < 2 * TILEB / 16; i += 64 * NW) y[i] = u32x4{0, 0, 0, 0};
     __syncthreads();
   }
 
-  f32x16 acc[DT];
+  f32x16 acc[RW][DT];
+  float m[RW], l[RW];
 #pragma unroll
-  for (int i = 0; i < DT; ++i) acc[i] = f32x16{};
-  float m = -INFINITY, l = 0.f;
+  for (int r = 0; r < RW; ++r) {
+#pragma unroll
+    for (int i = 0; i < DT; ++i) acc[r][i] = f32x16{};
+    m[r] = -INFINITY;
+    l[r] = 0.f;
+  }
 
-  // brings the wave's rows of a tile
+  // The rows of a tile that this wave brings lie within 16, on one page.
+  // Lane i holds the addresses of those 16 for tile tb + i, keys and values.
   const int piece = lane % CH, sub = lane / CH;
-  auto fetch = [&](int32_t i, int buf) {
-    const int32_t j0 = span.base(i) + MINE * w;
-    const AttnRows r = attn_rows(a, s, h, j0 & ~15);
+  uint32_t k_lo = 0, k_hi = 0, v_lo = 0, v_hi = 0;
+  int32_t tb = 0;
+  auto addresses = [&](int32_t i) {
+    tb = i;
+    const int32_t j16 = (span.base(i + lane) + MINE * w) & ~15, j = attn_row16(s, j16);
+    int64_t page = 0, in = s.key0 + j;
+    if (a.table) {
+      int32_t x = a.table[s.slot * a.table_stride + (j >> a.page_shift)];
+      page = x < 0 ? 0 : x >= a.pages ? a.pages - 1 : x;
+      in = j & ((1 << a.page_shift) - 1);
+    }
+    const uint64_t k = (uint64_t)(uintptr_t)a.k + 2 * (page * a.k_page + in * a.k_row + h * a.k_head);
+    const uint64_t v = (uint64_t)(uintptr_t)a.v + 2 * (page * a.v_page + in * a.v_row + h * a.v_head);
+    k_lo = (uint32_t)k, k_hi = (uint32_t)(k >> 32);
+    v_lo = (uint32_t)v, v_hi = (uint32_t)(v >> 32);
+  };
+  // each lane's place in those 16 rows, in bytes
+  uint32_t k_off[LD], v_off[LD];
+  auto offset = [&](int x, int32_t most, bool keys) -> uint32_t {
+    const int lr = MINE * w + x * RPI + sub;
+    const int32_t off = (lr & 15) < most ? (lr & 15) : most;
+    const int c = piece ^ (keys ? k_swizzle<CH>(lr) : v_swizzle<CH>(lr));
+    return 2 * ((uint32_t)off * (uint32_t)(keys ? a.k_row : a.v_row) + 8 * c);
+  };
 #pragma unroll
-    for (int x = 0; x < MINE / RPI; ++x) {
-      const int lr = MINE * w + x * RPI + sub;  // the row within the tile
-      const int off = (j0 & 15) + x * RPI + sub;
-      const int32_t rr = off < r.last ? off : r.last;
-      const int kc = piece ^ k_swizzle<CH>(lr), vc = piece ^ v_swizzle<CH>(lr);
-      const T *ks = static_cast<const T *>(a.k) + r.k + rr * (int32_t)a.k_row + 8 * kc;
-      const T *vs = static_cast<const T *>(a.v) + r.v + rr * (int32_t)a.v_row + 8 * vc;
-      const int at = (MINE * w + x * RPI) * ROWB;
-      if (8 * kc < a.d) load_to_lds(ks, kbuf[buf] + at);
-      if (8 * vc < a.d) load_to_lds(vs, vbuf[buf] + at);
+  for (int x = 0; x < LD; ++x) k_off[x] = offset(x, 15, true), v_off[x] = offset(x, 15, false);
+  const bool full = a.d == DP;
+  auto fetch = [&](int32_t i, lds_char *to, bool keys) {
+    const uint64_t base = keys ? lane_of(k_lo, k_hi, i - tb) : lane_of(v_lo, v_hi, i - tb);
+    const int32_t j0 = span.base(i) + MINE * w;
+    to += MINE * w * ROWB;
+    if (full && j0 + MINE <= s.L) {
+#pragma unroll
+      for (int x = 0; x < LD; ++x)
+        load_to_lds(base, keys ? k_off[x] : v_off[x], to + x * RPI * ROWB);
+      return;
+    }
+    // (the keys from L on read row L - 1, pieces past the head nothing)
+    const int32_t left = s.L - 1 - attn_row16(s, j0 & ~15);
+#pragma unroll
+    for (int x = 0; x < LD; ++x) {
+      const int lr = MINE * w + x * RPI + sub;
+      const int c = piece ^ (keys ? k_swizzle<CH>(lr) : v_swizzle<CH>(lr));
+      const uint32_t off = offset(x, left, keys);
+      if (8 * c < a.d) load_to_lds(base, off, to + x * RPI * ROWB);
     }
   };
 
   // lane's parts of the addresses of the reads
-  const int kx = h2 ^ k_swizzle<CH>(n);
   const int gi = lane & 15, va = gi >> 2, vhalf = (lane >> 4) & 1;
-  const int vrow = (4 * h2 + va) * ROWB + 8 * (gi & 1);
-  const int vx = (2 * vhalf + ((gi & 3) >> 1)) ^ v_swizzle<CH>(va);
+  const int k_at = n * ROWB + ((h2 ^ k_swizzle<CH>(n)) << 4);
+  const int v_at = (4 * h2 + va) * ROWB + 8 * (gi & 1) +
+                   (((2 * vhalf + ((gi & 3) >> 1)) ^ v_swizzle<CH>(va)) << 4);
+  // piece 2 x + h2 of key 32 u + n: the swizzle leaves bit operations only
+  auto key_piece = [&](int base, int x, int u) -> V8 {
+    return *(const lds_as V8 *)(uintptr_t)(uint32_t)((base ^ (x << 5)) + 32 * u * ROWB);
+  };
+  // dimensions 32 dt on of keys 16 u + 4 h2 .. + 3 and 8 further
+  auto value_piece = [&](int base, int dt, int u) -> V8 {
+    const int at = (base ^ (dt << 6)) + 16 * u * ROWB;
+    union {
+      i16x4 half[2];
+      V8 v;
+    } f;
+    f.half[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_as i16x4 *)(uintptr_t)(uint32_t)at);
+    f.half[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+        (lds_as i16x4 *)(uintptr_t)(uint32_t)(at + 8 * ROWB));
+    return f.v;
+  };
+  auto k_base = [&](const lds_char *buf) { return (int)(uintptr_t)buf + k_at; };
+  auto v_base = [&](const lds_char *buf) { return (int)(uintptr_t)buf + v_at; };
 
-  if (first < end) fetch(first, 0);
-  __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
-  __syncthreads();
-  for (int32_t i = first; i < end; ++i) {
-    const int cur = (i - first) & 1;
-    if (i + 1 < end) fetch(i + 1, cur ^ 1);
-    const int32_t kb = span.base(i);
-    // (a wave whose rows see none of the tile only brings its rows)
-    const bool any = kb <= q_hi && (a.window <= 0 || q_lo - (kb + KT - 1) < a.window || kb < a.sinks);
-    if (any) {
-      const char *kt = kbuf[cur] + n * ROWB;
-      f32x16 sc[2];
+  // register 16 u + x of the scores belongs to key 32 u + 8 (x / 4) + 4 h2 +
+  // x % 4 of the tile
+  auto scores = [&](const lds_char *buf, f32x16 (&sc)[RW][U]) {
+    const int kb = k_base(buf);
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        sc[u] = f32x16{};
+    for (int u = 0; u < U; ++u) {
 #pragma unroll
-        for (int x = 0; x < KS; ++x) {
-          const V8 k = *reinterpret_cast<const V8 *>(kt + 32 * u * ROWB + (((2 * x) ^ kx) << 4));
-          sc[u] = Mm<T>::mfma(k, q[x], sc[u]);
-        }
-      }
-      const bool whole = kb + KT - 1 <= q_lo &&
-                         (a.window <= 0 || q_hi - kb < a.window || kb + KT <= a.sinks);
-      bool odd = false;
-      if (!whole) {
+      for (int r = 0; r < RW; ++r) sc[r][u] = f32x16{};
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
+      for (int x = 0; x < KS; ++x) {
+        const V8 k = key_piece(kb, x, u);
 #pragma unroll
-          for (int x = 0; x < 16; ++x)
-            if (!attn_sees(a, pos, kb + 32 * u + 8 * (x >> 2) + 4 * h2 + (x & 3)))
-              sc[u][x] = -INFINITY;
-        // is every value of the tile finite?  (largest exponent field)
-        typedef __attribute__((ext_vector_type(2))) unsigned short u16x2;
-        u16x2 top = {0, 0};
-        const u32x4 *vt = reinterpret_cast<const u32x4 *>(vbuf[cur]);
-#pragma unroll 4
-        for (int x = lane; x < TILEB / 16; x += 64) {
-          const u32x4 y = vt[x];
-#pragma unroll
-          for (int z = 0; z < 4; ++z)
-            top = __builtin_elementwise_max(
-                top, __builtin_bit_cast(u16x2, y[z] & Mm<T>::EXP));
-        }
-        const unsigned short inf = (unsigned short)(Mm<T>::EXP & 0xFFFF);
-        odd = __any(top[0] == inf || top[1] == inf);
-      }
-      float tm = -INFINITY;
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int x = 0; x < 16; x += 2) tm = fmaxf(tm, fmaxf(sc[u][x], sc[u][x + 1]));
-      tm = fmaxf(tm, __shfl_xor(tm, 32));
-      const float nm = fmaxf(m, tm * a.scale_log2);
-      const float use = nm == -INFINITY ? 0.f : nm;
-      const float fade = attn_exp2(m - use);
-      m = nm;
-      l *= fade;
-#pragma unroll
-      for (int x = 0; x < DT; ++x) acc[x] *= fade;
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int x = 0; x < 16; ++x) {
-          sc[u][x] = attn_exp2(fmaf(sc[u][x], a.scale_log2, -use));
-          l += sc[u][x];
-        }
-      if (!odd) {
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          V8 p;
-#pragma unroll
-          for (int x = 0; x < 8; ++x) p[x] = (T)sc[u >> 1][8 * (u & 1) + x];
-#pragma unroll
-          for (int dt = 0; dt < DT; ++dt) {
-            const char *vt = vbuf[cur] + vrow + 16 * u * ROWB + (((4 * dt) ^ vx) << 4);
-            union {
-              i16x4 half[2];
-              V8 v;
-            } f;
-            f.half[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                (__attribute__((address_space(3))) i16x4 *)(lds_char *)vt);
-            f.half[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                (__attribute__((address_space(3))) i16x4 *)(lds_char *)(vt + 8 * ROWB));
-            acc[dt] = Mm<T>::mfma(f.v, p, acc[dt]);
-          }
-        }
-      } else {
-        // a value that is not finite, in a tile that not every row sees whole:
-        // its keys one at a time, each row takes only those it sees
-#pragma unroll 1
-        for (int j = 0; j < KT; ++j) {
-          float wt = 0.f;
-#pragma unroll
-          for (int u = 0; u < 2; ++u)
-#pragma unroll
-            for (int x = 0; x < 16; ++x)
-              wt = 32 * u + 8 * (x >> 2) + (x & 3) == (j & ~4) ? sc[u][x] : wt;
-          wt = __shfl(wt, n + 32 * ((j >> 2) & 1));
-          if (!attn_sees(a, pos, kb + j)) continue;
-#pragma unroll
-          for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-            for (int b = 0; b < 4; ++b) {
-              const int c = 4 * dt + b;
-              const T *v = reinterpret_cast<const T *>(vbuf[cur] + j * ROWB +
-                                                       ((c ^ v_swizzle<CH>(j)) << 4)) + 4 * h2;
-#pragma unroll
-              for (int x = 0; x < 4; ++x)
-                acc[dt][4 * b + x] = fmaf(wt, (float)v[x], acc[dt][4 * b + x]);
-            }
-        }
+        for (int r = 0; r < RW; ++r) sc[r][u] = Mm<T>::mfma(k, q[r][x], sc[r][u]);
       }
     }
-    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): the next tile has arrived
-    __syncthreads();
+  };
+  auto largest = [&](const f32x16 (&sc)[U]) {
+    float tm = max3(sc[0][0], sc[0][1], sc[0][2]);
+#pragma unroll
+    for (int x = 3; x < 16 * U - 1; x += 2)
+      tm = max3(tm, sc[x >> 4][x & 15], sc[(x + 1) >> 4][(x + 1) & 15]);
+    return xor32_max(max3(tm, sc[U - 1][15], sc[U - 1][15]));
+  };
+  // The sums are kept relative to m, which follows the largest score only when
+  // that has grown by 8 (in log2): weights up to 256 cost no precision, and
+  // the sums are seldom rescaled.
+  auto settle = [&](int r, float tm) {
+    const float top = tm * a.scale_log2;
+    if (!__any(top > m[r] + 8.f)) return;
+    const float nm = top > m[r] + 8.f ? top : m[r];
+    const float fade = nm == -INFINITY ? 1.f : attn_exp2(m[r] - nm);
+    m[r] = nm;
+    l[r] *= fade;
+#pragma unroll
+    for (int x = 0; x < DT; ++x) acc[r][x] *= fade;
+  };
+  // -inf for the keys that the row at this position does not see.  Bit c of a
+  // word is key c of the 32 that the word is for: comparisons a row, not a key.
+  auto up_to = [](int32_t x) -> uint32_t { return x < 0 ? 0u : x > 30 ? ~0u : (2u << x) - 1; };
+  auto hide = [&](f32x16 (&sc)[U], int32_t at, int32_t kb) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int32_t b = kb + 32 * u + 4 * h2;
+      uint32_t see = ~0u;
+      if (a.window > 0)
+        see = (at < a.window ? ~0u : ~up_to(at - a.window - b)) | up_to(a.sinks - 1 - b);
+      see &= up_to(at - b);
+#pragma unroll
+      for (int x = 0; x < 16; ++x) {
+        const uint32_t on = (uint32_t)((int32_t)(see << (31 - 8 * (x >> 2) - (x & 3))) >> 31);
+        sc[u][x] = __uint_as_float((on & __float_as_uint(sc[u][x])) | (~on & 0xFF800000u));
+      }
+    }
+  };
+  // is a value of the tile not finite?  (the largest exponent field)
+  auto not_finite = [&](const lds_char *vt) -> bool {
+    typedef __attribute__((ext_vector_type(2))) unsigned short u16x2;
+    u16x2 top = {0, 0};
+    const lds_as u32x4 *v4 = (const lds_as u32x4 *)vt;
+#pragma unroll 4
+    for (int x = lane; x < TILEB / 16; x += 64) {
+      const u32x4 y = v4[x];
+#pragma unroll
+      for (int z = 0; z < 4; ++z)
+        top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, y[z] & Mm<T>::EXP));
+    }
+    const unsigned short inf = (unsigned short)(Mm<T>::EXP & 0xFFFF);
+    return __any(top[0] == inf || top[1] == inf);
+  };
+  // a tile that not every row of the block sees whole
+  auto edge = [&](int32_t kb, const lds_char *kt, const lds_char *vt) {
+    // (a wave whose rows see none of it only brings its rows)
+    const bool any = kb <= q_hi && (a.window <= 0 || q_lo - (kb + KT - 1) < a.window || kb < a.sinks);
+    if (!any) return;
+    const bool whole = kb + KT - 1 <= q_lo &&
+                       (a.window <= 0 || q_hi - kb < a.window || kb + KT <= a.sinks);
+    if (whole || !not_finite(vt)) {
+      f32x16 sc[RW][U];
+      scores(kt, sc);
+      const int vb = v_base(vt);
+#pragma unroll
+      for (int r = 0; r < RW; ++r) {
+        if (!whole) hide(sc[r], pos[r], kb);
+        settle(r, largest(sc[r]));
+      }
+#pragma unroll
+      for (int u = 0; u < 2 * U; ++u) {
+        V8 p[RW];
+#pragma unroll
+        for (int r = 0; r < RW; ++r) {
+          const float use = m[r] == -INFINITY ? 0.f : m[r];
+#pragma unroll
+          for (int x = 0; x < 8; ++x) {
+            const float y = attn_exp2(fmaf(sc[r][u >> 1][8 * (u & 1) + x], a.scale_log2, -use));
+            l[r] += y;
+            p[r][x] = (T)y;
+          }
+        }
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) {
+          const V8 v = value_piece(vb, dt, u);
+#pragma unroll
+          for (int r = 0; r < RW; ++r) acc[r][dt] = Mm<T>::mfma(v, p[r], acc[r][dt]);
+        }
+      }
+      return;
+    }
+    // a masked place must not reach a sum, and 0 * NaN is NaN: the keys one at
+    // a time, each row takes only those it sees
+    f32x16 sc[RW][U];
+    scores(kt, sc);
+#pragma unroll
+    for (int r = 0; r < RW; ++r) {
+      hide(sc[r], pos[r], kb);
+      settle(r, largest(sc[r]));
+    }
+#pragma unroll 1
+    for (int j = 0; j < KT; ++j) {
+#pragma unroll
+      for (int r = 0; r < RW; ++r) {
+        float wt = 0.f;
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int x = 0; x < 16; ++x)
+            wt = 32 * u + 8 * (x >> 2) + (x & 3) == (j & ~4) ? sc[r][u][x] : wt;
+        wt = attn_exp2(fmaf(__shfl(wt, n + 32 * ((j >> 2) & 1)), a.scale_log2,
+                            m[r] == -INFINITY ? 0.f : -m[r]));
+        if (((j >> 2) & 1) == h2) l[r] += wt;
+        const bool sees = attn_sees(a, pos[r], kb + j);
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+          for (int b = 0; b < 4; ++b) {
+            const int c = 4 * dt + b;
+            const lds_as T *v =
+                (const lds_as T *)(vt + j * ROWB + ((c ^ v_swizzle<CH>(j)) << 4)) + 4 * h2;
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+              if (sees) acc[r][dt][4 * b + x] = fmaf(wt, (float)v[x], acc[r][dt][4 * b + x]);
+            __builtin_amdgcn_sched_barrier(0);  // (few registers, not speed)
+          }
+      }
+    }
+  };
+
+  // the tiles that every row of the block sees whole: from the window's edge
+  // of the last row to the first row's diagonal
+  int32_t hot0 = first, hot1 = first;
+  {
+    const int32_t lo = p0 + row0 / a.group, hi = p0 + last / a.group;
+    int32_t x0 = span.sink_tiles;
+    if (a.window > 0 && hi - span.lo >= a.window)
+      x0 += (hi - a.window - span.lo) / KT + 1;
+    const int32_t x1 = lo + 1 > span.lo ? span.sink_tiles + (lo + 1 - span.lo) / KT : 0;
+    hot0 = x0 > first ? x0 : first;
+    hot1 = x1 < end ? x1 : end;
   }
 
-  l += __shfl_xor(l, 32);
-  if (!real) return;
-  const int64_t out_row = (s.token0 + t) * a.heads + head;
-  if (parts > 1) {
-    const int64_t r = (int64_t)part * a.tokens * a.heads + out_row;
-    float *dst = a.part_o + r * DP;
+  int kslot = 0;  // (i - first) % 3
+  if (first < end) {
+    addresses(first);
+    fetch(first, kbuf, true);
+    fetch(first, vbuf, false);
+    if (first + 1 < end) fetch(first + 1, kbuf + TILEB, true);
+  }
+  __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
+  __syncthreads();
+
+  // a step's copies: the keys of tile i + 2, the values of tile i + 1
+  auto ahead = [&](int32_t i) {
+    if (i + 2 - tb >= 64) addresses(i + 1);
+    if (i + 2 < end) fetch(i + 2, kbuf + (kslot == 0 ? 2 : kslot - 1) * TILEB, true);
+    if (i + 1 < end) fetch(i + 1, vbuf + ((i + 1 - first) & 1) * TILEB, false);
+  };
+  auto done = [&]() {
+    kslot = kslot == 2 ? 0 : kslot + 1;
+    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): the copies have arrived
+    __syncthreads();
+  };
+
+  for (int32_t i = first; i < end;) {
+    if (i < hot0 || i >= hot1) {
+      ahead(i);
+      edge(span.base(i), kbuf + kslot * TILEB, vbuf + ((i - first) & 1) * TILEB);
+      done();
+      ++i;
+      continue;
+    }
+    // A step computes the scores of the next tile and the weights and sums of
+    // this one, the products on the matrix cores beside the exponentials on
+    // the vector unit: the order below is the order they are issued in, one
+    // piece of LDS, a read four pieces ahead, and a share of the vector work
+    // at a time (left to itself the compiler keeps one read in flight).  The
+    // last step's scores are not used: what follows is an edge, or nothing.
+    constexpr int NS = U * KS, NV = 2 * U * DT, AHEAD = 4;
+    f32x16 sc[RW][U];
+    scores(kbuf + kslot * TILEB, sc);
+#pragma unroll
+    for (int r = 0; r < RW; ++r) settle(r, largest(sc[r]));
+#pragma unroll 1
+    for (; i < hot1; ++i) {
+      ahead(i);
+      const int kb = k_base(kbuf + (kslot == 2 ? 0 : kslot + 1) * TILEB);
+      const int vb = v_base(vbuf + ((i - first) & 1) * TILEB);
+      f32x16 sn[RW][U];
+      V8 f[AHEAD], p[RW][2 * U];
+      float tm[RW], use[RW];
+#pragma unroll
+      for (int r = 0; r < RW; ++r) {
+        tm[r] = -INFINITY;
+        use[r] = m[r] == -INFINITY ? 0.f : m[r];
+#pragma unroll
+        for (int u = 0; u < U; ++u) sn[r][u] = f32x16{};
+      }
+      auto piece_of = [&](int g) -> V8 {
+        return g < NS ? key_piece(kb, g / U, g % U) : value_piece(vb, (g - NS) % DT, (g - NS) / DT);
+      };
+      auto weight = [&](int r, int e) {  // of register e of the scores
+        const float y = attn_exp2(fmaf(sc[r][e >> 4][e & 15], a.scale_log2, -use[r]));
+        l[r] += y;
+        p[r][e >> 3][e & 7] = (T)y;
+      };
+#pragma unroll
+      for (int g = 0; g < AHEAD; ++g) f[g] = piece_of(g);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int g = 0; g < NS + NV; ++g) {
+        const V8 x = f[g % AHEAD];
+#pragma unroll
+        for (int r = 0; r < RW; ++r) {
+          if (g < NS)
+            sn[r][g % U] = Mm<T>::mfma(x, q[r][g / U], sn[r][g % U]);
+          else
+            acc[r][(g - NS) % DT] =
+                Mm<T>::mfma(x, p[r][(g - NS) / DT], acc[r][(g - NS) % DT]);
+          if (r == RW - 1 && g + AHEAD < NS + NV) f[g % AHEAD] = piece_of(g + AHEAD);
+          // half of the weights beside the scores, half beside the first sums
+          if (g < NS) {
+#pragma unroll
+            for (int e = 8 * U * g / NS; e < 8 * U * (g + 1) / NS; ++e) weight(r, e);
+          } else if (g - NS < NV / 2) {
+#pragma unroll
+            for (int e = 8 * U * (g - NS) / (NV / 2); e < 8 * U * (g - NS + 1) / (NV / 2); ++e)
+              weight(r, 8 * U + e);
+          } else {
+            const int z = g - NS - NV / 2;
+#pragma unroll
+            for (int e = 8 * U * z / (NV / 2); e < 8 * U * (z + 1) / (NV / 2); ++e)
+              tm[r] = max3(tm[r], sn[r][e >> 3][2 * (e & 7)], sn[r][e >> 3][2 * (e & 7) + 1]);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < RW; ++r) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) sc[r][u] = sn[r][u];
+        if (i + 1 < hot1) settle(r, xor32_max(tm[r]));
+      }
+      done();
+    }
+  }
+
+#pragma unroll
+  for (int r = 0; r < RW; ++r) {
+    const float sum = xor32_sum(l[r]);
+    const int32_t row = w0 + 32 * r + n;
+    if (row > last) continue;
+    const int32_t t = row / a.group, head = h * a.group + row - t * a.group;
+    const int64_t out_row = (s.token0 + t) * a.heads + head;
+    if (parts > 1) {
+      const int64_t x = (int64_t)part * a.tokens * a.heads + out_row;
+      float *dst = a.part_o + x * DP;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+          *reinterpret_cast<f32x4 *>(dst + 32 * dt + 8 * b + 4 * h2) =
+              f32x4{acc[r][dt][4 * b], acc[r][dt][4 * b + 1], acc[r][dt][4 * b + 2],
+                    acc[r][dt][4 * b + 3]};
+      if (h2 == 0) {
+        a.part_ml[2 * x] = m[r];
+        a.part_ml[2 * x + 1] = sum;
+      }
+      continue;
+    }
+    const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+    T *dst = static_cast<T *>(a.out) + (s.token0 + t) * a.o_row + head * a.o_head;
+    typedef __attribute__((ext_vector_type(4))) T V4;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-      for (int b = 0; b < 4; ++b)
-        *reinterpret_cast<f32x4 *>(dst + 32 * dt + 8 * b + 4 * h2) =
-            f32x4{acc[dt][4 * b], acc[dt][4 * b + 1], acc[dt][4 * b + 2], acc[dt][4 * b + 3]};
-    if (h2 == 0) {
-      a.part_ml[2 * r] = m;
-      a.part_ml[2 * r + 1] = l;
-    }
-    return;
+      for (int b = 0; b < 4; ++b) {
+        const int e = 32 * dt + 8 * b + 4 * h2;
+        V4 y;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) y[x] = (T)(acc[r][dt][4 * b + x] * inv);
+        if (e < a.d) *reinterpret_cast<V4 *>(dst + e) = y;
+      }
+    if (a.lse && h2 == 0)
+      a.lse[out_row] = sum > 0.f ? (m[r] + __log2f(sum)) * 0.6931471805599453f
+                                 : sum != sum ? sum : -INFINITY;
   }
-  const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
-  T *dst = static_cast<T *>(a.out) + (s.token0 + t) * a.o_row + head * a.o_head;
-  typedef __attribute__((ext_vector_type(4))) T V4;
-#pragma unroll
-  for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-    for (int b = 0; b < 4; ++b) {
-      const int e = 32 * dt + 8 * b + 4 * h2;
-      V4 y;
-#pragma unroll
-      for (int x = 0; x < 4; ++x) y[x] = (T)(acc[dt][4 * b + x] * inv);
-      if (e < a.d) *reinterpret_cast<V4 *>(dst + e) = y;
-    }
-  if (a.lse && h2 == 0)
-    a.lse[out_row] = l > 0.f ? (m + __log2f(l)) * 0.6931471805599453f : l != l ? l : -INFINITY;
 }
 
 template <class T> void tile_of(hipStream_t st, const AttnArgs &a, int nw, unsigned g) {
   if (a.d <= 64) {
     if (nw == 8)
-      k_attn_tile<T, 64, 8><<<g, 512, 0, st>>>(a);
+      k_attn_tile<T, 64, 8, 1><<<g, 512, 0, st>>>(a);
     else
-      k_attn_tile<T, 64, 4><<<g, 256, 0, st>>>(a);
+      k_attn_tile<T, 64, 4, 1><<<g, 256, 0, st>>>(a);
   } else if (a.d <= 128) {
     if (nw == 8)
-      k_attn_tile<T, 128, 8><<<g, 512, 0, st>>>(a);
+      k_attn_tile<T, 128, 8, 1><<<g, 512, 0, st>>>(a);
     else
-      k_attn_tile<T, 128, 4><<<g, 256, 0, st>>>(a);
+      k_attn_tile<T, 128, 4, 1><<<g, 256, 0, st>>>(a);
   } else {
-    k_attn_tile<T, 256, 4><<<g, 256, 0, st>>>(a);
+    k_attn_tile<T, 256, 4, 1><<<g, 256, 0, st>>>(a);
   }
 }
 
