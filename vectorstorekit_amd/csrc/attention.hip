@@ -14,7 +14,7 @@ int32_t padded_head(int32_t d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
 // How a call's work is divided.
 struct Plan {
   int32_t tiles, splits, chunk;
-  bool split_keys;  // attn_rows: the waves of a block share a row tile's keys
+  int32_t share;  // attn_rows: waves that take a row tile's keys in turn
   int32_t waves;    // > 0: attn_tile, so many waves a block
 };
 
@@ -42,7 +42,7 @@ Plan plan_of(const vsk_ctx *ctx, const vsk_kv *kv, const vsk_new_tokens *news,
   p.splits = 1;
   p.chunk = 1 << 30;
   p.waves = 0;
-  p.split_keys = true;
+  p.share = 4;
   int64_t row_tile = 16, key_tile = kv->dtype == VSK_DTYPE_F32 ? 16 : 32, per = 4;
   int64_t want = 8 * (int64_t)ctx->cu_count;
   if (kv->dtype != VSK_DTYPE_F32 && rows >= 64 && aligned_operands(kv, args)) {
@@ -56,8 +56,10 @@ Plan plan_of(const vsk_ctx *ctx, const vsk_kv *kv, const vsk_new_tokens *news,
   const int64_t blocks = pairs * p.tiles;
   if (p.waves == 0) {
     // row tiles enough to fill the device: a wave each
-    p.split_keys = blocks < want || p.tiles < 4;
-    if (!p.split_keys) return p;
+    if (blocks >= want && p.tiles >= 4) {
+      p.share = 1;
+      return p;
+    }
   }
   int64_t keys = kv->table ? (int64_t)kv->width * kv->page_size : kv->pages;
   if (args->max_length > 0 && args->max_length < keys) keys = args->max_length;
@@ -69,6 +71,10 @@ Plan plan_of(const vsk_ctx *ctx, const vsk_kv *kv, const vsk_new_tokens *news,
   // parts as many as keep every compute unit supplied with blocks, of at least
   // a tile for each of the four waves that share them (two tiles)
   const int64_t tiles = ceil_div(keys, key_tile);
+  if (p.waves == 0 && kv->head_dim <= 128 && tiles <= 32) {
+    p.share = 8;
+    return p;
+  }
   const int64_t target = ceil_div(want, blocks);
   const int64_t chunk = ceil_div(ceil_div(tiles, target), per) * per;
   p.chunk = (int32_t)(chunk < per ? per : chunk);
@@ -196,7 +202,7 @@ vsk_status vsk_attention(vsk_ctx *ctx, void *stream, const vsk_kv *kv, int32_t l
   if (p.waves)
     launch_attn_tile(ctx, st, a, kv->dtype, p.waves);
   else
-    launch_attn_rows(ctx, st, a, kv->dtype, al, p.split_keys);
+    launch_attn_rows(ctx, st, a, kv->dtype, al, p.share);
   launch_attn_join(ctx, st, a, kv->dtype, al, p.waves ? 32 * p.waves : 16);
   finish_queued(ctx, st);
   VSK_API_END(ctx);

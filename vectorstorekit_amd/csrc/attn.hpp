@@ -162,6 +162,37 @@ __device__ inline AttnRows attn_rows(const AttnArgs &a, const AttnSeq &s, int32_
   return r;
 }
 
+#define lds_as __attribute__((address_space(3)))
+typedef lds_as char lds_char;
+
+// 16 bytes a lane from base + off to dst + 16 * lane (base and dst the same in
+// every lane).  Written as assembly because the compiler makes every read of
+// LDS after the builtin wait for it: here a tile's copies fly while the last
+// tile is computed with, and one wait before the barrier covers them.  (M0
+// holds the destination of such loads; nothing else in these kernels uses it.)
+__device__ inline void load_to_lds(uint64_t base, uint32_t off, const lds_char *dst) {
+  const uint32_t at = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)dst);
+  asm volatile(
+      "s_mov_b32 m0, %0\n\t"
+      "s_nop 0\n\t"
+      "global_load_lds_dwordx4 %1, %2"
+      :
+      : "s"(at), "v"(off), "s"(base)
+      : "memory");
+}
+
+__device__ inline uint64_t lane_of(uint32_t lo, uint32_t hi, int i) {
+  return (uint64_t)(uint32_t)__builtin_amdgcn_readlane(hi, i) << 32 |
+         (uint32_t)__builtin_amdgcn_readlane(lo, i);
+}
+
+// A row of CH 16-byte pieces in LDS: piece c of it is in slot c ^ swizzle(row),
+// so that the rows that a quarter (half) of a wave reads the same piece of
+// meet different banks.
+template <int CH> __device__ inline int k_swizzle(int row) {
+  return CH >= 16 ? row & 15 : (row & 7) ^ ((row >> 3) & 1);
+}
+
 __device__ inline float attn_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 // Exchanges between lanes 16 and 32 apart on the vector unit: of x twice, the
 // swap of the odd rows (the upper half) of the one with the even rows (the
@@ -206,8 +237,9 @@ void finish_queued(vsk_ctx *ctx, hipStream_t stream);
 
 // launches; attn_rows.hip; t: a VSK_DTYPE; aligned: every pointer and
 // stride takes 16-byte loads (8-byte stores)
+// share: waves that take a row tile's keys in turn: 8 (heads to 128), 4, or 1
 void launch_attn_rows(vsk_ctx *ctx, hipStream_t stream, const AttnArgs &a, int32_t t,
-                      bool aligned, bool split_keys);
+                      bool aligned, int32_t share);
 // keys of a tile of attn_tile.hip, by the (padded) head
 constexpr int attn_tile_keys(int d) { return d > 128 ? 32 : 64; }
 // attn_tile.hip: 16-bit types, aligned; waves: 8 or 4 a workgroup

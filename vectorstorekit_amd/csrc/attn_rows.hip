@@ -91,14 +91,17 @@ template <class T, int VW, int NB, bool ALIGNED> struct RowTile {
   static constexpr int WV = VW / E;         // words a lane takes of a row's block
   const AttnArgs &a;
   const AttnSeq &s;
+  // (aligned) the step's keys in LDS, this wave's own
+  static constexpr int ROWB = DV * (int)sizeof(T), CH = ROWB / 16, RPI = 64 / CH;
+  lds_char *const lds;
   const int32_t h, n, g;
   int32_t pos;  // position of this lane's row, -1 if there is none
   uint32_t q[KS][4];
   f32x4 acc[NB][VW];
   float m = -INFINITY, l = 0.f;
 
-  __device__ RowTile(const AttnArgs &a_, const AttnSeq &s_, int32_t h_, int lane)
-      : a(a_), s(s_), h(h_), n(lane & 15), g(lane >> 4) {}
+  __device__ RowTile(const AttnArgs &a_, const AttnSeq &s_, int32_t h_, int lane, lds_char *l_)
+      : a(a_), s(s_), lds(l_), h(h_), n(lane & 15), g(lane >> 4) {}
 
   __device__ void begin(int32_t row) {
     const int32_t t = row / a.group;
@@ -153,49 +156,165 @@ template <class T, int VW, int NB, bool ALIGNED> struct RowTile {
     }
   }
 
-  // q_lo, q_hi: the smallest and largest position of the tile's rows
-  __device__ void step(int32_t kb, int32_t q_lo, int32_t q_hi) {
-    uint32_t k[U][KS][4], v[U][4][NB][WV];
-    AttnRows r[U];
+  // Lane i holds the addresses of 16 keys: those of part i % U of the wave's
+  // step xb + i / U.
+  uint32_t k_lo, k_hi, v_lo, v_hi;
+  int32_t xb;
+  template <class Base> __device__ void addresses(int32_t x, int32_t steps, Base &&base) {
+    xb = x;
+    const int32_t lane = threadIdx.x & 63;
+    int32_t at = x + lane / U;
+    at = at < steps ? at : steps - 1;
+    const int32_t j = attn_row16(s, base(at) + 16 * (lane % U));
+    int64_t page = 0, in = s.key0 + j;
+    if (a.table) {
+      const int32_t y = a.table[s.slot * a.table_stride + (j >> a.page_shift)];
+      page = y < 0 ? 0 : y >= a.pages ? a.pages - 1 : y;
+      in = j & ((1 << a.page_shift) - 1);
+    }
+    const uint64_t kp = (uint64_t)(uintptr_t)a.k +
+                        (int64_t)sizeof(T) * (page * a.k_page + in * a.k_row + h * a.k_head);
+    const uint64_t vp = (uint64_t)(uintptr_t)a.v +
+                        (int64_t)sizeof(T) * (page * a.v_page + in * a.v_row + h * a.v_head);
+    k_lo = (uint32_t)kp, k_hi = (uint32_t)(kp >> 32);
+    v_lo = (uint32_t)vp, v_hi = (uint32_t)(vp >> 32);
+  }
+  // rows that may be read of the 16 from j16 on, less one
+  __device__ int32_t last_of(int32_t j16) const {
+    const int32_t left = s.L - 1 - attn_row16(s, j16);
+    return left < 15 ? left : 15;
+  }
+  // The keys from L on read row L - 1, and are masked.  Aligned operands go
+  // into LDS whole rows at a time (the products' layout straight from memory
+  // is 64 accesses of 16 bytes a load where whole rows are 16 of 64).
+  __device__ void load_keys(int32_t x, int32_t kb, uint32_t (&k)[U][KS][4]) {
+    const int32_t lane = threadIdx.x & 63, piece = lane % CH, sub = lane / CH;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      r[u] = attn_rows(a, s, h, kb + 16 * u, attn_page(a, s, kb + 16 * u));
-      const T *row = static_cast<const T *>(a.k) + r[u].k +
-                     (n < r[u].last ? n : r[u].last) * (int32_t)a.k_row;
+      const uint64_t base = lane_of(k_lo, k_hi, (x - xb) * U + u);
+      const uint32_t stride = (uint32_t)a.k_row * sizeof(T), most = last_of(kb + 16 * u) * stride;
+      if constexpr (ALIGNED) {
+        const bool full = a.d == DV;
 #pragma unroll
-      for (int i = 0; i < KS; ++i) load_row<T, 4, ALIGNED>(row, (4 * i + g) * KE, a.d, k[u][i]);
+        for (int y = 0; y < 16 / RPI; ++y) {
+          const int32_t r = y * RPI + sub, c = piece ^ k_swizzle<CH>(r);
+          const uint32_t at = (uint32_t)r * stride, row = at < most ? at : most;
+          lds_char *to = lds + (16 * u + y * RPI) * ROWB;
+          if (full)
+            load_to_lds(base, row + 16 * c, to);
+          else if (c * KE < a.d)
+            load_to_lds(base, row + 16 * c, to);
+        }
+      } else {
+        const uint32_t at = (uint32_t)n * stride, row = at < most ? at : most;
+#pragma unroll
+        for (int i = 0; i < KS; ++i)
+          load_row<T, 4, false>(reinterpret_cast<const T *>(base + row), (4 * i + g) * KE, a.d,
+                                k[u][i]);
+      }
     }
+  }
+  // Elements past the head are the last ones of it: their outputs are dropped.
+  __device__ void load_values(int32_t x, int32_t kb, uint32_t (&v)[U][4][NB][WV]) {
 #pragma unroll
-    for (int u = 0; u < U; ++u)
+    for (int u = 0; u < U; ++u) {
+      const char *base =
+          reinterpret_cast<const char *>((uintptr_t)lane_of(v_lo, v_hi, (x - xb) * U + u));
+      const uint32_t stride = (uint32_t)a.v_row * sizeof(T), most = last_of(kb + 16 * u) * stride;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const T *row = v_row(r[u], 4 * g + i);
+        const uint32_t at = (uint32_t)(4 * g + i) * stride, row = at < most ? at : most;
 #pragma unroll
-        for (int b = 0; b < NB; ++b)
-          load_row<T, WV, ALIGNED>(row, (16 * b + n) * VW, a.d, v[u][i][b]);
+        for (int b = 0; b < NB; ++b) {
+          const int32_t e = (16 * b + n) * VW;
+          if constexpr (ALIGNED) {
+            typedef __attribute__((ext_vector_type(WV))) uint32_t V;
+            const uint32_t in = sizeof(T) * (e < a.d ? e : a.d - VW);
+            const V y = *reinterpret_cast<const V *>(base + (row + in));
+#pragma unroll
+            for (int z = 0; z < WV; ++z) v[u][i][b][z] = y[z];
+          } else {
+            load_row<T, WV, false>(reinterpret_cast<const T *>(base + row), e, a.d, v[u][i][b]);
+          }
+        }
       }
-    f32x4 sc[U];
+    }
+  }
+
+  // The steps of a wave, `steps` of them, step x at key base(x).  q_lo, q_hi:
+  // the smallest and largest position of the tile's rows.  The next step's
+  // keys are asked for as soon as this one's are in the products, its values
+  // likewise: there are always loads in flight.
+  template <class Base>
+  __device__ void walk(int32_t steps, int32_t q_lo, int32_t q_hi, Base &&base) {
+    if (steps <= 0) return;
+    if (ALIGNED && a.d < DV) {
+      // pieces past the head are never loaded: they stay zero
+      lds_as u32x4 *z = (lds_as u32x4 *)lds;
+      for (int i = threadIdx.x & 63; i < KT * CH; i += 64) z[i] = u32x4{0, 0, 0, 0};
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    }
+    uint32_t k[U][KS][4], v[U][4][NB][WV];
+    addresses(0, steps, base);
+    int32_t kb = base(0);
+    load_keys(0, kb, k);
+    __builtin_amdgcn_sched_barrier(0);
+    load_values(0, kb, v);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll 1
+    for (int32_t x = 0;;) {
+      f32x4 sc[U];
+      // the step's keys have arrived (its values, asked for later, may not)
+      if constexpr (ALIGNED) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(4 * U * NB) : "memory");
+      scores(k, sc);
+      __builtin_amdgcn_sched_barrier(0);
+      const bool more = x + 1 < steps;
+      const int32_t nb = more ? base(x + 1) : 0;
+      if (more) {
+        if (x + 1 - xb >= 64 / U) addresses(x + 1, steps, base);
+        load_keys(x + 1, nb, k);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      float p[U][4];
+      // every row sees every key of most tiles
+      const bool whole = kb + KT - 1 <= q_lo &&
+                         (a.window <= 0 || q_hi - kb < a.window || kb + KT <= a.sinks);
+      weights(kb, whole, sc, p);
+      if (whole || !edge(kb, q_lo, q_hi, p, v)) weigh(p, v);
+      __builtin_amdgcn_sched_barrier(0);
+      if (!more) break;
+      load_values(++x, nb, v);
+      __builtin_amdgcn_sched_barrier(0);
+      kb = nb;
+    }
+  }
+
+  __device__ void scores(const uint32_t (&k)[U][KS][4], f32x4 (&sc)[U]) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       sc[u] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int i = 0; i < KS; ++i) {
+        u32x4 x;
+        if constexpr (ALIGNED)
+          x = *(const lds_as u32x4 *)(lds + (16 * u + n) * ROWB +
+                                      (((4 * i + g) ^ k_swizzle<CH>(n)) << 4));
+        else
+          x = u32x4{k[u][i][0], k[u][i][1], k[u][i][2], k[u][i][3]};
+        const u32x4 y = {q[i][0], q[i][1], q[i][2], q[i][3]};
         if constexpr (F32) {
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            sc[u] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, k[u][i][e]),
-                                                         __builtin_bit_cast(float, q[i][e]), sc[u],
-                                                         0, 0, 0);
+            sc[u] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(x[e]),
+                                                         __uint_as_float(y[e]), sc[u], 0, 0, 0);
         } else {
-          const u32x4 x = {k[u][i][0], k[u][i][1], k[u][i][2], k[u][i][3]};
-          const u32x4 y = {q[i][0], q[i][1], q[i][2], q[i][3]};
           sc[u] = Elem<T>::mfma(x, __builtin_bit_cast(typename Elem<T>::V8, y), sc[u]);
         }
       }
     }
-    // every row sees every key of most tiles
-    const bool whole = kb + KT - 1 <= q_lo &&
-                       (a.window <= 0 || q_hi - kb < a.window || kb + KT <= a.sinks);
+  }
+
+  __device__ void weights(int32_t kb, bool whole, f32x4 (&sc)[U], float (&p)[U][4]) {
     if (!whole) {
 #pragma unroll
       for (int u = 0; u < U; ++u)
@@ -211,7 +330,6 @@ template <class T, int VW, int NB, bool ALIGNED> struct RowTile {
     const float fade = attn_exp2(m - use);
     m = top;
     l *= fade;
-    float p[U][4];
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
@@ -223,20 +341,14 @@ template <class T, int VW, int NB, bool ALIGNED> struct RowTile {
     for (int b = 0; b < NB; ++b)
 #pragma unroll
       for (int t = 0; t < VW; ++t) acc[b][t] *= fade;
-    if (!whole && edge(r, kb, q_lo, q_hi, p, v)) return;
-    weigh(p, v);
   }
-  __device__ const T *v_row(const AttnRows &r, int32_t at) const {
-    return static_cast<const T *>(a.v) + r.v + (at < r.last ? at : r.last) * (int32_t)a.v_row;
-  }
-
   // A tile that not every row sees whole: what a masked place holds (memory
   // never written, for one) must not reach a sum, and 0 * NaN is NaN.  Rows of
   // V that no query row sees are cleared; if one that some rows see and some
   // do not is not finite, its keys go one at a time and each row takes only
   // those it sees (returns true).
-  __device__ bool edge(const AttnRows (&r)[U], int32_t kb, int32_t q_lo, int32_t q_hi,
-                       const float (&p)[U][4], uint32_t (&v)[U][4][NB][WV]) {
+  __device__ bool edge(int32_t kb, int32_t q_lo, int32_t q_hi, const float (&p)[U][4],
+                       uint32_t (&v)[U][4][NB][WV]) {
     bool odd = false;
 #pragma unroll
     for (int u = 0; u < U; ++u)
@@ -255,24 +367,22 @@ template <class T, int VW, int NB, bool ALIGNED> struct RowTile {
           }
       }
     if (q_lo == q_hi || !__any(odd)) return false;
-    one_by_one(r, kb, p);
+    one_by_one(kb, p);
     return true;
   }
-  __device__ void one_by_one(const AttnRows (&r)[U], int32_t kb, const float (&p)[U][4]) {
+  __device__ void one_by_one(int32_t kb, const float (&p)[U][4]) {
 #pragma unroll 1
     for (int32_t j = 0; j < KT; ++j) {
-      const int32_t at = j & 15;
+      const int32_t at = j & 15, j16 = kb + (j & 16);
       float w = 0.f;
-      AttnRows rr = r[0];
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (u == j >> 4) rr = r[u];
+      for (int u = 0; u < U; ++u)
 #pragma unroll
         for (int i = 0; i < 4; ++i) w = 16 * u + i == (j & ~12) ? p[u][i] : w;
-      }
       w = __shfl(w, n + 16 * (at >> 2));
+      const AttnRows r = attn_rows(a, s, h, j16, attn_page(a, s, j16));
       if (!attn_sees(a, pos, kb + j)) continue;
-      const T *row = v_row(rr, at);
+      const T *row = static_cast<const T *>(a.v) + r.v + (at < r.last ? at : r.last) * a.v_row;
 #pragma unroll
       for (int b = 0; b < NB; ++b)
 #pragma unroll
@@ -286,9 +396,9 @@ template <class T, int VW, int NB, bool ALIGNED> struct RowTile {
   }
 };
 
-// waves a SIMD, by the registers that the loads of a step take
+// waves a SIMD, by the registers that the values of a step and the sums take
 template <class T> constexpr int row_waves(int elems) {
-  return elems * (int)sizeof(T) < 16 ? 4 : elems * (int)sizeof(T) <= 16 ? 3 : elems * (int)sizeof(T) <= 32 ? 2 : 1;
+  return elems * (int)sizeof(T) <= 8 ? 4 : elems * (int)sizeof(T) <= 16 ? 3 : sizeof(T) == 4 && elems == 8 ? 2 : 1;
 }
 
 template <class T> __device__ inline void store4(T *dst, const float (&x)[4], int32_t left) {
@@ -302,9 +412,11 @@ template <class T> __device__ inline void store4(T *dst, const float (&x)[4], in
 }
 
 // One block: a row tile of one sequence and key head, over one part of its
-// keys that the four waves share (KSPLIT), or four row tiles, a wave each.
-template <class T, int VW, int NB, bool KSPLIT, bool ALIGNED>
-__global__ __launch_bounds__(256, row_waves<T>(VW * NB)) void
+// keys that the block's SHARE waves take in turn, or (SHARE 1) four row tiles,
+// a wave each.
+template <class T, int VW, int NB, int SHARE, bool ALIGNED>
+__global__ __launch_bounds__(SHARE > 4 ? 64 * SHARE : 256,
+                             SHARE > 4 ? SHARE / 4 : row_waves<T>(VW * NB)) void
 k_attn_rows(const AttnArgs a) {
   typedef RowTile<T, VW, NB, ALIGNED> Tile;
   constexpr int DV = Tile::DV;
@@ -314,37 +426,40 @@ k_attn_rows(const AttnArgs a) {
   uint32_t at = blockIdx.x;
   const int32_t h = at % a.kv_heads;
   at /= a.kv_heads;
-  const int32_t groups = KSPLIT ? a.tiles : (a.tiles + 3) / 4;
+  const int32_t groups = SHARE > 1 ? a.tiles : (a.tiles + 3) / 4;
   // (the last tiles see the most keys: they go first)
   const int32_t tg = groups - 1 - (int32_t)(at % groups);
   at /= groups;
   const int32_t part = at % a.splits;
   const AttnSeq s = attn_seq(a, at / a.splits);
-  const int32_t tile = KSPLIT ? tg : 4 * tg + w;
+  const int32_t tile = SHARE > 1 ? tg : 4 * tg + w;
   const int32_t row0 = tile * ROWS;
   const int32_t T_used = s.T < a.max_new ? s.T : a.max_new;
   const int32_t rows_all = T_used * a.group;
   const bool have = row0 < rows_all;
-  if (KSPLIT ? !have : 4 * tg * ROWS >= rows_all) return;
+  if (SHARE > 1 ? !have : 4 * tg * ROWS >= rows_all) return;
   const int32_t rows = !have ? 0 : rows_all - row0 < ROWS ? rows_all - row0 : ROWS;
   const int32_t t_lo = row0 / a.group, t_hi = (row0 + rows - 1) / a.group;
   const int32_t q_lo = s.L - s.T + t_lo, q_hi = s.L - s.T + t_hi;
   const auto span = attn_span<Tile::KT>(a, q_lo, have ? q_hi : -1);
   const int32_t parts = attn_parts(a, span.tiles);
   if (part >= parts) return;
-  const int32_t first = part * a.chunk;
-  const int32_t end = part == parts - 1 ? span.tiles : first + a.chunk;
+  const int32_t first = part * a.chunk + (SHARE > 1 ? w : 0);
+  const int32_t end = part == parts - 1 ? span.tiles : (part + 1) * a.chunk;
 
-  Tile tl(a, s, h, lane);
+  // the waves' keys and, after them, their sums: four waves' at a time
+  constexpr int SLOTS = 4, SUMB = SHARE > 1 ? SLOTS * ROWS * (DV + 4) * 4 : 0;
+  constexpr int KEYB = ALIGNED ? (SHARE > 4 ? SHARE : 4) * Tile::KT * Tile::ROWB : 16;
+  __shared__ __attribute__((aligned(1024))) char pool[KEYB > SUMB ? KEYB : SUMB];
+  Tile tl(a, s, h, lane, (lds_char *)pool + (ALIGNED ? w * Tile::KT * Tile::ROWB : 0));
   tl.begin(have ? row0 + tl.n : 0x3fffffff);
-  if (have)
-    for (int32_t t = KSPLIT ? first + w : first; t < end; t += KSPLIT ? 4 : 1)
-      tl.step(span.base(t), q_lo, q_hi);
+  tl.walk((end - first + SHARE - 1) / SHARE, q_lo, q_hi,
+          [&](int32_t x) { return span.base(first + SHARE * x); });
   tl.l = xor16_32_sum(tl.l);
 
   const bool partial = parts > 1;
   const int64_t row_of = (int64_t)part * a.tokens * a.heads;
-  if constexpr (!KSPLIT) {
+  if constexpr (SHARE == 1) {
     if (tl.n < rows) {
       const int32_t r = row0 + tl.n;
       const int64_t token = s.token0 + r / a.group;
@@ -375,51 +490,56 @@ k_attn_rows(const AttnArgs a) {
                        : tl.l != tl.l ? tl.l : -INFINITY;
     }
   } else {
-    __shared__ __attribute__((aligned(16))) float so[4][ROWS][DV + 4];
-    __shared__ float sm[4][ROWS], sl[4][ROWS];
+    typedef float Sums[ROWS][DV + 4];
+    Sums *so = reinterpret_cast<Sums *>(pool);
+    __shared__ float sm[SHARE][ROWS], sl[SHARE][ROWS];
     if (tl.g == 0) sm[w][tl.n] = tl.m, sl[w][tl.n] = tl.l;
     __syncthreads();
     float top = -INFINITY, sum = 0.f;
 #pragma unroll
-    for (int x = 0; x < 4; ++x) top = fmaxf(top, sm[x][tl.n]);
+    for (int x = 0; x < SHARE; ++x) top = fmaxf(top, sm[x][tl.n]);
     const float use = top == -INFINITY ? 0.f : top;
 #pragma unroll
-    for (int x = 0; x < 4; ++x) sum += sl[x][tl.n] * attn_exp2(sm[x][tl.n] - use);
+    for (int x = 0; x < SHARE; ++x) sum += sl[x][tl.n] * attn_exp2(sm[x][tl.n] - use);
     // rows of a part: the sums as they are; of the whole: the quotient
     float f = attn_exp2(tl.m - use);
     if (!partial) f *= sum > 0.f || sum != sum ? 1.f / sum : 0.f;
-    if (tl.n < rows) {
 #pragma unroll
-      for (int b = 0; b < NB; ++b)
+    for (int turn = 0; turn < (SHARE + SLOTS - 1) / SLOTS; ++turn) {
+      if (w / SLOTS == turn && tl.n < rows) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int b = 0; b < NB; ++b)
 #pragma unroll
-          for (int t = 0; t < VW; t += 4) {
-            f32x4 x;
+          for (int i = 0; i < 4; ++i)
 #pragma unroll
-            for (int y = 0; y < 4; ++y) x[y] = tl.acc[b][t + y][i] * f;
-            *reinterpret_cast<f32x4 *>(
-                &so[w][tl.n][16 * VW * b + VW * (4 * tl.g + i) + t]) = x;
-          }
-      if (w == 0 && tl.g == 0) {
-        const int32_t r = row0 + tl.n;
-        const int64_t row = (s.token0 + r / a.group) * a.heads + h * a.group + r % a.group;
-        if (partial) {
-          a.part_ml[2 * (row_of + row)] = top;
-          a.part_ml[2 * (row_of + row) + 1] = sum;
-        } else if (a.lse) {
-          a.lse[row] = sum > 0.f ? (top + __log2f(sum)) * 0.6931471805599453f
-                                 : sum != sum ? sum : -INFINITY;
-        }
+            for (int t = 0; t < VW; t += 4) {
+              f32x4 x;
+#pragma unroll
+              for (int y = 0; y < 4; ++y) x[y] = tl.acc[b][t + y][i] * f;
+              f32x4 *to = reinterpret_cast<f32x4 *>(
+                  &so[w % SLOTS][tl.n][16 * VW * b + VW * (4 * tl.g + i) + t]);
+              *to = turn ? *to + x : x;
+            }
+      }
+      __syncthreads();
+    }
+    if (w == 0 && tl.g == 0 && tl.n < rows) {
+      const int32_t r = row0 + tl.n;
+      const int64_t row = (s.token0 + r / a.group) * a.heads + h * a.group + r % a.group;
+      if (partial) {
+        a.part_ml[2 * (row_of + row)] = top;
+        a.part_ml[2 * (row_of + row) + 1] = sum;
+      } else if (a.lse) {
+        a.lse[row] = sum > 0.f ? (top + __log2f(sum)) * 0.6931471805599453f
+                               : sum != sum ? sum : -INFINITY;
       }
     }
-    __syncthreads();
-    for (int32_t x = threadIdx.x; x < rows * (DV / 4); x += 256) {
+    for (int32_t x = threadIdx.x; x < rows * (DV / 4); x += 64 * SHARE) {
       const int32_t rr = x / (DV / 4), e = 4 * (x % (DV / 4));
       if (e >= a.d) continue;
       f32x4 y = *reinterpret_cast<f32x4 *>(&so[0][rr][e]);
 #pragma unroll
-      for (int z = 1; z < 4; ++z) y += *reinterpret_cast<f32x4 *>(&so[z][rr][e]);
+      for (int z = 1; z < SLOTS; ++z) y += *reinterpret_cast<f32x4 *>(&so[z][rr][e]);
       const int32_t r = row0 + rr;
       const int64_t token = s.token0 + r / a.group;
       const int32_t head = h * a.group + r % a.group;
@@ -503,50 +623,58 @@ __global__ __launch_bounds__(256) void k_attn_join(const AttnArgs a, const int32
 }
 
 template <class T, int VW, int NB>
-void rows_of(hipStream_t st, const AttnArgs &a, bool aligned, bool split, unsigned grid) {
-  if (split) {
+void rows_of(hipStream_t st, const AttnArgs &a, bool aligned, int32_t share, unsigned grid) {
+  if (share == 8) {
+    // (a head of 256 takes the registers of a wave a SIMD)
+    if constexpr (16 * VW * NB <= 128) {
+      if (aligned)
+        k_attn_rows<T, VW, NB, 8, true><<<grid, 512, 0, st>>>(a);
+      else
+        k_attn_rows<T, VW, NB, 8, false><<<grid, 512, 0, st>>>(a);
+    }
+  } else if (share == 4) {
     if (aligned)
-      k_attn_rows<T, VW, NB, true, true><<<grid, 256, 0, st>>>(a);
+      k_attn_rows<T, VW, NB, 4, true><<<grid, 256, 0, st>>>(a);
     else
-      k_attn_rows<T, VW, NB, true, false><<<grid, 256, 0, st>>>(a);
+      k_attn_rows<T, VW, NB, 4, false><<<grid, 256, 0, st>>>(a);
   } else {
     if (aligned)
-      k_attn_rows<T, VW, NB, false, true><<<grid, 256, 0, st>>>(a);
+      k_attn_rows<T, VW, NB, 1, true><<<grid, 256, 0, st>>>(a);
     else
-      k_attn_rows<T, VW, NB, false, false><<<grid, 256, 0, st>>>(a);
+      k_attn_rows<T, VW, NB, 1, false><<<grid, 256, 0, st>>>(a);
   }
 }
 
 }  // namespace
 
 void launch_attn_rows(vsk_ctx *ctx, hipStream_t st, const AttnArgs &a, int32_t t, bool aligned,
-                      bool split) {
-  const int64_t groups = split ? a.tiles : (a.tiles + 3) / 4;
+                      int32_t share) {
+  const int64_t groups = share > 1 ? a.tiles : (a.tiles + 3) / 4;
   const int64_t grid = (int64_t)a.n * a.splits * groups * a.kv_heads;
   VSK_REQUIRE(grid <= 0x7FFFFFFFll, VSK_ERR_INVALID_BUFFER_SIZE, "too many query rows in one call");
   const unsigned g = (unsigned)grid;
   KernelTimer kt(ctx, "attn_rows", (double)a.tokens * a.heads, st);
   if (t == VSK_DTYPE_F32) {
     if (a.d <= 64)
-      rows_of<float, 4, 1>(st, a, aligned, split, g);
+      rows_of<float, 4, 1>(st, a, aligned, share, g);
     else if (a.d <= 128)
-      rows_of<float, 4, 2>(st, a, aligned, split, g);
+      rows_of<float, 4, 2>(st, a, aligned, share, g);
     else
-      rows_of<float, 4, 4>(st, a, aligned, split, g);
+      rows_of<float, 4, 4>(st, a, aligned, share, g);
   } else if (t == VSK_DTYPE_F16) {
     if (a.d <= 64)
-      rows_of<_Float16, 4, 1>(st, a, aligned, split, g);
+      rows_of<_Float16, 4, 1>(st, a, aligned, share, g);
     else if (a.d <= 128)
-      rows_of<_Float16, 8, 1>(st, a, aligned, split, g);
+      rows_of<_Float16, 8, 1>(st, a, aligned, share, g);
     else
-      rows_of<_Float16, 8, 2>(st, a, aligned, split, g);
+      rows_of<_Float16, 8, 2>(st, a, aligned, share, g);
   } else {
     if (a.d <= 64)
-      rows_of<__bf16, 4, 1>(st, a, aligned, split, g);
+      rows_of<__bf16, 4, 1>(st, a, aligned, share, g);
     else if (a.d <= 128)
-      rows_of<__bf16, 8, 1>(st, a, aligned, split, g);
+      rows_of<__bf16, 8, 1>(st, a, aligned, share, g);
     else
-      rows_of<__bf16, 8, 2>(st, a, aligned, split, g);
+      rows_of<__bf16, 8, 2>(st, a, aligned, share, g);
   }
   check_launch("attn_rows");
 }

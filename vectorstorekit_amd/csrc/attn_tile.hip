@@ -23,9 +23,6 @@ namespace {
 
 
 typedef __attribute__((ext_vector_type(4))) short i16x4;
-#define lds_as __attribute__((address_space(3)))
-typedef lds_as char lds_char;
-
 template <class T> struct Mm;
 template <> struct Mm<__bf16> {
   typedef bf16x8 V8;
@@ -42,36 +39,11 @@ template <> struct Mm<_Float16> {
   }
 };
 
-// The slot of a row's 16-byte piece c is c ^ swizzle(row).  K: the eight
-// (sixteen) rows that a quarter (half) of a wave reads the same piece of go to
-// different slots; V: the four rows of a transposing read.
-template <int CH> __device__ inline int k_swizzle(int row) {
-  return CH >= 16 ? row & 15 : (row & 7) ^ ((row >> 3) & 1);
-}
+// V's pieces in LDS: the four rows of a transposing read go to different
+// banks (K's: attn.hpp).
 template <int CH> __device__ inline int v_swizzle(int row) {
   const int x = row & 3;
   return CH >= 16 ? 4 * x + 2 * (x >> 1) : 2 * x;
-}
-
-// 16 bytes a lane from base + off to dst + 16 * lane (base and dst the same in
-// every lane).  Written as assembly because the compiler makes every read of
-// LDS after the builtin wait for it: here a tile's copies fly while the last
-// tile is computed with, and one wait before the barrier covers them.  (M0
-// holds the destination of such loads; nothing else in these kernels uses it.)
-__device__ inline void load_to_lds(uint64_t base, uint32_t off, const lds_char *dst) {
-  const uint32_t at = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)dst);
-  asm volatile(
-      "s_mov_b32 m0, %0\n\t"
-      "s_nop 0\n\t"
-      "global_load_lds_dwordx4 %1, %2"
-      :
-      : "s"(at), "v"(off), "s"(base)
-      : "memory");
-}
-
-__device__ inline uint64_t lane_of(uint32_t lo, uint32_t hi, int i) {
-  return (uint64_t)(uint32_t)__builtin_amdgcn_readlane(hi, i) << 32 |
-         (uint32_t)__builtin_amdgcn_readlane(lo, i);
 }
 
 // (fmaxf would first quiet each product, an instruction a value: the maximum
@@ -84,7 +56,7 @@ __device__ inline float max3(float a, float b, float c) {
 
 // RW: row tiles (of 32) of a wave.
 template <class T, int DP, int NW, int RW>
-__global__ __launch_bounds__(64 * NW, 2) void k_attn_tile(const AttnArgs a) {
+__global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void k_attn_tile(const AttnArgs a) {
   typedef typename Mm<T>::V8 V8;
   constexpr int KT = attn_tile_keys(DP), U = KT / 32;
   constexpr int CH = DP / 8;         // 16-byte pieces of a row
