@@ -44,19 +44,21 @@ Plan plan_of(const vsk_ctx *ctx, const vsk_kv *kv, const vsk_new_tokens *news,
   p.waves = 0;
   p.share = 4;
   int64_t row_tile = 16, key_tile = kv->dtype == VSK_DTYPE_F32 ? 16 : 32, per = 4;
-  int64_t want = 8 * (int64_t)ctx->cu_count;
+  // blocks that a compute unit holds at once (by their registers), twice over
+  // (a head of 256: once): fewer leave it idle at the end, more start too often
+  int64_t want = (kv->head_dim <= 64 ? 8 : kv->head_dim <= 128 ? 6 : 1) * (int64_t)ctx->cu_count;
   if (kv->dtype != VSK_DTYPE_F32 && rows >= 64 && aligned_operands(kv, args)) {
     p.waves = kv->head_dim > 128 || pairs * ceil_div(rows, 256) < ctx->cu_count ? 4 : 8;
     row_tile = 32 * p.waves;
     key_tile = attn_tile_keys(kv->head_dim);
-    per = 2;
+    per = 16;
     want = ctx->cu_count;
   }
   p.tiles = (int32_t)ceil_div(rows, row_tile);
   const int64_t blocks = pairs * p.tiles;
   if (p.waves == 0) {
     // row tiles enough to fill the device: a wave each
-    if (blocks >= want && p.tiles >= 4) {
+    if (blocks >= 8 * (int64_t)ctx->cu_count && p.tiles >= 4) {
       p.share = 1;
       return p;
     }
@@ -69,9 +71,11 @@ Plan plan_of(const vsk_ctx *ctx, const vsk_kv *kv, const vsk_new_tokens *news,
     if (seen < keys) keys = seen;
   }
   // parts as many as keep every compute unit supplied with blocks, of at least
-  // a tile for each of the four waves that share them (two tiles)
+  // a tile for each of the four waves that share them (16 tiles: joining a
+  // prompt's rows takes as long as some steps)
   const int64_t tiles = ceil_div(keys, key_tile);
-  if (p.waves == 0 && kv->head_dim <= 128 && tiles <= 32) {
+  if (p.waves == 0 && kv->head_dim <= 128 &&
+      tiles <= (blocks < ctx->cu_count ? 32 : 64)) {
     p.share = 8;
     return p;
   }

@@ -110,8 +110,24 @@ template <class T, int VW, int NB, bool ALIGNED> struct RowTile {
     const T *src = static_cast<const T *>(a.q) +
                    (real ? (s.token0 + t) * a.q_row + (h * a.group + row % a.group) * a.q_head : 0);
 #pragma unroll
-    for (int i = 0; i < KS; ++i)
-      load_row<T, 4, ALIGNED>(src, (4 * i + g) * KE, real ? a.d : 0, q[i]);
+    for (int i = 0; i < KS; ++i) {
+      const int32_t e = (4 * i + g) * KE;
+      if constexpr (ALIGNED) {
+        // (all of them in flight at once: no branch around any)
+        const u32x4 y = *reinterpret_cast<const u32x4 *>(src + (e < a.d ? e : a.d - KE));
+#pragma unroll
+        for (int z = 0; z < 4; ++z) q[i][z] = y[z];
+      } else {
+        load_row<T, 4, false>(src, e, real ? a.d : 0, q[i]);
+      }
+    }
+    if constexpr (ALIGNED) {
+#pragma unroll
+      for (int i = 0; i < KS; ++i)
+#pragma unroll
+        for (int z = 0; z < 4; ++z)
+          q[i][z] = real && (4 * i + g) * KE < a.d ? q[i][z] : 0u;
+    }
 #pragma unroll
     for (int b = 0; b < NB; ++b)
 #pragma unroll
@@ -572,6 +588,17 @@ __global__ __launch_bounds__(256) void k_attn_join(const AttnArgs a, const int32
   const AttnSeq s = attn_seq(a, blockIdx.x / per);
   const int32_t x = blockIdx.x % per, t = x / a.heads, head = x % a.heads;
   if (t >= s.T) return;
+  const int64_t stride = a.tokens * a.heads;
+  const int64_t at = (s.token0 + t) * a.heads + head;
+  // the first parts are asked for before it is known how many there are
+  const int e = 4 * (threadIdx.x % LANES), way = threadIdx.x / LANES;
+  const int32_t i0 = threadIdx.x & 63;
+  const int32_t w0 = way < a.splits ? way : 0;
+  const int32_t l0 = i0 < a.splits ? i0 : 0;
+  const float m0 = a.part_ml[2 * (l0 * stride + at)];
+  const int64_t r0 = w0 * stride + at;
+  const float fm0 = a.part_ml[2 * r0], fl0 = a.part_ml[2 * r0 + 1];
+  const f32x4 o0 = *reinterpret_cast<const f32x4 *>(a.part_o + r0 * DV + (e < a.d ? e : 0));
   // the parts of the row tile that computed this row
   const int32_t h = head / a.group, row = t * a.group + head - h * a.group;
   const int32_t row0 = row / RT * RT;
@@ -581,18 +608,21 @@ __global__ __launch_bounds__(256) void k_attn_join(const AttnArgs a, const int32
   const AttnSpan<KTILE> span = attn_span<KTILE>(a, p0 + row0 / a.group, p0 + last / a.group);
   const int32_t parts = attn_parts(a, span.tiles);
   if (parts == 1) return;  // written by the row tile itself
-  const int64_t stride = a.tokens * a.heads;
-  const int64_t at = (s.token0 + t) * a.heads + head;
-  float top = -INFINITY;
-  for (int32_t i = threadIdx.x & 63; i < parts; i += 64)
+  float top = i0 < parts ? m0 : -INFINITY;
+  for (int32_t i = i0 + 64; i < parts; i += 64)
     top = fmaxf(top, a.part_ml[2 * (i * stride + at)]);
-  for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+  for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+  top = xor16_32_max(top);
   const float use = top == -INFINITY ? 0.f : top;
-  const int e = 4 * (threadIdx.x % LANES), way = threadIdx.x / LANES;
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
   float sum = 0.f;
+  if (way < parts) {
+    const float f = attn_exp2(fm0 - use);
+    sum = f * fl0;
+    o = f * o0;
+  }
 #pragma unroll 4
-  for (int32_t i = way; i < parts; i += WAYS) {
+  for (int32_t i = way + WAYS; i < parts; i += WAYS) {
     const int64_t r = i * stride + at;
     const float f = attn_exp2(a.part_ml[2 * r] - use);
     sum += f * a.part_ml[2 * r + 1];

@@ -109,10 +109,12 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void k_attn_tile(const 
     const T *src = static_cast<const T *>(a.q) + (real ? (s.token0 + t) * a.q_row + head * a.q_head : 0);
 #pragma unroll
     for (int i = 0; i < KS; ++i) {
-      q[r][i] = V8{};
-      if (real && 16 * i + 8 * h2 < a.d)
-        q[r][i] = *reinterpret_cast<const V8 *>(src + 16 * i + 8 * h2);
+      const int e = 16 * i + 8 * h2;  // (no branch around a load: all are in flight)
+      q[r][i] = *reinterpret_cast<const V8 *>(src + (e < a.d ? e : a.d - 8));
     }
+#pragma unroll
+    for (int i = 0; i < KS; ++i)
+      if (!real || 16 * i + 8 * h2 >= a.d) q[r][i] = V8{};
   }
   if (a.d < DP) {
     // pieces past the head are never loaded: they stay zero

@@ -20,6 +20,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import struct
 
 import numpy as np
 import torch
@@ -31,8 +32,25 @@ from .engine import Context
 _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 
 
+# The call's structures as bytes: a decoder makes these calls dozens of times a
+# token, and setting a ctypes structure's fields takes several times as long.
+# Layouts: vsk_head_rows, vsk_new_tokens and vsk_attention_args of vsk_hip.h.
+_ROWS = struct.Struct("@QQqqqqixxxx")
+_NEWS = struct.Struct("@QQiiq")
+_ATTEND = struct.Struct("@QQqqqqixxxxQQQqfiii")
+assert _ATTEND.size == ctypes.sizeof(_lib.vsk_attention_args)
+assert _ROWS.size == ctypes.sizeof(_lib.vsk_head_rows)
+assert _NEWS.size == ctypes.sizeof(_lib.vsk_new_tokens)
+
+
 def _stream(device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    return torch._C._cuda_getCurrentRawStream(device.index or 0)
+
+
+def _empty(x):
+    """An uninitialised dense tensor like x."""
+    return torch.empty_like(x) if x.is_contiguous() else torch.empty(x.shape, dtype=x.dtype,
+                                                                     device=x.device)
 
 
 def _tensor(x, name, dtype=None, dims=None):
@@ -61,13 +79,10 @@ def _ints(x, name, device):
     return torch.from_numpy(a.astype(np.int32)).to(device)
 
 
-def _rows(src, dst):
-    r = _lib.vsk_head_rows()
-    r.src, r.src_row, r.src_head = src.data_ptr(), src.stride(0), src.stride(1)
-    if dst is not None:
-        r.dst, r.dst_row, r.dst_head = dst.data_ptr(), dst.stride(0), dst.stride(1)
-    r.heads = src.shape[1]
-    return r
+def _rows(src, dst=None):
+    x, y = src.stride(), dst.stride() if dst is not None else (0, 0)
+    return _ROWS.pack(src.data_ptr(), dst.data_ptr() if dst is not None else 0, x[0], x[1], y[0],
+                      y[1], src.shape[1])
 
 
 class RotaryEmbedding:
@@ -183,43 +198,44 @@ class RotaryEmbedding:
             outs = tensors
         else:
             tensors = [_dense_heads(x, "q") for x in tensors]
-            outs = [torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in tensors]
+            outs = [_empty(x) for x in tensors]
         if q.shape[0] and all(x.shape[1] for x in tensors):
-            rows = (_lib.vsk_head_rows * len(tensors))(*map(_rows, tensors, outs))
+            rows = b"".join(map(_rows, tensors, outs))
             self.ctx.check(self.ctx.lib.vsk_rotary_apply(
                 self.ctx.handle, _stream(q.device), self.handle, _TYPES[q.dtype], self.head_dim,
                 q.shape[0], positions.data_ptr(), 1 if inverse else 0, rows, len(tensors)))
         return outs[0] if k is None else tuple(outs)
 
 
-def _attend(ctx, kv, layer, q, news, k_starts, scale, window, sinks, max_length, out, lse):
+def _attend(ctx, kv, layer, q, news, k_starts, scale, window, sinks, max_length, return_lse):
     """The checked call of vsk_attention."""
-    head_dim = q.shape[2]
-    a = _lib.vsk_attention_args()
-    a.scale = head_dim ** -0.5 if scale is None else float(scale)
     if window is not None and window < 1:
         raise VSKError(-2, "window must be at least 1 (None: no window)")
     if sinks < 0:
         raise VSKError(-2, "sinks must not be negative")
-    a.window, a.sinks = int(window or 0), int(sinks)
-    a.max_length = int(max_length or 0)
-    a.q = _rows(q, out)
-    a.lse = lse.data_ptr() if lse is not None else None
-    a.k_starts = k_starts
-    need = ctx.lib.vsk_attention_workspace(ctx.handle, kv, ctypes.byref(news), ctypes.byref(a))
-    if need:
+    out, x = _empty(q), q.stride()
+    lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device) if return_lse else None
+    heads, y = q.shape[1], out.stride()
+    lib, handle, work, need = ctx.lib, ctx.handle, None, 0
+    scale = q.shape[2] ** -0.5 if scale is None else float(scale)
+    window, max_length = window or 0, max_length or 0
+    if max(window, sinks, max_length) >= 1 << 31:
+        raise VSKError(-9, "window, sinks and max_length are 32-bit")
+    while True:
+        a = _ATTEND.pack(q.data_ptr(), out.data_ptr(), x[0], x[1], y[0], y[1], heads,
+                         lse.data_ptr() if return_lse else 0, k_starts,
+                         work.data_ptr() if need else 0, need,
+                         scale, window, sinks, max_length)
+        if need:
+            break
+        need = lib.vsk_attention_workspace(handle, kv, news, a)
+        if not need:
+            break
         work = torch.empty(need, dtype=torch.uint8, device=q.device)
-        a.workspace, a.workspace_bytes = work.data_ptr(), need
-    ctx.check(ctx.lib.vsk_attention(ctx.handle, _stream(q.device), kv, layer, ctypes.byref(news),
-                                    ctypes.byref(a)))
-
-
-def _outputs(q, return_lse):
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    lse = None
-    if return_lse:
-        lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
-    return out, lse
+    status = lib.vsk_attention(handle, _stream(q.device), kv, layer, news, a)
+    if status:
+        ctx.check(status)
+    return (out, lse) if return_lse else out
 
 
 class PagedKVCache:
@@ -312,29 +328,24 @@ class PagedKVCache:
     # -- new tokens -----------------------------------------------------------
     def _news(self, x, starts, seqs, max_new):
         """vsk_new_tokens of the rows of x and what must outlive the call."""
-        n = _lib.vsk_new_tokens()
-        n.tokens = x.shape[0]
-        keep = []
-        if starts is None:
-            n.n, n.max_new = x.shape[0], 1
-        else:
-            s = _ints(starts, "starts", self.device)
-            keep.append(s)
-            if s.shape[0] < 1:
+        tokens = x.shape[0]
+        n, most, at = tokens, 1, None
+        if starts is not None:
+            at = _ints(starts, "starts", self.device)
+            n = at.shape[0] - 1
+            if n < 0:
                 raise VSKError(-4, "starts holds an offset a sequence and the end")
-            n.starts, n.n = s.data_ptr(), s.shape[0] - 1
-            n.max_new = x.shape[0] if max_new is None else min(int(max_new), x.shape[0])
-            if n.max_new < 0:
+            most = tokens if max_new is None else min(int(max_new), tokens)
+            if most < 0:
                 raise VSKError(-2, "max_new must not be negative")
         if seqs is not None:
-            q = _ints(seqs, "seqs", self.device)
-            keep.append(q)
-            if q.shape[0] != n.n:
-                raise VSKError(-4, f"{q.shape[0]} slots for {n.n} sequences")
-            n.seqs = q.data_ptr()
-        elif n.n > self.slots:
-            raise VSKError(-2, f"{n.n} sequences, {self.slots} slots")
-        return n, keep
+            seqs = _ints(seqs, "seqs", self.device)
+            if seqs.shape[0] != n:
+                raise VSKError(-4, f"{seqs.shape[0]} slots for {n} sequences")
+        elif n > self.slots:
+            raise VSKError(-2, f"{n} sequences, {self.slots} slots")
+        return _NEWS.pack(at.data_ptr() if at is not None else 0,
+                          seqs.data_ptr() if seqs is not None else 0, n, most, tokens), (at, seqs)
 
     def _heads(self, x, name, heads=None):
         _tensor(x, name, self.dtype, 3)
@@ -361,12 +372,11 @@ class PagedKVCache:
             q = self._heads(q, "q")
             if q.shape[0] != k.shape[0]:
                 raise VSKError(-4, f"{k.shape[0]} keys, {q.shape[0]} queries")
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-            qr = ctypes.byref(_rows(q, out))
+            out = _empty(q)
+            qr = _rows(q, out)
         if k.shape[0]:
             self.ctx.check(self.ctx.lib.vsk_kv_append(
-                self.ctx.handle, _stream(self.device), self._ref, layer, ctypes.byref(news),
-                ctypes.byref(_rows(k, None)), ctypes.byref(_rows(v, None)),
+                self.ctx.handle, _stream(self.device), self._ref, layer, news, _rows(k), _rows(v),
                 rotary.handle if rotary is not None else None, qr))
         return out
 
@@ -385,10 +395,8 @@ class PagedKVCache:
         if q.shape[1] % self.kv_heads or not q.shape[1]:
             raise VSKError(-4, f"{q.shape[1]} query heads over {self.kv_heads} key heads")
         news, keep = self._news(q, starts, seqs, max_new)
-        out, lse = _outputs(q, return_lse)
-        _attend(self.ctx, self._ref, layer, q, news, None, scale, window, sinks, max_length, out,
-                lse)
-        return (out, lse) if return_lse else out
+        return _attend(self.ctx, self._ref, layer, q, news, 0, scale, window, sinks, max_length,
+                       return_lse)
 
     # -- pages ------------------------------------------------------------------
     def _keeping(self):
@@ -483,13 +491,13 @@ def window_attention(ctx: Context, q, k, v, *, starts, k_starts=None, max_length
         raise VSKError(-4, "starts and k_starts hold an offset a sequence and the end")
     if k_starts is None and k.shape[0] != q.shape[0]:
         raise VSKError(-4, f"{q.shape[0]} queries, {k.shape[0]} keys: k_starts is wanted")
-    kv, news = _lib.vsk_kv(), _lib.vsk_new_tokens()
+    kv = _lib.vsk_kv()
     kv.k, kv.v, kv.dtype = k.data_ptr(), v.data_ptr(), _TYPES[q.dtype]
-    kv.k_row, kv.k_head, kv.v_row, kv.v_head = k.stride(0), k.stride(1), v.stride(0), v.stride(1)
-    kv.pages, kv.kv_heads, kv.head_dim, kv.layers = k.shape[0], k.shape[1], k.shape[2], 1
-    news.starts, news.n, news.tokens = s.data_ptr(), s.shape[0] - 1, q.shape[0]
-    news.max_new = q.shape[0] if max_length is None else min(int(max_length), q.shape[0])
-    out, lse = _outputs(q, return_lse)
-    _attend(ctx, ctypes.byref(kv), 0, q, news, ks.data_ptr(), scale, window, sinks,
-            max_length if k_starts is None else None, out, lse)
-    return (out, lse) if return_lse else out
+    kv.k_row, kv.k_head, _ = k.stride()
+    kv.v_row, kv.v_head, _ = v.stride()
+    kv.pages, kv.kv_heads, kv.head_dim = k.shape
+    kv.layers = 1
+    most = q.shape[0] if max_length is None else min(int(max_length), q.shape[0])
+    news = _NEWS.pack(s.data_ptr(), 0, s.shape[0] - 1, most, q.shape[0])
+    return _attend(ctx, ctypes.byref(kv), 0, q, news, ks.data_ptr(), scale, window, sinks,
+                   max_length if k_starts is None else None, return_lse)
