@@ -15,7 +15,7 @@ int32_t padded_head(int32_t d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
 struct Plan {
   int32_t tiles, splits, chunk;
   int32_t share;  // attn_rows: waves that take a row tile's keys in turn
-  int32_t waves;    // > 0: attn_tile, so many waves a block
+  bool tile;      // attn_tile
 };
 
 // 16-byte loads of every operand, and stores of four values.
@@ -41,22 +41,22 @@ Plan plan_of(const vsk_ctx *ctx, const vsk_kv *kv, const vsk_new_tokens *news,
   const int64_t rows = max_new * group, pairs = (int64_t)news->n * kv->kv_heads;
   p.splits = 1;
   p.chunk = 1 << 30;
-  p.waves = 0;
+  p.tile = false;
   p.share = 4;
   int64_t row_tile = 16, key_tile = kv->dtype == VSK_DTYPE_F32 ? 16 : 32, per = 4;
   // blocks that a compute unit holds at once (by their registers), twice over
   // (a head of 256: once): fewer leave it idle at the end, more start too often
   int64_t want = (kv->head_dim <= 64 ? 8 : kv->head_dim <= 128 ? 6 : 1) * (int64_t)ctx->cu_count;
   if (kv->dtype != VSK_DTYPE_F32 && rows >= 64 && aligned_operands(kv, args)) {
-    p.waves = kv->head_dim > 128 || pairs * ceil_div(rows, 256) < ctx->cu_count ? 4 : 8;
-    row_tile = 32 * p.waves;
+    p.tile = true;
+    row_tile = ATTN_TILE_ROWS;
     key_tile = attn_tile_keys(kv->head_dim);
     per = 16;
-    want = ctx->cu_count;
+    want = 2 * ctx->cu_count;
   }
   p.tiles = (int32_t)ceil_div(rows, row_tile);
   const int64_t blocks = pairs * p.tiles;
-  if (p.waves == 0) {
+  if (!p.tile) {
     // row tiles enough to fill the device: a wave each
     if (blocks >= 8 * (int64_t)ctx->cu_count && p.tiles >= 4) {
       p.share = 1;
@@ -74,12 +74,14 @@ Plan plan_of(const vsk_ctx *ctx, const vsk_kv *kv, const vsk_new_tokens *news,
   // a tile for each of the four waves that share them (16 tiles: joining a
   // prompt's rows takes as long as some steps)
   const int64_t tiles = ceil_div(keys, key_tile);
-  if (p.waves == 0 && kv->head_dim <= 128 &&
+  if (!p.tile && kv->head_dim <= 128 &&
       tiles <= (blocks < ctx->cu_count ? 32 : 64)) {
     p.share = 8;
     return p;
   }
-  const int64_t target = ceil_div(want, blocks);
+  // (a prompt's rows are many: parts only where a quarter of the device or less
+  // would work)
+  const int64_t target = p.tile && 4 * blocks > want ? 1 : ceil_div(want, blocks);
   const int64_t chunk = ceil_div(ceil_div(tiles, target), per) * per;
   p.chunk = (int32_t)(chunk < per ? per : chunk);
   p.splits = (int32_t)ceil_div(tiles, p.chunk);
@@ -203,11 +205,11 @@ vsk_status vsk_attention(vsk_ctx *ctx, void *stream, const vsk_kv *kv, int32_t l
   }
   const bool al = aligned_operands(kv, args);
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (p.waves)
-    launch_attn_tile(ctx, st, a, kv->dtype, p.waves);
+  if (p.tile)
+    launch_attn_tile(ctx, st, a, kv->dtype);
   else
     launch_attn_rows(ctx, st, a, kv->dtype, al, p.share);
-  launch_attn_join(ctx, st, a, kv->dtype, al, p.waves ? 32 * p.waves : 16);
+  launch_attn_join(ctx, st, a, kv->dtype, al, p.tile ? ATTN_TILE_ROWS : 16);
   finish_queued(ctx, st);
   VSK_API_END(ctx);
 }

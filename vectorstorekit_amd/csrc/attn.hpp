@@ -242,11 +242,11 @@ void launch_attn_rows(vsk_ctx *ctx, hipStream_t stream, const AttnArgs &a, int32
                       bool aligned, int32_t share);
 // keys of a tile of attn_tile.hip, by the (padded) head
 constexpr int attn_tile_keys(int d) { return d > 128 ? 32 : 64; }
-// attn_tile.hip: 16-bit types, aligned; waves: 8 or 4 a workgroup
-void launch_attn_tile(vsk_ctx *ctx, hipStream_t stream, const AttnArgs &a, int32_t t,
-                      int32_t waves);
-// joins the parts that row tiles of `rows` rows left: 16 (launch_attn_rows),
-// or 32 a wave (launch_attn_tile)
+// attn_tile.hip: 16-bit types, aligned, row tiles of ATTN_TILE_ROWS
+constexpr int ATTN_TILE_ROWS = 128;
+void launch_attn_tile(vsk_ctx *ctx, hipStream_t stream, const AttnArgs &a, int32_t t);
+// joins the parts that row tiles of `rows` rows left: 16 (launch_attn_rows) or
+// ATTN_TILE_ROWS
 void launch_attn_join(vsk_ctx *ctx, hipStream_t stream, const AttnArgs &a, int32_t t,
                       bool aligned, int32_t rows);
 

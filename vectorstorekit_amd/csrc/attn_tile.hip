@@ -1,5 +1,5 @@
 // attn_tile.hip -- attention of many query rows in 16 bits: 32 rows a wave,
-// eight (four) waves a workgroup, keys and values shared through LDS.
+// four waves a workgroup, keys and values shared through LDS.
 //
 // S^T = K Q^T and O^T = V^T P^T with 32x32x16 products.  As in
 // attn_rows.hip a lane owns one query row (lane % 32) and half of the keys of
@@ -23,6 +23,8 @@ namespace {
 
 
 typedef __attribute__((ext_vector_type(4))) short i16x4;
+constexpr int NW = 4;  // waves of a workgroup
+
 template <class T> struct Mm;
 template <> struct Mm<__bf16> {
   typedef bf16x8 V8;
@@ -54,19 +56,23 @@ __device__ inline float max3(float a, float b, float c) {
   return r;
 }
 
-// RW: row tiles (of 32) of a wave.
-template <class T, int DP, int NW, int RW>
+// DP: the head, padded to products.  Two workgroups of four waves share a
+// compute unit, so that one's start and end hide behind the other's products
+// (one of eight waves over twice the rows: 340 us where these take 308, 8
+// ragged prompts to 4,096 of 32 heads of 128, window 1,024).
+template <class T, int DP>
 __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void k_attn_tile(const AttnArgs a) {
   typedef typename Mm<T>::V8 V8;
   constexpr int KT = attn_tile_keys(DP), U = KT / 32;
-  constexpr int CH = DP / 8;         // 16-byte pieces of a row
-  constexpr int ROWB = 2 * DP;       // bytes of a row
+  constexpr int PITCH = DP <= 64 ? 64 : DP <= 128 ? 128 : 256;
+  constexpr int CH = PITCH / 8;      // 16-byte pieces of a row
+  constexpr int ROWB = 2 * PITCH;    // bytes of a row
   constexpr int TILEB = KT * ROWB;   // bytes of a tile
   constexpr int RPI = 64 / CH;       // rows that one load of a wave brings
   constexpr int MINE = KT / NW;      // rows of a tile that a wave brings
   constexpr int LD = MINE / RPI;     // loads that takes
   constexpr int KS = DP / 16, DT = DP / 32;
-  constexpr int ROWS = 32 * RW * NW; // query rows of the block
+  constexpr int ROWS = 32 * NW;      // query rows of the block
   // tile i's keys in kbuf[i % 3], two tiles ahead of their products, its
   // values in vbuf[i % 2], one ahead
   __shared__ __attribute__((aligned(1024))) char keys_lds[3 * TILEB];
@@ -96,27 +102,41 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void k_attn_tile(const 
   const int32_t end = part == parts - 1 ? span.tiles : first + a.chunk;
 
   // this wave's rows and what they see
-  const int32_t w0 = row0 + 32 * RW * w, w1 = w0 + 32 * RW - 1 < last ? w0 + 32 * RW - 1 : last;
+  const int32_t w0 = row0 + 32 * w, w1 = w0 + 31 < last ? w0 + 31 : last;
   const bool have = w0 <= last;
   const int32_t q_lo = p0 + w0 / a.group, q_hi = have ? p0 + w1 / a.group : -1;
-  int32_t pos[RW];
-  V8 q[RW][KS];
-#pragma unroll
-  for (int r = 0; r < RW; ++r) {
-    const int32_t row = w0 + 32 * r + n, t = row / a.group, head = h * a.group + row - t * a.group;
-    const bool real = row <= last;
-    pos[r] = real ? p0 + t : -1;
-    const T *src = static_cast<const T *>(a.q) + (real ? (s.token0 + t) * a.q_row + head * a.q_head : 0);
+  // (a head of 256 leaves no registers for the queries: each lane's wait in LDS)
+  constexpr bool QLDS = DP == 256;
+  __shared__ __attribute__((aligned(1024))) char queries_lds[QLDS ? NW * KS * 1024 : 16];
+  lds_char *const qbuf = (lds_char *)queries_lds + 16 * lane;
+  const int32_t my_row = w0 + n, my_t = my_row / a.group;
+  const int32_t my_head = h * a.group + my_row - my_t * a.group;
+  const bool real = my_row <= last;
+  const int32_t pos = real ? p0 + my_t : -1;
+  V8 q[QLDS ? 1 : KS];
+  auto query = [&](int x) -> V8 {
+    if constexpr (QLDS) return *(const lds_as V8 *)(qbuf + (w * KS + x) * 1024);
+    return q[QLDS ? 0 : x];
+  };
+  {
+    V8 mine[KS];
+    const T *src = static_cast<const T *>(a.q) +
+                   (real ? (s.token0 + my_t) * a.q_row + my_head * a.q_head : 0);
 #pragma unroll
     for (int i = 0; i < KS; ++i) {
       const int e = 16 * i + 8 * h2;  // (no branch around a load: all are in flight)
-      q[r][i] = *reinterpret_cast<const V8 *>(src + (e < a.d ? e : a.d - 8));
+      mine[i] = *reinterpret_cast<const V8 *>(src + (e < a.d ? e : a.d - 8));
     }
 #pragma unroll
-    for (int i = 0; i < KS; ++i)
-      if (!real || 16 * i + 8 * h2 >= a.d) q[r][i] = V8{};
+    for (int i = 0; i < KS; ++i) {
+      if (!real || 16 * i + 8 * h2 >= a.d) mine[i] = V8{};
+      if constexpr (QLDS)
+        *(lds_as V8 *)(qbuf + (w * KS + i) * 1024) = mine[i];
+      else
+        q[QLDS ? 0 : i] = mine[i];
+    }
   }
-  if (a.d < DP) {
+  if (a.d < PITCH) {
     // pieces past the head are never loaded: they stay zero
     u32x4 *z = reinterpret_cast<u32x4 *>(keys_lds), *y = reinterpret_cast<u32x4 *>(values_lds);
     for (int i = threadIdx.x; i < 3 * TILEB / 16; i += 64 * NW) z[i] = u32x4{0, 0, 0, 0};
@@ -124,15 +144,10 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void k_attn_tile(const 
     __syncthreads();
   }
 
-  f32x16 acc[RW][DT];
-  float m[RW], l[RW];
+  f32x16 acc[DT];
 #pragma unroll
-  for (int r = 0; r < RW; ++r) {
-#pragma unroll
-    for (int i = 0; i < DT; ++i) acc[r][i] = f32x16{};
-    m[r] = -INFINITY;
-    l[r] = 0.f;
-  }
+  for (int i = 0; i < DT; ++i) acc[i] = f32x16{};
+  float m = -INFINITY, l = 0.f;
 
   // The rows of a tile that this wave brings lie within 16, on one page.
   // Lane i holds the addresses of those 16 for tile tb + i, keys and values.
@@ -163,7 +178,7 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void k_attn_tile(const 
   };
 #pragma unroll
   for (int x = 0; x < LD; ++x) k_off[x] = offset(x, 15, true), v_off[x] = offset(x, 15, false);
-  const bool full = a.d == DP;
+  const bool full = a.d == PITCH;
   auto fetch = [&](int32_t i, lds_char *to, bool keys) {
     const uint64_t base = keys ? lane_of(k_lo, k_hi, i - tb) : lane_of(v_lo, v_hi, i - tb);
     const int32_t j0 = span.base(i) + MINE * w;
@@ -211,18 +226,13 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void k_attn_tile(const 
 
   // register 16 u + x of the scores belongs to key 32 u + 8 (x / 4) + 4 h2 +
   // x % 4 of the tile
-  auto scores = [&](const lds_char *buf, f32x16 (&sc)[RW][U]) {
+  auto scores = [&](const lds_char *buf, f32x16 (&sc)[U]) {
     const int kb = k_base(buf);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
+      sc[u] = f32x16{};
 #pragma unroll
-      for (int r = 0; r < RW; ++r) sc[r][u] = f32x16{};
-#pragma unroll
-      for (int x = 0; x < KS; ++x) {
-        const V8 k = key_piece(kb, x, u);
-#pragma unroll
-        for (int r = 0; r < RW; ++r) sc[r][u] = Mm<T>::mfma(k, q[r][x], sc[r][u]);
-      }
+      for (int x = 0; x < KS; ++x) sc[u] = Mm<T>::mfma(key_piece(kb, x, u), query(x), sc[u]);
     }
   };
   auto largest = [&](const f32x16 (&sc)[U]) {
@@ -235,27 +245,30 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void k_attn_tile(const 
   // The sums are kept relative to m, which follows the largest score only when
   // that has grown by 8 (in log2): weights up to 256 cost no precision, and
   // the sums are seldom rescaled.
-  auto settle = [&](int r, float tm) {
+  auto settle = [&](float tm) {
     const float top = tm * a.scale_log2;
-    if (!__any(top > m[r] + 8.f)) return;
-    const float nm = top > m[r] + 8.f ? top : m[r];
-    const float fade = nm == -INFINITY ? 1.f : attn_exp2(m[r] - nm);
-    m[r] = nm;
-    l[r] *= fade;
+    if (!__any(top > m + 8.f)) return;
+    const float nm = top > m + 8.f ? top : m;
+    const float fade = nm == -INFINITY ? 1.f : attn_exp2(m - nm);
+    m = nm;
+    l *= fade;
 #pragma unroll
-    for (int x = 0; x < DT; ++x) acc[r][x] *= fade;
+    for (int x = 0; x < DT; ++x) {
+      acc[x] *= fade;
+      if (DP == 256) __builtin_amdgcn_sched_barrier(0);  // (few registers at a time)
+    }
   };
-  // -inf for the keys that the row at this position does not see.  Bit c of a
+  // -inf for the keys that the lane's row does not see.  Bit c of a
   // word is key c of the 32 that the word is for: comparisons a row, not a key.
   auto up_to = [](int32_t x) -> uint32_t { return x < 0 ? 0u : x > 30 ? ~0u : (2u << x) - 1; };
-  auto hide = [&](f32x16 (&sc)[U], int32_t at, int32_t kb) {
+  auto hide = [&](f32x16 (&sc)[U], int32_t kb) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int32_t b = kb + 32 * u + 4 * h2;
       uint32_t see = ~0u;
       if (a.window > 0)
-        see = (at < a.window ? ~0u : ~up_to(at - a.window - b)) | up_to(a.sinks - 1 - b);
-      see &= up_to(at - b);
+        see = (pos < a.window ? ~0u : ~up_to(pos - a.window - b)) | up_to(a.sinks - 1 - b);
+      see &= up_to(pos - b);
 #pragma unroll
       for (int x = 0; x < 16; ++x) {
         const uint32_t on = (uint32_t)((int32_t)(see << (31 - 8 * (x >> 2) - (x & 3))) >> 31);
@@ -285,74 +298,59 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void k_attn_tile(const 
     if (!any) return;
     const bool whole = kb + KT - 1 <= q_lo &&
                        (a.window <= 0 || q_hi - kb < a.window || kb + KT <= a.sinks);
+    f32x16 sc[U];
     if (whole || !not_finite(vt)) {
-      f32x16 sc[RW][U];
       scores(kt, sc);
       const int vb = v_base(vt);
-#pragma unroll
-      for (int r = 0; r < RW; ++r) {
-        if (!whole) hide(sc[r], pos[r], kb);
-        settle(r, largest(sc[r]));
-      }
+      if (!whole) hide(sc, kb);
+      settle(largest(sc));
+      const float use = m == -INFINITY ? 0.f : m;
 #pragma unroll
       for (int u = 0; u < 2 * U; ++u) {
-        V8 p[RW];
+        V8 p;
 #pragma unroll
-        for (int r = 0; r < RW; ++r) {
-          const float use = m[r] == -INFINITY ? 0.f : m[r];
-#pragma unroll
-          for (int x = 0; x < 8; ++x) {
-            const float y = attn_exp2(fmaf(sc[r][u >> 1][8 * (u & 1) + x], a.scale_log2, -use));
-            l[r] += y;
-            p[r][x] = (T)y;
-          }
+        for (int x = 0; x < 8; ++x) {
+          const float y = attn_exp2(fmaf(sc[u >> 1][8 * (u & 1) + x], a.scale_log2, -use));
+          l += y;
+          p[x] = (T)y;
         }
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt) {
-          const V8 v = value_piece(vb, dt, u);
-#pragma unroll
-          for (int r = 0; r < RW; ++r) acc[r][dt] = Mm<T>::mfma(v, p[r], acc[r][dt]);
-        }
+        for (int dt = 0; dt < DT; ++dt) acc[dt] = Mm<T>::mfma(value_piece(vb, dt, u), p, acc[dt]);
       }
       return;
     }
     // a masked place must not reach a sum, and 0 * NaN is NaN: the keys one at
-    // a time, each row takes only those it sees
-    f32x16 sc[RW][U];
+    // a time, each row takes only those it sees.  (A rare path: the sums wait
+    // in memory meanwhile, so that it takes no registers from the others.)
     scores(kt, sc);
+    hide(sc, kb);
+    settle(largest(sc));
+    const float use = m == -INFINITY ? 0.f : m;
+    float held[16 * DT], wt[16 * U];
 #pragma unroll
-    for (int r = 0; r < RW; ++r) {
-      hide(sc[r], pos[r], kb);
-      settle(r, largest(sc[r]));
+    for (int x = 0; x < 16 * DT; ++x) held[x] = acc[x >> 4][x & 15];
+#pragma unroll
+    for (int x = 0; x < 16 * U; ++x) {
+      wt[x] = attn_exp2(fmaf(sc[x >> 4][x & 15], a.scale_log2, -use));
+      l += wt[x];
     }
 #pragma unroll 1
     for (int j = 0; j < KT; ++j) {
-#pragma unroll
-      for (int r = 0; r < RW; ++r) {
-        float wt = 0.f;
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-          for (int x = 0; x < 16; ++x)
-            wt = 32 * u + 8 * (x >> 2) + (x & 3) == (j & ~4) ? sc[r][u][x] : wt;
-        wt = attn_exp2(fmaf(__shfl(wt, n + 32 * ((j >> 2) & 1)), a.scale_log2,
-                            m[r] == -INFINITY ? 0.f : -m[r]));
-        if (((j >> 2) & 1) == h2) l[r] += wt;
-        const bool sees = attn_sees(a, pos[r], kb + j);
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-          for (int b = 0; b < 4; ++b) {
-            const int c = 4 * dt + b;
-            const lds_as T *v =
-                (const lds_as T *)(vt + j * ROWB + ((c ^ v_swizzle<CH>(j)) << 4)) + 4 * h2;
-#pragma unroll
-            for (int x = 0; x < 4; ++x)
-              if (sees) acc[r][dt][4 * b + x] = fmaf(wt, (float)v[x], acc[r][dt][4 * b + x]);
-            __builtin_amdgcn_sched_barrier(0);  // (few registers, not speed)
-          }
+      // key j is in register 16 (j / 32) + 4 (j / 8 % 4) + j % 4 of the lanes
+      // whose h2 is bit 2 of j
+      const float y = __shfl(wt[16 * (j >> 5) + 4 * ((j >> 3) & 3) + (j & 3)],
+                             n + 32 * ((j >> 2) & 1));
+      if (!attn_sees(a, pos, kb + j)) continue;
+#pragma unroll 1
+      for (int c = 0; c < 4 * DT; ++c) {
+        const lds_as T *v =
+            (const lds_as T *)(vt + j * ROWB + ((c ^ v_swizzle<CH>(j)) << 4)) + 4 * h2;
+#pragma unroll 1
+        for (int x = 0; x < 4; ++x) held[4 * c + x] = fmaf(y, (float)v[x], held[4 * c + x]);
       }
     }
+#pragma unroll
+    for (int x = 0; x < 16 * DT; ++x) acc[x >> 4][x & 15] = held[x];
   };
 
   // the tiles that every row of the block sees whole: from the window's edge
@@ -405,142 +403,123 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void k_attn_tile(const 
     // at a time (left to itself the compiler keeps one read in flight).  The
     // last step's scores are not used: what follows is an edge, or nothing.
     constexpr int NS = U * KS, NV = 2 * U * DT, AHEAD = 4;
-    f32x16 sc[RW][U];
+    f32x16 sc[U];
     scores(kbuf + kslot * TILEB, sc);
-#pragma unroll
-    for (int r = 0; r < RW; ++r) settle(r, largest(sc[r]));
+    settle(largest(sc));
 #pragma unroll 1
     for (; i < hot1; ++i) {
       ahead(i);
       const int kb = k_base(kbuf + (kslot == 2 ? 0 : kslot + 1) * TILEB);
       const int vb = v_base(vbuf + ((i - first) & 1) * TILEB);
-      f32x16 sn[RW][U];
-      V8 f[AHEAD], p[RW][2 * U];
-      float tm[RW], use[RW];
+      const float use = m == -INFINITY ? 0.f : m;
+      f32x16 sn[U];
+      V8 f[AHEAD], p[2 * U], qf[QLDS ? AHEAD : 1];
+      float tm = -INFINITY;
 #pragma unroll
-      for (int r = 0; r < RW; ++r) {
-        tm[r] = -INFINITY;
-        use[r] = m[r] == -INFINITY ? 0.f : m[r];
-#pragma unroll
-        for (int u = 0; u < U; ++u) sn[r][u] = f32x16{};
-      }
+      for (int u = 0; u < U; ++u) sn[u] = f32x16{};
       auto piece_of = [&](int g) -> V8 {
         return g < NS ? key_piece(kb, g / U, g % U) : value_piece(vb, (g - NS) % DT, (g - NS) / DT);
       };
-      auto weight = [&](int r, int e) {  // of register e of the scores
-        const float y = attn_exp2(fmaf(sc[r][e >> 4][e & 15], a.scale_log2, -use[r]));
-        l[r] += y;
-        p[r][e >> 3][e & 7] = (T)y;
+      auto weight = [&](int e) {  // of register e of the scores
+        const float y = attn_exp2(fmaf(sc[e >> 4][e & 15], a.scale_log2, -use));
+        l += y;
+        p[e >> 3][e & 7] = (T)y;
       };
 #pragma unroll
-      for (int g = 0; g < AHEAD; ++g) f[g] = piece_of(g);
+      for (int g = 0; g < AHEAD; ++g) {
+        f[g] = piece_of(g);
+        if (QLDS) qf[QLDS ? g : 0] = query(g / U);
+      }
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int g = 0; g < NS + NV; ++g) {
         const V8 x = f[g % AHEAD];
+        if (g < NS)
+          sn[g % U] = Mm<T>::mfma(x, QLDS ? qf[QLDS ? g % AHEAD : 0] : query(g / U), sn[g % U]);
+        else
+          acc[(g - NS) % DT] = Mm<T>::mfma(x, p[(g - NS) / DT], acc[(g - NS) % DT]);
+        if (g + AHEAD < NS + NV) f[g % AHEAD] = piece_of(g + AHEAD);
+        if (QLDS && g + AHEAD < NS) qf[QLDS ? g % AHEAD : 0] = query((g + AHEAD) / U);
+        // half of the weights beside the scores, half beside the first sums
+        if (g < NS) {
 #pragma unroll
-        for (int r = 0; r < RW; ++r) {
-          if (g < NS)
-            sn[r][g % U] = Mm<T>::mfma(x, q[r][g / U], sn[r][g % U]);
-          else
-            acc[r][(g - NS) % DT] =
-                Mm<T>::mfma(x, p[r][(g - NS) / DT], acc[r][(g - NS) % DT]);
-          if (r == RW - 1 && g + AHEAD < NS + NV) f[g % AHEAD] = piece_of(g + AHEAD);
-          // half of the weights beside the scores, half beside the first sums
-          if (g < NS) {
+          for (int e = 8 * U * g / NS; e < 8 * U * (g + 1) / NS; ++e) weight(e);
+        } else if (g - NS < NV / 2) {
 #pragma unroll
-            for (int e = 8 * U * g / NS; e < 8 * U * (g + 1) / NS; ++e) weight(r, e);
-          } else if (g - NS < NV / 2) {
+          for (int e = 8 * U * (g - NS) / (NV / 2); e < 8 * U * (g - NS + 1) / (NV / 2); ++e)
+            weight(8 * U + e);
+        } else {
+          const int z = g - NS - NV / 2;
 #pragma unroll
-            for (int e = 8 * U * (g - NS) / (NV / 2); e < 8 * U * (g - NS + 1) / (NV / 2); ++e)
-              weight(r, 8 * U + e);
-          } else {
-            const int z = g - NS - NV / 2;
-#pragma unroll
-            for (int e = 8 * U * z / (NV / 2); e < 8 * U * (z + 1) / (NV / 2); ++e)
-              tm[r] = max3(tm[r], sn[r][e >> 3][2 * (e & 7)], sn[r][e >> 3][2 * (e & 7) + 1]);
-          }
-          __builtin_amdgcn_sched_barrier(0);
+          for (int e = 8 * U * z / (NV / 2); e < 8 * U * (z + 1) / (NV / 2); ++e)
+            tm = max3(tm, sn[e >> 3][2 * (e & 7)], sn[e >> 3][2 * (e & 7) + 1]);
         }
+        __builtin_amdgcn_sched_barrier(0);
       }
 #pragma unroll
-      for (int r = 0; r < RW; ++r) {
-#pragma unroll
-        for (int u = 0; u < U; ++u) sc[r][u] = sn[r][u];
-        if (i + 1 < hot1) settle(r, xor32_max(tm[r]));
-      }
+      for (int u = 0; u < U; ++u) sc[u] = sn[u];
+      if (i + 1 < hot1) settle(xor32_max(tm));
       done();
     }
   }
 
-#pragma unroll
-  for (int r = 0; r < RW; ++r) {
-    const float sum = xor32_sum(l[r]);
-    const int32_t row = w0 + 32 * r + n;
-    if (row > last) continue;
-    const int32_t t = row / a.group, head = h * a.group + row - t * a.group;
-    const int64_t out_row = (s.token0 + t) * a.heads + head;
-    if (parts > 1) {
-      const int64_t x = (int64_t)part * a.tokens * a.heads + out_row;
-      float *dst = a.part_o + x * DP;
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-        for (int b = 0; b < 4; ++b)
-          *reinterpret_cast<f32x4 *>(dst + 32 * dt + 8 * b + 4 * h2) =
-              f32x4{acc[r][dt][4 * b], acc[r][dt][4 * b + 1], acc[r][dt][4 * b + 2],
-                    acc[r][dt][4 * b + 3]};
-      if (h2 == 0) {
-        a.part_ml[2 * x] = m[r];
-        a.part_ml[2 * x + 1] = sum;
-      }
-      continue;
-    }
-    const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
-    T *dst = static_cast<T *>(a.out) + (s.token0 + t) * a.o_row + head * a.o_head;
-    typedef __attribute__((ext_vector_type(4))) T V4;
+  const float sum = xor32_sum(l);
+  if (!real) return;
+  const int64_t out_row = (s.token0 + my_t) * a.heads + my_head;
+  if (parts > 1) {
+    const int64_t x = (int64_t)part * a.tokens * a.heads + out_row;
+    float *dst = a.part_o + x * PITCH;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-      for (int b = 0; b < 4; ++b) {
-        const int e = 32 * dt + 8 * b + 4 * h2;
-        V4 y;
-#pragma unroll
-        for (int x = 0; x < 4; ++x) y[x] = (T)(acc[r][dt][4 * b + x] * inv);
-        if (e < a.d) *reinterpret_cast<V4 *>(dst + e) = y;
-      }
-    if (a.lse && h2 == 0)
-      a.lse[out_row] = sum > 0.f ? (m[r] + __log2f(sum)) * 0.6931471805599453f
-                                 : sum != sum ? sum : -INFINITY;
+      for (int b = 0; b < 4; ++b)
+        *reinterpret_cast<f32x4 *>(dst + 32 * dt + 8 * b + 4 * h2) =
+            f32x4{acc[dt][4 * b], acc[dt][4 * b + 1], acc[dt][4 * b + 2], acc[dt][4 * b + 3]};
+    if (h2 == 0) {
+      a.part_ml[2 * x] = m;
+      a.part_ml[2 * x + 1] = sum;
+    }
+    return;
   }
+  const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+  T *dst = static_cast<T *>(a.out) + (s.token0 + my_t) * a.o_row + my_head * a.o_head;
+  typedef __attribute__((ext_vector_type(4))) T V4;
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+      const int e = 32 * dt + 8 * b + 4 * h2;
+      V4 y;
+#pragma unroll
+      for (int x = 0; x < 4; ++x) y[x] = (T)(acc[dt][4 * b + x] * inv);
+      if (e < a.d) *reinterpret_cast<V4 *>(dst + e) = y;
+    }
+  if (a.lse && h2 == 0)
+    a.lse[out_row] = sum > 0.f ? (m + __log2f(sum)) * 0.6931471805599453f
+                               : sum != sum ? sum : -INFINITY;
 }
 
-template <class T> void tile_of(hipStream_t st, const AttnArgs &a, int nw, unsigned g) {
-  if (a.d <= 64) {
-    if (nw == 8)
-      k_attn_tile<T, 64, 8, 1><<<g, 512, 0, st>>>(a);
-    else
-      k_attn_tile<T, 64, 4, 1><<<g, 256, 0, st>>>(a);
-  } else if (a.d <= 128) {
-    if (nw == 8)
-      k_attn_tile<T, 128, 8, 1><<<g, 512, 0, st>>>(a);
-    else
-      k_attn_tile<T, 128, 4, 1><<<g, 256, 0, st>>>(a);
-  } else {
-    k_attn_tile<T, 256, 4, 1><<<g, 256, 0, st>>>(a);
-  }
+template <class T> void tile_of(hipStream_t st, const AttnArgs &a, unsigned g) {
+  if (a.d <= 64)
+    k_attn_tile<T, 64><<<g, 64 * NW, 0, st>>>(a);
+  else if (a.d <= 96)
+    k_attn_tile<T, 96><<<g, 64 * NW, 0, st>>>(a);
+  else if (a.d <= 128)
+    k_attn_tile<T, 128><<<g, 64 * NW, 0, st>>>(a);
+  else
+    k_attn_tile<T, 256><<<g, 64 * NW, 0, st>>>(a);
 }
 
 }  // namespace
 
-void launch_attn_tile(vsk_ctx *ctx, hipStream_t st, const AttnArgs &a, int32_t t, int32_t nw) {
+void launch_attn_tile(vsk_ctx *ctx, hipStream_t st, const AttnArgs &a, int32_t t) {
   const int64_t grid = (int64_t)a.n * a.splits * a.tiles * a.kv_heads;
   VSK_REQUIRE(grid <= 0x7FFFFFFFll, VSK_ERR_INVALID_BUFFER_SIZE, "too many query rows in one call");
   KernelTimer kt(ctx, "attn_tile", (double)a.tokens * a.heads, st);
   if (t == VSK_DTYPE_F16)
-    tile_of<_Float16>(st, a, nw, (unsigned)grid);
+    tile_of<_Float16>(st, a, (unsigned)grid);
   else
-    tile_of<__bf16>(st, a, nw, (unsigned)grid);
+    tile_of<__bf16>(st, a, (unsigned)grid);
   check_launch("attn_tile");
 }
 
