@@ -58,7 +58,7 @@ struct Pool {
   int32_t *table, *lengths, *refs, *status, *scratch;
   int64_t table_stride;
   int32_t layers, pages, page_size, shift, kv_heads, d, size, slots, width;
-  // scratch: three lists of a page each, then five of a slot each
+  // scratch: three lists of a page each, then three of a slot each (reserve: the first)
   __device__ int32_t *page_list(int i) const { return scratch + (int64_t)i * pages; }
   __device__ int32_t *slot_list(int i) const {
     return scratch + 3 * (int64_t)pages + (int64_t)i * slots;
@@ -116,11 +116,15 @@ __device__ inline int32_t count_of(const int32_t *refs, int32_t i) {
 template <class F> __device__ int32_t take_free(const Pool &p, int32_t want, F &&take) {
   int32_t found = 0;
   for (int32_t c = 0; c < p.pages && found < want; c += 4 * NT) {
-    int32_t mask = 0;
+    int32_t mask = 0, count[4];
+#pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int32_t id = c + 4 * (int32_t)threadIdx.x + i;
-      if (id < p.pages && count_of(p.refs, id) <= 0) mask |= 1 << i;
+      count[i] = count_of(p.refs, id < p.pages ? id : p.pages - 1);
     }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (c + 4 * (int32_t)threadIdx.x + i < p.pages && count[i] <= 0) mask |= 1 << i;
     int32_t all;
     int32_t rank = found + scan(__popc(mask), &all);
     for (int i = 0; i < 4; ++i)
@@ -200,58 +204,71 @@ __global__ __launch_bounds__(NT) void k_kv_reserve(const Pool p, const int32_t *
   if (threadIdx.x == 0) p.status[0] = want - got + cut;
 }
 
+// A wave a child: its row's and its parent's entries are loaded together, and
+// the counts change by atomics that nothing waits for before free pages are
+// looked for.  Children go in batches of a workgroup's threads, one each; what
+// a batch needs again it finds in LDS.
 __global__ __launch_bounds__(NT) void k_kv_fork(const Pool p, const int32_t *parents,
                                                 const int32_t *children, int32_t n) {
   int32_t *src = p.slot_list(0), *dst = p.slot_list(1), *rows = p.slot_list(2);
-  int32_t *who = p.slot_list(3);
-  const int64_t cells = (int64_t)n * p.width;
-  for (int64_t x = threadIdx.x; x < cells; x += NT) {
-    const int32_t c = children[x / p.width];
-    if ((uint32_t)c < (uint32_t)p.slots) release(p, c, (int32_t)(x % p.width));
-  }
-  __syncthreads();
-  for (int64_t x = threadIdx.x; x < cells; x += NT) {
-    const int32_t i = (int32_t)(x / p.width), s = (int32_t)(x % p.width);
-    const int32_t c = children[i], f = parents[i];
-    if ((uint32_t)c >= (uint32_t)p.slots || (uint32_t)f >= (uint32_t)p.slots) continue;
-    if (s >= held(p, f) >> p.shift) continue;
-    const int32_t page = p.table[f * p.table_stride + s];
-    p.table[c * p.table_stride + s] = page;
-    if ((uint32_t)page < (uint32_t)p.pages) atomicAdd(p.refs + page, 1);
-  }
-  __syncthreads();
-  int32_t want = 0;
-  for (int32_t b = 0; b < n; b += NT) {
+  __shared__ int32_t sc[NT], sf[NT], sl[NT], who[NT], sd[NT];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  int32_t c = -1, f = -1, l = 0;
+  auto stage = [&](int32_t b) {
     const int32_t i = b + threadIdx.x;
-    int32_t part = 0;
+    c = f = -1, l = 0;
     if (i < n) {
-      const int32_t c = children[i], f = parents[i];
-      if ((uint32_t)c < (uint32_t)p.slots && (uint32_t)f < (uint32_t)p.slots)
-        part = held(p, f) & (p.page_size - 1);
-      rows[i] = part;
-      dst[i] = -1;
-      src[i] = part ? p.table[f * p.table_stride + (held(p, f) >> p.shift)] : -1;
+      c = children[i], f = parents[i];
+      if ((uint32_t)c >= (uint32_t)p.slots) c = -1;
+      if (c < 0 || (uint32_t)f >= (uint32_t)p.slots) f = -1;
+      if (f >= 0) l = held(p, f);
     }
-    int32_t all;
-    const int32_t before = scan(part > 0, &all);
-    if (part > 0) who[want + before] = i;
-    want += all;
+    __syncthreads();
+    sc[threadIdx.x] = c, sf[threadIdx.x] = f, sl[threadIdx.x] = l, sd[threadIdx.x] = -1;
+    __syncthreads();
+  };
+  for (int32_t b = 0; b < n; b += NT) {
+    stage(b);
+    const int32_t m = n - b < NT ? n - b : NT;
+    for (int32_t x = w; x < m; x += NT / 64) {
+      const int32_t to = sc[x], from = sf[x], full = sl[x] >> p.shift;
+      if (to < 0) continue;
+      int32_t *mine = p.table + to * p.table_stride;
+      const int32_t *its = p.table + (from < 0 ? to : from) * p.table_stride;
+#pragma unroll 4
+      for (int32_t y = lane; y < p.width; y += 64) {
+        const int32_t old = mine[y], now = y < full ? its[y] : -1;
+        mine[y] = now;
+        if ((uint32_t)old < (uint32_t)p.pages) atomicSub(p.refs + old, 1);
+        if ((uint32_t)now < (uint32_t)p.pages) atomicAdd(p.refs + now, 1);
+      }
+    }
   }
-  __syncthreads();
-  const int32_t got = take_free(p, want, [&](int32_t rank, int32_t page) {
-    const int32_t i = who[rank];
-    dst[i] = page;
-    p.refs[page] = 1;
-    p.table[children[i] * p.table_stride + (held(p, parents[i]) >> p.shift)] = page;
-  });
-  __syncthreads();
-  for (int32_t i = threadIdx.x; i < n; i += NT) {
-    const int32_t c = children[i], f = parents[i];
-    if ((uint32_t)c >= (uint32_t)p.slots) continue;
-    const int32_t l = (uint32_t)f < (uint32_t)p.slots ? held(p, f) : 0;
-    p.lengths[c] = rows[i] && dst[i] < 0 ? l & ~(p.page_size - 1) : l;
+  int32_t missing = 0;
+  for (int32_t b = 0; b < n; b += NT) {
+    if (n > NT) stage(b);
+    const int32_t i = b + threadIdx.x, part = l & (p.page_size - 1);
+    const int32_t last = part ? p.table[f * p.table_stride + (l >> p.shift)] : -1;
+    int32_t want;
+    const int32_t before = scan(part > 0, &want);
+    if (part > 0) who[before] = threadIdx.x;
+    __threadfence();  // the counts have arrived where take_free reads them
+    __syncthreads();
+    const int32_t got = take_free(p, want, [&](int32_t rank, int32_t page) {
+      const int32_t x = who[rank];
+      sd[x] = page;
+      p.refs[page] = 1;
+      p.table[sc[x] * p.table_stride + (sl[x] >> p.shift)] = page;
+    });
+    __syncthreads();
+    if (i < n) {
+      const int32_t to = sd[threadIdx.x];
+      src[i] = last, dst[i] = to, rows[i] = part;
+      if (c >= 0) p.lengths[c] = part && to < 0 ? l & ~(p.page_size - 1) : l;
+    }
+    missing += want - got;
   }
-  if (threadIdx.x == 0) p.status[0] = want - got;
+  if (threadIdx.x == 0) p.status[0] = missing;
 }
 
 __global__ __launch_bounds__(256) void k_kv_free(const Pool p, const int32_t *seqs, int32_t n) {
@@ -266,41 +283,47 @@ __global__ __launch_bounds__(256) void k_kv_free(const Pool p, const int32_t *se
 
 // Lists the free pages below the number of pages in use and the used ones at
 // or above it, each in order: there are as many of the one as of the other.
+// place[id]: a moved page's number in the list, -1 for a free one.
 __global__ __launch_bounds__(NT) void k_kv_plan(const Pool p) {
   int32_t *hole = p.page_list(0), *mover = p.page_list(1), *place = p.page_list(2);
   int32_t used = 0;
+#pragma unroll 8
   for (int32_t id = threadIdx.x; id < p.pages; id += NT) used += p.refs[id] > 0;
   int32_t live;
   scan(used, &live);
   int32_t moves = 0, holes = 0;
+  auto load = [&](int32_t c, int32_t (&on)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int32_t id = c + 4 * (int32_t)threadIdx.x + i;
+      on[i] = p.refs[id < p.pages ? id : p.pages - 1];
+    }
+  };
+  int32_t next[4];
+  load(0, next);
   for (int32_t c = 0; c < p.pages; c += 4 * NT) {
     // (at most 4,096 of each a step: two counts in one word)
     int32_t count = 0, kind[4];
+#pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int32_t id = c + 4 * (int32_t)threadIdx.x + i;
-      const bool on = id < p.pages && p.refs[id] > 0;
+      const bool on = next[i] > 0;
       kind[i] = id >= p.pages ? 0 : id < live ? (on ? 0 : 1) : (on ? 1 << 16 : 0);
       count += kind[i];
     }
+    load(c + 4 * NT, next);
     int32_t all;
     int32_t before = scan(count, &all);
+#pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int32_t id = c + 4 * (int32_t)threadIdx.x + i;
       if (kind[i] == 1) hole[holes + (before & 0xFFFF)] = id;
       if (kind[i] > 1) mover[moves + (before >> 16)] = id;
-      // (an entry that names a free page keeps its number)
-      if (id < p.pages && id >= live && !kind[i]) place[id] = id;
+      if (id < p.pages && id >= live) place[id] = kind[i] ? moves + (before >> 16) : -1;
       before += kind[i];
     }
     holes += all & 0xFFFF;
     moves += all >> 16;
-  }
-  __syncthreads();
-  for (int32_t i = threadIdx.x; i < moves; i += NT) {
-    const int32_t from = mover[i], to = hole[i];
-    place[from] = to;
-    p.refs[to] = p.refs[from];
-    p.refs[from] = 0;
   }
   if (threadIdx.x == 0) {
     p.status[1] = live;
@@ -334,7 +357,9 @@ __global__ __launch_bounds__(256) void k_kv_move(const Pool p, const MoveArgs m,
     const int64_t cells = (int64_t)p.slots * p.width;
     for (int64_t x = blockIdx.x * 256ll + threadIdx.x; x < cells; x += gridDim.x * 256ll) {
       int32_t *e = p.table + x / p.width * p.table_stride + x % p.width;
-      if (*e >= live && *e < p.pages) *e = place[*e];
+      // (an entry that names a free page keeps its number)
+      const int32_t r = *e >= live && *e < p.pages ? place[*e] : -1;
+      if (r >= 0) *e = m.dst[r];
     }
   }
   const int32_t n = m.count ? *m.count : m.n;
@@ -347,6 +372,10 @@ __global__ __launch_bounds__(256) void k_kv_move(const Pool p, const MoveArgs m,
     const int32_t layer = (int32_t)(y % p.layers), i = (int32_t)(y / p.layers);
     const int32_t from = m.src[i], to = m.dst[i];
     if ((uint32_t)from >= (uint32_t)p.pages || (uint32_t)to >= (uint32_t)p.pages) continue;
+    if (place && piece == 0 && layer == 0 && !val && threadIdx.x == 0) {
+      p.refs[to] = p.refs[from];
+      p.refs[from] = 0;
+    }
     const int32_t rows = m.rows ? m.rows[i] : p.page_size;
     const int64_t page = val ? p.v_page : p.k_page, lay = val ? p.v_layer : p.k_layer;
     char *at = (val ? p.v : p.k) + layer * lay * p.size;
@@ -429,7 +458,7 @@ using namespace vsk;
 extern "C" {
 
 int64_t vsk_kv_scratch_ints(int32_t pages, int32_t slots) {
-  return pages < 0 || slots < 0 ? 0 : 3 * (int64_t)pages + 5 * (int64_t)slots;
+  return pages < 0 || slots < 0 ? 0 : 3 * ((int64_t)pages + slots);
 }
 
 vsk_status vsk_kv_reserve(vsk_ctx *ctx, void *stream, const vsk_kv *kv, const int32_t *seqs,

@@ -61,22 +61,7 @@ template <class T> __device__ inline void sin_cos(uint32_t phase, float *s, floa
   }
 }
 
-// V elements at once; V = 1: any alignment and parity
-template <class T, int V>
-__device__ inline void get(const T *p, float (&x)[V]) {
-  typedef __attribute__((ext_vector_type(V))) T VT;
-  const VT v = *reinterpret_cast<const VT *>(p);
-#pragma unroll
-  for (int i = 0; i < V; ++i) x[i] = (float)v[i];
-}
-template <class T, int V> __device__ inline void put(T *p, const float (&x)[V]) {
-  typedef __attribute__((ext_vector_type(V))) T VT;
-  VT v;
-#pragma unroll
-  for (int i = 0; i < V; ++i) v[i] = (T)x[i];
-  *reinterpret_cast<VT *>(p) = v;
-}
-
+// V: elements of an access; 1: any alignment and parity.
 // Unit u of a head: pairs [u V, u V + V) while they last, then 2 V values of
 // those that pass through.  In a copied tensor: 2 V values from 2 V u on.
 template <class T, int V>
@@ -127,68 +112,90 @@ __global__ __launch_bounds__(256) void k_rotary(const RotaryArgs a) {
       s[i] *= a.inverse ? -a.amplitude : a.amplitude;
     }
   }
-  for (int32_t h = h0; h < a.heads; h += a.hs) {
-    int32_t k = 0, hh = h;
-    if (hh >= a.x[0].heads) hh -= a.x[0].heads, k = 1;
-    if (k == 1 && hh >= a.x[1].heads) hh -= a.x[1].heads, k = 2;
-    const HeadRows &x = a.x[k];
-    if (x.paged && page < 0) continue;
-    const T *src = static_cast<const T *>(x.src) + row * x.src_row + hh * x.src_head;
-    T *dst = static_cast<T *>(x.dst) + hh * x.dst_head +
-             (x.paged ? page * x.dst_page + in_page * x.dst_row : row * x.dst_row);
-    int32_t e0, e1;  // the two runs of V values
-    if (!x.turn) {
-      e0 = 2 * V * u;
-      e1 = e0 + V;
-    } else if (!turned) {
-      e0 = 2 * a.pairs + 2 * (V * u - a.pairs);
-      e1 = e0 + V;
-    } else if (a.interleaved) {
-      e0 = 2 * V * u;
-      e1 = e0 + V;
-    } else {
-      e0 = V * u;
-      e1 = a.pairs + V * u;
+  // where a head's two runs of V values lie
+  struct Place {
+    const T *src;
+    T *dst;
+    int32_t e0, e1;
+    bool turn;
+  };
+  auto place = [&](int32_t h, Place &p) -> bool {
+    int32_t hh = h;
+    const bool second = hh >= a.x[0].heads;
+    if (second) hh -= a.x[0].heads;
+    const bool third = second && hh >= a.x[1].heads;
+    if (third) hh -= a.x[1].heads;
+    const HeadRows &x = third ? a.x[2] : second ? a.x[1] : a.x[0];
+    if (h >= a.heads || (x.paged && page < 0)) return false;
+    p.src = static_cast<const T *>(x.src) + row * x.src_row + hh * x.src_head;
+    p.dst = static_cast<T *>(x.dst) + hh * x.dst_head +
+            (x.paged ? page * x.dst_page + in_page * x.dst_row : row * x.dst_row);
+    p.turn = x.turn && turned;
+    p.e0 = 2 * V * u;
+    p.e1 = p.e0 + V;
+    if (p.turn && !a.interleaved) {
+      p.e0 = V * u;
+      p.e1 = a.pairs + V * u;
     }
-    if constexpr (V == 1) {
+    return true;
+  };
+  if constexpr (V == 1) {
+    for (int32_t h = h0; h < a.heads; h += a.hs) {
+      Place p;
+      if (!place(h, p)) continue;
       // (an odd head: the last unit holds one value)
-      const bool two = e1 < a.d;
-      const T p0 = src[e0], p1 = two ? src[e1] : T(0.f);
-      if (x.turn && turned) {
+      const bool two = p.e1 < a.d;
+      const T p0 = p.src[p.e0], p1 = two ? p.src[p.e1] : T(0.f);
+      if (p.turn) {
         const float f0 = (float)p0, f1 = (float)p1;
-        dst[e0] = (T)(f0 * c[0] - f1 * s[0]);
-        dst[e1] = (T)(f0 * s[0] + f1 * c[0]);
+        p.dst[p.e0] = (T)(f0 * c[0] - f1 * s[0]);
+        p.dst[p.e1] = (T)(f0 * s[0] + f1 * c[0]);
       } else {
-        dst[e0] = p0;
-        if (two) dst[e1] = p1;
+        p.dst[p.e0] = p0;
+        if (two) p.dst[p.e1] = p1;
       }
-    } else {
-      typedef __attribute__((ext_vector_type(V))) T VT;
-      if (x.turn && turned) {
-        float f0[V], f1[V], o0[V], o1[V];
-        get<T, V>(src + e0, f0);
-        get<T, V>(src + e1, f1);
+    }
+  } else {
+    typedef __attribute__((ext_vector_type(V))) T VT;
+    // WAYS heads at a time: their loads are in flight together
+    constexpr int WAYS = 2;
+    for (int32_t h = h0; h < a.heads; h += WAYS * a.hs) {
+      Place p[WAYS];
+      VT v0[WAYS], v1[WAYS];
+      bool on[WAYS];
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          if (a.interleaved) {
-            const int j = 2 * i;
-            const float p0 = j < V ? f0[j % V] : f1[j % V];
-            const float p1 = j < V ? f0[(j + 1) % V] : f1[(j + 1) % V];
-            const float r0 = p0 * c[i] - p1 * s[i], r1 = p0 * s[i] + p1 * c[i];
-            (j < V ? o0[j % V] : o1[j % V]) = r0;
-            (j < V ? o0[(j + 1) % V] : o1[(j + 1) % V]) = r1;
-          } else {
-            o0[i] = f0[i] * c[i] - f1[i] * s[i];
-            o1[i] = f0[i] * s[i] + f1[i] * c[i];
+      for (int y = 0; y < WAYS; ++y) {
+        on[y] = place(h + y * a.hs, p[y]);
+        if (on[y]) {
+          v0[y] = *reinterpret_cast<const VT *>(p[y].src + p[y].e0);
+          v1[y] = *reinterpret_cast<const VT *>(p[y].src + p[y].e1);
+        }
+      }
+#pragma unroll
+      for (int y = 0; y < WAYS; ++y) {
+        if (!on[y]) continue;
+        if (p[y].turn) {
+          const VT x0 = v0[y], x1 = v1[y];
+#pragma unroll
+          for (int i = 0; i < V; ++i) {
+            if (a.interleaved) {
+              const int j = 2 * i;
+              const float p0 = (float)(j < V ? x0[j % V] : x1[j % V]);
+              const float p1 = (float)(j < V ? x0[(j + 1) % V] : x1[(j + 1) % V]);
+              const T r0 = (T)(p0 * c[i] - p1 * s[i]), r1 = (T)(p0 * s[i] + p1 * c[i]);
+              if (j < V)
+                v0[y][j % V] = r0, v0[y][(j + 1) % V] = r1;
+              else
+                v1[y][j % V] = r0, v1[y][(j + 1) % V] = r1;
+            } else {
+              const float p0 = (float)x0[i], p1 = (float)x1[i];
+              v0[y][i] = (T)(p0 * c[i] - p1 * s[i]);
+              v1[y][i] = (T)(p0 * s[i] + p1 * c[i]);
+            }
           }
         }
-        put<T, V>(dst + e0, o0);
-        put<T, V>(dst + e1, o1);
-      } else {
-        const VT v0 = *reinterpret_cast<const VT *>(src + e0);
-        const VT v1 = *reinterpret_cast<const VT *>(src + e1);
-        *reinterpret_cast<VT *>(dst + e0) = v0;
-        *reinterpret_cast<VT *>(dst + e1) = v1;
+        *reinterpret_cast<VT *>(p[y].dst + p[y].e0) = v0[y];
+        *reinterpret_cast<VT *>(p[y].dst + p[y].e1) = v1[y];
       }
     }
   }
@@ -230,7 +237,7 @@ void launch_rotary(vsk_ctx *ctx, hipStream_t st, RotaryArgs &a, int32_t dtype) {
   // cosines are a thread's, whatever the number of its heads
   const int64_t one = (int64_t)a.n * a.max_new * a.units;
   a.hs = 1;
-  while (a.hs < a.heads && one * a.hs < (int64_t)ctx->cu_count * 2048) a.hs *= 2;
+  while (a.hs < a.heads && one * a.hs < (int64_t)ctx->cu_count * 4096) a.hs *= 2;
   if (a.hs > a.heads) a.hs = a.heads;
   const int64_t blocks = ceil_div((int64_t)a.max_new * a.hs * a.units, 256) * a.n;
   VSK_REQUIRE(blocks <= 0x7FFFFFFFll, VSK_ERR_INVALID_BUFFER_SIZE, "too many tokens in one call");
