@@ -89,32 +89,35 @@ __device__ inline AttnSeq attn_seq(const AttnArgs &a, int32_t b) {
   return s;
 }
 
-// The keys that query positions q0 .. q1 see between them, in tiles of KT
-// keys: the sinks' tiles from 0, then the tiles from lo on.
-template <int KT> struct AttnSpan {
-  int32_t lo, hi, sink_tiles, tiles;
-  __device__ int32_t base(int32_t t) const {
-    return t < sink_tiles ? KT * t : lo + KT * (t - sink_tiles);
+// The keys that query positions q0 .. q1 see between them, in groups of G keys
+// and tiles of KT: the sinks' groups from 0, then the groups from lo on.
+template <int KT, int G> struct AttnSpan {
+  int32_t lo, hi, sink_groups, tiles;
+  // first key of a group
+  __device__ int32_t group(int32_t g) const {
+    return g < sink_groups ? G * g : lo + G * (g - sink_groups);
   }
+  __device__ int32_t base(int32_t t) const { return group(KT / G * t); }
 };
-template <int KT>
-__device__ inline AttnSpan<KT> attn_span(const AttnArgs &a, int32_t q0, int32_t q1) {
-  AttnSpan<KT> s;
+template <int KT, int G>
+__device__ inline AttnSpan<KT, G> attn_span(const AttnArgs &a, int32_t q0, int32_t q1) {
+  AttnSpan<KT, G> s;
   s.hi = q1 + 1 > 0 ? q1 + 1 : 0;
   s.lo = 0;
-  s.sink_tiles = 0;
+  s.sink_groups = 0;
   if (a.window > 0) {
     const int64_t first = (int64_t)q0 - a.window + 1;
     if (first > 0) {
-      const int32_t lo = (int32_t)first & ~(KT - 1);
-      const int32_t st = a.sinks / KT + (a.sinks % KT != 0);
-      if ((int64_t)st * KT < lo) {
+      const int32_t lo = (int32_t)first & ~(G - 1);
+      const int32_t st = a.sinks / G + (a.sinks % G != 0);
+      if ((int64_t)st * G < lo) {
         s.lo = lo;
-        s.sink_tiles = st;
+        s.sink_groups = st;
       }
     }
   }
-  s.tiles = s.sink_tiles + (s.hi > s.lo ? (s.hi - s.lo + KT - 1) / KT : 0);
+  const int32_t groups = s.sink_groups + (s.hi > s.lo ? (s.hi - s.lo + G - 1) / G : 0);
+  s.tiles = (groups + KT / G - 1) / (KT / G);
   return s;
 }
 
@@ -244,6 +247,7 @@ void launch_attn_rows(vsk_ctx *ctx, hipStream_t stream, const AttnArgs &a, int32
 constexpr int attn_tile_keys(int d) { return d > 128 ? 32 : 64; }
 // attn_tile.hip: 16-bit types, aligned, row tiles of ATTN_TILE_ROWS
 constexpr int ATTN_TILE_ROWS = 128;
+constexpr int ATTN_TILE_GROUP = 16;  // keys that lie together in a tile
 void launch_attn_tile(vsk_ctx *ctx, hipStream_t stream, const AttnArgs &a, int32_t t);
 // joins the parts that row tiles of `rows` rows left: 16 (launch_attn_rows) or
 // ATTN_TILE_ROWS

@@ -457,7 +457,7 @@ k_attn_rows(const AttnArgs a) {
   const int32_t rows = !have ? 0 : rows_all - row0 < ROWS ? rows_all - row0 : ROWS;
   const int32_t t_lo = row0 / a.group, t_hi = (row0 + rows - 1) / a.group;
   const int32_t q_lo = s.L - s.T + t_lo, q_hi = s.L - s.T + t_hi;
-  const auto span = attn_span<Tile::KT>(a, q_lo, have ? q_hi : -1);
+  const auto span = attn_span<Tile::KT, Tile::KT>(a, q_lo, have ? q_hi : -1);
   const int32_t parts = attn_parts(a, span.tiles);
   if (part >= parts) return;
   const int32_t first = part * a.chunk + (SHARE > 1 ? w : 0);
@@ -579,7 +579,7 @@ k_attn_rows(const AttnArgs a) {
 // Joins the parts of one output row: sum of the parts' values and sums, each
 // times 2^(its maximum - the largest).  A block a row; the threads take four
 // values each of several parts at a time.
-template <class T, int DV, int KTILE, bool ALIGNED>
+template <class T, int DV, int KTILE, int G, bool ALIGNED>
 __global__ __launch_bounds__(256) void k_attn_join(const AttnArgs a, const int32_t RT) {
   constexpr int LANES = DV / 4, WAYS = 256 / LANES;
   __shared__ __attribute__((aligned(16))) float so[WAYS][DV];
@@ -605,7 +605,7 @@ __global__ __launch_bounds__(256) void k_attn_join(const AttnArgs a, const int32
   const int32_t all = (s.T < a.max_new ? s.T : a.max_new) * a.group;
   const int32_t last = row0 + RT < all ? row0 + RT - 1 : all - 1;
   const int32_t p0 = s.L - s.T;
-  const AttnSpan<KTILE> span = attn_span<KTILE>(a, p0 + row0 / a.group, p0 + last / a.group);
+  const auto span = attn_span<KTILE, G>(a, p0 + row0 / a.group, p0 + last / a.group);
   const int32_t parts = attn_parts(a, span.tiles);
   if (parts == 1) return;  // written by the row tile itself
   float top = i0 < parts ? m0 : -INFINITY;
@@ -715,11 +715,11 @@ void join_head(hipStream_t st, const AttnArgs &a, bool aligned, int32_t rows, un
   constexpr int KR = 16 * SUBS<T>, KB = attn_tile_keys(DV);
   if (rows == ROWS) {
     if (aligned)
-      k_attn_join<T, DV, KR, true><<<g, 256, 0, st>>>(a, rows);
+      k_attn_join<T, DV, KR, KR, true><<<g, 256, 0, st>>>(a, rows);
     else
-      k_attn_join<T, DV, KR, false><<<g, 256, 0, st>>>(a, rows);
+      k_attn_join<T, DV, KR, KR, false><<<g, 256, 0, st>>>(a, rows);
   } else if constexpr (sizeof(T) == 2) {  // (tiles are for 16-bit, aligned operands)
-    k_attn_join<T, DV, KB, true><<<g, 256, 0, st>>>(a, rows);
+    k_attn_join<T, DV, KB, ATTN_TILE_GROUP, true><<<g, 256, 0, st>>>(a, rows);
   }
 }
 template <class T>

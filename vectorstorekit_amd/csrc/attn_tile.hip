@@ -12,6 +12,10 @@
 // fetches the piece that belongs in its slot), so that the reads of K (32 rows
 // of one piece) and of V (4 rows of 32 bytes) meet every bank once.
 //
+// A tile's keys are four groups (of a head over 128 two) of 16 that lie
+// together: the few first keys that a window leaves visible share a tile with
+// the first that it shows.
+//
 // The weights are rounded to the type of V before the second product, with an
 // error of the size of the output's own rounding; sums stay in fp32.
 #include "attn.hpp"
@@ -20,7 +24,6 @@
 namespace vsk {
 
 namespace {
-
 
 typedef __attribute__((ext_vector_type(4))) short i16x4;
 constexpr int NW = 4;  // waves of a workgroup
@@ -63,7 +66,7 @@ __device__ inline float max3(float a, float b, float c) {
 template <class T, int DP>
 __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void k_attn_tile(const AttnArgs a) {
   typedef typename Mm<T>::V8 V8;
-  constexpr int KT = attn_tile_keys(DP), U = KT / 32;
+  constexpr int KT = attn_tile_keys(DP), U = KT / 32, G = ATTN_TILE_GROUP;
   constexpr int PITCH = DP <= 64 ? 64 : DP <= 128 ? 128 : 256;
   constexpr int CH = PITCH / 8;      // 16-byte pieces of a row
   constexpr int ROWB = 2 * PITCH;    // bytes of a row
@@ -95,7 +98,7 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void k_attn_tile(const 
   if (row0 >= rows_all) return;
   const int32_t last = row0 + ROWS < rows_all ? row0 + ROWS - 1 : rows_all - 1;
   const int32_t p0 = s.L - s.T;
-  const AttnSpan<KT> span = attn_span<KT>(a, p0 + row0 / a.group, p0 + last / a.group);
+  const auto span = attn_span<KT, G>(a, p0 + row0 / a.group, p0 + last / a.group);
   const int32_t parts = attn_parts(a, span.tiles);
   if (part >= parts) return;
   const int32_t first = part * a.chunk;
@@ -156,7 +159,7 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void k_attn_tile(const 
   int32_t tb = 0;
   auto addresses = [&](int32_t i) {
     tb = i;
-    const int32_t j16 = (span.base(i + lane) + MINE * w) & ~15, j = attn_row16(s, j16);
+    const int32_t j = attn_row16(s, span.group(KT / G * (i + lane) + MINE * w / G));
     int64_t page = 0, in = s.key0 + j;
     if (a.table) {
       int32_t x = a.table[s.slot * a.table_stride + (j >> a.page_shift)];
@@ -181,7 +184,7 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void k_attn_tile(const 
   const bool full = a.d == PITCH;
   auto fetch = [&](int32_t i, lds_char *to, bool keys) {
     const uint64_t base = keys ? lane_of(k_lo, k_hi, i - tb) : lane_of(v_lo, v_hi, i - tb);
-    const int32_t j0 = span.base(i) + MINE * w;
+    const int32_t j0 = span.group(KT / G * i + MINE * w / G) + MINE * w % G;
     to += MINE * w * ROWB;
     if (full && j0 + MINE <= s.L) {
 #pragma unroll
@@ -261,14 +264,18 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void k_attn_tile(const 
   // -inf for the keys that the lane's row does not see.  Bit c of a
   // word is key c of the 32 that the word is for: comparisons a row, not a key.
   auto up_to = [](int32_t x) -> uint32_t { return x < 0 ? 0u : x > 30 ? ~0u : (2u << x) - 1; };
-  auto hide = [&](f32x16 (&sc)[U], int32_t kb) {
+  auto sees = [&](int32_t b) -> uint32_t {
+    uint32_t see = ~0u;
+    if (a.window > 0)
+      see = (pos < a.window ? ~0u : ~up_to(pos - a.window - b)) | up_to(a.sinks - 1 - b);
+    return see & up_to(pos - b);
+  };
+  auto hide = [&](f32x16 (&sc)[U], int32_t i) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int32_t b = kb + 32 * u + 4 * h2;
-      uint32_t see = ~0u;
-      if (a.window > 0)
-        see = (pos < a.window ? ~0u : ~up_to(pos - a.window - b)) | up_to(a.sinks - 1 - b);
-      see &= up_to(pos - b);
+      const int32_t b = span.group(KT / G * i + 2 * u), c = span.group(KT / G * i + 2 * u + 1);
+      uint32_t see = sees(b + 4 * h2);
+      if (c != b + G) see = (see & 0xFFFFu) | (sees(c - G + 4 * h2) & 0xFFFF0000u);
 #pragma unroll
       for (int x = 0; x < 16; ++x) {
         const uint32_t on = (uint32_t)((int32_t)(see << (31 - 8 * (x >> 2) - (x & 3))) >> 31);
@@ -291,18 +298,19 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void k_attn_tile(const 
     const unsigned short inf = (unsigned short)(Mm<T>::EXP & 0xFFFF);
     return __any(top[0] == inf || top[1] == inf);
   };
-  // a tile that not every row of the block sees whole
-  auto edge = [&](int32_t kb, const lds_char *kt, const lds_char *vt) {
+  // tile i, that not every row of the block sees whole
+  auto edge = [&](int32_t i, const lds_char *kt, const lds_char *vt) {
     // (a wave whose rows see none of it only brings its rows)
-    const bool any = kb <= q_hi && (a.window <= 0 || q_lo - (kb + KT - 1) < a.window || kb < a.sinks);
+    const int32_t kb = span.base(i), ke = span.group(KT / G * (i + 1) - 1) + G;  // (end)
+    const bool any = kb <= q_hi && (a.window <= 0 || q_lo - ke < a.window - 1 || kb < a.sinks);
     if (!any) return;
-    const bool whole = kb + KT - 1 <= q_lo &&
-                       (a.window <= 0 || q_hi - kb < a.window || kb + KT <= a.sinks);
+    const bool whole = ke == kb + KT && ke <= q_lo + 1 &&
+                       (a.window <= 0 || q_hi - kb < a.window || ke <= a.sinks);
     f32x16 sc[U];
     if (whole || !not_finite(vt)) {
       scores(kt, sc);
       const int vb = v_base(vt);
-      if (!whole) hide(sc, kb);
+      if (!whole) hide(sc, i);
       settle(largest(sc));
       const float use = m == -INFINITY ? 0.f : m;
 #pragma unroll
@@ -323,7 +331,7 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void k_attn_tile(const 
     // a time, each row takes only those it sees.  (A rare path: the sums wait
     // in memory meanwhile, so that it takes no registers from the others.)
     scores(kt, sc);
-    hide(sc, kb);
+    hide(sc, i);
     settle(largest(sc));
     const float use = m == -INFINITY ? 0.f : m;
     float held[16 * DT], wt[16 * U];
@@ -340,7 +348,7 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void k_attn_tile(const 
       // whose h2 is bit 2 of j
       const float y = __shfl(wt[16 * (j >> 5) + 4 * ((j >> 3) & 3) + (j & 3)],
                              n + 32 * ((j >> 2) & 1));
-      if (!attn_sees(a, pos, kb + j)) continue;
+      if (!attn_sees(a, pos, span.group(KT / G * i + j / G) + j % G)) continue;
 #pragma unroll 1
       for (int c = 0; c < 4 * DT; ++c) {
         const lds_as T *v =
@@ -358,10 +366,10 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void k_attn_tile(const 
   int32_t hot0 = first, hot1 = first;
   {
     const int32_t lo = p0 + row0 / a.group, hi = p0 + last / a.group;
-    int32_t x0 = span.sink_tiles;
-    if (a.window > 0 && hi - span.lo >= a.window)
-      x0 += (hi - a.window - span.lo) / KT + 1;
-    const int32_t x1 = lo + 1 > span.lo ? span.sink_tiles + (lo + 1 - span.lo) / KT : 0;
+    int32_t x0 = G * span.sink_groups;
+    const int32_t x1 = lo + 1 > span.lo ? (x0 + lo + 1 - span.lo) / KT : 0;
+    if (a.window > 0 && hi - span.lo >= a.window) x0 += hi - a.window - span.lo + 1;
+    x0 = (x0 + KT - 1) / KT;
     hot0 = x0 > first ? x0 : first;
     hot1 = x1 < end ? x1 : end;
   }
@@ -391,7 +399,7 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void k_attn_tile(const 
   for (int32_t i = first; i < end;) {
     if (i < hot0 || i >= hot1) {
       ahead(i);
-      edge(span.base(i), kbuf + kslot * TILEB, vbuf + ((i - first) & 1) * TILEB);
+      edge(i, kbuf + kslot * TILEB, vbuf + ((i - first) & 1) * TILEB);
       done();
       ++i;
       continue;
