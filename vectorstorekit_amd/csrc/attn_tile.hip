@@ -472,9 +472,9 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void k_attn_tile(const 
   }
 
   const float sum = xor32_sum(l);
-  if (!real) return;
   const int64_t out_row = (s.token0 + my_t) * a.heads + my_head;
   if (parts > 1) {
+    if (!real) return;
     const int64_t x = (int64_t)part * a.tokens * a.heads + out_row;
     float *dst = a.part_o + x * PITCH;
 #pragma unroll
@@ -490,19 +490,30 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void k_attn_tile(const 
     return;
   }
   const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
-  T *dst = static_cast<T *>(a.out) + (s.token0 + my_t) * a.o_row + my_head * a.o_head;
+  // The outputs leave by way of LDS (no wave reads keys any more), so that a
+  // store of a wave is whole rows and not eight bytes of each.
   typedef __attribute__((ext_vector_type(4))) T V4;
+  lds_char *const obuf = (QLDS ? (lds_char *)queries_lds : kbuf) + 32 * w * ROWB;
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
     for (int b = 0; b < 4; ++b) {
-      const int e = 32 * dt + 8 * b + 4 * h2;
       V4 y;
 #pragma unroll
       for (int x = 0; x < 4; ++x) y[x] = (T)(acc[dt][4 * b + x] * inv);
-      if (e < a.d) *reinterpret_cast<V4 *>(dst + e) = y;
+      *(lds_as V4 *)(obuf + n * ROWB + (((4 * dt + b) ^ k_swizzle<CH>(n)) << 4) + 8 * h2) = y;
     }
-  if (a.lse && h2 == 0)
+  const int64_t to = real ? (s.token0 + my_t) * a.o_row + my_head * a.o_head : INT64_MIN;
+#pragma unroll
+  for (int x = 0; x < 32 / RPI; ++x) {
+    const int r = x * RPI + sub;
+    typedef __attribute__((ext_vector_type(4), aligned(8))) uint32_t Piece;
+    const u32x4 y = *(const lds_as u32x4 *)(obuf + r * ROWB + ((piece ^ k_swizzle<CH>(r)) << 4));
+    const int64_t row = __shfl(to, r);
+    if (row != INT64_MIN && 8 * piece < a.d)
+      *reinterpret_cast<Piece *>(static_cast<T *>(a.out) + row + 8 * piece) = y;
+  }
+  if (a.lse && h2 == 0 && real)
     a.lse[out_row] = sum > 0.f ? (m + __log2f(sum)) * 0.6931471805599453f
                                : sum != sum ? sum : -INFINITY;
 }
