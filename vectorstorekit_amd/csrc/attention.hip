@@ -47,7 +47,21 @@ Plan plan_of(const vsk_ctx *ctx, const vsk_kv *kv, const vsk_new_tokens *news,
   // blocks that a compute unit holds at once (by their registers), twice over
   // (a head of 256: once): fewer leave it idle at the end, more start too often
   int64_t want = (kv->head_dim <= 64 ? 8 : kv->head_dim <= 128 ? 6 : 1) * (int64_t)ctx->cu_count;
-  if (kv->dtype != VSK_DTYPE_F32 && rows >= 64 && aligned_operands(kv, args)) {
+  int64_t keys = kv->table ? (int64_t)kv->width * kv->page_size : kv->pages;
+  if (args->max_length > 0 && args->max_length < keys) keys = args->max_length;
+  // Row tiles of 128 where there are rows to fill them and work for the
+  // device.  Under 64 rows of a key head most of a tile would be empty; with
+  // few rows in all, or few products, tiles of 16 spread over more waves and
+  // end sooner.  Measured in 16 bits, tiles of 128 against tiles of 16 (us):
+  // one prompt of 1,000 tokens, 8 heads of 64 of their own 21 / 13, 32 heads
+  // of 128 on 8 27 / 72 (over the bound on rows); 64 new tokens of those 8
+  // heads after 4,000 keys 23 / 15, after 30,000 25 / 33 (over the bound on
+  // products); 4 prompts of 64 after 2,000 of those 32 45 / 42, 16 of 32 61 / 79.
+  const int64_t most = args->window > 0 && args->window + (int64_t)args->sinks < keys
+                           ? args->window + (int64_t)args->sinks : keys;
+  const bool few = pairs * rows < 32 * (int64_t)ctx->cu_count &&
+                   pairs * rows * most < 32768 * (int64_t)ctx->cu_count;
+  if (kv->dtype != VSK_DTYPE_F32 && rows >= 64 && !few && aligned_operands(kv, args)) {
     p.tile = true;
     row_tile = ATTN_TILE_ROWS;
     key_tile = attn_tile_keys(kv->head_dim);
@@ -63,8 +77,6 @@ Plan plan_of(const vsk_ctx *ctx, const vsk_kv *kv, const vsk_new_tokens *news,
       return p;
     }
   }
-  int64_t keys = kv->table ? (int64_t)kv->width * kv->page_size : kv->pages;
-  if (args->max_length > 0 && args->max_length < keys) keys = args->max_length;
   if (args->window > 0) {
     const int64_t seen = (int64_t)args->window + args->sinks + ceil_div(row_tile, group) +
                          2 * key_tile;
