@@ -603,6 +603,147 @@ def test_other_stream_and_graph(ctx):
 
 # ------------------------------------------------------------------------ refusals
 
+# -------------------------------------------- many rows: tiles of 128 query rows
+
+def attended_at_once(q, k, v, scale, window, sinks):
+    """``attended``, all heads and tokens in one product."""
+    t, heads, d = q.shape
+    u = U[q.dtype]
+    q, k, v = (x.detach().cpu().double().transpose(0, 1) for x in (q, k, v))
+    length, group = k.shape[1], heads // k.shape[0]
+    if t == 0 or length == 0:
+        zero = torch.zeros(t, heads, d, dtype=torch.float64)
+        return zero, torch.full((t, heads), -math.inf, dtype=torch.float64), zero
+    k, v = (x.repeat_interleave(group, 0) for x in (k, v))
+    j, pos = torch.arange(length)[None], torch.arange(length - t, length)[:, None]
+    see = j <= pos
+    if window:
+        see = see & ((pos - j < window) | (j < sinks))
+    some = see.any(1)[None, :, None]
+    s = (q @ k.transpose(1, 2) * scale).masked_fill(~see, -math.inf)
+    lse = torch.logsumexp(s, 2)
+    w = torch.exp(s - lse[..., None].masked_fill(~some, 0.0)).masked_fill(~see, 0.0)
+    out = w @ v
+    products = (q.abs() @ k.abs().transpose(1, 2)).masked_fill(~see, 0.0)
+    e = 2.0 ** -24 * (d + 8) * scale * products.amax(2, keepdim=True)
+    peak = torch.where(see[None], v.abs().amax(2)[:, None], 0.0).amax(2, keepdim=True)
+    tol = u * out.abs() + peak * (2 * (e + 2.0 ** -21 + 2.0 ** -24 * (length + 16)) + u)
+    return out.transpose(0, 1), lse.transpose(0, 1), tol.transpose(0, 1)
+
+
+def kernels_of(ctx, f):
+    ctx.profile_reset()
+    ctx.profile(True)
+    try:
+        out = f()
+        return out, set(ctx.profile_stats())
+    finally:
+        ctx.profile(False)
+        ctx.profile_reset()
+
+
+@pytest.mark.parametrize("dtype", [BF, F16])
+@pytest.mark.parametrize("order", ["nhd", "hnd"])
+@pytest.mark.parametrize("news,lengths,page,heads,kv,d,window,sinks", [
+    ([70, 130], [200, 130], 32, 64, 8, 128, 33, 4),
+    ([65, 64, 63], [65, 100, 63], 16, 48, 48, 64, 16, 16),
+    ([300], [300], 64, 32, 4, 96, 64, 0),
+    ([40, 9, 0], [64, 20, 5], 16, 80, 10, 256, None, 0),
+    ([260], [900], 64, 36, 9, 80, 200, 70),    # the sinks' last tile holds window too
+    ([129], [1500], 16, 64, 8, 128, 300, 17),
+    ([1, 512], [1, 512], 16, 16, 2, 40, 100, 1),
+    ([150], [1000], 128, 60, 20, 256, 333, 40),
+    ([64], [20000], 64, 8, 1, 128, None, 0),   # few rows, many keys: in parts
+    ([64], [9000], 32, 16, 2, 256, None, 0),
+    ([64], [9000], 32, 16, 16, 64, 8500, 3),
+])
+def test_prompt_attention_of_many_rows(ctx, dtype, order, news, lengths, page, heads, kv, d,
+                                       window, sinks):
+    cache, seqs = filled(ctx, lengths, page, kv, d, dtype, order=order, seed=d + 2)
+    starts = [0] + list(np.cumsum(news))
+    q = normal(gen(11), starts[-1], heads, d, dtype=dtype)
+    (out, lse), used = kernels_of(ctx, lambda: cache.attend(
+        q, starts=starts, max_new=max(news), window=window, sinks=sinks, return_lse=True))
+    assert "attn_tile" in used
+    for i, (kk, vv) in enumerate(seqs):
+        a, b = starts[i], starts[i + 1]
+        o, l, t = attended_at_once(q[a:b], kk[0], vv[0], d ** -0.5, window, sinks)
+        check(out[a:b], o, t)
+        check_norm(out[a:b], o, dtype)
+        check(lse[a:b], l, 2.0 ** -16 * (1 + l.abs()))
+
+
+@pytest.mark.parametrize("dtype", [BF, F16])
+@pytest.mark.parametrize("lengths,heads,kv,d,window,sinks", [
+    ([520, 31], 8, 2, 128, 100, 130),
+    ([333, 0, 1], 12, 12, 64, 90, 5),
+    ([130], 64, 64, 128, None, 0),
+    ([190, 75], 32, 4, 256, 32, 0),
+    ([1030], 8, 8, 96, 64, 4),
+    ([500], 33, 11, 72, 1, 1),
+])
+def test_window_attention_of_many_rows(ctx, dtype, lengths, heads, kv, d, window, sinks):
+    from vectorstorekit_amd import window_attention
+
+    starts = [0] + list(np.cumsum(lengths))
+    packed = normal(gen(d + 3), starts[-1], heads + 2 * kv, d, dtype=dtype)
+    q, k, v = packed[:, :heads], packed[:, heads:heads + kv], packed[:, heads + kv:]
+    (out, lse), used = kernels_of(ctx, lambda: window_attention(
+        ctx, q, k, v, starts=starts, max_length=max(lengths), window=window, sinks=sinks,
+        return_lse=True))
+    assert "attn_tile" in used
+    for i in range(len(lengths)):
+        a, b = starts[i], starts[i + 1]
+        o, l, t = attended_at_once(q[a:b], k[a:b], v[a:b], d ** -0.5, window, sinks)
+        check(out[a:b], o, t)
+        check_norm(out[a:b], o, dtype)
+        check(lse[a:b], l, 2.0 ** -16 * (1 + l.abs()))
+
+
+def test_many_queries_before_the_keys(ctx):
+    from vectorstorekit_amd import window_attention
+
+    q, k, v = (normal(gen(12), n, 32, 64, dtype=BF) for n in (300, 250, 250))
+    out, lse = window_attention(ctx, q, k, v, starts=[0, 290, 300], k_starts=[0, 250, 250],
+                                return_lse=True)
+    assert not out[:40].any() and not out[290:].any()
+    assert bool(torch.isneginf(lse[:40]).all()) and bool(torch.isneginf(lse[290:]).all())
+    o, _, t = attended_at_once(q[40:290], k, v, 64 ** -0.5, None, 0)
+    check(out[40:290], o, t)
+
+
+@pytest.mark.parametrize("dtype", [BF, F16])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("heads,kv,d,n", [(64, 32, 128, 150), (24, 24, 64, 400),
+                                          (128, 16, 256, 70)])
+def test_masked_places_of_many_rows(ctx, dtype, bad, heads, kv, d, n):
+    """As above, and a hidden key between the sinks and the window."""
+    from vectorstorekit_amd import window_attention
+
+    g = gen(13)
+    q, k, v = (normal(g, n, h, d, dtype=dtype) for h in (heads, kv, kv))
+    window, sinks = 20, 3
+    clean, _, t = attended_at_once(q, k, v, d ** -0.5, window, sinks)
+    for x, j in ((k, n - 45), (v, n - 45), (v, 1), (v, 7), (k, 7)):
+        y = [z.clone() for z in (k, v)]
+        (y[0] if x is k else y[1])[j, 0, d // 2] = bad
+        out = window_attention(ctx, q, *y, starts=[0, n], window=window, sinks=sinks)
+        rows = torch.arange(n)
+        see = (rows >= j) & ((rows - j < window) | (j < sinks))
+        first = slice(0, heads // kv)
+        hidden = torch.ones(n, heads, dtype=torch.bool)
+        hidden[see, first] = False
+        got = out.cpu().double()
+        assert bool(((got - clean).abs() <= t)[hidden].all())
+        if x is v:
+            assert not bool(torch.isfinite(got[see][:, first, d // 2]).any())
+            rest = torch.ones(d, dtype=torch.bool)
+            rest[d // 2] = False
+            assert bool(((got - clean).abs() <= t)[see][:, first][..., rest].all())
+        elif math.isnan(bad):
+            assert bool(torch.isnan(got[see][:, first]).all())
+
+
 def test_refusals(ctx):
     from vectorstorekit_amd import PagedKVCache, RotaryEmbedding, VSKError, window_attention
 
