@@ -43,19 +43,19 @@ assert _ROWS.size == ctypes.sizeof(_lib.vsk_head_rows)
 assert _NEWS.size == ctypes.sizeof(_lib.vsk_new_tokens)
 
 
-def _stream(device) -> int:
-    return torch._C._cuda_getCurrentRawStream(device.index or 0)
+def _stream(gpu: int) -> int:
+    return torch._C._cuda_getCurrentRawStream(gpu)
 
 
 def _empty(x):
     """An uninitialised dense tensor like x."""
-    return torch.empty_like(x) if x.is_contiguous() else torch.empty(x.shape, dtype=x.dtype,
-                                                                     device=x.device)
+    return torch.empty_like(x, memory_format=torch.contiguous_format)
 
 
-def _tensor(x, name, dtype=None, dims=None):
-    if not isinstance(x, torch.Tensor) or not x.is_cuda:
-        raise VSKError(-2, f"{name} must be a tensor on the GPU")
+def _tensor(gpu, x, name, dtype=None, dims=None):
+    """x, checked to be a tensor on that GPU."""
+    if not isinstance(x, torch.Tensor) or x.get_device() != gpu:
+        raise VSKError(-2, f"{name} must be a tensor on GPU {gpu}, the context's")
     if dtype is not None and x.dtype != dtype:
         raise VSKError(-2, f"{name} is {x.dtype}, not {dtype}")
     if dims is not None and x.dim() != dims:
@@ -63,20 +63,20 @@ def _tensor(x, name, dtype=None, dims=None):
     return x
 
 
-def _dense_heads(x, name):
+def _dense_heads(x):
     """x itself, or a copy whose innermost dimension is dense."""
     return x if x.stride(-1) == 1 or x.shape[-1] == 1 else x.contiguous()
 
 
-def _ints(x, name, device):
-    """A dense int32 vector on the device; a host sequence is copied there."""
+def _ints(gpu, x, name):
+    """A dense int32 vector on that GPU; a host sequence is copied there."""
     if isinstance(x, torch.Tensor):
-        _tensor(x, name, torch.int32, 1)
+        _tensor(gpu, x, name, torch.int32, 1)
         return x if x.is_contiguous() else x.contiguous()
     a = np.asarray(x)
     if a.ndim != 1 or (a.size and a.dtype.kind not in "iu"):
         raise VSKError(-2, f"{name} must be a vector of whole numbers")
-    return torch.from_numpy(a.astype(np.int32)).to(device)
+    return torch.from_numpy(a.astype(np.int32)).to(torch.device("cuda", gpu))
 
 
 def _rows(src, dst=None):
@@ -180,31 +180,42 @@ class RotaryEmbedding:
         ``inverse`` turns back (with the same factor): the gradient of
         ``apply``, and, with positions p - p', a cached key's move from p to
         p'."""
-        tensors = [x for x in (q, k) if x is not None]
-        for x, name in zip(tensors, ("q", "k")):
-            _tensor(x, name, q.dtype, 3)
-            if x.shape[2] != self.head_dim or x.shape[0] != q.shape[0]:
-                raise VSKError(-4, f"{name} is {tuple(x.shape)}: head_dim is {self.head_dim}, "
-                               f"tokens are {q.shape[0]}")
-        if q.dtype not in _TYPES:
-            raise VSKError(-8, f"{q.dtype} is not supported")
-        _tensor(positions, "positions", torch.int32, 1)
-        if positions.shape[0] != q.shape[0]:
-            raise VSKError(-4, f"{positions.shape[0]} positions for {q.shape[0]} tokens")
+        ctx, gpu = self.ctx, self.ctx.device
+        tokens, dtype = self._checked(_tensor(gpu, q, "q", None, 3), "q", None), q.dtype
+        if k is not None:
+            self._checked(_tensor(gpu, k, "k", dtype, 3), "k", tokens)
+        if dtype not in _TYPES:
+            raise VSKError(-8, f"{dtype} is not supported")
+        if _tensor(gpu, positions, "positions", torch.int32, 1).shape[0] != tokens:
+            raise VSKError(-4, f"{positions.shape[0]} positions for {tokens} tokens")
         positions = positions.contiguous()
         if inplace:
-            if any(x.stride(-1) != 1 for x in tensors):
+            if q.stride(-1) != 1 or k is not None and k.stride(-1) != 1:
                 raise VSKError(-2, "inplace needs dense heads")
-            outs = tensors
+            to_q, to_k = q, k
         else:
-            tensors = [_dense_heads(x, "q") for x in tensors]
-            outs = [_empty(x) for x in tensors]
-        if q.shape[0] and all(x.shape[1] for x in tensors):
-            rows = b"".join(map(_rows, tensors, outs))
-            self.ctx.check(self.ctx.lib.vsk_rotary_apply(
-                self.ctx.handle, _stream(q.device), self.handle, _TYPES[q.dtype], self.head_dim,
-                q.shape[0], positions.data_ptr(), 1 if inverse else 0, rows, len(tensors)))
-        return outs[0] if k is None else tuple(outs)
+            q = _dense_heads(q)
+            to_q, to_k = _empty(q), None
+            if k is not None:
+                k = _dense_heads(k)
+                to_k = _empty(k)
+        rows = _rows(q, to_q) if q.shape[1] else b""
+        if k is not None and k.shape[1]:
+            rows += _rows(k, to_k)
+        if tokens and rows:
+            status = ctx.lib.vsk_rotary_apply(
+                ctx.handle, _stream(gpu), self.handle, _TYPES[dtype], self.head_dim, tokens,
+                positions.data_ptr(), 1 if inverse else 0, rows, len(rows) // _ROWS.size)
+            if status:
+                ctx.check(status)
+        return to_q if k is None else (to_q, to_k)
+
+    def _checked(self, x, name, tokens):
+        n, _, d = x.shape
+        if d != self.head_dim or tokens is not None and n != tokens:
+            raise VSKError(-4, f"{name} is {tuple(x.shape)}: head_dim is {self.head_dim}"
+                           + (f", tokens are {tokens}" if tokens is not None else ""))
+        return n
 
 
 def _attend(ctx, kv, layer, q, news, k_starts, scale, window, sinks, max_length, return_lse):
@@ -232,7 +243,7 @@ def _attend(ctx, kv, layer, q, news, k_starts, scale, window, sinks, max_length,
         if not need:
             break
         work = torch.empty(need, dtype=torch.uint8, device=q.device)
-    status = lib.vsk_attention(handle, _stream(q.device), kv, layer, news, a)
+    status = lib.vsk_attention(handle, _stream(ctx.device), kv, layer, news, a)
     if status:
         ctx.check(status)
     return (out, lse) if return_lse else out
@@ -279,7 +290,7 @@ class PagedKVCache:
 
     def _hold(self, ctx, k, v, table, lengths, refs):
         for x, name in ((k, "k"), (v, "v")):
-            _tensor(x, name)
+            _tensor(ctx.device, x, name)
             if x.dim() not in (4, 5):
                 raise VSKError(-4, f"{name} must be (layers x) pages x page_size x kv_heads x "
                                "head_dim")
@@ -289,8 +300,8 @@ class PagedKVCache:
                 raise VSKError(-2, f"the heads of {name} must be dense")
         if k.shape != v.shape or k.dtype != v.dtype:
             raise VSKError(-4, "k and v differ in shape or type")
-        _tensor(table, "table", torch.int32, 2)
-        _tensor(lengths, "lengths", torch.int32, 1)
+        _tensor(ctx.device, table, "table", torch.int32, 2)
+        _tensor(ctx.device, lengths, "lengths", torch.int32, 1)
         if table.shape[0] != lengths.shape[0] or table.stride(1) != 1 and table.shape[1] != 1:
             raise VSKError(-4, "table must be slots x width, dense rows, lengths of slots")
         if lengths.stride(0) != 1 and lengths.shape[0] != 1:
@@ -304,7 +315,7 @@ class PagedKVCache:
         self.layers, self.pages, self.page_size = layers, pages, page_size
         self.kv_heads, self.head_dim, self.dtype = kv_heads, head_dim, k.dtype
         self.slots, self.width = table.shape
-        self.device = k.device
+        self.device, self.gpu = k.device, ctx.device
         kv = _lib.vsk_kv()
         kv.k, kv.v = k.data_ptr(), v.data_ptr()
         kv.k_layer, kv.k_page, kv.k_row, kv.k_head = k5.stride()[:4]
@@ -314,7 +325,7 @@ class PagedKVCache:
         kv.dtype, kv.layers, kv.pages, kv.page_size = _TYPES[k.dtype], layers, pages, page_size
         kv.kv_heads, kv.head_dim, kv.slots, kv.width = kv_heads, head_dim, self.slots, self.width
         if refs is not None:
-            _tensor(refs, "refs", torch.int32, 1)
+            _tensor(ctx.device, refs, "refs", torch.int32, 1)
             if refs.shape[0] != pages or refs.stride(0) != 1 and pages != 1:
                 raise VSKError(-4, "refs must be a dense vector of a count a page")
             self.status = torch.zeros(4, dtype=torch.int32, device=k.device)
@@ -331,7 +342,7 @@ class PagedKVCache:
         tokens = x.shape[0]
         n, most, at = tokens, 1, None
         if starts is not None:
-            at = _ints(starts, "starts", self.device)
+            at = _ints(self.gpu, starts, "starts")
             n = at.shape[0] - 1
             if n < 0:
                 raise VSKError(-4, "starts holds an offset a sequence and the end")
@@ -339,7 +350,7 @@ class PagedKVCache:
             if most < 0:
                 raise VSKError(-2, "max_new must not be negative")
         if seqs is not None:
-            seqs = _ints(seqs, "seqs", self.device)
+            seqs = _ints(self.gpu, seqs, "seqs")
             if seqs.shape[0] != n:
                 raise VSKError(-4, f"{seqs.shape[0]} slots for {n} sequences")
         elif n > self.slots:
@@ -348,11 +359,11 @@ class PagedKVCache:
                           seqs.data_ptr() if seqs is not None else 0, n, most, tokens), (at, seqs)
 
     def _heads(self, x, name, heads=None):
-        _tensor(x, name, self.dtype, 3)
+        _tensor(self.gpu, x, name, self.dtype, 3)
         if x.shape[2] != self.head_dim or heads is not None and x.shape[1] != heads:
             raise VSKError(-4, f"{name} is {tuple(x.shape)}: heads of {self.head_dim} are wanted"
                            + (f", {heads} of them" if heads is not None else ""))
-        return _dense_heads(x, name)
+        return _dense_heads(x)
 
     def append(self, k, v, *, starts=None, seqs=None, max_new=None, layer: int = 0,
                rotary: RotaryEmbedding | None = None, q=None):
@@ -376,7 +387,7 @@ class PagedKVCache:
             qr = _rows(q, out)
         if k.shape[0]:
             self.ctx.check(self.ctx.lib.vsk_kv_append(
-                self.ctx.handle, _stream(self.device), self._ref, layer, news, _rows(k), _rows(v),
+                self.ctx.handle, _stream(self.gpu), self._ref, layer, news, _rows(k), _rows(v),
                 rotary.handle if rotary is not None else None, qr))
         return out
 
@@ -407,10 +418,10 @@ class PagedKVCache:
         """Grows the sequences in these slots by these numbers of tokens,
         taking the lowest free pages; ``missing()`` tells of a shortage."""
         self._keeping()
-        s, c = _ints(seqs, "seqs", self.device), _ints(counts, "counts", self.device)
+        s, c = _ints(self.gpu, seqs, "seqs"), _ints(self.gpu, counts, "counts")
         if s.shape != c.shape:
             raise VSKError(-4, f"{s.shape[0]} slots, {c.shape[0]} counts")
-        self.ctx.check(self.ctx.lib.vsk_kv_reserve(self.ctx.handle, _stream(self.device),
+        self.ctx.check(self.ctx.lib.vsk_kv_reserve(self.ctx.handle, _stream(self.gpu),
                                                    self._ref, s.data_ptr(), c.data_ptr(),
                                                    s.shape[0]))
 
@@ -428,34 +439,34 @@ class PagedKVCache:
             c = list(children)
             if len(set(c)) != len(c) or set(c) & set(parents):
                 raise VSKError(-2, "children must be distinct and none of them a parent")
-        p, c = _ints(parents, "parents", self.device), _ints(children, "children", self.device)
+        p, c = _ints(self.gpu, parents, "parents"), _ints(self.gpu, children, "children")
         if p.shape != c.shape:
             raise VSKError(-4, f"{p.shape[0]} parents, {c.shape[0]} children")
-        self.ctx.check(self.ctx.lib.vsk_kv_fork(self.ctx.handle, _stream(self.device), self._ref,
+        self.ctx.check(self.ctx.lib.vsk_kv_fork(self.ctx.handle, _stream(self.gpu), self._ref,
                                                 p.data_ptr(), c.data_ptr(), p.shape[0]))
 
     def free(self, seqs):
         """Releases the pages of the sequences in these slots."""
         self._keeping()
-        s = _ints(seqs, "seqs", self.device)
-        self.ctx.check(self.ctx.lib.vsk_kv_free(self.ctx.handle, _stream(self.device), self._ref,
+        s = _ints(self.gpu, seqs, "seqs")
+        self.ctx.check(self.ctx.lib.vsk_kv_free(self.ctx.handle, _stream(self.gpu), self._ref,
                                                 s.data_ptr(), s.shape[0]))
 
     def compact(self):
         """Moves the pages in use to the low end of the pool, as few as that
         takes; returns their number (an int32 tensor, the cache's own)."""
         self._keeping()
-        self.ctx.check(self.ctx.lib.vsk_kv_compact(self.ctx.handle, _stream(self.device),
+        self.ctx.check(self.ctx.lib.vsk_kv_compact(self.ctx.handle, _stream(self.gpu),
                                                    self._ref))
         return self.status[1]
 
     def copy_pages(self, src, dst):
         """Copies pages ``src`` to pages ``dst`` in every layer."""
         self._keeping()
-        s, d = _ints(src, "src", self.device), _ints(dst, "dst", self.device)
+        s, d = _ints(self.gpu, src, "src"), _ints(self.gpu, dst, "dst")
         if s.shape != d.shape:
             raise VSKError(-4, f"{s.shape[0]} sources, {d.shape[0]} destinations")
-        self.ctx.check(self.ctx.lib.vsk_kv_copy(self.ctx.handle, _stream(self.device), self._ref,
+        self.ctx.check(self.ctx.lib.vsk_kv_copy(self.ctx.handle, _stream(self.gpu), self._ref,
                                                 s.data_ptr(), d.data_ptr(), s.shape[0]))
 
     def missing(self) -> int:
@@ -474,8 +485,9 @@ def window_attention(ctx: Context, q, k, v, *, starts, k_starts=None, max_length
     ``k_starts`` (default: ``starts``), the queries standing at the keys' end.
     ``max_length`` bounds the sequences' queries (default: all rows); window,
     sinks, scale and return_lse as in ``PagedKVCache.attend``."""
-    for x, name in ((q, "q"), (k, "k"), (v, "v")):
-        _tensor(x, name, q.dtype if isinstance(q, torch.Tensor) else None, 3)
+    gpu = ctx.device
+    dtype = _tensor(gpu, q, "q", None, 3).dtype
+    _tensor(gpu, k, "k", dtype, 3), _tensor(gpu, v, "v", dtype, 3)
     if q.dtype not in _TYPES:
         raise VSKError(-8, f"{q.dtype} is not supported")
     if k.shape != v.shape or q.shape[2] != k.shape[2]:
@@ -484,9 +496,9 @@ def window_attention(ctx: Context, q, k, v, *, starts, k_starts=None, max_length
         raise VSKError(-4, f"{q.shape[1]} query heads over {k.shape[1]} key heads")
     if not k.shape[0] and q.shape[0]:
         raise VSKError(-3, "no keys")
-    q, k, v = (_dense_heads(x, "q") for x in (q, k, v))
-    s = _ints(starts, "starts", q.device)
-    ks = s if k_starts is None else _ints(k_starts, "k_starts", q.device)
+    q, k, v = _dense_heads(q), _dense_heads(k), _dense_heads(v)
+    s = _ints(gpu, starts, "starts")
+    ks = s if k_starts is None else _ints(gpu, k_starts, "k_starts")
     if s.shape[0] < 1 or ks.shape != s.shape:
         raise VSKError(-4, "starts and k_starts hold an offset a sequence and the end")
     if k_starts is None and k.shape[0] != q.shape[0]:
