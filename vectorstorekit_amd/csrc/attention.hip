@@ -43,10 +43,7 @@ Plan plan_of(const vsk_ctx *ctx, const vsk_kv *kv, const vsk_new_tokens *news,
   p.chunk = 1 << 30;
   p.tile = false;
   p.share = 4;
-  int64_t row_tile = 16, key_tile = kv->dtype == VSK_DTYPE_F32 ? 16 : 32, per = 4;
-  // blocks that a compute unit holds at once (by their registers), twice over
-  // (a head of 256: once): fewer leave it idle at the end, more start too often
-  int64_t want = (kv->head_dim <= 64 ? 8 : kv->head_dim <= 128 ? 6 : 1) * (int64_t)ctx->cu_count;
+  int64_t row_tile = 16, key_tile = kv->dtype == VSK_DTYPE_F32 ? 16 : 32;
   int64_t keys = kv->table ? (int64_t)kv->width * kv->page_size : kv->pages;
   if (args->max_length > 0 && args->max_length < keys) keys = args->max_length;
   // Row tiles of 128 where there are rows to fill them and work for the
@@ -65,8 +62,6 @@ Plan plan_of(const vsk_ctx *ctx, const vsk_kv *kv, const vsk_new_tokens *news,
     p.tile = true;
     row_tile = ATTN_TILE_ROWS;
     key_tile = attn_tile_keys(kv->head_dim);
-    per = 16;
-    want = 2 * ctx->cu_count;
   }
   p.tiles = (int32_t)ceil_div(rows, row_tile);
   const int64_t blocks = pairs * p.tiles;
@@ -82,19 +77,31 @@ Plan plan_of(const vsk_ctx *ctx, const vsk_kv *kv, const vsk_new_tokens *news,
                          2 * key_tile;
     if (seen < keys) keys = seen;
   }
-  // parts as many as keep every compute unit supplied with blocks, of at least
-  // a tile for each of the four waves that share them (16 tiles: joining a
-  // prompt's rows takes as long as some steps)
   const int64_t tiles = ceil_div(keys, key_tile);
   if (!p.tile && kv->head_dim <= 128 &&
       tiles <= (blocks < ctx->cu_count ? 32 : 64)) {
     p.share = 8;
     return p;
   }
-  // (a prompt's rows are many: parts only where a quarter of the device or less
-  // would work)
-  const int64_t target = p.tile && 4 * blocks > want ? 1 : ceil_div(want, blocks);
-  const int64_t chunk = ceil_div(ceil_div(tiles, target), per) * per;
+  // Parts as many as keep the device supplied with blocks.
+  int64_t want, per;
+  const int64_t cus = ctx->cu_count;
+  if (p.tile) {
+    // a prompt's rows are many and joining them takes as long as some steps:
+    // parts of at least 16 tiles, and only where a quarter of the blocks that
+    // fit or less would work
+    per = 16;
+    want = 2 * blocks > cus ? 1 : 2 * cus;
+  } else {
+    // a tile for each of the four waves that share a part at least, and no
+    // more parts of a row than 64 while there is a block for every compute unit
+    per = 4;
+    const int64_t most = kv->head_dim > 128 ? 1 : kv->dtype == VSK_DTYPE_F32 ? 2
+                         : kv->head_dim > 64 ? 6 : 8;
+    want = most * cus < 64 * blocks ? most * cus : 64 * blocks;
+    if (want < cus) want = cus;
+  }
+  const int64_t chunk = ceil_div(ceil_div(tiles, ceil_div(want, blocks)), per) * per;
   p.chunk = (int32_t)(chunk < per ? per : chunk);
   p.splits = (int32_t)ceil_div(tiles, p.chunk);
   if (p.splits < 1) p.splits = 1;

@@ -577,21 +577,24 @@ k_attn_rows(const AttnArgs a) {
 }
 
 // Joins the parts of one output row: sum of the parts' values and sums, each
-// times 2^(its maximum - the largest).  A block a row; the threads take four
-// values each of several parts at a time.
-template <class T, int DV, int KTILE, int G, bool ALIGNED>
+// times 2^(its maximum - the largest).  A block a row, or, SL, a block SL
+// values of one; the threads take four values each of several parts at a time.
+template <class T, int DV, int SL, int KTILE, int G, bool ALIGNED>
 __global__ __launch_bounds__(256) void k_attn_join(const AttnArgs a, const int32_t RT) {
-  constexpr int LANES = DV / 4, WAYS = 256 / LANES;
-  __shared__ __attribute__((aligned(16))) float so[WAYS][DV];
+  constexpr int LANES = SL / 4, WAYS = 256 / LANES;
+  __shared__ __attribute__((aligned(16))) float so[WAYS][SL];
   __shared__ float ss[WAYS];
   const uint32_t per = (uint32_t)a.max_new * a.heads;
-  const AttnSeq s = attn_seq(a, blockIdx.x / per);
-  const int32_t x = blockIdx.x % per, t = x / a.heads, head = x % a.heads;
+  const uint32_t block = blockIdx.x / (DV / SL);
+  const int e0 = blockIdx.x % (DV / SL) * SL;
+  if (e0 >= a.d) return;
+  const AttnSeq s = attn_seq(a, block / per);
+  const int32_t x = block % per, t = x / a.heads, head = x % a.heads;
   if (t >= s.T) return;
   const int64_t stride = a.tokens * a.heads;
   const int64_t at = (s.token0 + t) * a.heads + head;
   // the first parts are asked for before it is known how many there are
-  const int e = 4 * (threadIdx.x % LANES), way = threadIdx.x / LANES;
+  const int e = e0 + 4 * (threadIdx.x % LANES), way = threadIdx.x / LANES;
   const int32_t i0 = threadIdx.x & 63;
   const int32_t w0 = way < a.splits ? way : 0;
   const int32_t l0 = i0 < a.splits ? i0 : 0;
@@ -628,17 +631,17 @@ __global__ __launch_bounds__(256) void k_attn_join(const AttnArgs a, const int32
     sum += f * a.part_ml[2 * r + 1];
     if (e < a.d) o += f * *reinterpret_cast<const f32x4 *>(a.part_o + r * DV + e);
   }
-  *reinterpret_cast<f32x4 *>(&so[way][e]) = o;
+  *reinterpret_cast<f32x4 *>(&so[way][e - e0]) = o;
   if (threadIdx.x % LANES == 0) ss[way] = sum;
   __syncthreads();
   if (way) return;
-#pragma unroll
+#pragma unroll 8
   for (int i = 1; i < WAYS; ++i) {
-    o += *reinterpret_cast<f32x4 *>(&so[i][e]);
+    o += *reinterpret_cast<f32x4 *>(&so[i][e - e0]);
     sum += ss[i];
   }
   const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
-  if (threadIdx.x == 0 && a.lse)
+  if (e == 0 && a.lse)
     a.lse[at] = sum > 0.f ? (top + __log2f(sum)) * 0.6931471805599453f
                           : sum != sum ? sum : -INFINITY;
   if (e >= a.d) return;
@@ -710,26 +713,38 @@ void launch_attn_rows(vsk_ctx *ctx, hipStream_t st, const AttnArgs &a, int32_t t
 }
 
 namespace {
-template <class T, int DV>
-void join_head(hipStream_t st, const AttnArgs &a, bool aligned, int32_t rows, unsigned g) {
+template <class T, int DV, int SL>
+void join_slice(hipStream_t st, const AttnArgs &a, bool aligned, int32_t rows, unsigned g) {
   constexpr int KR = 16 * SUBS<T>, KB = attn_tile_keys(DV);
   if (rows == ROWS) {
     if (aligned)
-      k_attn_join<T, DV, KR, KR, true><<<g, 256, 0, st>>>(a, rows);
+      k_attn_join<T, DV, SL, KR, KR, true><<<g, 256, 0, st>>>(a, rows);
     else
-      k_attn_join<T, DV, KR, KR, false><<<g, 256, 0, st>>>(a, rows);
+      k_attn_join<T, DV, SL, KR, KR, false><<<g, 256, 0, st>>>(a, rows);
   } else if constexpr (sizeof(T) == 2) {  // (tiles are for 16-bit, aligned operands)
-    k_attn_join<T, DV, KB, ATTN_TILE_GROUP, true><<<g, 256, 0, st>>>(a, rows);
+    k_attn_join<T, DV, SL, KB, ATTN_TILE_GROUP, true><<<g, 256, 0, st>>>(a, rows);
   }
 }
-template <class T>
-void join_of(hipStream_t st, const AttnArgs &a, bool aligned, int32_t rows, unsigned g) {
-  if (a.d <= 64)
-    join_head<T, 64>(st, a, aligned, rows, g);
-  else if (a.d <= 128)
-    join_head<T, 128>(st, a, aligned, rows, g);
+template <class T, int DV>
+void join_head(hipStream_t st, const AttnArgs &a, bool aligned, int32_t rows, uint64_t g,
+               uint64_t cus) {
+  // slices of 16 values where all of them find a compute unit each: one context
+  // of 100,000 under 8 heads of 128 on one takes 30 us, 67 without them; 4 of
+  // 30,000 under 32 on 8 would take 58 and take 51.
+  if (g * (DV / 16) <= cus)
+    join_slice<T, DV, 16>(st, a, aligned, rows, g * (DV / 16));
   else
-    join_head<T, 256>(st, a, aligned, rows, g);
+    join_slice<T, DV, DV>(st, a, aligned, rows, g);
+}
+template <class T>
+void join_of(hipStream_t st, const AttnArgs &a, bool aligned, int32_t rows, uint64_t g,
+             uint64_t cus) {
+  if (a.d <= 64)
+    join_head<T, 64>(st, a, aligned, rows, g, cus);
+  else if (a.d <= 128)
+    join_head<T, 128>(st, a, aligned, rows, g, cus);
+  else
+    join_head<T, 256>(st, a, aligned, rows, g, cus);
 }
 }  // namespace
 
@@ -740,11 +755,11 @@ void launch_attn_join(vsk_ctx *ctx, hipStream_t st, const AttnArgs &a, int32_t t
   VSK_REQUIRE(grid <= 0x7FFFFFFFll, VSK_ERR_INVALID_BUFFER_SIZE, "too many query rows in one call");
   KernelTimer kt(ctx, "attn_join", (double)grid, st);
   if (t == VSK_DTYPE_F32)
-    join_of<float>(st, a, aligned, rows, (unsigned)grid);
+    join_of<float>(st, a, aligned, rows, grid, ctx->cu_count);
   else if (t == VSK_DTYPE_F16)
-    join_of<_Float16>(st, a, aligned, rows, (unsigned)grid);
+    join_of<_Float16>(st, a, aligned, rows, grid, ctx->cu_count);
   else
-    join_of<__bf16>(st, a, aligned, rows, (unsigned)grid);
+    join_of<__bf16>(st, a, aligned, rows, grid, ctx->cu_count);
   check_launch("attn_join");
 }
 
