@@ -93,11 +93,18 @@ Plan plan_of(const vsk_ctx *ctx, const vsk_kv *kv, const vsk_new_tokens *news,
     per = 16;
     want = 2 * blocks > cus ? 1 : 2 * cus;
   } else {
-    // a tile for each of the four waves that share a part at least, and no
-    // more parts of a row than 64 while there is a block for every compute unit
+    // A tile for each of the four waves that share a part at least.  Contexts
+    // differ in length, so several rounds of blocks share the work more evenly
+    // than one; each starts and is joined, so the fewer the longer a block is
+    // by its head.  Measured, blocks a compute unit / us: 64 contexts to 8,192
+    // of 8 key heads of 128 2 / 228, 6 / 195, 12 / 197; 200 to 4,000 of 8 heads
+    // of 64 8 / 192, 16 / 164, 24 / 203; 17 of 16 f32 heads of 96, window
+    // 2,048, 2 / 76, 6 / 86; 60 to 2,000 of 2 heads of 256 1 / 38, 4 / 47.  No
+    // more than 64 parts a row, while there is a block for every compute unit:
+    // 2 contexts of 100,000 of 8 heads of 128 121 us, in 96 parts 129.
     per = 4;
-    const int64_t most = kv->head_dim > 128 ? 1 : kv->dtype == VSK_DTYPE_F32 ? 2
-                         : kv->head_dim > 64 ? 6 : 8;
+    const int64_t most = kv->head_dim <= 64 ? 16 : kv->head_dim > 128 ? 1
+                         : kv->dtype == VSK_DTYPE_F32 ? 2 : 6;
     want = most * cus < 64 * blocks ? most * cus : 64 * blocks;
     if (want < cus) want = cus;
   }
