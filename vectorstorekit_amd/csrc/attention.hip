@@ -43,6 +43,7 @@ Plan plan_of(const vsk_ctx *ctx, const vsk_kv *kv, const vsk_new_tokens *news,
   p.chunk = 1 << 30;
   p.tile = false;
   p.share = 4;
+  const int64_t cus = ctx->cu_count;
   int64_t row_tile = 16, key_tile = kv->dtype == VSK_DTYPE_F32 ? 16 : 32;
   int64_t keys = kv->table ? (int64_t)kv->width * kv->page_size : kv->pages;
   if (args->max_length > 0 && args->max_length < keys) keys = args->max_length;
@@ -56,8 +57,7 @@ Plan plan_of(const vsk_ctx *ctx, const vsk_kv *kv, const vsk_new_tokens *news,
   // products); 4 prompts of 64 after 2,000 of those 32 45 / 42, 16 of 32 61 / 79.
   const int64_t most = args->window > 0 && args->window + (int64_t)args->sinks < keys
                            ? args->window + (int64_t)args->sinks : keys;
-  const bool few = pairs * rows < 32 * (int64_t)ctx->cu_count &&
-                   pairs * rows * most < 32768 * (int64_t)ctx->cu_count;
+  const bool few = pairs * rows < 32 * cus && pairs * rows * most < 32768 * cus;
   if (kv->dtype != VSK_DTYPE_F32 && rows >= 64 && !few && aligned_operands(kv, args)) {
     p.tile = true;
     row_tile = ATTN_TILE_ROWS;
@@ -65,31 +65,41 @@ Plan plan_of(const vsk_ctx *ctx, const vsk_kv *kv, const vsk_new_tokens *news,
   }
   p.tiles = (int32_t)ceil_div(rows, row_tile);
   const int64_t blocks = pairs * p.tiles;
-  if (!p.tile) {
-    // row tiles enough to fill the device: a wave each
-    if (blocks >= 8 * (int64_t)ctx->cu_count && p.tiles >= 4) {
-      p.share = 1;
-      return p;
-    }
-  }
   if (args->window > 0) {
     const int64_t seen = (int64_t)args->window + args->sinks + ceil_div(row_tile, group) +
                          2 * key_tile;
     if (seen < keys) keys = seen;
   }
   const int64_t tiles = ceil_div(keys, key_tile);
-  if (!p.tile && kv->head_dim <= 128 &&
-      tiles <= (blocks < ctx->cu_count ? 32 : 64)) {
-    p.share = 8;
-    return p;
+  if (!p.tile) {
+    // A wave each for row tiles that fill the device several times over, or
+    // with few keys twice; measured against four waves each (us): 8 f32 prompts
+    // of 1,000, 32 heads of 128 on 8, window 100 (16,000 row tiles) 160 / 263;
+    // one of 4,000, 8 heads of 64, window 64 (2,000) 18 / 88; 8 f16 prompts of
+    // 500, 10 heads of 100 (2,560) 330 / 204.
+    if (p.tiles >= 4 && (blocks >= 16 * cus || (blocks >= 4 * cus && keys <= 384))) {
+      p.share = 1;
+      return p;
+    }
+    // Eight waves and no parts for short contexts: nothing to join.  Heads over
+    // 64 leave room for one such block a compute unit only, in 32 bits with
+    // half the bytes in flight.  Against four (us): one context of 777, 32 heads
+    // of 128 on 8, 12 / 13; 100 of up to 1,000 37 / 42; 300 117 / 100; with
+    // heads of 64 45 / 65; 64 of up to 300 in 32 bits 27 / 22, heads of 64 14 / 22.
+    const bool many = kv->head_dim <= 64 || (kv->head_dim <= 128 && kv->dtype != VSK_DTYPE_F32 &&
+                                             blocks <= 6 * cus);
+    if (many && tiles <= (blocks < cus ? 32 : 64)) {
+      p.share = 8;
+      return p;
+    }
   }
   // Parts as many as keep the device supplied with blocks.
   int64_t want, per;
-  const int64_t cus = ctx->cu_count;
   if (p.tile) {
-    // a prompt's rows are many and joining them takes as long as some steps:
+    // A prompt's rows are many and joining them takes as long as some steps:
     // parts of at least 16 tiles, and only where a quarter of the blocks that
-    // fit or less would work
+    // fit or less would work.  Unsplit / split after 30,000 keys, 32 heads of
+    // 128 on 8 (us): 512 tokens (128 blocks) 519 / 284, 2,000 (504) 893 / 998.
     per = 16;
     want = 2 * blocks > cus ? 1 : 2 * cus;
   } else {

@@ -14,13 +14,10 @@
 namespace vsk {
 
 typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
-typedef __attribute__((ext_vector_type(4))) __bf16 bf16x4;
 typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
-typedef __attribute__((ext_vector_type(4))) _Float16 f16x4;
 typedef __attribute__((ext_vector_type(4))) float f32x4;
 typedef __attribute__((ext_vector_type(16))) float f32x16;
 typedef __attribute__((ext_vector_type(4))) uint32_t u32x4;
-typedef __attribute__((ext_vector_type(2))) uint32_t u32x2;
 
 // The operands of a call, by value to every kernel.  Strides in elements.
 struct AttnArgs {
@@ -240,7 +237,8 @@ void finish_queued(vsk_ctx *ctx, hipStream_t stream);
 
 // launches; attn_rows.hip; t: a VSK_DTYPE; aligned: every pointer and
 // stride takes 16-byte loads (8-byte stores)
-// share: waves that take a row tile's keys in turn: 8 (heads to 128), 4, or 1
+// share: waves that take a row tile's keys in turn: 8 (heads to 128, in 32 bits
+// to 64), 4, or 1
 void launch_attn_rows(vsk_ctx *ctx, hipStream_t stream, const AttnArgs &a, int32_t t,
                       bool aligned, int32_t share);
 // keys of a tile of attn_tile.hip, by the (padded) head

@@ -658,8 +658,7 @@ __global__ __launch_bounds__(256) void k_attn_join(const AttnArgs a, const int32
 template <class T, int VW, int NB>
 void rows_of(hipStream_t st, const AttnArgs &a, bool aligned, int32_t share, unsigned grid) {
   if (share == 8) {
-    // (a head of 256 takes the registers of a wave a SIMD)
-    if constexpr (16 * VW * NB <= 128) {
+    if constexpr (16 * VW * NB <= (sizeof(T) == 4 ? 64 : 128)) {
       if (aligned)
         k_attn_rows<T, VW, NB, 8, true><<<grid, 512, 0, st>>>(a);
       else
