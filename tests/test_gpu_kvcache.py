@@ -744,6 +744,24 @@ def test_masked_places_of_many_rows(ctx, dtype, bad, heads, kv, d, n):
             assert bool(torch.isnan(got[see][:, first]).all())
 
 
+def test_example(capsys):
+    """The example's decoder over the cache against itself without one.  Both
+    round activations to bf16 at the same places, in another order of sums:
+    eight roundings a layer of 2^-8 of a value, four layers, added as
+    independent errors, are 2^-8 sqrt(32) = 0.022 of a logit's size, twice
+    that for the largest of them."""
+    import importlib.util
+    import os
+
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples",
+                        "answer_over_retrieved.py")
+    spec = importlib.util.spec_from_file_location("answer_over_retrieved", path)
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    assert example.main(branches=3, steps=6) <= 0.044
+    assert "documents [123" in capsys.readouterr().out
+
+
 def test_refusals(ctx):
     from vectorstorekit_amd import PagedKVCache, RotaryEmbedding, VSKError, window_attention
 

@@ -1,6 +1,5 @@
-// attn_rows.hip -- attention over 16 query rows a wave, keys and values from
-// memory straight into registers: one new token over a long cache, few new
-// tokens, and 32-bit prompts.
+// attn_rows.hip -- attention over 16 query rows a wave: one new token over a
+// long cache, few new tokens, and 32-bit prompts.
 //
 // S^T = K Q^T and O^T = V^T P^T on the matrix cores, 16 rows (columns of the
 // transposed products) at a time.  In the products' layout a lane owns one
@@ -10,13 +9,22 @@
 // none.  The keys of a product may come in any order as long as both operands
 // agree on it: P stays in the registers that S^T was computed in, and a lane
 // loads V's rows for just those keys, 16 bytes of each, and turns the 8 x 8
-// block of 16-bit values around with byte permutes.  No shared memory is
-// touched before the waves' results are joined.
+// block of 16-bit values around with byte permutes.  K's fragments straight
+// from memory would be 64 accesses of 16 bytes a load: whole rows go into LDS
+// that belongs to the wave, and no wave waits for another before the join.
 //
 // One new token reads K and V once and does 4 * 16 * d operations a key for
 // up to 16 heads: far under what the matrix cores do in the time the bytes
 // take, so a group's heads ride along at no cost, and P goes in as a sum of
 // two 16-bit values (its rounding would be as large as the output's).
+//
+// What bounds it: the bytes of K and V.  Measured, bf16 and f16, heads of 128:
+// 64 contexts to 8,192, 32 heads on 8, 195 us, 5.0 TB/s; 3 to 200,003, 64 on 8,
+// 204 us, 5.0 TB/s (a kernel that only reads: 5.8); one of 100,000, 8 on 1,
+// 20 us, 2.5 TB/s: what a launch of few blocks and the join take.  f32, heads
+// of 96 of their own, 17 contexts, window 2,048: 75 us, 5.1 TB/s.  Prompts in
+// 32 bits are bound by the products (16x16x4, 157 TFLOP/s): 2 of 2,048, 32
+// heads of 128 on 8, 388 us, 90 TFLOP/s.
 #include "attn.hpp"
 #include "vsk_api.hpp"
 
@@ -577,8 +585,10 @@ k_attn_rows(const AttnArgs a) {
 }
 
 // Joins the parts of one output row: sum of the parts' values and sums, each
-// times 2^(its maximum - the largest).  A block a row, or, SL, a block SL
-// values of one; the threads take four values each of several parts at a time.
+// times 2^(its maximum - the largest).  A block a row, or a block for SL values
+// of one; the threads take four values each of several parts at a time.  Its
+// bytes are few: it is bound by the chain count, maximum, parts, each a trip to
+// memory (5 us behind 64 parts of 192 rows of 128).
 template <class T, int DV, int SL, int KTILE, int G, bool ALIGNED>
 __global__ __launch_bounds__(256) void k_attn_join(const AttnArgs a, const int32_t RT) {
   constexpr int LANES = SL / 4, WAYS = 256 / LANES;
