@@ -18,6 +18,8 @@
  *    by the caller (the reference makes every engine/index an actor); calls
  *    on distinct contexts may run concurrently.  Every call returns after
  *    its results are in the caller's buffers.
+ *    The calls of the last section (key-value cache and attention) are other:
+ *    they take device memory only and are queued on a stream of the caller's.
  *  - Results are ordered ascending by (distance, tie key); the tie key is
  *    the row id (flat, SQ, PQ), the centroid index (IVF probe) or the
  *    position of the row in the probe-ordered candidate list (IVF search),
