@@ -819,6 +819,12 @@ def test_refusals(ctx):
     refused(bad, window_attention, ctx, x, x.half(), x, starts=[0, 3])
     big = torch.zeros(1, 1, 320, device=DEV)
     refused("unsupportedOperation", window_attention, ctx, big, big, big, starts=[0, 1])
+    # more keys than positions hold (one row, seen very often)
+    far = torch.zeros(1, 1, 8, device=DEV).expand((1 << 30) + 1, 1, 8)
+    refused("invalidBufferSize", window_attention, ctx, x[..., :8], far, far, starts=[0, 3],
+            k_starts=[0, 3])
+    far = torch.zeros(1, 16, 1, 8, device=DEV).expand(1 << 31, 16, 1, 8)
+    refused("invalidBufferSize", PagedKVCache.over, ctx, far, far, t, n)
     assert cache.attend(q[:0]).shape == (0, 4, 64)
     # nothing was lost on the way
     assert int(cache.lengths[0]) == 20 and cache.missing() == 0

@@ -184,6 +184,8 @@ vsk_status vsk_attention(vsk_ctx *ctx, void *stream, const vsk_kv *kv, int32_t l
   } else {
     VSK_REQUIRE(kv->page_size == 0 && layer == 0, VSK_ERR_INVALID_ARGUMENT,
                 "dense keys have no pages or layers");
+    // (positions a few thousand past a sequence's end are formed in 32 bits)
+    VSK_REQUIRE(kv->pages <= (1 << 30), VSK_ERR_INVALID_BUFFER_SIZE, "at most 2^30 keys");
     VSK_REQUIRE(args->k_starts && is_device_ptr(args->k_starts), VSK_ERR_INVALID_ARGUMENT,
                 "dense keys need k_starts in device memory");
     VSK_REQUIRE(kv->k_row >= 0 && kv->v_row >= 0 && kv->k_row <= (1 << 26) &&

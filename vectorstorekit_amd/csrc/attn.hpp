@@ -113,7 +113,7 @@ __device__ inline AttnSpan<KT, G> attn_span(const AttnArgs &a, int32_t q0, int32
       }
     }
   }
-  const int32_t groups = s.sink_groups + (s.hi > s.lo ? (s.hi - s.lo + G - 1) / G : 0);
+  const int32_t groups = s.sink_groups + (s.hi > s.lo ? (s.hi - s.lo - 1) / G + 1 : 0);
   s.tiles = (groups + KT / G - 1) / (KT / G);
   return s;
 }

@@ -308,6 +308,8 @@ class PagedKVCache:
             raise VSKError(-2, "lengths must be dense")
         k5, v5 = (x if x.dim() == 5 else x[None] for x in (k, v))
         layers, pages, page_size, kv_heads, head_dim = k5.shape
+        if max(layers, pages, kv_heads, *table.shape) >= 1 << 31:
+            raise VSKError(-9, "the cache's counts are 32-bit")
         if page_size < 16 or page_size & (page_size - 1):
             raise VSKError(-8, "page_size must be a power of two of at least 16")
         self.ctx, self.k, self.v = ctx, k, v
@@ -503,6 +505,8 @@ def window_attention(ctx: Context, q, k, v, *, starts, k_starts=None, max_length
         raise VSKError(-4, "starts and k_starts hold an offset a sequence and the end")
     if k_starts is None and k.shape[0] != q.shape[0]:
         raise VSKError(-4, f"{q.shape[0]} queries, {k.shape[0]} keys: k_starts is wanted")
+    if k.shape[0] > 1 << 30:
+        raise VSKError(-9, f"{k.shape[0]} keys: at most 2^30")
     kv = _lib.vsk_kv()
     kv.k, kv.v, kv.dtype = k.data_ptr(), v.data_ptr(), _TYPES[q.dtype]
     kv.k_row, kv.k_head, _ = k.stride()
