@@ -557,6 +557,33 @@ def test_pages(ctx, dtype, kv, d, order, pages):
     assert short > 0 or pages > 100
 
 
+@pytest.mark.parametrize("pages", [3500, 33000])
+def test_fork_many(ctx, pages):
+    """More branches than a workgroup has threads, twice: the second drops the
+    first's; with 3,500 pages some find no last page."""
+    from vectorstorekit_amd import PagedKVCache
+
+    page, slots, width, roots = 16, 1700, 3, 200
+    g = gen(pages)
+    k, v = (torch.randn((1, pages, page, 1, 4), generator=g).to(F16).to(DEV) for _ in range(2))
+    refs = (torch.rand(pages, generator=g) < 0.55).int()  # held by others
+    cache = PagedKVCache.over(ctx, k, v, torch.full((slots, width), -1, dtype=torch.int32,
+                                                    device=DEV), ints([0] * slots), refs.to(DEV))
+    m = Model(cache)
+    rng = np.random.default_rng(pages)
+    counts = rng.integers(0, page * width + 1, roots).tolist()
+    assert m.reserve(range(roots), counts) == 0
+    cache.reserve(list(range(roots)), counts)
+    for _ in range(2):
+        children = (roots + rng.permutation(slots - roots)).tolist()
+        parents = rng.integers(0, roots, len(children)).tolist()
+        missing = m.fork(parents, children)
+        cache.fork(parents, children)
+        assert cache.missing() == missing
+        assert (missing > 0) == (pages < 10000)
+        m.same(cache)
+
+
 def test_copy_pages(ctx):
     cache, _ = filled(ctx, [100], 32, 2, 40, F16, layers=3, seed=1, poison=False)
     k, v = cache.k.cpu().clone(), cache.v.cpu().clone()

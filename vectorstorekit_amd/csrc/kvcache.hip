@@ -109,21 +109,23 @@ __device__ inline int32_t scan(int32_t x, int32_t *total) {
   return before + y - x;
 }
 
-// The counts were changed by atomics of this workgroup: read past the L1.
-__device__ inline int32_t count_of(const int32_t *refs, int32_t i) {
+// A count that atomics of this workgroup may have changed: read past the L1.
+__device__ inline int32_t shared_count(const int32_t *refs, int32_t i) {
   return __hip_atomic_load(refs + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
-// take(rank, page) for the `want` lowest free pages in order; returns how many
-// there were.  Called by the whole workgroup.
-template <class F> __device__ int32_t take_free(const Pool &p, int32_t want, F &&take) {
+// take(rank, page) for the `want` lowest free pages in order, count(id) the
+// sequences that hold one; returns how many there were.  Called by the whole
+// workgroup.
+template <class C, class F>
+__device__ int32_t take_free(const Pool &p, int32_t want, C &&count_of, F &&take) {
   int32_t found = 0;
   for (int32_t c = 0; c < p.pages && found < want; c += 4 * NT) {
     int32_t mask = 0, count[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int32_t id = c + 4 * (int32_t)threadIdx.x + i;
-      count[i] = count_of(p.refs, id < p.pages ? id : p.pages - 1);
+      count[i] = count_of(id < p.pages ? id : p.pages - 1);
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -171,7 +173,8 @@ __global__ __launch_bounds__(NT) void k_kv_reserve(const Pool p, const int32_t *
     want += all;
   }
   __syncthreads();
-  const int32_t got = take_free(p, want, [&](int32_t rank, int32_t page) {
+  const auto count = [&](int32_t id) { return p.refs[id]; };
+  const int32_t got = take_free(p, want, count, [&](int32_t rank, int32_t page) {
     int32_t lo = 0, hi = n;  // the last sequence whose first rank is at most this one
     while (hi - lo > 1) {
       const int32_t mid = (lo + hi) / 2;
@@ -208,16 +211,32 @@ __global__ __launch_bounds__(NT) void k_kv_reserve(const Pool p, const int32_t *
 }
 
 // A wave a child: its row's and its parent's entries are loaded together, and
-// the counts change by atomics that nothing waits for before free pages are
-// looked for.  Children go in batches of a workgroup's threads, one each; what
-// a batch needs again it finds in LDS.  48 branches of contexts to 2,000 over
-// 8,192 pages: 16 us (20 with a wait for each child's counts), and 4.4 for the
-// last pages' copies.
+// nothing waits for the counts before free pages are looked for.  Children go
+// in batches of a workgroup's threads, one each; what a batch needs again it
+// finds in LDS.
+//
+// Counts change twice for every page of every child.  LOCAL: in LDS, where
+// they are all read at the start and written at the end; else by atomics in
+// memory, one a cycle from one workgroup.  48 branches of contexts to 2,000
+// over 8,192 pages: 7.1 us, 4 more for the last pages' copies (16.4 by
+// atomics behind a fence); a fork over 32,768 pages 13.4 us, over 33,000, by
+// atomics, 18.5.
+constexpr int32_t LOCAL_PAGES = 32768;
+template <bool LOCAL>
 __global__ __launch_bounds__(NT) void k_kv_fork(const Pool p, const int32_t *parents,
                                                 const int32_t *children, int32_t n) {
   int32_t *src = p.slot_list(0), *dst = p.slot_list(1), *rows = p.slot_list(2);
   __shared__ int32_t sc[NT], sf[NT], sl[NT], who[NT], sd[NT];
+  __shared__ int32_t held_by[LOCAL ? LOCAL_PAGES : 1];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  if (LOCAL) {
+#pragma unroll 8
+    for (int32_t i = threadIdx.x; i < p.pages; i += NT) held_by[i] = p.refs[i];
+  }
+  auto change = [&](int32_t page, int32_t by) {
+    if ((uint32_t)page >= (uint32_t)p.pages) return;
+    atomicAdd(LOCAL ? held_by + page : p.refs + page, by);
+  };
   int32_t c = -1, f = -1, l = 0;
   auto stage = [&](int32_t b) {
     const int32_t i = b + threadIdx.x;
@@ -244,8 +263,8 @@ __global__ __launch_bounds__(NT) void k_kv_fork(const Pool p, const int32_t *par
       for (int32_t y = lane; y < p.width; y += 64) {
         const int32_t old = mine[y], now = y < full ? its[y] : -1;
         mine[y] = now;
-        if ((uint32_t)old < (uint32_t)p.pages) atomicSub(p.refs + old, 1);
-        if ((uint32_t)now < (uint32_t)p.pages) atomicAdd(p.refs + now, 1);
+        change(old, -1);
+        change(now, 1);
       }
     }
   }
@@ -257,12 +276,14 @@ __global__ __launch_bounds__(NT) void k_kv_fork(const Pool p, const int32_t *par
     int32_t want;
     const int32_t before = scan(part > 0, &want);
     if (part > 0) who[before] = threadIdx.x;
-    __threadfence();  // the counts have arrived where take_free reads them
+    // (this wave's atomics are done: the barrier alone would not wait for them)
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
-    const int32_t got = take_free(p, want, [&](int32_t rank, int32_t page) {
+    const auto count = [&](int32_t id) { return LOCAL ? held_by[id] : shared_count(p.refs, id); };
+    const int32_t got = take_free(p, want, count, [&](int32_t rank, int32_t page) {
       const int32_t x = who[rank];
       sd[x] = page;
-      p.refs[page] = 1;
+      (LOCAL ? held_by : p.refs)[page] = 1;
       p.table[sc[x] * p.table_stride + (sl[x] >> p.shift)] = page;
     });
     __syncthreads();
@@ -274,6 +295,10 @@ __global__ __launch_bounds__(NT) void k_kv_fork(const Pool p, const int32_t *par
     missing += want - got;
   }
   if (threadIdx.x == 0) p.status[0] = missing;
+  if (LOCAL) {
+#pragma unroll 8
+    for (int32_t i = threadIdx.x; i < p.pages; i += NT) p.refs[i] = held_by[i];
+  }
 }
 
 __global__ __launch_bounds__(256) void k_kv_free(const Pool p, const int32_t *seqs, int32_t n) {
@@ -500,7 +525,10 @@ vsk_status vsk_kv_fork(vsk_ctx *ctx, void *stream, const vsk_kv *kv, const int32
   hipStream_t st = static_cast<hipStream_t>(stream);
   {
     KernelTimer kt(ctx, "kv_fork", n, st);
-    k_kv_fork<<<1, NT, 0, st>>>(p, parents, children, n);
+    if (p.pages <= LOCAL_PAGES)
+      k_kv_fork<true><<<1, NT, 0, st>>>(p, parents, children, n);
+    else
+      k_kv_fork<false><<<1, NT, 0, st>>>(p, parents, children, n);
     check_launch("kv_fork");
   }
   MoveArgs m{};
