@@ -673,7 +673,7 @@ def kernels_of(ctx, f):
 @pytest.mark.parametrize("order", ["nhd", "hnd"])
 @pytest.mark.parametrize("news,lengths,page,heads,kv,d,window,sinks", [
     ([70, 130], [200, 130], 32, 64, 8, 128, 33, 4),
-    ([65, 64, 63], [65, 100, 63], 16, 48, 48, 64, 16, 16),
+    ([65, 64, 63], [65, 100, 63], 16, 96, 96, 64, 16, 16),
     ([300], [300], 64, 32, 4, 96, 64, 0),
     ([40, 9, 0], [64, 20, 5], 16, 80, 10, 256, None, 0),
     ([260], [900], 64, 36, 9, 80, 200, 70),    # the sinks' last tile holds window too
@@ -703,7 +703,7 @@ def test_prompt_attention_of_many_rows(ctx, dtype, order, news, lengths, page, h
 @pytest.mark.parametrize("dtype", [BF, F16])
 @pytest.mark.parametrize("lengths,heads,kv,d,window,sinks", [
     ([520, 31], 8, 2, 128, 100, 130),
-    ([333, 0, 1], 12, 12, 64, 90, 5),
+    ([333, 0, 1], 24, 24, 64, 90, 5),
     ([130], 64, 64, 128, None, 0),
     ([190, 75], 32, 4, 256, 32, 0),
     ([1030], 8, 8, 96, 64, 4),
@@ -741,7 +741,7 @@ def test_many_queries_before_the_keys(ctx):
 
 @pytest.mark.parametrize("dtype", [BF, F16])
 @pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
-@pytest.mark.parametrize("heads,kv,d,n", [(64, 32, 128, 150), (24, 24, 64, 400),
+@pytest.mark.parametrize("heads,kv,d,n", [(64, 32, 128, 150), (48, 48, 64, 400),
                                           (128, 16, 256, 70)])
 def test_masked_places_of_many_rows(ctx, dtype, bad, heads, kv, d, n):
     """As above, and a hidden key between the sinks and the window."""

@@ -49,15 +49,19 @@ Plan plan_of(const vsk_ctx *ctx, const vsk_kv *kv, const vsk_new_tokens *news,
   if (args->max_length > 0 && args->max_length < keys) keys = args->max_length;
   // Row tiles of 128 where there are rows to fill them and work for the
   // device.  Under 64 rows of a key head most of a tile would be empty; with
-  // few rows in all, or few products, tiles of 16 spread over more waves and
-  // end sooner.  Measured in 16 bits, tiles of 128 against tiles of 16 (us):
-  // one prompt of 1,000 tokens, 8 heads of 64 of their own 21 / 13, 32 heads
-  // of 128 on 8 27 / 72 (over the bound on rows); 64 new tokens of those 8
-  // heads after 4,000 keys 23 / 15, after 30,000 25 / 33 (over the bound on
-  // products); 4 prompts of 64 after 2,000 of those 32 45 / 42, 16 of 32 61 / 79.
-  const int64_t most = args->window > 0 && args->window + (int64_t)args->sinks < keys
-                           ? args->window + (int64_t)args->sinks : keys;
-  const bool few = pairs * rows < 32 * cus && pairs * rows * most < 32768 * cus;
+  // few rows in all, and few products, tiles of 16 spread over more waves and
+  // end sooner; fewer still where keys are many and parts of them keep the
+  // device busy either way.  Measured in
+  // 16 bits, tiles of 128 against tiles of 16 (us): one prompt of 2,000 tokens,
+  // 8 heads of 64 47 / 27, of 4,000 60 / 122; 4 heads of 128 on one 41 / 27; of
+  // 333, 32 heads of 128 on 8, 16 / 22; 64 new tokens of 8 heads of 64 after
+  // 4,000 keys 23 / 15, after 30,000 25 / 33; of one head after 30,000 24 / 16.
+  int64_t seen = keys - (max_new < keys ? max_new : keys) / 2;
+  if (args->window > 0 && args->window + (int64_t)args->sinks < seen)
+    seen = args->window + (int64_t)args->sinks;
+  const int64_t unit = (kv->head_dim <= 64 ? 64 : 32) * cus;
+  const bool few = pairs * rows < unit &&
+                   pairs * rows * seen < (seen <= 8192 ? 1024 : 256) * unit;
   if (kv->dtype != VSK_DTYPE_F32 && rows >= 64 && !few && aligned_operands(kv, args)) {
     p.tile = true;
     row_tile = ATTN_TILE_ROWS;
@@ -66,9 +70,9 @@ Plan plan_of(const vsk_ctx *ctx, const vsk_kv *kv, const vsk_new_tokens *news,
   p.tiles = (int32_t)ceil_div(rows, row_tile);
   const int64_t blocks = pairs * p.tiles;
   if (args->window > 0) {
-    const int64_t seen = (int64_t)args->window + args->sinks + ceil_div(row_tile, group) +
-                         2 * key_tile;
-    if (seen < keys) keys = seen;
+    const int64_t reach = (int64_t)args->window + args->sinks + ceil_div(row_tile, group) +
+                          2 * key_tile;
+    if (reach < keys) keys = reach;
   }
   const int64_t tiles = ceil_div(keys, key_tile);
   if (!p.tile) {
@@ -77,7 +81,8 @@ Plan plan_of(const vsk_ctx *ctx, const vsk_kv *kv, const vsk_new_tokens *news,
     // of 1,000, 32 heads of 128 on 8, window 100 (16,000 row tiles) 160 / 263;
     // one of 4,000, 8 heads of 64, window 64 (2,000) 18 / 88; 8 f16 prompts of
     // 500, 10 heads of 100 (2,560) 330 / 204.
-    if (p.tiles >= 4 && (blocks >= 16 * cus || (blocks >= 4 * cus && keys <= 384))) {
+    if (p.tiles >= 4 && (blocks >= 16 * cus || (blocks >= 4 * cus && keys <= 384) ||
+                         (blocks >= 2 * cus && keys <= 128))) {
       p.share = 1;
       return p;
     }
