@@ -50,12 +50,12 @@ Plan plan_of(const vsk_ctx *ctx, const vsk_kv *kv, const vsk_new_tokens *news,
   // Row tiles of 128 where there are rows to fill them and work for the
   // device.  Under 64 rows of a key head most of a tile would be empty; with
   // few rows in all, and few products, tiles of 16 spread over more waves and
-  // end sooner; fewer still where keys are many and parts of them keep the
-  // device busy either way.  Measured in
-  // 16 bits, tiles of 128 against tiles of 16 (us): one prompt of 2,000 tokens,
-  // 8 heads of 64 47 / 27, of 4,000 60 / 122; 4 heads of 128 on one 41 / 27; of
-  // 333, 32 heads of 128 on 8, 16 / 22; 64 new tokens of 8 heads of 64 after
-  // 4,000 keys 23 / 15, after 30,000 25 / 33; of one head after 30,000 24 / 16.
+  // end sooner; fewer still where keys are many, whose parts keep the device
+  // busy either way.  Measured in 16 bits, tiles of 128 against tiles of 16
+  // (us): one prompt of 2,000 tokens, 8 heads of 64 47 / 27, of 4,000 60 / 122;
+  // 4 heads of 128 on one 41 / 27; of 333, 32 heads of 128 on 8, 16 / 22; 64
+  // new tokens of 8 heads of 64 after 4,000 keys 23 / 15, after 30,000 25 / 33;
+  // of one head after 30,000 24 / 16.
   int64_t seen = keys - (max_new < keys ? max_new : keys) / 2;
   if (args->window > 0 && args->window + (int64_t)args->sinks < seen)
     seen = args->window + (int64_t)args->sinks;
