@@ -741,9 +741,13 @@ void join_head(hipStream_t st, const AttnArgs &a, bool aligned, int32_t rows, ui
                uint64_t cus) {
   // slices of 16 values where all of them find a compute unit each: one context
   // of 100,000 under 8 heads of 128 on one takes 30 us, 67 without them; 4 of
-  // 30,000 under 32 on 8 would take 58 and take 51.
+  // 30,000 under 32 on 8 would take 58 and take 51.  Up to a row a compute unit,
+  // slices of 64: 4 f32 contexts to 30,000, 8 heads of 256 on one, 44 us, 49
+  // without them; 3 f16 to 200,003, 64 of 128 on 8, 209 / 212.
   if (g * (DV / 16) <= cus)
     join_slice<T, DV, 16>(st, a, aligned, rows, g * (DV / 16));
+  else if (DV > 64 && g <= cus)
+    join_slice<T, DV, 64>(st, a, aligned, rows, g * (DV / 64));
   else
     join_slice<T, DV, DV>(st, a, aligned, rows, g);
 }
