@@ -789,6 +789,18 @@ def test_example(capsys):
     assert "documents [123" in capsys.readouterr().out
 
 
+def test_offsets_out_of_order(ctx):
+    """Offsets that fall, as far apart as 32 bits allow: no token is treated."""
+    for starts in ([2 ** 31 - 1, -2 ** 31], [5, 2], [9, 9]):
+        cache, ks, vs, order = filled(ctx, [40], 16, 2, 64, BF, poison=False)
+        k, v = cache.k.clone(), cache.v.clone()
+        x = normal(gen(3), 8, 2, 64, dtype=BF)
+        cache.append(x, x, starts=ints(starts), seqs=ints([0]))
+        cache.attend(x, starts=ints(starts), seqs=ints([0]))
+        torch.cuda.synchronize()
+        assert torch.equal(cache.k, k) and torch.equal(cache.v, v)
+
+
 def test_refusals(ctx):
     from vectorstorekit_amd import PagedKVCache, RotaryEmbedding, VSKError, window_attention
 

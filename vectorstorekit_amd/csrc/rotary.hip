@@ -92,7 +92,7 @@ __global__ __launch_bounds__(256) void k_rotary(const RotaryArgs a) {
     if (a.starts) {
       t0 = a.starts[b] < 0 ? 0 : a.starts[b];
       const int32_t t1 = a.starts[b + 1] > a.tokens ? (int32_t)a.tokens : a.starts[b + 1];
-      count = t1 - t0;
+      count = t1 > t0 ? t1 - t0 : 0;  // (offsets out of order: t1 - t0 may not fit 32 bits)
     }
     if (t >= count) return;
     row = t0 + t;
