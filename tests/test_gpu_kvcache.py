@@ -801,6 +801,35 @@ def test_offsets_out_of_order(ctx):
         assert torch.equal(cache.k, k) and torch.equal(cache.v, v)
 
 
+def test_refusals_of_lost_meaning(ctx):
+    """What would otherwise pass and mean something else."""
+    from vectorstorekit_amd import RotaryEmbedding, VSKError, window_attention
+
+    def refused(kind, f, *a, **k):
+        with pytest.raises(VSKError) as e:
+            f(*a, **k)
+        assert e.value.kind == kind, e.value
+
+    cache, _ = filled(ctx, [20, 4], 16, 2, 64, F32, poison=False)
+    x, pos = torch.ones(2, 2, 64, device=DEV), ints([0, 1])
+    rope = RotaryEmbedding(ctx, 64)
+    rope.free()  # (not "no rotation")
+    refused("invalidArgument", cache.append, x, x, rotary=rope)
+    refused("invalidArgument", rope.apply, x, positions=pos)
+    for far in (1 << 32, -(1 << 32), 1 << 31):  # (not slot 0)
+        refused("invalidArgument", cache.free, [far])
+        refused("invalidArgument", cache.reserve, [0], [far])
+    assert cache.lengths.tolist() == [20, 4]
+    rope, y = RotaryEmbedding(ctx, 64), x.clone().requires_grad_()
+    refused("unsupportedOperation", rope.apply, y, positions=pos)
+    refused("unsupportedOperation", cache.attend, y)
+    refused("unsupportedOperation", cache.append, x, y)
+    refused("unsupportedOperation", window_attention, ctx, x, y, x, starts=[0, 2])
+    with torch.no_grad():
+        assert torch.equal(rope.apply(y, positions=pos), rope.apply(x, positions=pos))
+        assert torch.equal(cache.attend(y), cache.attend(x))
+
+
 def test_refusals(ctx):
     from vectorstorekit_amd import PagedKVCache, RotaryEmbedding, VSKError, window_attention
 

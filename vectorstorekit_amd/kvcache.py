@@ -11,7 +11,8 @@ answers over retrieved vectors calls next to the search.
 
 Tensors are torch tensors on the context's GPU.  Unlike the search calls,
 these are queued on torch's current stream and do not wait: a decoder makes
-dozens a token.  They allocate through torch, so a captured graph may hold
+dozens a token.  They record no gradients (a tensor that wants one is refused
+outside ``torch.no_grad()``).  They allocate through torch, so a captured graph may hold
 them.  The reference keeps its language-model layer on the application's side
 (LLM/, Core/ML/Shaders/OptimizedMLShaders.metal:523); there is no CPU
 fallback.
@@ -56,6 +57,10 @@ def _tensor(gpu, x, name, dtype=None, dims=None):
     """x, checked to be a tensor on that GPU."""
     if not isinstance(x, torch.Tensor) or x.get_device() != gpu:
         raise VSKError(-2, f"{name} must be a tensor on GPU {gpu}, the context's")
+    if x.requires_grad and torch.is_grad_enabled():
+        # (a result without its history would train on silently)
+        raise VSKError(-8, f"{name} requires a gradient, which these calls do not record: detach "
+                       "it or call under torch.no_grad()")
     if dtype is not None and x.dtype != dtype:
         raise VSKError(-2, f"{name} is {x.dtype}, not {dtype}")
     if dims is not None and x.dim() != dims:
@@ -76,6 +81,8 @@ def _ints(gpu, x, name):
     a = np.asarray(x)
     if a.ndim != 1 or (a.size and a.dtype.kind not in "iu"):
         raise VSKError(-2, f"{name} must be a vector of whole numbers")
+    if a.size and (int(a.min()) < -1 << 31 or int(a.max()) >= 1 << 31):
+        raise VSKError(-2, f"{name} does not fit 32 bits")
     return torch.from_numpy(a.astype(np.int32)).to(torch.device("cuda", gpu))
 
 
@@ -377,8 +384,11 @@ class PagedKVCache:
         k, v = self._heads(k, "k", self.kv_heads), self._heads(v, "v", self.kv_heads)
         if v.shape[0] != k.shape[0]:
             raise VSKError(-4, f"{k.shape[0]} keys, {v.shape[0]} values")
-        if rotary is not None and rotary.head_dim != self.head_dim:
-            raise VSKError(-4, f"rotary is for heads of {rotary.head_dim}")
+        if rotary is not None:
+            if not rotary.handle:
+                raise VSKError(-2, "the rotary embedding has been freed")
+            if rotary.head_dim != self.head_dim:
+                raise VSKError(-4, f"rotary is for heads of {rotary.head_dim}")
         news, keep = self._news(k, starts, seqs, max_new)
         out, qr = None, None
         if q is not None:
