@@ -792,13 +792,45 @@ def test_example(capsys):
 def test_offsets_out_of_order(ctx):
     """Offsets that fall, as far apart as 32 bits allow: no token is treated."""
     for starts in ([2 ** 31 - 1, -2 ** 31], [5, 2], [9, 9]):
-        cache, ks, vs, order = filled(ctx, [40], 16, 2, 64, BF, poison=False)
+        cache, _ = filled(ctx, [40], 16, 2, 64, BF, poison=False)
         k, v = cache.k.clone(), cache.v.clone()
         x = normal(gen(3), 8, 2, 64, dtype=BF)
         cache.append(x, x, starts=ints(starts), seqs=ints([0]))
         cache.attend(x, starts=ints(starts), seqs=ints([0]))
         torch.cuda.synchronize()
         assert torch.equal(cache.k, k) and torch.equal(cache.v, v)
+
+
+@pytest.mark.parametrize("dtype", [BF, F16, F32])
+@pytest.mark.parametrize("new,n", [(1, 100003), (1, 900), (2, 6000), (70, 20000)])
+def test_small_weights_of_many_keys(ctx, dtype, new, n):
+    """One first key of value 0 takes nearly all of a row's weight; the others,
+    2^-27 each, are the whole output: w (n - 1) / (1 + w (n - 1)) of them.
+    Scores are sums of products of powers of two, so they are exact: the weight
+    is off by 2^-21, the sum of n by 2^-24 (n + 16) at the most, an f16 or bf16
+    weight and output by u each (an f16 output under 2^-14 by 2^-25)."""
+    from vectorstorekit_amd import window_attention
+
+    heads, d = 32, 64
+    k = torch.zeros(n, heads, d, dtype=dtype, device=DEV)
+    v = torch.ones(n, heads, d, dtype=dtype, device=DEV)
+    k[0, :, 0], v[0] = 32.0, 0.0
+    q = torch.zeros(new, heads, d, dtype=dtype, device=DEV)
+    q[:, :, 0] = 32.0
+    scale = 27 * math.log(2) / 1024
+    out, lse = window_attention(ctx, q, k, v, starts=[0, new], k_starts=[0, n], scale=scale,
+                                return_lse=True)
+    # (the scale as the call takes it, in fp32)
+    w = math.exp(-1024 * float(np.float32(scale)))
+    others = w * torch.arange(n - new, n, dtype=torch.float64)[:, None, None]
+    want = (others / (1 + others)).expand(new, heads, d)
+    u = U[dtype] if dtype != F32 else 0.0
+    # (the first score, 27 in log2, is rounded twice to 2^-20 of it: 2^-19 of w)
+    tol = want * (2 * U[dtype] + u + 2 * 2.0 ** -19 + 2.0 ** -24 * (n + 16)) + 2.0 ** -25
+    check(out, want, tol if dtype == F16 else tol - 2.0 ** -25)
+    top = 1024 * float(np.float32(scale))
+    check(lse, (top + torch.log1p(others))[..., 0].expand(new, heads),
+          torch.full((new, heads), 2.0 ** -16 * 28, dtype=torch.float64))
 
 
 def test_refusals_of_lost_meaning(ctx):

@@ -42,7 +42,7 @@ struct AttnArgs {
   int32_t chunk;        // key tiles of a part
   float scale_log2;     // scale * log2(e)
   float *part_o;        // splits x tokens x heads x d
-  float *part_ml;       // splits x tokens x heads x 2: maximum (log2), sum
+  float *part_ml;       // splits x tokens x heads x 2: reference (log2), sum
 };
 
 // One sequence of the call.

@@ -35,14 +35,19 @@ namespace vsk {
 namespace {
 
 // What a type's 32-bit words hold: E elements; 16 bytes hold 4 * E.
+// TOP: log2 of the largest weight, the sums' reference being 2^-TOP of it.  An
+// f16 of 1 at most loses a weight under 2^-25, and a long context may hold many
+// of them behind one large first key; bf16 has fp32's exponents.
 template <class T> struct Elem;
 template <> struct Elem<float> {
   static constexpr int E = 1;
+  static constexpr float TOP = 0.f;
   static constexpr uint32_t EXP = 0x7F800000u;  // an infinity's or NaN's exponent
 };
 template <> struct Elem<__bf16> {
   typedef bf16x8 V8;
   static constexpr int E = 2;
+  static constexpr float TOP = 0.f;
   static constexpr uint32_t EXP = 0x7F80u;
   static __device__ f32x4 mfma(u32x4 a, V8 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(V8, a), b, c, 0, 0, 0);
@@ -51,6 +56,7 @@ template <> struct Elem<__bf16> {
 template <> struct Elem<_Float16> {
   typedef f16x8 V8;
   static constexpr int E = 2;
+  static constexpr float TOP = 15.f;
   static constexpr uint32_t EXP = 0x7C00u;
   static __device__ f32x4 mfma(u32x4 a, V8 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(V8, a), b, c, 0, 0, 0);
@@ -351,7 +357,7 @@ template <class T, int VW, int NB, bool ALIGNED> struct RowTile {
     float top = fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3]));
     if constexpr (U == 2)
       top = fmaxf(top, fmaxf(fmaxf(sc[1][0], sc[1][1]), fmaxf(sc[1][2], sc[1][3])));
-    top = fmaxf(m, xor16_32_max(top) * a.scale_log2);
+    top = fmaxf(m, xor16_32_max(top) * a.scale_log2 - Elem<T>::TOP);
     const float use = top == -INFINITY ? 0.f : top;
     const float fade = attn_exp2(m - use);
     m = top;

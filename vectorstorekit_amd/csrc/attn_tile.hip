@@ -38,9 +38,12 @@ namespace {
 typedef __attribute__((ext_vector_type(4))) short i16x4;
 constexpr int NW = 4;  // waves of a workgroup
 
+// TOP: log2 of a weight where its score sets the reference; weights grow to
+// 2^(TOP + 8).  In f16 as large as fits, so that small ones are not lost.
 template <class T> struct Mm;
 template <> struct Mm<__bf16> {
   typedef bf16x8 V8;
+  static constexpr float TOP = 0.f;
   static constexpr uint32_t EXP = 0x7F807F80u;
   static __device__ f32x16 mfma(V8 a, V8 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
@@ -48,6 +51,7 @@ template <> struct Mm<__bf16> {
 };
 template <> struct Mm<_Float16> {
   typedef f16x8 V8;
+  static constexpr float TOP = 7.f;
   static constexpr uint32_t EXP = 0x7C007C00u;
   static __device__ f32x16 mfma(V8 a, V8 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
@@ -255,11 +259,11 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void k_attn_tile(const 
       tm = max3(tm, sc[x >> 4][x & 15], sc[(x + 1) >> 4][(x + 1) & 15]);
     return xor32_max(max3(tm, sc[U - 1][15], sc[U - 1][15]));
   };
-  // The sums are kept relative to m, which follows the largest score only when
-  // that has grown by 8 (in log2): weights up to 256 cost no precision, and
-  // the sums are seldom rescaled.
+  // The sums are kept relative to m, which follows the largest score (less TOP)
+  // only when that has grown by 8 (in log2): weights 256 times as large cost no
+  // precision, and the sums are seldom rescaled.
   auto settle = [&](float tm) {
-    const float top = tm * a.scale_log2;
+    const float top = tm * a.scale_log2 - Mm<T>::TOP;
     if (!__any(top > m + 8.f)) return;
     const float nm = top > m + 8.f ? top : m;
     const float fade = nm == -INFINITY ? 1.f : attn_exp2(m - nm);
