@@ -40,5 +40,6 @@ def __getattr__(name):
     if name in _KVCACHE:
         from . import kvcache
 
-        return getattr(kvcache, name)
+        # (kept: an import within a loop is then a plain lookup)
+        return globals().setdefault(name, getattr(kvcache, name))
     raise AttributeError(f"module {__name__!r} has no attribute {name!r}")

@@ -35,11 +35,14 @@ _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 
 # The call's structures as bytes: a decoder makes these calls dozens of times a
 # token, and setting a ctypes structure's fields takes several times as long.
-# Layouts: vsk_head_rows, vsk_new_tokens and vsk_attention_args of vsk_hip.h.
+# Layouts: vsk_kv, vsk_head_rows, vsk_new_tokens and vsk_attention_args of
+# vsk_hip.h.
+_KV = struct.Struct("@QQqqqqqqqqQQQQQqiiiiiiii")
 _ROWS = struct.Struct("@QQqqqqixxxx")
 _NEWS = struct.Struct("@QQiiq")
 _ATTEND = struct.Struct("@QQqqqqixxxxQQQqfiii")
 assert _ATTEND.size == ctypes.sizeof(_lib.vsk_attention_args)
+assert _KV.size == ctypes.sizeof(_lib.vsk_kv)
 assert _ROWS.size == ctypes.sizeof(_lib.vsk_head_rows)
 assert _NEWS.size == ctypes.sizeof(_lib.vsk_new_tokens)
 
@@ -515,15 +518,14 @@ def window_attention(ctx: Context, q, k, v, *, starts, k_starts=None, max_length
         raise VSKError(-4, "starts and k_starts hold an offset a sequence and the end")
     if k_starts is None and k.shape[0] != q.shape[0]:
         raise VSKError(-4, f"{q.shape[0]} queries, {k.shape[0]} keys: k_starts is wanted")
-    if k.shape[0] > 1 << 30:
-        raise VSKError(-9, f"{k.shape[0]} keys: at most 2^30")
-    kv = _lib.vsk_kv()
-    kv.k, kv.v, kv.dtype = k.data_ptr(), v.data_ptr(), _TYPES[q.dtype]
-    kv.k_row, kv.k_head, _ = k.stride()
-    kv.v_row, kv.v_head, _ = v.stride()
-    kv.pages, kv.kv_heads, kv.head_dim = k.shape
-    kv.layers = 1
+    rows, heads, d = k.shape
+    if max(rows, heads, q.shape[1]) > 1 << 30:
+        raise VSKError(-9, f"{rows} keys of {heads} heads: at most 2^30")
+    x, y = k.stride(), v.stride()
+    # (dense rows: no table, no pages, no layers but one)
+    kv = _KV.pack(k.data_ptr(), v.data_ptr(), 0, 0, x[0], x[1], 0, 0, y[0], y[1], 0, 0, 0, 0, 0,
+                  0, _TYPES[dtype], 1, rows, 0, heads, d, 0, 0)
     most = q.shape[0] if max_length is None else min(int(max_length), q.shape[0])
     news = _NEWS.pack(s.data_ptr(), 0, s.shape[0] - 1, most, q.shape[0])
-    return _attend(ctx, ctypes.byref(kv), 0, q, news, ks.data_ptr(), scale, window, sinks,
+    return _attend(ctx, kv, 0, q, news, ks.data_ptr(), scale, window, sinks,
                    max_length if k_starts is None else None, return_lse)
