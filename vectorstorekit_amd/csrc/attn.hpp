@@ -163,6 +163,10 @@ __device__ inline AttnRows attn_rows(const AttnArgs &a, const AttnSeq &s, int32_
 }
 
 #define lds_as __attribute__((address_space(3)))
+// A pointer made of an integer is generic unless it says where it points, and
+// a generic (flat) load counts as one of LDS too: only a wait for none of them
+// is sound behind it.
+#define global_as __attribute__((address_space(1)))
 typedef lds_as char lds_char;
 
 // 16 bytes a lane from base + off to dst + 16 * lane (base and dst the same in

@@ -70,18 +70,18 @@ template <class T> __device__ inline bool not_finite(uint32_t w) {
 
 // W words (16 or 8 bytes) of a row from element e on, zero from element d on
 template <class T, int W, bool ALIGNED>
-__device__ inline void load_row(const T *row, int32_t e, int32_t d, uint32_t (&x)[W]) {
+__device__ inline void load_row(const global_as T *row, int32_t e, int32_t d, uint32_t (&x)[W]) {
   if constexpr (ALIGNED) {
     typedef __attribute__((ext_vector_type(W))) uint32_t VW;
     VW v = {};
-    if (e < d) v = *reinterpret_cast<const VW *>(row + e);
+    if (e < d) v = *reinterpret_cast<const global_as VW *>(row + e);
 #pragma unroll
     for (int i = 0; i < W; ++i) x[i] = v[i];
   } else if constexpr (sizeof(T) == 4) {
 #pragma unroll
     for (int i = 0; i < W; ++i) x[i] = e + i < d ? __builtin_bit_cast(uint32_t, row[e + i]) : 0u;
   } else {
-    const uint16_t *h = reinterpret_cast<const uint16_t *>(row);
+    const global_as uint16_t *h = reinterpret_cast<const global_as uint16_t *>(row);
 #pragma unroll
     for (int i = 0; i < W; ++i) {
       x[i] = e + 2 * i < d ? h[e + 2 * i] : 0u;
@@ -134,7 +134,7 @@ template <class T, int VW, int NB, bool ALIGNED> struct RowTile {
 #pragma unroll
         for (int z = 0; z < 4; ++z) q[i][z] = y[z];
       } else {
-        load_row<T, 4, false>(src, e, real ? a.d : 0, q[i]);
+        load_row<T, 4, false>((const global_as T *)src, e, real ? a.d : 0, q[i]);
       }
     }
     if constexpr (ALIGNED) {
@@ -241,8 +241,7 @@ template <class T, int VW, int NB, bool ALIGNED> struct RowTile {
         const uint32_t at = (uint32_t)n * stride, row = at < most ? at : most;
 #pragma unroll
         for (int i = 0; i < KS; ++i)
-          load_row<T, 4, false>(reinterpret_cast<const T *>(base + row), (4 * i + g) * KE, a.d,
-                                k[u][i]);
+          load_row<T, 4, false>((const global_as T *)(base + row), (4 * i + g) * KE, a.d, k[u][i]);
       }
     }
   }
@@ -250,8 +249,7 @@ template <class T, int VW, int NB, bool ALIGNED> struct RowTile {
   __device__ void load_values(int32_t x, int32_t kb, uint32_t (&v)[U][4][NB][WV]) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const char *base =
-          reinterpret_cast<const char *>((uintptr_t)lane_of(v_lo, v_hi, (x - xb) * U + u));
+      const global_as char *base = (const global_as char *)lane_of(v_lo, v_hi, (x - xb) * U + u);
       const uint32_t stride = (uint32_t)a.v_row * sizeof(T), most = last_of(kb + 16 * u) * stride;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -262,11 +260,12 @@ template <class T, int VW, int NB, bool ALIGNED> struct RowTile {
           if constexpr (ALIGNED) {
             typedef __attribute__((ext_vector_type(WV))) uint32_t V;
             const uint32_t in = sizeof(T) * (e < a.d ? e : a.d - VW);
-            const V y = *reinterpret_cast<const V *>(base + (row + in));
+            const V y = *reinterpret_cast<const global_as V *>(base + (row + in));
 #pragma unroll
             for (int z = 0; z < WV; ++z) v[u][i][b][z] = y[z];
           } else {
-            load_row<T, WV, false>(reinterpret_cast<const T *>(base + row), e, a.d, v[u][i][b]);
+            load_row<T, WV, false>(reinterpret_cast<const global_as T *>(base + row), e, a.d,
+                                   v[u][i][b]);
           }
         }
       }
@@ -275,8 +274,11 @@ template <class T, int VW, int NB, bool ALIGNED> struct RowTile {
 
   // The steps of a wave, `steps` of them, step x at key base(x).  q_lo, q_hi:
   // the smallest and largest position of the tile's rows.  The next step's
-  // keys are asked for as soon as this one's are in the products, its values
-  // likewise: there are always loads in flight.
+  // keys are asked for as soon as this one's are in the products and arrive
+  // while the weights are computed: the compiler does not count the copies into
+  // LDS, so its wait for this step's values is one for them too.  The next
+  // step's values arrive during its first product.  The rest of the time to
+  // memory is hidden by other waves.
   template <class Base>
   __device__ void walk(int32_t steps, int32_t q_lo, int32_t q_hi, Base &&base) {
     if (steps <= 0) return;
@@ -296,7 +298,8 @@ template <class T, int VW, int NB, bool ALIGNED> struct RowTile {
 #pragma unroll 1
     for (int32_t x = 0;;) {
       f32x4 sc[U];
-      // the step's keys have arrived (its values, asked for later, may not)
+      // the step's keys have arrived (its values, asked for later, may not:
+      // 4 * U * NB global loads, which return in order)
       if constexpr (ALIGNED) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(4 * U * NB) : "memory");
       scores(k, sc);
       __builtin_amdgcn_sched_barrier(0);
