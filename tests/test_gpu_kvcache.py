@@ -801,6 +801,29 @@ def test_offsets_out_of_order(ctx):
         assert torch.equal(cache.k, k) and torch.equal(cache.v, v)
 
 
+@pytest.mark.parametrize("d,lengths", [(64, [20]), (128, [9000]), (256, [70, 30])])
+def test_no_rows_to_treat(ctx, d, lengths):
+    """Bounds of no new token at all: nothing is done, however long the keys."""
+    from vectorstorekit_amd import window_attention
+
+    cache, seqs = filled(ctx, lengths, 16, 2, d, BF, width=600, seed=d)
+    starts = [0] + list(range(1, len(lengths) + 1))
+    q = normal(gen(d), len(lengths), 4, d, dtype=BF)
+    out, lse = cache.attend(q, starts=starts, max_new=0, return_lse=True)
+    assert out.shape == q.shape and lse.shape == q.shape[:2]
+    k = cache.k.clone()
+    cache.append(q[:, :2], q[:, 2:], starts=starts, max_new=0)
+    assert torch.equal(cache.k.view(torch.int16), k.view(torch.int16))
+    x = normal(gen(1), 5000, 2, d, dtype=BF)
+    assert window_attention(ctx, x, x, x, starts=[0, 5000], max_length=0).shape == x.shape
+    assert cache.attend(q[:0], starts=[0], max_new=0).shape == (0, 4, d)
+    # and the calls after them are as ever
+    out = cache.attend(q, starts=starts, max_new=1)
+    for i, (kk, vv) in enumerate(seqs):
+        o, _, t = attended(q[i:i + 1], kk[0], vv[0], d ** -0.5, None, 0)
+        check(out[i:i + 1], o, t)
+
+
 @pytest.mark.parametrize("dtype", [BF, F16, F32])
 @pytest.mark.parametrize("new,n", [(1, 100003), (1, 900), (2, 6000), (70, 20000)])
 def test_small_weights_of_many_keys(ctx, dtype, new, n):

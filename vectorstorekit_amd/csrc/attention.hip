@@ -166,9 +166,14 @@ extern "C" {
 
 int64_t vsk_attention_workspace(vsk_ctx *ctx, const vsk_kv *kv, const vsk_new_tokens *news,
                                 const vsk_attention_args *args) {
-  if (!ctx || !kv || !news || !args || kv->kv_heads < 1 || args->q.heads < 1 || news->n < 1 ||
-      args->q.heads % kv->kv_heads || news->max_new < 0 || news->tokens < 1)
-    return 0;
+  if (!ctx) return 0;
+  try {
+    check_shapes(kv, news, args);
+  } catch (const Error &) {
+    return 0;  // (vsk_attention says why)
+  }
+  // (no rows: nothing to divide)
+  if (news->n == 0 || news->tokens == 0 || news->max_new == 0) return 0;
   return workspace_of(plan_of(ctx, kv, news, args), kv, news, args);
 }
 
