@@ -856,6 +856,48 @@ def test_small_weights_of_many_keys(ctx, dtype, new, n):
           torch.full((new, heads), 2.0 ** -16 * 28, dtype=torch.float64))
 
 
+@pytest.mark.parametrize("dtype", [BF, F16, F32])
+@pytest.mark.parametrize("new,n", [(1, 60), (1, 40003), (3, 500), (70, 300), (70, 20000), (600, 700)])
+@pytest.mark.parametrize("scale", [0.2, 0.9, 3.7, 1e3, 1e6])
+def test_scores_that_differ_by_one_rounding(ctx, dtype, new, n, scale):
+    """Scores of +-2^24 and more times ``scale``: in 32 bits a softmax of such
+    scores is the mean over the largest, which many keys share here.  Scores
+    are one product of two values, exact in fp32, so the weights are 1 (off by
+    2^-21 at the most) and 0; the sum, weight and output are as above."""
+    from vectorstorekit_amd import window_attention
+
+    heads, d = 32, 64
+    g = gen(n + new)
+    k = torch.zeros(n, heads, d)
+    # large negative ones first, then, for some of the heads, larger ones, and
+    # zeros for the last: the running maximum climbs as far as it can
+    k[:, :, 0] = torch.where(torch.rand(n, heads, generator=g) < 0.3, -1168.0, -1200.0)
+    later = torch.arange(n)[:, None] >= n // 2
+    some = torch.rand(n, heads, generator=g) < 0.4
+    k[:, 8:16, 0] = torch.where(later & some, 1168.0, k[:, :, 0])[:, 8:16]
+    k[:, 16:24, 0] = torch.where(later & some, 1e-3, k[:, :, 0])[:, 16:24]
+    k[:, 24:, 0] = k[:, 24:, 0].neg()
+    k, v = k.to(dtype).to(DEV), normal(g, n, heads, d, dtype=dtype)
+    q = torch.zeros(new, heads, d, dtype=dtype, device=DEV)
+    q[:, :, 0] = 14592.0  # 57 * 2^8
+    out, lse = window_attention(ctx, q, k, v, starts=[0, new], k_starts=[0, n], scale=scale,
+                                return_lse=True)
+    u = U[dtype]
+    rows = [0, 1, new // 2, new - 1]
+    for i in sorted(set(r for r in rows if r < new)):
+        m = n - new + i + 1
+        s = q[i, :, :1].cpu().double() * k[:m, :, 0].cpu().double().T  # heads x keys
+        s *= float(np.float32(scale))
+        w = torch.softmax(s, 1)
+        vv = v[:m].cpu().double()
+        want = torch.einsum("hm,mhd->hd", w, vv)
+        tol = u * want.abs() + float(vv.abs().max()) * (
+            2 * (2.0 ** -21 + 2.0 ** -24 * (n + 16)) + (u if dtype != F32 else 0))
+        check(out[i], want, tol)
+        le = torch.logsumexp(s, 1)
+        check(lse[i], le, 2.0 ** -16 + 2.0 ** -21 * s.abs().amax(1))
+
+
 def test_refusals_of_lost_meaning(ctx):
     """What would otherwise pass and mean something else."""
     from vectorstorekit_amd import RotaryEmbedding, VSKError, window_attention

@@ -42,7 +42,7 @@ struct AttnArgs {
   int32_t chunk;        // key tiles of a part
   float scale_log2;     // scale * log2(e)
   float *part_o;        // splits x tokens x heads x d
-  float *part_ml;       // splits x tokens x heads x 2: reference (log2), sum
+  float *part_ml;       // splits x tokens x heads x 2: reference (a score), sum
 };
 
 // One sequence of the call.
@@ -198,6 +198,10 @@ template <int CH> __device__ inline int k_swizzle(int row) {
 }
 
 __device__ inline float attn_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
+// log of a row's sum, whose weights are 2^(score * scale_log2 - ref)
+__device__ inline float attn_lse(float ref, float sum) {
+  return sum > 0.f ? (ref + __log2f(sum)) * 0.6931471805599453f : sum != sum ? sum : -INFINITY;
+}
 // Exchanges between lanes 16 and 32 apart on the vector unit: of x twice, the
 // swap of the odd rows (the upper half) of the one with the even rows (the
 // lower half) of the other leaves each pair's two values in the two results.

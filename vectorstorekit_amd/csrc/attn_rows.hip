@@ -35,8 +35,7 @@ namespace vsk {
 namespace {
 
 // What a type's 32-bit words hold: E elements; 16 bytes hold 4 * E.
-// TOP: log2 of the largest weight, the sums' reference being 2^-TOP of it.  An
-// f16 of 1 at most loses a weight under 2^-25, and a long context may hold many
+// TOP: log2 of the largest weight.  An f16 of 1 at most loses a weight under 2^-25, and a long context may hold many
 // of them behind one large first key; bf16 has fp32's exponents.
 template <class T> struct Elem;
 template <> struct Elem<float> {
@@ -114,7 +113,8 @@ template <class T, int VW, int NB, bool ALIGNED> struct RowTile {
   int32_t pos;  // position of this lane's row, -1 if there is none
   uint32_t q[KS][4];
   f32x4 acc[NB][VW];
-  float m = -INFINITY, l = 0.f;
+  float m = -INFINITY;  // the largest score, unscaled
+  float l = 0.f;
 
   __device__ RowTile(const AttnArgs &a_, const AttnSeq &s_, int32_t h_, int lane, lds_char *l_)
       : a(a_), s(s_), lds(l_), h(h_), n(lane & 15), g(lane >> 4) {}
@@ -360,16 +360,19 @@ template <class T, int VW, int NB, bool ALIGNED> struct RowTile {
     float top = fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3]));
     if constexpr (U == 2)
       top = fmaxf(top, fmaxf(fmaxf(sc[1][0], sc[1][1]), fmaxf(sc[1][2], sc[1][3])));
-    top = fmaxf(m, xor16_32_max(top) * a.scale_log2 - Elem<T>::TOP);
+    // The largest score is subtracted before the scale comes in: its product
+    // with the scale, rounded, would be off by more than a weight's range where
+    // scores pass 2^24.
+    top = fmaxf(m, xor16_32_max(top));
     const float use = top == -INFINITY ? 0.f : top;
-    const float fade = attn_exp2(m - use);
+    const float fade = attn_exp2((m - use) * a.scale_log2);
     m = top;
     l *= fade;
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        p[u][i] = attn_exp2(fmaf(sc[u][i], a.scale_log2, -use));
+        p[u][i] = attn_exp2(fmaf(sc[u][i] - use, a.scale_log2, Elem<T>::TOP));
         l += p[u][i];
       }
 #pragma unroll
@@ -521,8 +524,7 @@ k_attn_rows(const AttnArgs a) {
         }
       if (a.lse && tl.g == 0)
         a.lse[token * a.heads + head] =
-            tl.l > 0.f ? (tl.m + __log2f(tl.l)) * 0.6931471805599453f
-                       : tl.l != tl.l ? tl.l : -INFINITY;
+            attn_lse(tl.m * a.scale_log2 - Elem<T>::TOP, tl.l);
     }
   } else {
     typedef float Sums[ROWS][DV + 4];
@@ -535,10 +537,12 @@ k_attn_rows(const AttnArgs a) {
     for (int x = 0; x < SHARE; ++x) top = fmaxf(top, sm[x][tl.n]);
     const float use = top == -INFINITY ? 0.f : top;
 #pragma unroll
-    for (int x = 0; x < SHARE; ++x) sum += sl[x][tl.n] * attn_exp2(sm[x][tl.n] - use);
-    // rows of a part: the sums as they are; of the whole: the quotient
-    float f = attn_exp2(tl.m - use);
-    if (!partial) f *= sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+    for (int x = 0; x < SHARE; ++x)
+      sum += sl[x][tl.n] * attn_exp2((sm[x][tl.n] - use) * a.scale_log2);
+    // rows of a part: the sums with weights up to 1; of the whole: the quotient
+    constexpr float ONE = Elem<T>::TOP > 0.f ? 1.f / 32768.f : 1.f;  // 2^-TOP
+    float f = attn_exp2((tl.m - use) * a.scale_log2);
+    f *= partial ? ONE : sum > 0.f || sum != sum ? 1.f / sum : 0.f;
 #pragma unroll
     for (int turn = 0; turn < (SHARE + SLOTS - 1) / SLOTS; ++turn) {
       if (w / SLOTS == turn && tl.n < rows) {
@@ -563,10 +567,9 @@ k_attn_rows(const AttnArgs a) {
       const int64_t row = (s.token0 + r / a.group) * a.heads + h * a.group + r % a.group;
       if (partial) {
         a.part_ml[2 * (row_of + row)] = top;
-        a.part_ml[2 * (row_of + row) + 1] = sum;
+        a.part_ml[2 * (row_of + row) + 1] = sum * ONE;
       } else if (a.lse) {
-        a.lse[row] = sum > 0.f ? (top + __log2f(sum)) * 0.6931471805599453f
-                               : sum != sum ? sum : -INFINITY;
+        a.lse[row] = attn_lse(top * a.scale_log2 - Elem<T>::TOP, sum);
       }
     }
     for (int32_t x = threadIdx.x; x < rows * (DV / 4); x += 64 * SHARE) {
@@ -596,7 +599,7 @@ k_attn_rows(const AttnArgs a) {
 }
 
 // Joins the parts of one output row: sum of the parts' values and sums, each
-// times 2^(its maximum - the largest).  A block a row, or a block for SL values
+// times exp(its reference less the largest, scaled).  A block a row, or a block for SL values
 // of one; the threads take four values each of several parts at a time.  Its
 // bytes are few: it is bound by the chain count, maximum, parts, each a trip to
 // memory (5 us behind 64 parts of 192 rows of 128).
@@ -641,14 +644,14 @@ __global__ __launch_bounds__(256) void k_attn_join(const AttnArgs a, const int32
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
   float sum = 0.f;
   if (way < parts) {
-    const float f = attn_exp2(fm0 - use);
+    const float f = attn_exp2((fm0 - use) * a.scale_log2);
     sum = f * fl0;
     o = f * o0;
   }
 #pragma unroll 4
   for (int32_t i = way + WAYS; i < parts; i += WAYS) {
     const int64_t r = i * stride + at;
-    const float f = attn_exp2(a.part_ml[2 * r] - use);
+    const float f = attn_exp2((a.part_ml[2 * r] - use) * a.scale_log2);
     sum += f * a.part_ml[2 * r + 1];
     if (e < a.d) o += f * *reinterpret_cast<const f32x4 *>(a.part_o + r * DV + e);
   }
@@ -662,9 +665,7 @@ __global__ __launch_bounds__(256) void k_attn_join(const AttnArgs a, const int32
     sum += ss[i];
   }
   const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
-  if (e == 0 && a.lse)
-    a.lse[at] = sum > 0.f ? (top + __log2f(sum)) * 0.6931471805599453f
-                          : sum != sum ? sum : -INFINITY;
+  if (e == 0 && a.lse) a.lse[at] = attn_lse(top * a.scale_log2, sum);
   if (e >= a.d) return;
   T *dst = static_cast<T *>(a.out) + (s.token0 + t) * a.o_row + head * a.o_head + e;
   const float z[4] = {o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};

@@ -80,6 +80,7 @@ __device__ inline float max3(float a, float b, float c) {
 template <class T, int DP>
 __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void k_attn_tile(const AttnArgs a) {
   typedef typename Mm<T>::V8 V8;
+  typedef __attribute__((ext_vector_type(4))) T V4;
   constexpr int KT = attn_tile_keys(DP), U = KT / 32, G = ATTN_TILE_GROUP;
   constexpr int PITCH = DP <= 64 ? 64 : DP <= 128 ? 128 : 256;
   constexpr int CH = PITCH / 8;      // 16-byte pieces of a row
@@ -259,12 +260,19 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void k_attn_tile(const 
       tm = max3(tm, sc[x >> 4][x & 15], sc[(x + 1) >> 4][(x + 1) & 15]);
     return xor32_max(max3(tm, sc[U - 1][15], sc[U - 1][15]));
   };
+  // Past FAR the product of a score and the scale, and so m, is rounded by more
+  // than an eighth of one in log2, further on (2^24) by more than the room that
+  // f16's weights have, then fp32's.  Rows with such scores, which no model
+  // makes, are computed again at the end.
+  constexpr float FAR = 2097152.f;
+  bool far = false;
   // The sums are kept relative to m, which follows the largest score (less TOP)
   // only when that has grown by 8 (in log2): weights 256 times as large cost no
   // precision, and the sums are seldom rescaled.
   auto settle = [&](float tm) {
     const float top = tm * a.scale_log2 - Mm<T>::TOP;
     if (!__any(top > m + 8.f)) return;
+    far |= fabsf(top) > FAR && fabsf(tm) < INFINITY;
     const float nm = top > m + 8.f ? top : m;
     const float fade = nm == -INFINITY ? 1.f : attn_exp2(m - nm);
     m = nm;
@@ -485,10 +493,65 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void k_attn_tile(const 
     }
   }
 
-  const float sum = xor32_sum(l);
+  float sum = xor32_sum(l);
+  // Key by key on the vector unit, the largest score subtracted before the
+  // scale comes in.  Of a row's products a lane has half, of its outputs those
+  // in its registers.
+  float ref = -INFINITY;  // by_key: the largest score, unscaled
+  const bool by_key = __any(far);
+  if (by_key) {
+#pragma unroll
+    for (int x = 0; x < DT; ++x) acc[x] = f32x16{};
+    sum = 0.f;
+#pragma unroll 1
+    for (int32_t x = first * KT; x < end * KT; ++x) {
+      const int32_t j = span.group(x / G) + x % G;
+      const bool see = attn_sees(a, pos, j);
+      if (!__any(see)) continue;
+      const AttnRows r = attn_rows(a, s, h, j & ~15, attn_page(a, s, j & ~15));
+      const T *kr = static_cast<const T *>(a.k) + r.k + (j & 15) * a.k_row;
+      const T *vr = static_cast<const T *>(a.v) + r.v + (j & 15) * a.v_row;
+      float sc = 0.f;
+#pragma unroll
+      for (int i = 0; i < KS; ++i) {
+        const int e = 16 * i + 8 * h2;
+        if (e >= a.d) continue;
+        const V8 kv = *reinterpret_cast<const V8 *>(kr + e), qv = query(i);
+#pragma unroll
+        for (int y = 0; y < 8; ++y) sc = fmaf((float)qv[y], (float)kv[y], sc);
+      }
+      sc = xor32_sum(sc);
+      const float top = see ? fmaxf(ref, sc) : ref, use = top == -INFINITY ? 0.f : top;
+      const float fade = attn_exp2((ref - use) * a.scale_log2);
+      const float p = see ? attn_exp2((sc - use) * a.scale_log2) : 0.f;
+      ref = top;
+      sum = sum * fade + p;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) {
+        acc[dt] *= fade;
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+          const int e = 32 * dt + 8 * b + 4 * h2;
+          if (!see || e >= a.d) continue;
+          const V4 vv = *reinterpret_cast<const V4 *>(vr + e);
+#pragma unroll
+          for (int y = 0; y < 4; ++y) acc[dt][4 * b + y] = fmaf(p, (float)vv[y], acc[dt][4 * b + y]);
+        }
+      }
+    }
+    m = ref * a.scale_log2;
+  }
   const int64_t out_row = (s.token0 + my_t) * a.heads + my_head;
   if (parts > 1) {
     if (!real) return;
+    // a part's reference is a score: the one that m was made of, or near it
+    if (!by_key && m != -INFINITY) {
+      ref = (m + Mm<T>::TOP) / a.scale_log2;
+      const float f = attn_exp2(-fmaf(ref, a.scale_log2, -m));
+      sum *= f;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) acc[dt] *= f;
+    }
     const int64_t x = (int64_t)part * a.tokens * a.heads + out_row;
     float *dst = a.part_o + x * PITCH;
 #pragma unroll
@@ -498,7 +561,7 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void k_attn_tile(const 
         *reinterpret_cast<f32x4 *>(dst + 32 * dt + 8 * b + 4 * h2) =
             f32x4{acc[dt][4 * b], acc[dt][4 * b + 1], acc[dt][4 * b + 2], acc[dt][4 * b + 3]};
     if (h2 == 0) {
-      a.part_ml[2 * x] = m;
+      a.part_ml[2 * x] = ref;
       a.part_ml[2 * x + 1] = sum;
     }
     return;
@@ -506,7 +569,6 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void k_attn_tile(const 
   const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
   // The outputs leave by way of LDS (no wave reads keys any more), so that a
   // store of a wave is whole rows and not eight bytes of each.
-  typedef __attribute__((ext_vector_type(4))) T V4;
   lds_char *const obuf = (QLDS ? (lds_char *)queries_lds : kbuf) + 32 * w * ROWB;
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt)
@@ -528,8 +590,7 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void k_attn_tile(const 
       *reinterpret_cast<Piece *>(static_cast<T *>(a.out) + row + 8 * piece) = y;
   }
   if (a.lse && h2 == 0 && real)
-    a.lse[out_row] = sum > 0.f ? (m + __log2f(sum)) * 0.6931471805599453f
-                               : sum != sum ? sum : -INFINITY;
+    a.lse[out_row] = attn_lse(m, sum);
 }
 
 template <class T> void tile_of(hipStream_t st, const AttnArgs &a, unsigned g) {
