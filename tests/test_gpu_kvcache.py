@@ -898,6 +898,46 @@ def test_scores_that_differ_by_one_rounding(ctx, dtype, new, n, scale):
         check(lse[i], le, 2.0 ** -16 + 2.0 ** -21 * s.abs().amax(1))
 
 
+@pytest.mark.parametrize("dtype", [BF, F16, F32])
+@pytest.mark.parametrize("heads,kv,d,new,n", [(8, 2, 128, 1, 700), (8, 8, 64, 1, 90),
+                                              (4, 1, 256, 1, 9000), (6, 3, 100, 1, 300),
+                                              (4, 2, 128, 40, 300), (5, 5, 33, 20, 130),
+                                              (64, 32, 128, 130, 300), (48, 48, 64, 400, 400),
+                                              (128, 16, 256, 70, 200)])
+def test_infinite_values(ctx, dtype, heads, kv, d, new, n):
+    """A visible infinity is the sum of its column, with its sign; two of
+    different signs are NaN; a row that does not see it is as without it.  The
+    weight is an ordinary one, and one of 2^-40 of the largest."""
+    from vectorstorekit_amd import window_attention
+
+    g = gen(d + new)
+    q, k, v = (normal(g, m, h, d, dtype=dtype) for m, h in ((new, heads), (n, kv), (n, kv)))
+    window, sinks = n - new // 2, 3
+    # key 5 of key head 1 has a score 40 in log2 below every other's largest
+    low = 1 if kv > 1 else 0
+    q[..., 0], k[..., 0] = 8.0, 0.0
+    k[5, low] = 0.0
+    k[5, low, 0] = -64.0
+    scale = 40 * math.log(2) / 512
+    clean, _, t = attended_at_once(q, k, v, scale, window, sinks)
+    for where in ([(n - new, 1.0)], [(2, -1.0)], [(5, 1.0)], [(n - new, 1.0), (n // 2, -1.0)]):
+        bad, want = v.clone(), clean.clone()
+        for j, sign in where:
+            bad[j, low, d // 2] = sign * math.inf
+        for i in range(new):
+            pos = n - new + i
+            signs = {sign for j, sign in where if j <= pos and (pos - j < window or j < sinks)}
+            if signs:
+                one = slice(low * (heads // kv), (low + 1) * (heads // kv))
+                want[i, one, d // 2] = math.nan if len(signs) > 1 else signs.pop() * math.inf
+        out = window_attention(ctx, q, k, bad, starts=[0, new], k_starts=[0, n], scale=scale,
+                               window=window, sinks=sinks).cpu().double()
+        odd = ~torch.isfinite(want)
+        assert torch.equal(torch.isnan(out), torch.isnan(want))
+        assert torch.equal(out[torch.isinf(want)], want[torch.isinf(want)])
+        check(out.masked_fill(odd, 0.0), want.masked_fill(odd, 0.0), t.masked_fill(odd, 0.0))
+
+
 def test_refusals_of_lost_meaning(ctx):
     """What would otherwise pass and mean something else."""
     from vectorstorekit_amd import RotaryEmbedding, VSKError, window_attention

@@ -67,6 +67,15 @@ template <class T> __device__ inline bool not_finite(uint32_t w) {
   return (w & X) == X || ((w >> 16) & X) == X;
 }
 
+// x, as a value that the compiler computes nothing from beforehand: what it
+// would (comparisons, a division's reciprocal) waits in registers through the
+// loop over the keys, or, with too few of them, in scratch memory, which alone
+// costs 64 contexts to 8,192 2 us.
+__device__ inline int32_t hidden(int32_t x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+
 // W words (16 or 8 bytes) of a row from element e on, zero from element d on
 template <class T, int W, bool ALIGNED>
 __device__ inline void load_row(const global_as T *row, int32_t e, int32_t d, uint32_t (&x)[W]) {
@@ -109,7 +118,8 @@ template <class T, int VW, int NB, bool ALIGNED> struct RowTile {
   // (aligned) the step's keys in LDS, this wave's own
   static constexpr int ROWB = DV * (int)sizeof(T), CH = ROWB / 16, RPI = 64 / CH;
   lds_char *const lds;
-  const int32_t h, n, g;
+  const int32_t h;
+  int32_t n, g;
   int32_t pos;  // position of this lane's row, -1 if there is none
   uint32_t q[KS][4];
   f32x4 acc[NB][VW];
@@ -194,7 +204,7 @@ template <class T, int VW, int NB, bool ALIGNED> struct RowTile {
   int32_t xb;
   template <class Base> __device__ void addresses(int32_t x, int32_t steps, Base &&base) {
     xb = x;
-    const int32_t lane = threadIdx.x & 63;
+    const int32_t lane = hidden(threadIdx.x & 63);
     int32_t at = x + lane / U;
     at = at < steps ? at : steps - 1;
     const int32_t j = attn_row16(s, base(at) + 16 * (lane % U));
@@ -432,6 +442,74 @@ template <class T, int VW, int NB, bool ALIGNED> struct RowTile {
           }
     }
   }
+  // Has a sum become NaN while the weights are numbers?  Of a weight's two
+  // 16-bit parts the second is negative or zero half of the time: the products
+  // of an infinite value have both signs, or are NaN.
+  __device__ bool lost() const {
+    bool odd = false;
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int t = 0; t < VW; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; i += 2)
+          odd |= __builtin_isunordered(acc[b][t][i], acc[b][t][i + 1]);
+    const float sum = xor16_32_sum(l);
+    return odd && sum == sum;
+  }
+  // Then the steps once more, key by key on the vector unit, with weights in 32
+  // bits.  (A rare path: few registers at a time, so that it takes none from
+  // the others.)
+  template <class Base> __device__ void by_key(int32_t steps, Base &&base) {
+    m = -INFINITY, l = 0.f;
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int t = 0; t < VW; ++t) acc[b][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+    for (int32_t x = 0; x < steps * KT; ++x) {
+      const int32_t j = base(x / KT) + x % KT, j16 = j & ~15;
+      const bool see = attn_sees(a, pos, j);
+      if (!__any(see)) continue;
+      const int32_t d = hidden(a.d);
+      const AttnRows r = attn_rows(a, s, h, j16, attn_page(a, s, j16));
+      const T *kr = static_cast<const T *>(a.k) + r.k + (j & 15) * a.k_row;
+      const T *vr = static_cast<const T *>(a.v) + r.v + (j & 15) * a.v_row;
+      float sc = 0.f;
+#pragma unroll
+      for (int i = 0; i < KS; ++i) {
+        const int32_t e = (4 * i + g) * KE;
+#pragma unroll
+        for (int y = 0; y < KE; ++y)
+          if (e + y < d) sc = fmaf(query(i, y), (float)kr[e + y], sc);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      sc = xor16_32_sum(sc);
+      const float top = see ? fmaxf(m, sc) : m, use = top == -INFINITY ? 0.f : top;
+      const float fade = attn_exp2((m - use) * a.scale_log2);
+      const float p = see ? attn_exp2(fmaf(sc - use, a.scale_log2, Elem<T>::TOP)) : 0.f;
+      m = top;
+      l = l * fade + (g == 0 ? p : 0.f);  // (the row's four lanes are added up later)
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int t = 0; t < VW; ++t) {
+          acc[b][t] *= fade;
+#pragma unroll
+          for (int y = 0; y < 4; ++y) {
+            const int32_t e = (16 * b + 4 * g + y) * VW + t;
+            if (see && e < d) acc[b][t][y] = fmaf(p, (float)vr[e], acc[b][t][y]);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+  }
+  // element y of the query's piece i
+  __device__ float query(int i, int y) const {
+    typedef __attribute__((ext_vector_type(KE))) T V;
+    const u32x4 w = {q[i][0], q[i][1], q[i][2], q[i][3]};
+    return (float)__builtin_bit_cast(V, w)[y];
+  }
 };
 
 // waves a SIMD, by the registers that the values of a step and the sums take
@@ -491,17 +569,26 @@ k_attn_rows(const AttnArgs a) {
   __shared__ __attribute__((aligned(1024))) char pool[KEYB > SUMB ? KEYB : SUMB];
   Tile tl(a, s, h, lane, (lds_char *)pool + (ALIGNED ? w * Tile::KT * Tile::ROWB : 0));
   tl.begin(have ? row0 + tl.n : 0x3fffffff);
-  tl.walk((end - first + SHARE - 1) / SHARE, q_lo, q_hi,
-          [&](int32_t x) { return span.base(first + SHARE * x); });
+  const auto base = [&](int32_t x) { return span.base(first + SHARE * x); };
+  const int32_t steps = (end - first + SHARE - 1) / SHARE;
+  tl.walk(steps, q_lo, q_hi, base);
+  {
+    // (the lane's place anew)
+    const int32_t tid = hidden(threadIdx.x);
+    tl.n = tid & 15, tl.g = (tid >> 4) & 3;
+  }
+  if constexpr (!Tile::F32)
+    if (__any(tl.lost())) tl.by_key(steps, base);
   tl.l = xor16_32_sum(tl.l);
 
   const bool partial = parts > 1;
+  const int32_t group = hidden(a.group);
   const int64_t row_of = (int64_t)part * a.tokens * a.heads;
   if constexpr (SHARE == 1) {
     if (tl.n < rows) {
       const int32_t r = row0 + tl.n;
-      const int64_t token = s.token0 + r / a.group;
-      const int32_t head = h * a.group + r % a.group;
+      const int64_t token = s.token0 + r / group;
+      const int32_t head = h * group + r % group;
       const float inv = tl.l > 0.f || tl.l != tl.l ? 1.f / tl.l : 0.f;
       T *dst = static_cast<T *>(a.out) + token * a.o_row + head * a.o_head;
 #pragma unroll
@@ -564,7 +651,7 @@ k_attn_rows(const AttnArgs a) {
     }
     if (w == 0 && tl.g == 0 && tl.n < rows) {
       const int32_t r = row0 + tl.n;
-      const int64_t row = (s.token0 + r / a.group) * a.heads + h * a.group + r % a.group;
+      const int64_t row = (s.token0 + r / group) * a.heads + h * group + r % group;
       if (partial) {
         a.part_ml[2 * (row_of + row)] = top;
         a.part_ml[2 * (row_of + row) + 1] = sum * ONE;
@@ -579,8 +666,8 @@ k_attn_rows(const AttnArgs a) {
 #pragma unroll
       for (int z = 1; z < SLOTS; ++z) y += *reinterpret_cast<f32x4 *>(&so[z][rr][e]);
       const int32_t r = row0 + rr;
-      const int64_t token = s.token0 + r / a.group;
-      const int32_t head = h * a.group + r % a.group;
+      const int64_t token = s.token0 + r / group;
+      const int32_t head = h * group + r % group;
       if (partial) {
         float *dst = a.part_o + (row_of + token * a.heads + head) * DV + e;
         *reinterpret_cast<f32x4 *>(dst) = y;

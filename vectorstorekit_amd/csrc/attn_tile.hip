@@ -265,14 +265,14 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void k_attn_tile(const 
   // f16's weights have, then fp32's.  Rows with such scores, which no model
   // makes, are computed again at the end.
   constexpr float FAR = 2097152.f;
-  bool far = false;
+  bool again = false;
   // The sums are kept relative to m, which follows the largest score (less TOP)
   // only when that has grown by 8 (in log2): weights 256 times as large cost no
   // precision, and the sums are seldom rescaled.
   auto settle = [&](float tm) {
     const float top = tm * a.scale_log2 - Mm<T>::TOP;
     if (!__any(top > m + 8.f)) return;
-    far |= fabsf(top) > FAR && fabsf(tm) < INFINITY;
+    again |= fabsf(top) > FAR && fabsf(tm) < INFINITY;
     const float nm = top > m + 8.f ? top : m;
     const float fade = nm == -INFINITY ? 1.f : attn_exp2(m - nm);
     m = nm;
@@ -494,11 +494,20 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void k_attn_tile(const 
   }
 
   float sum = xor32_sum(l);
+  // An f16 weight may have been rounded to zero, and zero times an infinite
+  // value is NaN.
+  if constexpr (Mm<T>::TOP > 0.f) {
+    bool odd = false;
+#pragma unroll
+    for (int x = 0; x < 16 * DT; x += 2)
+      odd |= __builtin_isunordered(acc[x >> 4][x & 15], acc[x >> 4][(x & 15) + 1]);
+    again |= odd && sum == sum;
+  }
   // Key by key on the vector unit, the largest score subtracted before the
   // scale comes in.  Of a row's products a lane has half, of its outputs those
   // in its registers.
   float ref = -INFINITY;  // by_key: the largest score, unscaled
-  const bool by_key = __any(far);
+  const bool by_key = __any(again);
   if (by_key) {
 #pragma unroll
     for (int x = 0; x < DT; ++x) acc[x] = f32x16{};
