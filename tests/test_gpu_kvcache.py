@@ -557,6 +557,25 @@ def test_pages(ctx, dtype, kv, d, order, pages):
     assert short > 0 or pages > 100
 
 
+@pytest.mark.parametrize("slots,width", [(32, 4), (33, 1 << 26)])
+def test_reserve_more_than_32_bits_of_pages(ctx, slots, width):
+    """Pages wanted in all pass 2^31: they are counted as far as that, and the
+    first sequences get what there is."""
+    from vectorstorekit_amd import PagedKVCache
+
+    cache = PagedKVCache(ctx, pages=40, page_size=16, kv_heads=1, head_dim=8, slots=slots,
+                         width=width, dtype=F16)
+    cache.reserve(list(range(slots)), [2 ** 31 - 1] * slots)
+    assert cache.missing() == 2 ** 31 - 1
+    each = min(width, 40)
+    want = [16 * max(0, min(each, 40 - i * each)) for i in range(slots)]
+    assert cache.lengths.tolist() == want
+    assert cache.refs.tolist() == [1] * 40
+    for i, n in enumerate(want):
+        assert cache.table[i, :n // 16].tolist() == list(range(i * each, i * each + n // 16))
+        assert bool((cache.table[i, n // 16:] == -1).all())
+
+
 @pytest.mark.parametrize("pages", [3500, 33000])
 def test_fork_many(ctx, pages):
     """More branches than a workgroup has threads, twice: the second drops the

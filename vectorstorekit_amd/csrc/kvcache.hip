@@ -89,18 +89,18 @@ Pool pool_of(const vsk_kv *kv) {
 }
 
 // Sum of x over the threads before this one; *total: over all.
-__device__ inline int32_t scan(int32_t x, int32_t *total) {
-  __shared__ int32_t waves[NT / 64];
+template <class I> __device__ inline I scan(I x, I *total) {
+  __shared__ I waves[NT / 64];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  int32_t y = x;
+  I y = x;
   for (int o = 1; o < 64; o <<= 1) {
-    const int32_t z = __shfl_up(y, o);
+    const I z = __shfl_up(y, o);
     if (lane >= o) y += z;
   }
   __syncthreads();
   if (lane == 63) waves[w] = y;
   __syncthreads();
-  int32_t before = 0, all = 0;
+  I before = 0, all = 0;
   for (int i = 0; i < NT / 64; ++i) {
     if (i < w) before += waves[i];
     all += waves[i];
@@ -131,7 +131,7 @@ __device__ int32_t take_free(const Pool &p, int32_t want, C &&count_of, F &&take
     for (int i = 0; i < 4; ++i)
       if (c + 4 * (int32_t)threadIdx.x + i < p.pages && count[i] <= 0) mask |= 1 << i;
     int32_t all;
-    int32_t rank = found + scan(__popc(mask), &all);
+    int32_t rank = found + scan((int32_t)__popc(mask), &all);
     for (int i = 0; i < 4; ++i)
       if (mask >> i & 1) {
         if (rank < want) take(rank, c + 4 * (int32_t)threadIdx.x + i);
@@ -156,25 +156,28 @@ __device__ inline void release(const Pool &p, int32_t slot, int32_t i) {
 
 __global__ __launch_bounds__(NT) void k_kv_reserve(const Pool p, const int32_t *seqs,
                                                    const int32_t *counts, int32_t n) {
+  // base: pages that the sequences before want, as far as 32 bits count (there
+  // are fewer)
   int32_t *base = p.slot_list(0);
-  int32_t want = 0;
+  int64_t want = 0;
+  const auto counted = [](int64_t x) { return x < INT32_MAX ? (int32_t)x : INT32_MAX; };
   for (int32_t c = 0; c < n; c += NT) {
     const int32_t i = c + threadIdx.x;
-    int32_t need = 0;
+    int64_t need = 0;
     if (i < n && (uint32_t)seqs[i] < (uint32_t)p.slots) {
       const int32_t l = held(p, seqs[i]), most = p.width << p.shift;
       const int32_t add = counts[i] > 0 ? counts[i] : 0;
       const int32_t to = add > most - l ? most : l + add;
       need = ((to + p.page_size - 1) >> p.shift) - ((l + p.page_size - 1) >> p.shift);
     }
-    int32_t all;
-    const int32_t before = scan(need, &all);
-    if (i < n) base[i] = want + before;
+    int64_t all;
+    const int64_t before = scan(need, &all);
+    if (i < n) base[i] = counted(want + before);
     want += all;
   }
   __syncthreads();
   const auto count = [&](int32_t id) { return p.refs[id]; };
-  const int32_t got = take_free(p, want, count, [&](int32_t rank, int32_t page) {
+  const int32_t got = take_free(p, counted(want), count, [&](int32_t rank, int32_t page) {
     int32_t lo = 0, hi = n;  // the last sequence whose first rank is at most this one
     while (hi - lo > 1) {
       const int32_t mid = (lo + hi) / 2;
@@ -189,7 +192,7 @@ __global__ __launch_bounds__(NT) void k_kv_reserve(const Pool p, const int32_t *
     p.refs[page] = 1;
   });
   __syncthreads();
-  __shared__ int32_t cut;
+  __shared__ unsigned long long cut;
   if (threadIdx.x == 0) cut = 0;
   __syncthreads();
   for (int32_t i = threadIdx.x; i < n; i += NT) {
@@ -197,17 +200,17 @@ __global__ __launch_bounds__(NT) void k_kv_reserve(const Pool p, const int32_t *
     const int32_t l = held(p, seqs[i]), most = p.width << p.shift;
     const int32_t add = counts[i] > 0 ? counts[i] : 0;
     const int32_t to = add > most - l ? most : l + add;
-    const int32_t end = i + 1 < n ? base[i + 1] : want;
+    const int32_t end = i + 1 < n ? base[i + 1] : counted(want);
     int32_t have = got - base[i];
     have = have < 0 ? 0 : have > end - base[i] ? end - base[i] : have;
     const int64_t reach = ((int64_t)((l + p.page_size - 1) >> p.shift) + have) << p.shift;
     p.lengths[seqs[i]] = to < reach ? to : (int32_t)reach;
     // pages past the table's width are missing too
     const int64_t wide = ((int64_t)l + add + p.page_size - 1) >> p.shift;
-    if (wide > p.width) atomicAdd(&cut, (int32_t)(wide - p.width));
+    if (wide > p.width) atomicAdd(&cut, (unsigned long long)(wide - p.width));
   }
   __syncthreads();
-  if (threadIdx.x == 0) p.status[0] = want - got + cut;
+  if (threadIdx.x == 0) p.status[0] = counted(want - got + (int64_t)cut);
 }
 
 // A wave a child: its row's and its parent's entries are loaded together, and
@@ -274,7 +277,7 @@ __global__ __launch_bounds__(NT) void k_kv_fork(const Pool p, const int32_t *par
     const int32_t i = b + threadIdx.x, part = l & (p.page_size - 1);
     const int32_t last = part ? p.table[f * p.table_stride + (l >> p.shift)] : -1;
     int32_t want;
-    const int32_t before = scan(part > 0, &want);
+    const int32_t before = scan((int32_t)(part > 0), &want);
     if (part > 0) who[before] = threadIdx.x;
     // (this wave's atomics are done: the barrier alone would not wait for them)
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
