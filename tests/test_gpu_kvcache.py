@@ -986,6 +986,17 @@ def test_refusals_of_lost_meaning(ctx):
         assert torch.equal(cache.attend(y), cache.attend(x))
 
 
+def test_page_keeping_beyond_its_counts(ctx):
+    """More pages or slots than the kernels count are refused, not launched."""
+    import ctypes
+
+    cache, _ = filled(ctx, [20, 4], 16, 2, 64, F32, poison=False)
+    for field in ("pages", "slots"):
+        kv = type(cache._kv).from_buffer_copy(cache._kv)
+        setattr(kv, field, (1 << 30) + 1)
+        assert ctx.lib.vsk_kv_compact(ctx.handle, None, ctypes.byref(kv)) == -9
+
+
 def test_refusals(ctx):
     from vectorstorekit_amd import PagedKVCache, RotaryEmbedding, VSKError, window_attention
 

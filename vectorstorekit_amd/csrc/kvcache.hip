@@ -73,6 +73,9 @@ Pool pool_of(const vsk_kv *kv) {
   VSK_REQUIRE(kv->refs && kv->status && kv->scratch && is_device_ptr(kv->refs) &&
                   is_device_ptr(kv->status) && is_device_ptr(kv->scratch),
               VSK_ERR_INVALID_ARGUMENT, "page keeping needs refs, status and scratch");
+  // (the kernels step past the last page and slot in 32 bits)
+  VSK_REQUIRE(kv->pages <= (1 << 30) && kv->slots <= (1 << 30), VSK_ERR_INVALID_BUFFER_SIZE,
+              "page keeping for at most 2^30 pages and slots");
   Pool p;
   p.k = static_cast<char *>(kv->k);
   p.v = static_cast<char *>(kv->v);
