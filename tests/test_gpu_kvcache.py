@@ -986,6 +986,31 @@ def test_refusals_of_lost_meaning(ctx):
         assert torch.equal(cache.attend(y), cache.attend(x))
 
 
+def test_tangents_are_refused(ctx):
+    """Forward-mode and functional gradients are not dropped silently."""
+    from torch.autograd import forward_ad
+
+    from vectorstorekit_amd import RotaryEmbedding, VSKError, window_attention
+
+    cache, _ = filled(ctx, [20, 4], 16, 2, 64, F32, poison=False)
+    x, pos, rope = torch.ones(2, 2, 64, device=DEV), ints([0, 1]), RotaryEmbedding(ctx, 64)
+    calls = (lambda y: rope.apply(y, positions=pos), cache.attend,
+             lambda y: cache.append(x, y), lambda y: cache.append(x, x, q=y),
+             lambda y: window_attention(ctx, x, y, x, starts=[0, 2]))
+    for grads in (True, False):
+        with forward_ad.dual_level(), torch.set_grad_enabled(grads):
+            for f in calls:
+                with pytest.raises(VSKError) as e:
+                    f(forward_ad.make_dual(x, x))
+                assert e.value.kind == "unsupportedOperation"
+            rope.apply(x, positions=pos)  # one without a tangent is as ever
+    for f in calls:
+        with pytest.raises((VSKError, RuntimeError)):
+            torch.func.jvp(f, (x,), (x,))
+        with pytest.raises((VSKError, RuntimeError)):
+            torch.func.vjp(f, x)
+
+
 def test_page_keeping_beyond_its_counts(ctx):
     """More pages or slots than the kernels count are refused, not launched."""
     import ctypes

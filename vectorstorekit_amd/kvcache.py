@@ -12,7 +12,7 @@ answers over retrieved vectors calls next to the search.
 Tensors are torch tensors on the context's GPU.  Unlike the search calls,
 these are queued on torch's current stream and do not wait: a decoder makes
 dozens a token.  They record no gradients (a tensor that wants one is refused
-outside ``torch.no_grad()``).  They allocate through torch, so a captured graph may hold
+outside ``torch.no_grad()``, one with a forward-mode tangent always).  They allocate through torch, so a captured graph may hold
 them.  The reference keeps its language-model layer on the application's side
 (LLM/, Core/ML/Shaders/OptimizedMLShaders.metal:523); there is no CPU
 fallback.
@@ -25,6 +25,7 @@ import struct
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import VSKError
@@ -64,6 +65,8 @@ def _tensor(gpu, x, name, dtype=None, dims=None):
         # (a result without its history would train on silently)
         raise VSKError(-8, f"{name} requires a gradient, which these calls do not record: detach "
                        "it or call under torch.no_grad()")
+    if forward_ad._current_level >= 0 and forward_ad.unpack_dual(x).tangent is not None:
+        raise VSKError(-8, f"{name} carries a tangent, which these calls do not pass on")
     if dtype is not None and x.dtype != dtype:
         raise VSKError(-2, f"{name} is {x.dtype}, not {dtype}")
     if dims is not None and x.dim() != dims:
