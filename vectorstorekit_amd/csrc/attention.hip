@@ -179,7 +179,7 @@ int64_t vsk_attention_workspace(vsk_ctx *ctx, const vsk_kv *kv, const vsk_new_to
 
 vsk_status vsk_attention(vsk_ctx *ctx, void *stream, const vsk_kv *kv, int32_t layer,
                          const vsk_new_tokens *news, const vsk_attention_args *args) {
-  VSK_API_BEGIN(ctx);
+  QUEUED_API_BEGIN(ctx);
   check_shapes(kv, news, args);
   VSK_REQUIRE(std::isfinite(args->scale) && args->scale > 0, VSK_ERR_INVALID_ARGUMENT,
               "scale must be positive and finite");

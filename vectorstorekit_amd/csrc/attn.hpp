@@ -9,7 +9,15 @@
 // once for all of them.
 #pragma once
 
+#include "device_scope.hpp"
 #include "vsk_core.hpp"
+
+// VSK_API_BEGIN (vsk_api.hpp) of a call that a program makes between its own:
+// the current device is what it was when the call returns.
+#define QUEUED_API_BEGIN(ctx)                              \
+  if (!(ctx)) return VSK_ERR_INVALID_ARGUMENT;             \
+  const ::vsk::DeviceScope vsk_device_scope_((ctx)->device); \
+  VSK_API_BEGIN(ctx)
 
 namespace vsk {
 

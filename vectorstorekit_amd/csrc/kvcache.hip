@@ -502,7 +502,7 @@ int64_t vsk_kv_scratch_ints(int32_t pages, int32_t slots) {
 
 vsk_status vsk_kv_reserve(vsk_ctx *ctx, void *stream, const vsk_kv *kv, const int32_t *seqs,
                           const int32_t *counts, int32_t n) {
-  VSK_API_BEGIN(ctx);
+  QUEUED_API_BEGIN(ctx);
   VSK_REQUIRE(kv, VSK_ERR_INVALID_ARGUMENT, "null argument");
   const Pool p = pool_of(kv);
   check_list(seqs, n);
@@ -521,7 +521,7 @@ vsk_status vsk_kv_reserve(vsk_ctx *ctx, void *stream, const vsk_kv *kv, const in
 
 vsk_status vsk_kv_fork(vsk_ctx *ctx, void *stream, const vsk_kv *kv, const int32_t *parents,
                        const int32_t *children, int32_t n) {
-  VSK_API_BEGIN(ctx);
+  QUEUED_API_BEGIN(ctx);
   VSK_REQUIRE(kv, VSK_ERR_INVALID_ARGUMENT, "null argument");
   const Pool p = pool_of(kv);
   check_list(parents, n);
@@ -550,7 +550,7 @@ vsk_status vsk_kv_fork(vsk_ctx *ctx, void *stream, const vsk_kv *kv, const int32
 
 vsk_status vsk_kv_free(vsk_ctx *ctx, void *stream, const vsk_kv *kv, const int32_t *seqs,
                        int32_t n) {
-  VSK_API_BEGIN(ctx);
+  QUEUED_API_BEGIN(ctx);
   VSK_REQUIRE(kv, VSK_ERR_INVALID_ARGUMENT, "null argument");
   const Pool p = pool_of(kv);
   check_list(seqs, n);
@@ -567,7 +567,7 @@ vsk_status vsk_kv_free(vsk_ctx *ctx, void *stream, const vsk_kv *kv, const int32
 }
 
 vsk_status vsk_kv_compact(vsk_ctx *ctx, void *stream, const vsk_kv *kv) {
-  VSK_API_BEGIN(ctx);
+  QUEUED_API_BEGIN(ctx);
   VSK_REQUIRE(kv, VSK_ERR_INVALID_ARGUMENT, "null argument");
   const Pool p = pool_of(kv);
   hipStream_t st = static_cast<hipStream_t>(stream);
@@ -587,7 +587,7 @@ vsk_status vsk_kv_compact(vsk_ctx *ctx, void *stream, const vsk_kv *kv) {
 
 vsk_status vsk_kv_copy(vsk_ctx *ctx, void *stream, const vsk_kv *kv, const int32_t *src,
                        const int32_t *dst, int32_t n) {
-  VSK_API_BEGIN(ctx);
+  QUEUED_API_BEGIN(ctx);
   VSK_REQUIRE(kv, VSK_ERR_INVALID_ARGUMENT, "null argument");
   const Pool p = pool_of(kv);
   check_list(src, n);

@@ -291,7 +291,7 @@ extern "C" {
 
 vsk_status vsk_rotary_create(vsk_ctx *ctx, const double *inv_freq, int32_t pairs, int32_t layout,
                              double amplitude, vsk_rotary **out) {
-  VSK_API_BEGIN(ctx);
+  QUEUED_API_BEGIN(ctx);
   VSK_REQUIRE(out, VSK_ERR_INVALID_ARGUMENT, "out is null");
   *out = nullptr;
   VSK_REQUIRE(inv_freq, VSK_ERR_INVALID_ARGUMENT, "inv_freq is null");
@@ -324,7 +324,9 @@ vsk_status vsk_rotary_create(vsk_ctx *ctx, const double *inv_freq, int32_t pairs
 
 vsk_status vsk_rotary_free(vsk_ctx *ctx, vsk_rotary *rotary) {
   if (!rotary) return VSK_OK;
-  if (ctx) (void)hipSetDevice(ctx->device);
+  int device = 0;
+  (void)hipGetDevice(&device);
+  const DeviceScope scope(ctx ? ctx->device : device);
   // (the release waits for the device: work queued on any stream may read it)
   (void)hipDeviceSynchronize();
   delete rotary;
@@ -334,7 +336,7 @@ vsk_status vsk_rotary_free(vsk_ctx *ctx, vsk_rotary *rotary) {
 vsk_status vsk_rotary_apply(vsk_ctx *ctx, void *stream, const vsk_rotary *rotary, int32_t dtype,
                             int32_t d, int64_t tokens, const int32_t *positions, int32_t inverse,
                             const vsk_head_rows *tensors, int32_t n_tensors) {
-  VSK_API_BEGIN(ctx);
+  QUEUED_API_BEGIN(ctx);
   VSK_REQUIRE(rotary && tensors, VSK_ERR_INVALID_ARGUMENT, "null argument");
   VSK_REQUIRE(dtype >= VSK_DTYPE_F32 && dtype <= VSK_DTYPE_BF16, VSK_ERR_UNSUPPORTED,
               "unknown data type");
@@ -371,7 +373,7 @@ vsk_status vsk_kv_append(vsk_ctx *ctx, void *stream, const vsk_kv *kv, int32_t l
                          const vsk_new_tokens *news, const vsk_head_rows *k,
                          const vsk_head_rows *v, const vsk_rotary *rotary,
                          const vsk_head_rows *q) {
-  VSK_API_BEGIN(ctx);
+  QUEUED_API_BEGIN(ctx);
   VSK_REQUIRE(kv && news && k && v, VSK_ERR_INVALID_ARGUMENT, "null argument");
   check_kv(kv);
   check_news(news);
