@@ -1011,6 +1011,19 @@ def test_tangents_are_refused(ctx):
             torch.func.vjp(f, x)
 
 
+def test_layers_past_32_bits(ctx):
+    from vectorstorekit_amd import VSKError
+
+    cache, _ = filled(ctx, [20, 4], 16, 2, 64, F32, poison=False)
+    k, x = cache.k.clone(), torch.ones(2, 2, 64, device=DEV)
+    for layer in (1, -1, 1 << 32, -(1 << 32)):  # (not layer 0)
+        for f in (lambda: cache.append(x, x, layer=layer), lambda: cache.attend(x, layer=layer)):
+            with pytest.raises(VSKError) as e:
+                f()
+            assert e.value.kind == "invalidArgument"
+    assert torch.equal(cache.k, k)
+
+
 def test_page_keeping_beyond_its_counts(ctx):
     """More pages or slots than the kernels count are refused, not launched."""
     import ctypes

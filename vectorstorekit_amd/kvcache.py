@@ -352,6 +352,10 @@ class PagedKVCache:
         self._ref = ctypes.byref(kv)
 
     # -- new tokens -----------------------------------------------------------
+    def _layer(self, layer):
+        if not 0 <= layer < self.layers:  # (the call would take its low 32 bits)
+            raise VSKError(-2, f"no layer {layer}: the cache has {self.layers}")
+
     def _news(self, x, starts, seqs, max_new):
         """vsk_new_tokens of the rows of x and what must outlive the call."""
         tokens = x.shape[0]
@@ -387,6 +391,7 @@ class PagedKVCache:
         i), has the rows ``starts[i] .. starts[i + 1]`` (default: row i), at
         most ``max_new``; they are the last of its length.  ``rotary`` turns
         the keys by their positions, and ``q``, returned turned, with them."""
+        self._layer(layer)
         k, v = self._heads(k, "k", self.kv_heads), self._heads(v, "v", self.kv_heads)
         if v.shape[0] != k.shape[0]:
             raise VSKError(-4, f"{k.shape[0]} keys, {v.shape[0]} values")
@@ -420,6 +425,7 @@ class PagedKVCache:
         bounds the lengths, to divide the work by (default: the table's
         width).  Returns the outputs, with ``return_lse`` also the logarithm
         of each row's sum (-inf, and zeros, where a row sees nothing)."""
+        self._layer(layer)
         q = self._heads(q, "q")
         if q.shape[1] % self.kv_heads or not q.shape[1]:
             raise VSKError(-4, f"{q.shape[1]} query heads over {self.kv_heads} key heads")
