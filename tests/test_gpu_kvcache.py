@@ -1011,6 +1011,27 @@ def test_tangents_are_refused(ctx):
             torch.func.vjp(f, x)
 
 
+def test_expanded_tensors_are_not_turned_in_place(ctx):
+    """Tokens (or heads) at one place would be turned once each, one after
+    another, or not; out of place they are read only."""
+    from vectorstorekit_amd import RotaryEmbedding, VSKError
+
+    rope, pos = RotaryEmbedding(ctx, 64), ints(range(1, 8))
+    one, head = normal(gen(1), 1, 2, 64), normal(gen(2), 7, 1, 64)
+    x = normal(gen(3), 7, 2, 64)
+    for y in (one.expand(7, 2, 64), head.expand(7, 2, 64)):
+        before = y.clone()
+        for q, k in ((y, None), (y, x.clone()), (x.clone(), y)):
+            with pytest.raises(VSKError) as e:
+                rope.apply(q, k, positions=pos, inplace=True)
+            assert e.value.kind == "invalidArgument"
+        assert torch.equal(y, before)
+        assert torch.equal(rope.apply(y, positions=pos), rope.apply(before, positions=pos))
+    z = one.clone().expand(1, 2, 64)
+    assert torch.equal(rope.apply(z, positions=pos[:1], inplace=True),
+                       rope.apply(one, positions=pos[:1]))
+
+
 def test_layers_past_32_bits(ctx):
     from vectorstorekit_amd import VSKError
 

@@ -74,6 +74,12 @@ def _tensor(gpu, x, name, dtype=None, dims=None):
     return x
 
 
+def _shared(x):
+    """Do tokens or heads of x lie at one place (an expanded tensor)?"""
+    (n, h), (a, b) = x.shape[:2], x.stride()[:2]
+    return n > 1 and a == 0 or h > 1 and b == 0
+
+
 def _dense_heads(x):
     """x itself, or a copy whose innermost dimension is dense."""
     return x if x.stride(-1) == 1 or x.shape[-1] == 1 else x.contiguous()
@@ -205,6 +211,9 @@ class RotaryEmbedding:
         if inplace:
             if q.stride(-1) != 1 or k is not None and k.stride(-1) != 1:
                 raise VSKError(-2, "inplace needs dense heads")
+            if _shared(q) or k is not None and _shared(k):
+                # (threads would turn what others have turned already)
+                raise VSKError(-2, "inplace needs tokens and heads with memory of their own")
             to_q, to_k = q, k
         else:
             q = _dense_heads(q)
