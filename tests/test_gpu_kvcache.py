@@ -1032,6 +1032,30 @@ def test_expanded_tensors_are_not_turned_in_place(ctx):
                        rope.apply(one, positions=pos[:1]))
 
 
+def test_slots_known_on_the_host(ctx):
+    """A slot twice would lose the pages taken for it first, one that is not
+    there would grow nothing: refused where the host knows, like a fork's."""
+    from vectorstorekit_amd import VSKError
+
+    cache, _ = filled(ctx, [20, 4], 16, 2, 64, F32, poison=False)
+    table, refs = cache.table.clone(), cache.refs.clone()
+    for f, *a in ((cache.reserve, [0, 0], [16, 16]), (cache.reserve, np.array([1, 2]), [1, 1]),
+                  (cache.reserve, [-1], [1]), (cache.free, [2]), (cache.free, [-1]),
+                  (cache.fork, [0], [2]), (cache.fork, [0, 0], [1, 1])):
+        with pytest.raises(VSKError) as e:
+            f(*a)
+        assert e.value.kind == "invalidArgument"
+    assert torch.equal(cache.table, table) and torch.equal(cache.refs, refs)
+    assert cache.lengths.tolist() == [20, 4]
+    cache.reserve([], [])
+    cache.free([])
+    cache.reserve((1, 0), np.array([1, 2]))
+    assert cache.lengths.tolist() == [22, 5]
+    cache.fork([0], np.array([1]))
+    cache.free(ints([1, 1, 7]))  # (on the GPU: slots out of range hold nothing)
+    assert cache.lengths.tolist() == [22, 0]
+
+
 def test_layers_past_32_bits(ctx):
     from vectorstorekit_amd import VSKError
 

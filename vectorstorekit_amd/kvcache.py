@@ -447,10 +447,23 @@ class PagedKVCache:
         if self.refs is None:
             raise VSKError(-8, "a cache without refs keeps no pages")
 
+    def _known(self, x, name, distinct=False):
+        """Checks slots that are known on the host (those on the GPU are the
+        caller's to keep in range and distinct)."""
+        if isinstance(x, torch.Tensor):
+            return
+        a = np.asarray(x)
+        if a.size and (a.min() < 0 or a.max() >= self.slots):
+            raise VSKError(-2, f"{name} outside the {self.slots} slots")
+        if distinct and np.unique(a).size != a.size:
+            raise VSKError(-2, f"{name} must be distinct")
+
     def reserve(self, seqs, counts):
-        """Grows the sequences in these slots by these numbers of tokens,
-        taking the lowest free pages; ``missing()`` tells of a shortage."""
+        """Grows the sequences in these slots (distinct) by these numbers of
+        tokens, taking the lowest free pages; ``missing()`` tells of a
+        shortage."""
         self._keeping()
+        self._known(seqs, "seqs", distinct=True)
         s, c = _ints(self.gpu, seqs, "seqs"), _ints(self.gpu, counts, "counts")
         if s.shape != c.shape:
             raise VSKError(-4, f"{s.shape[0]} slots, {c.shape[0]} counts")
@@ -463,15 +476,11 @@ class PagedKVCache:
         ``parents``: whole pages are shared, a last page that is not full is
         copied.  What the children held is released."""
         self._keeping()
-        for x, name in ((parents, "parents"), (children, "children")):
-            if not isinstance(x, torch.Tensor):
-                a = np.asarray(x)
-                if a.size and (a.min() < 0 or a.max() >= self.slots):
-                    raise VSKError(-2, f"{name} outside the {self.slots} slots")
+        self._known(parents, "parents")
+        self._known(children, "children", distinct=True)
         if not isinstance(parents, torch.Tensor) and not isinstance(children, torch.Tensor):
-            c = list(children)
-            if len(set(c)) != len(c) or set(c) & set(parents):
-                raise VSKError(-2, "children must be distinct and none of them a parent")
+            if set(children) & set(parents):
+                raise VSKError(-2, "a child must not be a parent")
         p, c = _ints(self.gpu, parents, "parents"), _ints(self.gpu, children, "children")
         if p.shape != c.shape:
             raise VSKError(-4, f"{p.shape[0]} parents, {c.shape[0]} children")
@@ -481,6 +490,7 @@ class PagedKVCache:
     def free(self, seqs):
         """Releases the pages of the sequences in these slots."""
         self._keeping()
+        self._known(seqs, "seqs")
         s = _ints(self.gpu, seqs, "seqs")
         self.ctx.check(self.ctx.lib.vsk_kv_free(self.ctx.handle, _stream(self.gpu), self._ref,
                                                 s.data_ptr(), s.shape[0]))
