@@ -1032,6 +1032,55 @@ def test_expanded_tensors_are_not_turned_in_place(ctx):
                        rope.apply(one, positions=pos[:1]))
 
 
+def off_by_one(x):
+    """x's values one element past an aligned place."""
+    flat = torch.empty(x.numel() + 1, dtype=x.dtype, device=x.device)
+    y = flat[1:].view(x.shape)
+    return y.copy_(x)
+
+
+@pytest.mark.parametrize("dtype", [BF, F16, F32])
+@pytest.mark.parametrize("d,shift", [(68, 0), (100, 0), (101, 0), (77, 0), (128, 1), (64, 1),
+                                     (256, 1), (250, 0)])
+@pytest.mark.parametrize("news,lengths,heads,kv,window,sinks", [
+    ([1, 1, 1], [700, 1, 0], 8, 2, None, 0),
+    ([1], [5000], 5, 5, 900, 3),
+    ([1] * 40, [60 + i for i in range(40)], 6, 1, 33, 1),
+    ([40, 3, 0, 90], [300, 3, 9, 90], 6, 3, 50, 2),
+    ([200, 150], [200, 150], 4, 4, None, 0),
+    ([100] * 6, [100] * 6, 32, 8, 70, 5),  # a wave a row tile
+])
+def test_operands_without_wide_loads(ctx, dtype, d, shift, news, lengths, heads, kv, window, sinks):
+    """Heads that are not whole 16-byte pieces, and bases off by an element:
+    tokens, prompts and dense keys."""
+    from vectorstorekit_amd import PagedKVCache, window_attention
+
+    cache, seqs = filled(ctx, lengths, 16, kv, d, dtype, seed=d + shift)
+    if shift:
+        cache = PagedKVCache.over(ctx, off_by_one(cache.k), off_by_one(cache.v), cache.table,
+                                  cache.lengths)
+    starts = [0] + list(np.cumsum(news))
+    q = normal(gen(d), starts[-1], heads, d, dtype=dtype)
+    given = {"window": window, "sinks": sinks, "return_lse": True}
+    if max(news) > 1:
+        given.update(starts=starts, max_new=max(news))
+    results = [cache.attend(q, **given)]
+    if shift:
+        results.append(cache.attend(off_by_one(q), **given))
+    if news == lengths:
+        k, v = (torch.cat([x[i][0] for x in seqs]).to(DEV) for i in (0, 1))
+        results.append(window_attention(ctx, q, *((off_by_one(x) if shift else x) for x in (k, v)),
+                                        starts=starts, max_length=max(news), window=window,
+                                        sinks=sinks, return_lse=True))
+    for i, (kk, vv) in enumerate(seqs):
+        a, b = starts[i], starts[i + 1]
+        o, l, t = attended_at_once(q[a:b], kk[0], vv[0], d ** -0.5, window, sinks)
+        for out, lse in results:
+            check(out[a:b], o, t)
+            check_norm(out[a:b], o, dtype)
+            check(lse[a:b], l, 2.0 ** -16 * (1 + l.abs()))
+
+
 def test_slots_known_on_the_host(ctx):
     """A slot twice would lose the pages taken for it first, one that is not
     there would grow nothing: refused where the host knows, like a fork's."""
