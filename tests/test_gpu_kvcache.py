@@ -191,6 +191,24 @@ def test_rotary_strides_and_gradient(ctx):
     assert abs(slope - float((e.double() * grad.double()).sum())) <= 2.0 ** -20 * size
 
 
+@pytest.mark.parametrize("scaling", [None, {"type": "yarn", "factor": 8.0,
+                                            "original_length": 512}])
+def test_moved_keys(ctx, scaling):
+    """A turned key moved to another position, by the inverse, is that key
+    turned there, times the factor.  Three rotations, each off by 2^-24 of the
+    value and 2^-21 of the pair's size."""
+    from vectorstorekit_amd import RotaryEmbedding
+
+    rope = RotaryEmbedding(ctx, 64, scaling=scaling)
+    a = rope.amplitude
+    assert (a == 1.0) == (scaling is None)
+    x, p, to = normal(gen(4), 30, 2, 64), ints(range(1000, 1030)), ints(range(30))
+    moved = rope.apply(rope.apply(x, positions=p), positions=p - to, inverse=True)
+    want = rope.apply(x, positions=to).cpu().double() * a
+    size = x.cpu().double().abs().amax(-1, keepdim=True) * a * a
+    check(moved, want, 3 * (2.0 ** -24 * want.abs() + 2.0 ** -20 * size))
+
+
 # ---------------------------------------------------------------------- the cache
 
 def filled(ctx, lengths, page, kv, d, dtype, *, layers=1, order="nhd", seed=0, width=None,

@@ -196,9 +196,10 @@ class RotaryEmbedding:
     def apply(self, q, k=None, *, positions, inverse: bool = False, inplace: bool = False):
         """q (and k), tokens x heads x head_dim, turned by positions (int32,
         one a token): new tensors, or the given ones with ``inplace``.
-        ``inverse`` turns back (with the same factor): the gradient of
-        ``apply``, and, with positions p - p', a cached key's move from p to
-        p'."""
+        ``inverse`` turns back, with the same factor on the rotated values:
+        the gradient of ``apply``.  With positions p - p' it moves a cached
+        key from p to p', times that factor (``amplitude``): divide by it where
+        it is not 1 (yarn)."""
         ctx, gpu = self.ctx, self.ctx.device
         tokens, dtype = self._checked(_tensor(gpu, q, "q", None, 3), "q", None), q.dtype
         if k is not None:
