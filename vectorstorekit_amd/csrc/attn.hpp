@@ -148,9 +148,10 @@ __device__ inline int32_t attn_row16(const AttnSeq &s, int32_t j16) {
   const int32_t tail = (s.L - 1) & ~15;
   return j16 < tail ? j16 : tail;
 }
-// the page that holds them, as the table has it (dense: 0).  The index is
-// hidden from the compiler, which would turn the value into a scalar, and wait
-// for it, at once: it is asked for a step before it is used.
+// The page that holds them, as the table has it (dense: 0): for the paths that
+// take keys one at a time.  The index is hidden from the compiler: a scalar load
+// of it would keep scalars that the loops around have no registers for (one
+// context of 777: 11.3 us, 11.1 with it).
 __device__ inline int32_t attn_page(const AttnArgs &a, const AttnSeq &s, int32_t j16) {
   if (!a.table) return 0;
   int32_t i = attn_row16(s, j16) >> a.page_shift;

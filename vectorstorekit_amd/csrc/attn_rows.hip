@@ -76,16 +76,10 @@ __device__ inline int32_t hidden(int32_t x) {
   return x;
 }
 
-// W words (16 or 8 bytes) of a row from element e on, zero from element d on
-template <class T, int W, bool ALIGNED>
+// W words of a row of any alignment from element e on, zero from element d on
+template <class T, int W>
 __device__ inline void load_row(const global_as T *row, int32_t e, int32_t d, uint32_t (&x)[W]) {
-  if constexpr (ALIGNED) {
-    typedef __attribute__((ext_vector_type(W))) uint32_t VW;
-    VW v = {};
-    if (e < d) v = *reinterpret_cast<const global_as VW *>(row + e);
-#pragma unroll
-    for (int i = 0; i < W; ++i) x[i] = v[i];
-  } else if constexpr (sizeof(T) == 4) {
+  if constexpr (sizeof(T) == 4) {
 #pragma unroll
     for (int i = 0; i < W; ++i) x[i] = e + i < d ? __builtin_bit_cast(uint32_t, row[e + i]) : 0u;
   } else {
@@ -144,7 +138,7 @@ template <class T, int VW, int NB, bool ALIGNED> struct RowTile {
 #pragma unroll
         for (int z = 0; z < 4; ++z) q[i][z] = y[z];
       } else {
-        load_row<T, 4, false>((const global_as T *)src, e, real ? a.d : 0, q[i]);
+        load_row<T, 4>((const global_as T *)src, e, real ? a.d : 0, q[i]);
       }
     }
     if constexpr (ALIGNED) {
@@ -251,7 +245,7 @@ template <class T, int VW, int NB, bool ALIGNED> struct RowTile {
         const uint32_t at = (uint32_t)n * stride, row = at < most ? at : most;
 #pragma unroll
         for (int i = 0; i < KS; ++i)
-          load_row<T, 4, false>((const global_as T *)(base + row), (4 * i + g) * KE, a.d, k[u][i]);
+          load_row<T, 4>((const global_as T *)(base + row), (4 * i + g) * KE, a.d, k[u][i]);
       }
     }
   }
@@ -274,8 +268,7 @@ template <class T, int VW, int NB, bool ALIGNED> struct RowTile {
 #pragma unroll
             for (int z = 0; z < WV; ++z) v[u][i][b][z] = y[z];
           } else {
-            load_row<T, WV, false>(reinterpret_cast<const global_as T *>(base + row), e, a.d,
-                                   v[u][i][b]);
+            load_row<T, WV>(reinterpret_cast<const global_as T *>(base + row), e, a.d, v[u][i][b]);
           }
         }
       }
