@@ -620,8 +620,9 @@ vsk_status vsk_rotary_apply(vsk_ctx *ctx, void *stream, const vsk_rotary *rotary
  * counts the sequences that hold a page (0: free).  page_size is a power of
  * two of at least 16.  refs, status and scratch serve the page calls only.
  * status (4 ints): [0] pages that were missing in the last vsk_kv_reserve or
- * vsk_kv_fork, [1] pages in use and [2] pages moved by the last
- * vsk_kv_compact.  scratch: vsk_kv_scratch_ints() ints. */
+ * vsk_kv_fork (2^31 - 1: that many or more), [1] pages in use and [2] pages moved by the last
+ * vsk_kv_compact.  scratch: vsk_kv_scratch_ints() ints.  The page calls take
+ * at most 2^30 pages and slots. */
 typedef struct {
   void *k, *v;
   int64_t k_layer, k_page, k_row, k_head;
@@ -658,7 +659,8 @@ vsk_status vsk_kv_copy(vsk_ctx *ctx, void *stream, const vsk_kv *kv, const int32
 /* The new tokens of n sequences: sequence i (slot seqs[i], or i without
  * seqs) has rows starts[i] .. starts[i + 1] of q, k and v (starts NULL: row i
  * alone), which are the last tokens of its length.  max_new bounds the new
- * tokens of a sequence: rows past it are not treated. */
+ * tokens of a sequence.  Rows past it, and rows of no sequence, are not
+ * treated: nothing is written for them. */
 typedef struct {
   const int32_t *starts, *seqs;
   int32_t n, max_new;
@@ -677,7 +679,12 @@ vsk_status vsk_kv_append(vsk_ctx *ctx, void *stream, const vsk_kv *kv, int32_t l
  * multiple of kv_heads, consecutive heads share a key head.  lse (may be
  * NULL): tokens x heads, log of the sum.  max_length: the longest length, for
  * the division of the work only (0: what the table holds).  Masked places of
- * the cache may hold anything, infinities and NaN included.
+ * the cache may hold anything, infinities and NaN included; an infinite value
+ * that a token sees is its output's, as long as its weight is not 0 in 32 bits
+ * (under 2^-126 of the largest: NaN).
+ * Scores, sums and outputs are computed in 32 bits; in 16 bits a weight enters
+ * its product with a value as two 16-bit parts (few rows) or rounded once to
+ * the values' type (many).
  * kv for dense keys and values: table NULL, page_size 0, `pages` rows of k
  * and v (k_row, k_head, v_row, v_head apart) and k_starts[n + 1] their
  * sequences' offsets; else k_starts is unused.

@@ -838,6 +838,31 @@ def test_offsets_out_of_order(ctx):
         assert torch.equal(cache.k, k) and torch.equal(cache.v, v)
 
 
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("heads,kv,d,news,most", [(4, 2, 64, [9, 3, 1], 4), (32, 8, 128, [200, 70], 96),
+                                                  (6, 6, 100, [40, 2], 1)])
+def test_bound_under_the_new_tokens(ctx, dtype, heads, kv, d, news, most):
+    """A sequence's first max_new rows are treated, each at its own place."""
+    lengths = [x + 50 for x in news]
+    cache, seqs = filled(ctx, lengths, 16, kv, d, dtype, seed=d)
+    starts = [0] + list(np.cumsum(news))
+    q = normal(gen(3), starts[-1], heads, d, dtype=dtype)
+    out, lse = cache.attend(q, starts=starts, max_new=most, window=60, sinks=2, return_lse=True)
+    k = cache.k.clone()
+    x = normal(gen(4), starts[-1], kv, d, dtype=dtype)
+    cache.append(x, x, starts=starts, max_new=most)
+    for i, (kk, vv) in enumerate(seqs):
+        a, n = starts[i], min(news[i], most)
+        o, l, t = attended_at_once(q[a:starts[i + 1]], kk[0], vv[0], d ** -0.5, 60, 2)
+        check(out[a:a + n], o[:n], t[:n])
+        check(lse[a:a + n], l[:n], 2.0 ** -16 * (1 + l[:n].abs()))
+        for p in range(lengths[i]):
+            page, row = int(cache.table[i, p // 16]), p % 16
+            new = p - 50
+            want = x[a + new] if 0 <= new < n else k[0, page, row]
+            assert torch.equal(cache.k[0, page, row], want)
+
+
 @pytest.mark.parametrize("d,lengths", [(64, [20]), (128, [9000]), (256, [70, 30])])
 def test_no_rows_to_treat(ctx, d, lengths):
     """Bounds of no new token at all: nothing is done, however long the keys."""

@@ -11,7 +11,9 @@ answers over retrieved vectors calls next to the search.
 
 Tensors are torch tensors on the context's GPU.  Unlike the search calls,
 these are queued on torch's current stream and do not wait: a decoder makes
-dozens a token.  They record no gradients (a tensor that wants one is refused
+dozens a token.  (Offsets, slots and counts given as host sequences are copied
+to the GPU first, which does wait and cannot be captured; int32 tensors there
+are used as they are.)  They record no gradients (a tensor that wants one is refused
 outside ``torch.no_grad()``, one with a forward-mode tangent always).  They allocate through torch, so a captured graph may hold
 them.  The reference keeps its language-model layer on the application's side
 (LLM/, Core/ML/Shaders/OptimizedMLShaders.metal:523); there is no CPU
@@ -398,9 +400,13 @@ class PagedKVCache:
                rotary: RotaryEmbedding | None = None, q=None):
         """Writes the new tokens' keys and values (tokens x kv_heads x
         head_dim) to their places.  Sequence i, in slot ``seqs[i]`` (default:
-        i), has the rows ``starts[i] .. starts[i + 1]`` (default: row i), at
-        most ``max_new``; they are the last of its length.  ``rotary`` turns
-        the keys by their positions, and ``q``, returned turned, with them."""
+        i), has the rows ``starts[i] .. starts[i + 1]`` (default: row i); they
+        are the last of its length.  No sequence has more than ``max_new``
+        (default: all the rows; the nearer the bound, the fewer blocks start
+        for nothing).  ``rotary`` turns the keys by their positions, and ``q``,
+        returned turned, with them.  Rows of no sequence, and a sequence's
+        past ``max_new``, are not treated: what is returned for them is
+        undefined."""
         self._layer(layer)
         k, v = self._heads(k, "k", self.kv_heads), self._heads(v, "v", self.kv_heads)
         if v.shape[0] != k.shape[0]:
@@ -434,7 +440,13 @@ class PagedKVCache:
         first ``sinks``.  ``scale`` defaults to head_dim^-0.5; ``max_length``
         bounds the lengths, to divide the work by (default: the table's
         width).  Returns the outputs, with ``return_lse`` also the logarithm
-        of each row's sum (-inf, and zeros, where a row sees nothing)."""
+        of each row's sum (-inf, and zeros, where a row sees nothing; undefined
+        for rows that are not treated).
+
+        Scores, sums and outputs are computed in 32 bits.  In 16 bits a weight
+        is rounded before it multiplies a value: for few rows to two 16-bit
+        parts, for many (prompts) once to the values' type, which is off by as
+        much as the output's own rounding."""
         self._layer(layer)
         q = self._heads(q, "q")
         if q.shape[1] % self.kv_heads or not q.shape[1]:
@@ -475,7 +487,8 @@ class PagedKVCache:
     def fork(self, parents, children):
         """The sequences in slots ``children`` become branches of those in
         ``parents``: whole pages are shared, a last page that is not full is
-        copied.  What the children held is released."""
+        copied; ``missing()`` tells of children that found none for it, which
+        keep the whole pages only.  What the children held is released."""
         self._keeping()
         self._known(parents, "parents")
         self._known(children, "children", distinct=True)
@@ -505,7 +518,8 @@ class PagedKVCache:
         return self.status[1]
 
     def copy_pages(self, src, dst):
-        """Copies pages ``src`` to pages ``dst`` in every layer."""
+        """Copies pages ``src`` to pages ``dst`` in every layer.  No page may be
+        written twice, or be both read and written."""
         self._keeping()
         s, d = _ints(self.gpu, src, "src"), _ints(self.gpu, dst, "dst")
         if s.shape != d.shape:
@@ -528,7 +542,8 @@ def window_attention(ctx: Context, q, k, v, *, starts, k_starts=None, max_length
     starts[i + 1]``; k and v are rows x kv_heads x head_dim with the offsets
     ``k_starts`` (default: ``starts``), the queries standing at the keys' end.
     ``max_length`` bounds the sequences' queries (default: all rows); window,
-    sinks, scale and return_lse as in ``PagedKVCache.attend``."""
+    sinks, scale, return_lse, the rounding of weights and the rows that are not
+    treated as in ``PagedKVCache.attend``."""
     gpu = ctx.device
     dtype = _tensor(gpu, q, "q", None, 3).dtype
     _tensor(gpu, k, "k", dtype, 3), _tensor(gpu, v, "v", dtype, 3)
