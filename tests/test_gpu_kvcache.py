@@ -1000,6 +1000,64 @@ def test_infinite_values(ctx, dtype, heads, kv, d, new, n):
         check(out.masked_fill(odd, 0.0), want.masked_fill(odd, 0.0), t.masked_fill(odd, 0.0))
 
 
+@pytest.mark.parametrize("dtype", [BF, F16, F32])
+@pytest.mark.parametrize("heads,kv,d,news,lengths", [
+    (8, 2, 128, [1, 1], [300, 41]), (8, 8, 64, [1], [20000]), (6, 3, 100, [1, 1], [90, 500]),
+    (4, 2, 64, [20, 3], [130, 33]), (64, 16, 128, [140, 70], [300, 80]),
+    (32, 8, 256, [90], [200]), (8, 8, 64, [64], [20000]),
+])
+def test_key_by_key_over_pages(ctx, dtype, heads, kv, d, news, lengths):
+    """Scores that differ by one rounding and infinite values in a paged cache
+    whose other places hold NaN: as over dense keys."""
+    from vectorstorekit_amd import window_attention
+
+    cache, seqs = filled(ctx, lengths, 32, kv, d, dtype, seed=heads + d)
+    g = gen(d)
+    starts = [0] + list(np.cumsum(news))
+    kstarts = [0] + list(np.cumsum(lengths))
+    k, v = (torch.cat([x[i][0] for x in seqs]) for i in (0, 1))
+    # a few of each sequence's keys have the largest score, and one value is
+    # infinite
+    k[:], best = 0.0, torch.rand(k.shape[:2], generator=g) < 0.2
+    k[..., 0] = torch.where(best, -1168.0, -1200.0).to(dtype)
+    for a in kstarts[:-1]:
+        k[a, :, 0] = -1168.0
+    odd = [a + 7 for a in kstarts[:-1]]
+    k[odd, :, 0] = -1168.0
+    peak = float(v.abs().max())
+    v[odd, 0, d // 2] = math.inf
+    q = torch.zeros(starts[-1], heads, d, dtype=dtype, device=DEV)
+    q[:, :, 0] = 14592.0
+    table = cache.table.cpu()
+    for i, n in enumerate(lengths):
+        for p in range(0, n, 32):
+            page, m, at = int(table[i, p // 32]), min(32, n - p), kstarts[i] + p
+            cache.k[0, page, :m], cache.v[0, page, :m] = k[at:at + m].to(DEV), v[at:at + m].to(DEV)
+    for scale in (3.7, 1e6):
+        given = {"scale": scale, "window": 10 ** 6, "sinks": 0, "return_lse": True}
+        out, lse = cache.attend(q, starts=starts, max_new=max(news), **given)
+        same, also = window_attention(ctx, q, k.to(DEV), v.to(DEV), starts=starts, k_starts=kstarts,
+                                      **given)
+        for i, n in enumerate(lengths):
+            for t in {0, news[i] // 2, news[i] - 1}:
+                r, m = starts[i] + t, n - news[i] + t + 1
+                s = q[r, :, :1].cpu().double() * k[kstarts[i]:kstarts[i] + m].repeat_interleave(
+                    heads // kv, 1)[..., 0].double().T * float(np.float32(scale))
+                w = torch.softmax(s, 1)
+                vv = v[kstarts[i]:kstarts[i] + m].double().repeat_interleave(heads // kv, 1)
+                want = torch.where(w.T[..., None] > 0, w.T[..., None] * vv, 0.0).sum(0)
+                u = U[dtype]
+                tol = u * want.abs() + peak * (2 * (2.0 ** -21 + 2.0 ** -24 * (n + 16))
+                                               + (u if dtype != F32 else 0))
+                inf = torch.isinf(want)
+                for x, y in ((out[r], lse[r]), (same[r], also[r])):
+                    x = x.cpu().double()
+                    assert torch.equal(x[inf], want[inf])
+                    check(x.masked_fill(inf, 0.0), want.masked_fill(inf, 0.0),
+                          tol.masked_fill(inf, 0.0))
+                    check(y, torch.logsumexp(s, 1), 2.0 ** -16 + 2.0 ** -21 * s.abs().amax(1))
+
+
 def test_refusals_of_lost_meaning(ctx):
     """What would otherwise pass and mean something else."""
     from vectorstorekit_amd import RotaryEmbedding, VSKError, window_attention
