@@ -80,7 +80,7 @@ Plan plan_of(const vsk_ctx *ctx, const vsk_kv *kv, const vsk_new_tokens *news,
     // with few keys twice; measured against four waves each (us): 8 f32 prompts
     // of 1,000, 32 heads of 128 on 8, window 100 (16,000 row tiles) 160 / 263;
     // one of 4,000, 8 heads of 64, window 64 (2,000) 18 / 88; 8 f16 prompts of
-    // 500, 10 heads of 100 (2,560) 330 / 204.
+    // 500, 10 heads of 100 (2,560) 357 / 297.
     if (p.tiles >= 4 && (blocks >= 16 * cus || (blocks >= 4 * cus && keys <= 384) ||
                          (blocks >= 2 * cus && keys <= 128))) {
       p.share = 1;

@@ -19,14 +19,17 @@
 // two 16-bit values (its rounding would be as large as the output's).
 //
 // What bounds it: the bytes of K and V.  Measured, bf16 and f16, heads of 128:
-// 64 contexts to 8,192, 32 heads on 8, 195 us, 5.0 TB/s; 3 to 200,003, 64 on 8,
-// 204 us, 5.0 TB/s (a kernel that only reads: 5.8); one of 100,000, 8 on 1,
+// 64 contexts to 8,192, 32 heads on 8, 197 us, 5.0 TB/s; 3 to 200,003, 64 on 8,
+// 202 us, 5.1 TB/s (a kernel that only reads: 5.8); one of 100,000, 8 on 1,
 // 20 us, 2.5 TB/s: what a launch of few blocks and the join take; one of 777,
 // 32 on 8, 11 us: one compute unit a key head, and its L1 passes 64 bytes a
-// cycle, which is 1 us a round of eight waves and 32 keys.  f32, heads
-// of 96 of their own, 17 contexts, window 2,048: 75 us, 5.1 TB/s.  Prompts in
-// 32 bits are bound by the products (16x16x4, 157 TFLOP/s): 2 of 2,048, 32
-// heads of 128 on 8, 388 us, 90 TFLOP/s.
+// cycle, which is 1 us a round of eight waves and 32 keys; a wave waits for
+// memory twice a step (walk).  f32, heads of 96 of their own, 17 contexts,
+// window 2,048: 78 us, 4.9 TB/s.  Prompts in 32 bits are bound by the products
+// (16x16x4, 157 TFLOP/s) and by keys and values that each wave brings for
+// itself: 2 of 2,048, 32 heads of 128 on 8, 731 us, 94 TFLOP/s.  Operands
+// without 16-byte alignment are loaded a value at a time: 32 contexts of 4,000,
+// 10 f16 heads of 100, 595 us where heads of 104 take 125.
 #include "attn.hpp"
 #include "vsk_api.hpp"
 

@@ -22,12 +22,14 @@
 // What bounds it: the products, 4 d operations a visible key and row (half of
 // them each product), and beside them the exponentials, one a score, on the
 // vector unit.  Measured, bf16, 32 heads of 128 on 8: 16,384 tokens, window
-// 4,096, 927 us, 1,041 TFLOP/s of visible work, 1,270 in the loop over whole
-// tiles (a library product of 16,384 cubed: 1,360); 8 ragged prompts to 4,096,
-// window 1,024, 285 us, 775 TFLOP/s: 17.3 tiles a block where 16 hold what is
-// seen, three of them partly masked and outside the pipelined loop, and a
-// block's start and end.  4 prompts of 4,096, 8 heads of 256 on one: 155 us,
-// 488 TFLOP/s (one block a compute unit, queries in LDS).
+// 4,096, 910 to 1,020 us by the card (and its power limit), 945 to 1,060 TFLOP/s
+// of visible work, 1,270 in the loop over whole tiles (a library product of
+// 16,384 cubed: 1,360); 8 ragged prompts to 4,096, window 1,024, 294 to 310 us,
+// 715 to 750 TFLOP/s: 17.3 tiles a block where 16 hold what is seen, three of
+// them partly masked and outside the pipelined loop, and a block's start and
+// end.  4 prompts of 4,096, 8 heads of 256 on one: 363 us, 758 TFLOP/s (one
+// block a compute unit, queries in LDS).  One of 4,000, 8 heads of 64: 60 us,
+// 273 TFLOP/s: 16 products a step beside 138 vector instructions, which bound it.
 #include "attn.hpp"
 #include "vsk_api.hpp"
 
