@@ -182,7 +182,7 @@ typedef lds_as char lds_char;
 // every lane).  Written as assembly because the compiler makes every read of
 // LDS after the builtin wait for it: here a tile's copies fly while the last
 // tile is computed with, and one wait before the barrier covers them.  (M0
-// holds the destination of such loads; nothing else in these kernels uses it.)
+// holds the destination of such loads; the compiler is told.)
 __device__ inline void load_to_lds(uint64_t base, uint32_t off, const lds_char *dst) {
   const uint32_t at = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)dst);
   asm volatile(
@@ -191,7 +191,7 @@ __device__ inline void load_to_lds(uint64_t base, uint32_t off, const lds_char *
       "global_load_lds_dwordx4 %1, %2"
       :
       : "s"(at), "v"(off), "s"(base)
-      : "memory");
+      : "memory", "m0");
 }
 
 __device__ inline uint64_t lane_of(uint32_t lo, uint32_t hi, int i) {
