@@ -169,7 +169,7 @@ int64_t vsk_attention_workspace(vsk_ctx *ctx, const vsk_kv *kv, const vsk_new_to
   if (!ctx) return 0;
   try {
     check_shapes(kv, news, args);
-  } catch (const Error &) {
+  } catch (...) {
     return 0;  // (vsk_attention says why)
   }
   // (no rows: nothing to divide)
