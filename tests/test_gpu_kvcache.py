@@ -839,6 +839,24 @@ def test_offsets_out_of_order(ctx):
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("new,lengths", [(1, [900] * 12), (3, [7000, 20, 0, 300]), (80, [2000, 90])])
+def test_bound_of_dense_keys(ctx, dtype, new, lengths):
+    """It only divides the work, wrong ones included."""
+    from vectorstorekit_amd import window_attention
+
+    g, n = gen(new), len(lengths)
+    ks, starts = [0] + list(np.cumsum(lengths)), list(range(0, n * new + 1, new))
+    q, k, v = (normal(g, m, h, 64, dtype=dtype) for m, h in ((n * new, 8), (ks[-1], 2), (ks[-1], 2)))
+    for bound in (None, max(lengths), 1, 10 ** 6):
+        out = window_attention(ctx, q, k, v, starts=ints(starts), k_starts=ints(ks), max_length=new,
+                               max_keys=bound)
+        for i in range(n):
+            a, b = starts[i], starts[i + 1]
+            o, _, t = attended_at_once(q[a:b], k[ks[i]:ks[i + 1]], v[ks[i]:ks[i + 1]], 0.125, None, 0)
+            check(out[a:b], o, t)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
 @pytest.mark.parametrize("heads,kv,d,news,most", [(4, 2, 64, [9, 3, 1], 4), (32, 8, 128, [200, 70], 96),
                                                   (6, 6, 100, [40, 2], 1)])
 def test_bound_under_the_new_tokens(ctx, dtype, heads, kv, d, news, most):

@@ -535,13 +535,15 @@ class PagedKVCache:
 
 
 def window_attention(ctx: Context, q, k, v, *, starts, k_starts=None, max_length: int | None = None,
-                     scale: float | None = None, window: int | None = None, sinks: int = 0,
-                     return_lse: bool = False):
+                     max_keys: int | None = None, scale: float | None = None,
+                     window: int | None = None, sinks: int = 0, return_lse: bool = False):
     """Causal attention of ragged sequences over dense keys and values: q is
     tokens x heads x head_dim, sequence i its rows ``starts[i] ..
     starts[i + 1]``; k and v are rows x kv_heads x head_dim with the offsets
     ``k_starts`` (default: ``starts``), the queries standing at the keys' end.
-    ``max_length`` bounds the sequences' queries (default: all rows); window,
+    ``max_length`` bounds the sequences' queries (default: all rows),
+    ``max_keys`` their keys, to divide the work by (default: ``max_length``
+    without ``k_starts``, else all rows); window,
     sinks, scale, return_lse, the rounding of weights and the rows that are not
     treated as in ``PagedKVCache.attend``."""
     gpu = ctx.device
@@ -571,5 +573,6 @@ def window_attention(ctx: Context, q, k, v, *, starts, k_starts=None, max_length
                   0, _TYPES[dtype], 1, rows, 0, heads, d, 0, 0)
     most = q.shape[0] if max_length is None else min(int(max_length), q.shape[0])
     news = _NEWS.pack(s.data_ptr(), 0, s.shape[0] - 1, most, q.shape[0])
-    return _attend(ctx, kv, 0, q, news, ks.data_ptr(), scale, window, sinks,
-                   max_length if k_starts is None else None, return_lse)
+    if max_keys is None and k_starts is None:
+        max_keys = max_length
+    return _attend(ctx, kv, 0, q, news, ks.data_ptr(), scale, window, sinks, max_keys, return_lse)
