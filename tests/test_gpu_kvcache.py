@@ -191,6 +191,27 @@ def test_rotary_strides_and_gradient(ctx):
     assert abs(slope - float((e.double() * grad.double()).sum())) <= 2.0 ** -20 * size
 
 
+def test_given_frequencies(ctx):
+    """Frequencies of the caller's own, zeros and fast ones among them."""
+    from vectorstorekit_amd import RotaryEmbedding, VSKError
+
+    inv = np.concatenate([[0.0, 3.0, 1e-7], 7.0 ** -np.arange(17)])
+    x, pos = normal(gen(6), 40, 3, 64), ints(range(0, 40 * 5003, 5003))
+    for scaling, a in (({"type": "given", "inv_freq": inv}, 1.0),
+                       ({"type": "given", "inv_freq": inv.tolist(), "attention_factor": 1.25}, 1.25)):
+        rope = RotaryEmbedding(ctx, 64, rotary_dim=40, scaling=scaling)
+        assert rope.amplitude == a and rope.inv_freq.tolist() == inv.tolist()
+        want = rotated(x, pos, inv, a, "half")
+        check(rope.apply(x, positions=pos), want, 2.0 ** -24 * want.abs()
+              + 2.0 ** -20 * x.cpu().double().abs().amax(-1, keepdim=True) * a)
+    for bad in ({"type": "given"}, {"type": "given", "inv_freq": inv[:3]},
+                {"type": "given", "inv_freq": inv, "factor": 2.0},
+                {"type": "given", "inv_freq": -inv}, {"type": "given", "inv_freq": inv + math.inf}):
+        with pytest.raises(VSKError) as e:
+            RotaryEmbedding(ctx, 64, rotary_dim=40, scaling=bad)
+        assert e.value.kind == "invalidArgument"
+
+
 @pytest.mark.parametrize("scaling", [None, {"type": "yarn", "factor": 8.0,
                                             "original_length": 512}])
 def test_moved_keys(ctx, scaling):

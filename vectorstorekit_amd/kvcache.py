@@ -122,7 +122,10 @@ class RotaryEmbedding:
       more than ``beta_fast`` (32) times over n positions stay, those under
       ``beta_slow`` (1) are divided by f, those between are blended, and the
       rotated values are multiplied by ``attention_factor``
-      (0.1 ln f + 1)."""
+      (0.1 ln f + 1);
+    * ``{"type": "given", "inv_freq": x}``: the pairs' radians a position
+      themselves (``rotary_dim / 2`` of them, whatever the base), and an
+      ``attention_factor`` (1)."""
 
     LAYOUTS = {"half": 0, "interleaved": 1}
 
@@ -153,10 +156,19 @@ class RotaryEmbedding:
         if not scaling:
             return inv, 1.0
         s = dict(scaling)
-        kind, f = s.pop("type", None), float(s.pop("factor", 0))
+        kind, amplitude = s.pop("type", None), 1.0
+        if kind == "given":
+            given = s.pop("inv_freq", None)
+            inv = np.array(() if given is None else given, np.float64)
+            if inv.shape != (r // 2,):
+                raise VSKError(-2, f"inv_freq must hold a value for each of {r // 2} pairs")
+            amplitude = float(s.pop("attention_factor", 1.0))
+            if s:
+                raise VSKError(-2, f"unknown scaling options {sorted(s)}")
+            return inv, amplitude
+        f = float(s.pop("factor", 0))
         if not f >= 1:
             raise VSKError(-2, "scaling needs a factor of at least 1")
-        amplitude = 1.0
         if kind == "linear":
             inv = inv / f
         elif kind == "ntk":
