@@ -38,8 +38,9 @@ namespace vsk {
 namespace {
 
 // What a type's 32-bit words hold: E elements; 16 bytes hold 4 * E.
-// TOP: log2 of the largest weight.  An f16 of 1 at most loses a weight under 2^-25, and a long context may hold many
-// of them behind one large first key; bf16 has fp32's exponents.
+// TOP: log2 of the largest weight.  An f16 of 1 at most loses a weight under
+// 2^-25, and a long context may hold many of them behind one large first key;
+// bf16 has fp32's exponents.
 template <class T> struct Elem;
 template <> struct Elem<float> {
   static constexpr int E = 1;
