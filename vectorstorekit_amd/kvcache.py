@@ -13,11 +13,11 @@ Tensors are torch tensors on the context's GPU.  Unlike the search calls,
 these are queued on torch's current stream and do not wait: a decoder makes
 dozens a token.  (Offsets, slots and counts given as host sequences are copied
 to the GPU first, which does wait and cannot be captured; int32 tensors there
-are used as they are.)  They record no gradients (a tensor that wants one is refused
-outside ``torch.no_grad()``, one with a forward-mode tangent always).  They allocate through torch, so a captured graph may hold
-them.  The reference keeps its language-model layer on the application's side
-(LLM/, Core/ML/Shaders/OptimizedMLShaders.metal:523); there is no CPU
-fallback.
+are used as they are.)  They record no gradients (a tensor that wants one is
+refused outside ``torch.no_grad()``, one with a forward-mode tangent always).
+They allocate through torch, so a captured graph may hold them.  The reference
+keeps its language-model layer on the application's side (LLM/,
+Core/ML/Shaders/OptimizedMLShaders.metal:523); there is no CPU fallback.
 """
 from __future__ import annotations
 
