@@ -703,6 +703,46 @@ int64_t vsk_attention_workspace(vsk_ctx *ctx, const vsk_kv *kv, const vsk_new_to
 vsk_status vsk_attention(vsk_ctx *ctx, void *stream, const vsk_kv *kv, int32_t layer,
                          const vsk_new_tokens *news, const vsk_attention_args *args);
 
+/* ---- linear layers in 8-bit integers ---------------------------------------
+ * The projections of the model that answers: matrixMultiply's counterpart
+ * (Acceleration/MetalAccelerationEngine.swift:209-229) over codes as the
+ * scalar quantizer's (symmetric, of at most 127), with a scale for each output
+ * channel of the weights and each token of the activations.  Queued on
+ * `stream` like the calls above.
+ *
+ * Weights are packed once into the order that the matrix cores read, into
+ * vsk_int8_packed_bytes(outputs, inputs) bytes, 16-byte aligned. */
+#define VSK_DTYPE_I8 3 /* vsk_int8_pack only */
+int64_t vsk_int8_packed_bytes(int64_t rows, int32_t inputs);
+typedef struct {
+  void *packed;
+  float *scales;     /* outputs                */
+  const float *bias; /* outputs, or NULL       */
+  int32_t outputs, inputs;
+} vsk_int8_weight;
+/* rows: outputs x inputs of dtype.  Numbers are quantised, scale = the row's
+ * largest magnitude / 127 (a row that holds an infinity or NaN: scale NaN);
+ * VSK_DTYPE_I8: codes with the scales that w->scales holds already. */
+vsk_status vsk_int8_pack(vsk_ctx *ctx, void *stream, int32_t dtype, const void *rows,
+                         int64_t row_stride, const vsk_int8_weight *w);
+/* tokens x inputs in, tokens x outputs out: each token is quantised as above
+ * (code = x * (127 / largest), rounded to even) and
+ * out = code . weights * token's scale * channel's scale + bias.  The sums are
+ * exact; a token that holds an infinity or NaN has NaN outputs.  inputs at
+ * most 131,072.  workspace: vsk_int8_linear_workspace() bytes, 16-byte
+ * aligned. */
+typedef struct {
+  const void *x;
+  void *out;
+  int64_t x_row, out_row, tokens;
+  void *workspace;
+  int64_t workspace_bytes;
+  int32_t x_dtype, out_dtype;
+} vsk_int8_rows;
+int64_t vsk_int8_linear_workspace(const vsk_int8_weight *w, int64_t tokens);
+vsk_status vsk_int8_linear(vsk_ctx *ctx, void *stream, const vsk_int8_weight *w,
+                           const vsk_int8_rows *rows);
+
 #ifdef __cplusplus
 }
 #endif

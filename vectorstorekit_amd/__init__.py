@@ -32,14 +32,17 @@ from .quantization import (  # noqa: F401,E402
     SQ8Database,
 )
 
-# the cache and its attention work on torch tensors; torch is imported with them
-_KVCACHE = ("PagedKVCache", "RotaryEmbedding", "window_attention")
+# the cache, its attention and the linear layers work on torch tensors; torch is
+# imported with them
+_QUEUED = {"PagedKVCache": "kvcache", "RotaryEmbedding": "kvcache", "window_attention": "kvcache",
+           "Int8Linear": "linear"}
 
 
 def __getattr__(name):
-    if name in _KVCACHE:
-        from . import kvcache
+    if name in _QUEUED:
+        from importlib import import_module
 
         # (kept: an import within a loop is then a plain lookup)
-        return globals().setdefault(name, getattr(kvcache, name))
+        module = import_module("." + _QUEUED[name], __name__)
+        return globals().setdefault(name, getattr(module, name))
     raise AttributeError(f"module {__name__!r} has no attribute {name!r}")

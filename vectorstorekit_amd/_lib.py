@@ -110,6 +110,17 @@ class vsk_attention_args(ctypes.Structure):
                 ("window", c_int32), ("sinks", c_int32), ("max_length", c_int32)]
 
 
+class vsk_int8_weight(ctypes.Structure):
+    _fields_ = [("packed", c_void_p), ("scales", c_void_p), ("bias", c_void_p),
+                ("outputs", c_int32), ("inputs", c_int32)]
+
+
+class vsk_int8_rows(ctypes.Structure):
+    _fields_ = [("x", c_void_p), ("out", c_void_p), ("x_row", c_int64), ("out_row", c_int64),
+                ("tokens", c_int64), ("workspace", c_void_p), ("workspace_bytes", c_int64),
+                ("x_dtype", c_int32), ("out_dtype", c_int32)]
+
+
 KERNEL_AUTO, KERNEL_EXACT, KERNEL_SCREEN, KERNEL_BF16X3, KERNEL_FP32 = 0, 1, 2, 3, 4
 
 P = c_void_p  # every buffer argument is passed as a raw address
@@ -204,6 +215,10 @@ SIGNATURES = {
     "vsk_kv_append": (c_int32, [P, P, P, c_int32, P, P, P, P, P]),
     "vsk_attention_workspace": (c_int64, [P, P, P, P]),
     "vsk_attention": (c_int32, [P, P, P, c_int32, P, P]),
+    "vsk_int8_packed_bytes": (c_int64, [c_int64, c_int32]),
+    "vsk_int8_pack": (c_int32, [P, P, c_int32, P, c_int64, P]),
+    "vsk_int8_linear_workspace": (c_int64, [P, c_int64]),
+    "vsk_int8_linear": (c_int32, [P, P, P, P]),
 }
 
 _lib = None
