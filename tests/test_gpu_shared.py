@@ -1,0 +1,585 @@
+"""Cross attention and attention over shared prefixes, against their
+definitions in 64 bits.
+
+Tolerances as in test_gpu_kvcache.py: with u the unit roundoff of the output's
+type (2^-8 bf16, 2^-11 f16, 2^-24 f32), the score of fp32 products is off by at
+most e = 2^-24 (d + 8) scale max sum |q k|, a weight by a factor within
+e + 2^-21, the sum of L weights by 2^-24 (L + 16); 16-bit types may round each
+weight once (u); so |err| <= u |o| + max |v| (2 (e + 2^-21 + 2^-24 (L + 16)) +
+(16-bit) u).  Parts that are joined are scaled by one more exponential, within
+the same 2^-21."""
+import ctypes
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+U = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11, torch.float32: 2.0 ** -24}
+BF, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+DEV = "cuda:0"
+
+
+def ints(x):
+    return torch.tensor(list(x), dtype=torch.int32, device=DEV)
+
+
+def gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def normal(g, *shape, dtype=F32):
+    return torch.randn(*shape, generator=g, dtype=torch.float32).to(dtype).to(DEV)
+
+
+def attended(q, k, v, pos, scale):
+    """q (T x H x d) over k, v (L x Hkv x d), query i sees the keys up to
+    pos[i]; in 64 bits on the CPU.  Outputs, logarithms of the sums,
+    tolerances."""
+    t, heads, d = q.shape
+    u, group = U[q.dtype], heads // k.shape[1]
+    q, k, v = (x.detach().cpu().double() for x in (q, k, v))
+    length = k.shape[0]
+    if not length:
+        zero = torch.zeros(t, heads, d, dtype=torch.float64)
+        return zero, torch.full((t, heads), -math.inf, dtype=torch.float64), zero
+    k, v = (x.repeat_interleave(group, 1).transpose(0, 1) for x in (k, v))
+    see = torch.arange(length) <= torch.as_tensor(pos)[:, None]
+    # what no query sees enters no sum
+    k, v = (torch.where(see.any(0)[:, None], x, 0.0) for x in (k, v))
+    q = q.transpose(0, 1)
+    s = (q @ k.transpose(1, 2) * scale).masked_fill(~see, -math.inf)
+    lse = torch.logsumexp(s, -1)
+    w = torch.where(torch.isfinite(lse)[..., None], torch.exp(s - lse[..., None]), 0.0)
+    out = w @ v
+    size = (q.abs() @ k.abs().transpose(1, 2)).masked_fill(~see, 0.0).amax(-1)
+    e = 2.0 ** -24 * (d + 8) * scale * size
+    w = 2 * (e + 2.0 ** -20 + 2.0 ** -24 * (length + 16)) + (u if u > 2.0 ** -20 else 0.0)
+    most = v.abs().amax((1, 2))[:, None]
+    tol = u * out.abs() + (most * w)[..., None]
+    return out.transpose(0, 1), lse.T, tol.transpose(0, 1)
+
+
+def check(got, want, tol):
+    got = got.detach().cpu().double()
+    fine = torch.isfinite(want)
+    assert torch.equal(torch.isfinite(got), fine)
+    err = (got - want).abs()[fine]
+    assert bool((err <= tol[fine]).all()), float((err - tol[fine]).max())
+
+
+def starts_of(counts):
+    return [0] + list(torch.tensor(counts).cumsum(0).tolist())
+
+
+def check_lse(got, want):
+    got = got.cpu().double()
+    assert torch.equal(torch.isfinite(got), torch.isfinite(want))
+    fine = torch.isfinite(want)
+    # the sum's bound, and a logarithm's own rounding
+    assert bool(((got - want).abs()[fine] <= 2.0 ** -17 * (1 + want.abs()[fine])).all())
+
+
+# --------------------------------------------------------------- cross attention
+
+HEADS = [(8, 2, 64), (4, 4, 128), (5, 5, 80), (3, 1, 37), (8, 1, 256), (14, 2, 96)]
+
+
+@pytest.mark.parametrize("dtype", [BF, F16, F32])
+@pytest.mark.parametrize("heads,kv,d", HEADS)
+@pytest.mark.parametrize("new,keys", [
+    ([1], [1]), ([1, 1, 1, 1], [300, 0, 17, 1]), ([3, 0, 40, 1], [33, 5, 0, 1200]),
+    ([200, 7], [15, 129]), ([70, 130, 1], [257, 64, 700])])
+def test_cross_ragged(ctx, dtype, heads, kv, d, new, keys):
+    from vectorstorekit_amd import cross_attention
+
+    g = gen(d + sum(keys))
+    q = normal(g, sum(new), heads, d, dtype=dtype)
+    k, v = (normal(g, sum(keys), kv, d, dtype=dtype) for _ in range(2))
+    at, ks = starts_of(new), starts_of(keys)
+    out, lse = cross_attention(ctx, q, k, v, starts=at, k_starts=ks, max_length=max(new),
+                               max_keys=max(keys), return_lse=True)
+    bare = cross_attention(ctx, q, k, v, starts=ints(at), k_starts=ints(ks))
+    for i in range(len(new)):
+        a, b = slice(at[i], at[i + 1]), slice(ks[i], ks[i + 1])
+        want, sums, tol = attended(q[a], k[b], v[b], [keys[i]] * new[i], d ** -0.5)
+        check(out[a], want, tol)
+        check(bare[a], want, tol)
+        check_lse(lse[a], sums)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("layout", ["dense", "heads first", "fused"])
+@pytest.mark.parametrize("new", [1, 5, 90])
+def test_cross_padded(ctx, dtype, layout, new):
+    """A padded batch in the layouts that projections leave, with memory never
+    written behind the lengths."""
+    from vectorstorekit_amd import cross_attention
+
+    g = gen(new)
+    n, most, heads, kv, d = 5, 150, 6, 3, 64
+    lengths = [150, 0, 1, 77, 128]
+    if layout == "dense":
+        k, v = (normal(g, n, most, kv, d, dtype=dtype) for _ in range(2))
+    elif layout == "heads first":
+        k, v = (normal(g, n, kv, most, d, dtype=dtype).transpose(1, 2) for _ in range(2))
+    else:
+        k, v = normal(g, n, most, 2, kv, d, dtype=dtype).unbind(2)
+    for i, x in enumerate(lengths):
+        k[i, x:], v[i, x:] = math.nan, math.inf
+    q = normal(g, n * new, heads, d, dtype=dtype)
+    at = None if new == 1 else [new * i for i in range(n + 1)]
+    out = cross_attention(ctx, q, k, v, starts=at, k_lengths=lengths, max_length=new)
+    for i, x in enumerate(lengths):
+        a = slice(new * i, new * (i + 1))
+        want, _, tol = attended(q[a], k[i, :x], v[i, :x], [x] * new, d ** -0.5)
+        check(out[a], want, tol)
+    whole = cross_attention(ctx, q[:new], k[:1], v[:1], starts=[0, new])
+    assert torch.equal(whole, out[:new])
+
+
+@pytest.mark.parametrize("dtype", [BF, F16, F32])
+def test_cross_sets(ctx, dtype):
+    """Several sequences of one set, sets that are not there."""
+    from vectorstorekit_amd import cross_attention
+
+    g = gen(3)
+    new, which, keys = [4, 1, 9, 2, 60, 3], [1, 1, -1, 0, 2, 7], [40, 333, 100]
+    q = normal(g, sum(new), 4, 128, dtype=dtype)
+    k, v = (normal(g, sum(keys), 2, 128, dtype=dtype) for _ in range(2))
+    at, ks = starts_of(new), starts_of(keys)
+    out = cross_attention(ctx, q, k, v, starts=at, k_starts=ks, sets=ints(which), scale=0.2)
+    pad = torch.zeros(3, 333, 2, 128, dtype=dtype, device=DEV)
+    pv = torch.zeros_like(pad)
+    for i in range(3):
+        pad[i, :keys[i]], pv[i, :keys[i]] = k[ks[i]:ks[i + 1]], v[ks[i]:ks[i + 1]]
+    same = cross_attention(ctx, q, pad, pv, starts=at, k_lengths=ints(keys), sets=which, scale=0.2)
+    for i, z in enumerate(which):
+        a = slice(at[i], at[i + 1])
+        b = slice(ks[z], ks[z + 1]) if 0 <= z < 3 else slice(0, 0)
+        want, _, tol = attended(q[a], k[b], v[b], [10 ** 6] * new[i], 0.2)
+        check(out[a], want, tol)
+        check(same[a], want, tol)
+
+
+@pytest.mark.parametrize("dtype", [BF, F16, F32])
+@pytest.mark.parametrize("new,heads,kv", [(1, 8, 8), (6, 4, 1), (100, 4, 2)])
+def test_cross_long(ctx, dtype, new, heads, kv):
+    """Keys in parts, and the last part longer than the bound said."""
+    from vectorstorekit_amd import cross_attention
+
+    g = gen(new)
+    d, length = 64, 9001
+    q = normal(g, new, heads, d, dtype=dtype)
+    k, v = (normal(g, 1, length, kv, d, dtype=dtype) for _ in range(2))
+    want, sums, tol = attended(q, k[0], v[0], [length] * new, d ** -0.5)
+    for most in (None, 9001, 500):
+        out, lse = cross_attention(ctx, q, k, v, starts=[0, new], max_keys=most, return_lse=True)
+        check(out, want, tol)
+        check_lse(lse, sums)
+
+
+@pytest.mark.parametrize("dtype", [BF, F16, F32])
+def test_cross_visible_infinities(ctx, dtype):
+    """An infinite value is its column's result, a NaN score its row's."""
+    from vectorstorekit_amd import cross_attention
+
+    g = gen(5)
+    q = normal(g, 80, 2, 64, dtype=dtype)
+    k, v = (normal(g, 70, 2, 64, dtype=dtype) for _ in range(2))
+    v[3, 0, 5], v[69, 1, 6] = math.inf, -math.inf
+    q[7, 1, 0] = math.nan
+    for new in (1, 80):
+        out = cross_attention(ctx, q[:new], k, v, starts=[0, new], k_starts=[0, 70]).cpu()
+        assert bool((out[:, 0, 5] == math.inf).all())
+        bad = torch.isnan(out[:, 1]).all(-1)
+        assert bad.tolist() == [i == 7 for i in range(new)]
+        assert bool((out[~bad][:, 1, 6] == -math.inf).all())
+        out[:, 0, 5] = out[:, 1, 6] = 0
+        assert bool(torch.isfinite(out[~bad]).all())
+
+
+def test_cross_empty(ctx):
+    from vectorstorekit_amd import cross_attention
+
+    q = normal(gen(1), 3, 4, 64, dtype=BF)
+    k = torch.empty(0, 2, 64, dtype=BF, device=DEV)
+    out, lse = cross_attention(ctx, q, k, k, k_starts=[0, 0, 0, 0], return_lse=True)
+    assert not out.any() and bool((lse == -math.inf).all())
+    k = torch.empty(3, 0, 2, 64, dtype=BF, device=DEV)
+    assert not cross_attention(ctx, q, k, k).any()
+    k = torch.empty(0, 5, 2, 64, dtype=BF, device=DEV)
+    assert not cross_attention(ctx, q, k, k, sets=[-1, -1, -1]).any()
+    k = torch.ones(1, 5, 2, 64, dtype=BF, device=DEV)
+    assert cross_attention(ctx, q[:0], k, k).shape == (0, 4, 64)
+    assert cross_attention(ctx, q, k, k, starts=[0, 3], max_length=0).shape == (3, 4, 64)
+
+
+# ---------------------------------------------------------------- shared prefixes
+
+def cache_of(ctx, g, groups, page, kv, d, dtype, order=None):
+    """A cache whose groups' members share a prefix: groups is a list of
+    (shared tokens, whole pages; each member's own tokens).  Pages lie all over
+    the pool, slots in the given order.  Returns the cache and the slots."""
+    from vectorstorekit_amd import PagedKVCache
+
+    pages = sum(p // page + sum(-(-x // page) for x in own) for p, own in groups) + 2
+    width = max(p // page + -(-max(own + [1]) // page) for p, own in groups) + 1
+    ids = torch.randperm(pages, generator=g).tolist()
+    rows, lengths = [], []
+    for p, own in groups:
+        first = [ids.pop() for _ in range(p // page)]
+        for x in own:
+            row = first + [ids.pop() for _ in range(-(-x // page))]
+            rows.append(row + [-1] * (width - len(row)))
+            lengths.append(p + x)
+    n = len(rows)
+    order = list(range(n)) if order is None else order
+    table = torch.full((n + 1, width), -1, dtype=torch.int32)
+    held = torch.zeros(n + 1, dtype=torch.int32)
+    for i, slot in enumerate(order):
+        table[slot], held[slot] = torch.tensor(rows[i], dtype=torch.int32), lengths[i]
+    k, v = (normal(g, pages, page, kv, d, dtype=dtype) for _ in range(2))
+    return PagedKVCache.over(ctx, k, v, table.to(DEV), held.to(DEV)), order
+
+
+def keys_of(cache, slot):
+    length = int(cache.lengths[slot])
+    ids = cache.table[slot, :-(-length // cache.page_size)].long()
+    return (x[ids].flatten(0, 1)[:length] for x in (cache.k, cache.v))
+
+
+def check_shared(cache, slots, q, starts, out, scale, lse=None):
+    at = starts if starts is not None else list(range(len(slots) + 1))
+    for i, slot in enumerate(slots[:len(at) - 1]):
+        a, (k, v) = slice(at[i], at[i + 1]), keys_of(cache, slot)
+        t, length = at[i + 1] - at[i], k.shape[0]
+        want, sums, tol = attended(q[a], k, v, range(length - t, length), scale)
+        check(out[a], want, tol)
+        if lse is not None:
+            check_lse(lse[a], sums)
+
+
+GROUPS = [
+    [(64, [1, 5, 30])],
+    [(512, [40, 3, 17, 100]), (0, [7, 20]), (96, [33])],
+    [(1600, [1] * 9 + [200]), (32, [64, 1])],
+]
+
+
+@pytest.mark.parametrize("dtype", [BF, F16, F32])
+@pytest.mark.parametrize("heads,kv,d", HEADS)
+@pytest.mark.parametrize("groups", GROUPS)
+def test_shared_tokens(ctx, dtype, heads, kv, d, groups):
+    g = gen(d)
+    cache, slots = cache_of(ctx, g, groups, 32, kv, d, dtype)
+    n = len(slots)
+    q = normal(g, n, heads, d, dtype=dtype)
+    offsets = starts_of([len(own) for _, own in groups])
+    plan = cache.share(offsets)
+    want = [p if len(own) > 1 else 0 for p, own in groups for _ in own] + [0]
+    assert plan.prefix.tolist() == want
+    out, lse = cache.attend(q, shared=plan, return_lse=True)
+    check_shared(cache, slots, q, None, out, d ** -0.5, lse)
+    hinted = cache.share(offsets, prefix=groups[0][0])
+    out = cache.attend(q, shared=hinted, max_length=int(cache.lengths.max()), scale=0.1)
+    check_shared(cache, slots, q, None, out, 0.1)
+
+
+@pytest.mark.parametrize("dtype", [BF, F16, F32])
+@pytest.mark.parametrize("heads,kv,d", [(8, 2, 64), (4, 4, 128), (8, 1, 256), (3, 3, 50)])
+@pytest.mark.parametrize("new", [[2, 3, 1, 5, 4, 0, 1], [1, 0, 0, 70, 9, 20, 33]])
+def test_shared_several_tokens(ctx, dtype, heads, kv, d, new):
+    """Ragged new tokens, none among them; slots in an order of their own."""
+    g = gen(d + len(new))
+    groups = [(256, [9, 3, 1, 80]), (128, [12, 25, 33])]
+    cache, slots = cache_of(ctx, g, groups, 16, kv, d, dtype, order=[3, 0, 6, 1, 7, 2, 4])
+    at = starts_of(new)
+    q = normal(g, at[-1], heads, d, dtype=dtype)
+    plan = cache.share(ints([0, 4, 7]), seqs=ints(slots), members=4)
+    assert plan.prefix.tolist() == [256] * 4 + [128] * 3
+    out, lse = cache.attend(q, shared=plan, starts=at, max_new=max(new), return_lse=True)
+    check_shared(cache, slots, q, at, out, d ** -0.5, lse)
+    same = cache.attend(q, starts=at, seqs=slots, max_new=max(new), window=100, sinks=3)
+    assert torch.equal(same, cache.attend(q, shared=plan, starts=at, max_new=max(new), window=100,
+                                          sinks=3))
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_shared_rows_within_the_prefix(ctx, dtype):
+    """New tokens that reach back into the shared pages see what stands before
+    them, no more."""
+    g = gen(8)
+    cache, slots = cache_of(ctx, g, [(128, [5, 1, 9]), (64, [2, 2])], 16, 2, 64, dtype)
+    new = [40, 100, 9, 66, 3]
+    at = starts_of(new)
+    q = normal(g, at[-1], 4, 64, dtype=dtype)
+    out = cache.attend(q, shared=cache.share([0, 3, 5]), starts=at, max_new=100)
+    check_shared(cache, slots, q, at, out, 0.125)
+
+
+@pytest.mark.parametrize("dtype", [BF, F16])
+def test_shared_many_rows(ctx, dtype):
+    """A prefix for many branches (row tiles of 128), in parts."""
+    g = gen(9)
+    groups = [(4096, torch.randint(1, 90, (40,), generator=g).tolist()), (2048, [50, 700])]
+    cache, slots = cache_of(ctx, g, groups, 64, 2, 128, dtype)
+    q = normal(g, 42, 16, 128, dtype=dtype)
+    plan = cache.share([0, 40, 42], prefix=4096)
+    out, lse = cache.attend(q, shared=plan, return_lse=True)
+    check_shared(cache, slots, q, None, out, 128 ** -0.5, lse)
+
+
+def test_shared_sequences_in_no_group(ctx):
+    """Sequences before the first group and behind the last, an empty group,
+    and fewer sequences than the plan knows."""
+    g = gen(10)
+    cache, slots = cache_of(ctx, g, [(64, [3, 4, 5, 6]), (64, [1, 2])], 32, 2, 64, BF)
+    q = normal(g, 6, 4, 64, dtype=BF)
+    plan = cache.share([1, 3, 3, 6])
+    # (slot 3 shares nothing with slots 4 and 5)
+    assert plan.prefix.tolist() == [0, 64, 64, 0, 0, 0, 0]
+    check_shared(cache, slots, q, None, cache.attend(q, shared=plan), 0.125)
+    plan = cache.share([0, 4, 6])
+    check_shared(cache, slots, q[:2], None, cache.attend(q[:2], shared=plan), 0.125)
+    check_shared(cache, slots, q[:5], None, cache.attend(q[:5], shared=plan), 0.125)
+    for none in ([], [0], [2, 2]):
+        if not none:
+            continue
+        out = cache.attend(q, shared=cache.share(none))
+        assert torch.equal(out, cache.attend(q))
+
+
+def test_share_finds_what_tables_agree_on(ctx):
+    g = gen(11)
+    cache, _ = cache_of(ctx, g, [(160, [20, 20, 20])], 16, 1, 16, F32)
+    assert cache.share([0, 3]).prefix.tolist() == [160, 160, 160, 0]
+    cache.table[2, 7] = cache.table[2, 11]
+    assert cache.share([0, 3]).prefix.tolist() == [112, 112, 112, 0]
+    assert cache.share([0, 2]).prefix.tolist() == [160, 160, 0, 0]
+    cache.lengths[1] = 47  # two whole pages
+    assert cache.share([0, 3]).prefix.tolist() == [32, 32, 32, 0]
+    cache.lengths[1] = 0
+    assert cache.share([0, 3]).prefix.tolist() == [0, 0, 0, 0]
+    cache.lengths[1] = 180
+    cache.table[:, 3] = -1
+    assert cache.share([0, 3]).prefix.tolist() == [48, 48, 48, 0]
+    # the same slot twice agrees with itself; one that is not there with none
+    assert cache.share([0, 2], seqs=[2, 2]).prefix.tolist() == [48, 48]
+    assert cache.share([0, 2], seqs=ints([2, 9])).prefix.tolist() == [0, 0]
+
+
+def test_shared_nan_in_masked_places(ctx):
+    """Rows of pages behind a sequence's end hold NaN."""
+    g = gen(12)
+    cache, slots = cache_of(ctx, g, [(64, [3, 17, 30]), (32, [1, 16])], 16, 2, 64, BF)
+    for s in slots:
+        length = int(cache.lengths[s])
+        page = int(cache.table[s, (length - 1) // 16])
+        if length % 16:
+            cache.k[page, length % 16:] = math.nan
+            cache.v[page, length % 16:] = math.inf
+    q = normal(g, 5, 4, 64, dtype=BF)
+    out = cache.attend(q, shared=cache.share([0, 3, 5]))
+    check_shared(cache, slots, q, None, out, 0.125)
+
+
+def forked(ctx, dtype=BF, branches=5, tokens=200):
+    """A real cache: one context, forked, each branch grown by a few tokens."""
+    from vectorstorekit_amd import PagedKVCache
+
+    g = gen(13)
+    cache = PagedKVCache(ctx, pages=64, page_size=16, kv_heads=2, head_dim=64,
+                         slots=branches + 2, width=20, dtype=dtype)
+    cache.reserve([0], [tokens])
+    k, v = (normal(g, tokens, 2, 64, dtype=dtype) for _ in range(2))
+    cache.append(k, v, starts=[0, tokens], seqs=[0])
+    slots = ints(range(1, branches + 1))
+    cache.fork(torch.zeros_like(slots), slots)
+    return cache, slots, g
+
+
+def view(cache, slots):
+    """(the helpers above look at one layer)"""
+    class One:
+        k, v, table, lengths = cache.k[0], cache.v[0], cache.table, cache.lengths
+        page_size = cache.page_size
+    return One, slots.tolist()
+
+
+def test_shared_after_forks(ctx):
+    cache, slots, g = forked(ctx)
+    plan = cache.share([0, 5], seqs=slots, prefix=192)
+    assert plan.prefix.tolist() == [192] * 5
+    for step in range(3):
+        cache.reserve(slots, torch.ones_like(slots))
+        k, v = (normal(g, 5, 2, 64, dtype=BF) for _ in range(2))
+        cache.append(k, v, seqs=slots)
+        q = normal(g, 5, 8, 64, dtype=BF)
+        one, order = view(cache, slots)
+        check_shared(one, order, q, None, cache.attend(q, shared=plan), 0.125)
+    # packing the pool renames pages in every table: what was found stays true
+    cache.free([0])
+    cache.compact()
+    one, order = view(cache, slots)
+    check_shared(one, order, q, None, cache.attend(q, shared=plan), 0.125)
+    # a branch dropped and forked from another that has grown
+    cache.fork([2], [5])
+    plan.update()
+    one, order = view(cache, slots)
+    check_shared(one, order, q, None, cache.attend(q, shared=plan), 0.125)
+    last = cache.share([0, 2], seqs=[2, 5])
+    assert last.prefix.tolist() == [192, 192]
+
+
+def test_shared_graph_and_stream(ctx):
+    """Captured with the plan made anew in the graph, replayed over changed
+    lengths with other work between; two streams at once."""
+    cache, slots, g = forked(ctx)
+    q = normal(g, 5, 8, 64, dtype=BF)
+    ones = torch.ones_like(slots)
+    plan = cache.share([0, 5], seqs=slots)
+    cache.attend(q, shared=plan)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        plan.update()
+        out = cache.attend(q, shared=plan)
+    for step in range(4):
+        cache.reserve(slots, ones)
+        cache.append(*(normal(g, 5, 2, 64, dtype=BF) for _ in range(2)), seqs=slots)
+        q.copy_(normal(g, 5, 8, 64, dtype=BF))
+        graph.replay()
+        got = out.clone()
+        torch.cuda.synchronize()
+        assert torch.equal(got, cache.attend(q, shared=plan))
+        one, order = view(cache, slots)
+        check_shared(one, order, q, None, got, 0.125)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        there = [cache.attend(q, shared=plan) for _ in range(3)]
+    here = [cache.attend(q, shared=plan) for _ in range(3)]
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, got) for x in there + here)
+
+
+def test_indices_out_of_range(ctx):
+    """What device memory holds is held to its buffers: no group, slot, offset
+    or prefix reads past them, and the other groups are not touched."""
+    g = gen(14)
+    cache, slots = cache_of(ctx, g, [(64, [3, 4]), (64, [5, 6])], 32, 2, 64, BF)
+    q = normal(g, 4, 4, 64, dtype=BF)
+    plan = cache.share([0, 2, 4])
+    want = cache.attend(q, shared=plan)
+    plan.prefix[:2] = 1 << 30
+    assert torch.equal(cache.attend(q, shared=plan)[2:], want[2:])
+    plan.prefix[:2] = -5
+    assert torch.equal(cache.attend(q, shared=plan)[2:], want[2:])
+    plan.update()
+    plan.groups[0] = -100
+    cache.attend(q, shared=plan)
+    plan.groups.copy_(ints([5, 2, 1 << 30]))
+    plan.update()
+    cache.attend(q, shared=plan)
+    torch.cuda.synchronize()
+
+
+# ---------------------------------------------------------------------- refusals
+
+def test_refusals(ctx):
+    from vectorstorekit_amd import VSKError, cross_attention
+
+    g = gen(15)
+    q, k = normal(g, 4, 4, 64, dtype=BF), normal(g, 10, 2, 64, dtype=BF)
+    pad = normal(g, 4, 5, 2, 64, dtype=BF)
+    bad = [
+        lambda: cross_attention(ctx, q.cpu(), k, k, k_starts=[0, 10]),
+        lambda: cross_attention(ctx, q, k.half(), k, k_starts=[0, 10]),
+        lambda: cross_attention(ctx, q, k, k[:9], starts=[0, 4], k_starts=[0, 10]),
+        lambda: cross_attention(ctx, q, k, k, starts=[0, 4]),
+        lambda: cross_attention(ctx, q, k, k, starts=[0, 4], k_starts=[0, 10], k_lengths=[10]),
+        lambda: cross_attention(ctx, q, pad, pad, k_starts=[0, 5]),
+        lambda: cross_attention(ctx, q, pad, pad, k_lengths=[5, 5]),
+        lambda: cross_attention(ctx, q, k, k, k_starts=[0, 10]),
+        lambda: cross_attention(ctx, q, k, k, k_starts=[0, 10], sets=[0, 0]),
+        lambda: cross_attention(ctx, q[:, :3], k, k, starts=[0, 4], k_starts=[0, 10]),
+        lambda: cross_attention(ctx, q, k, k, starts=[0, 4], k_starts=[0, 10], scale=0.0),
+        lambda: cross_attention(ctx, q, k, k, starts=[0, 4], k_starts=[0, 10], max_length=-1),
+        lambda: cross_attention(ctx, q, k, k, starts=[], k_starts=[0, 10]),
+        lambda: cross_attention(ctx, q.long(), k.long(), k.long(), starts=[0, 4], k_starts=[0, 10]),
+        lambda: cross_attention(ctx, q.clone().requires_grad_(), k, k, starts=[0, 4],
+                                k_starts=[0, 10]),
+    ]
+    cache, _ = cache_of(ctx, g, [(32, [3, 4])], 32, 2, 64, BF)
+    other, _ = cache_of(ctx, g, [(32, [3, 4])], 32, 2, 64, BF)
+    plan = cache.share([0, 2], seqs=[0, 1])
+    bad += [
+        lambda: cache.share([]),
+        lambda: cache.share([0, 9]),
+        lambda: cache.share([2, 1]),
+        lambda: cache.share([-1, 1]),
+        lambda: cache.share([0, 2], seqs=[0, 7]),
+        lambda: cache.share([0, 2], members=-1),
+        lambda: cache.share([0, 2], prefix=-1),
+        lambda: cache.share(ints([0, 2]).long()),
+        lambda: cache.attend(q[:2], shared=plan, seqs=[0, 1]),
+        lambda: other.attend(q[:2], shared=plan),
+        lambda: cache.attend(q[:2], shared=[0, 2]),
+        lambda: cache.attend(q[:3], shared=plan),
+    ]
+    for i, call in enumerate(bad):
+        with pytest.raises(VSKError):
+            call()
+            pytest.fail(f"call {i} was taken")
+
+
+def test_c_refusals(ctx):
+    """The C calls' own checks (of what Python checks before)."""
+    from vectorstorekit_amd import _lib
+
+    g = gen(16)
+    cache, _ = cache_of(ctx, g, [(32, [3, 4])], 32, 2, 64, BF)
+    q, out = normal(g, 2, 4, 64, dtype=BF), torch.empty(2, 4, 64, dtype=BF, device=DEV)
+    lib, h = ctx.lib, ctx.handle
+    plan = cache.share([0, 2])
+    news = _lib.vsk_new_tokens(None, None, 2, 1, 2)
+    args = _lib.vsk_attention_args()
+    args.q = _lib.vsk_head_rows(q.data_ptr(), out.data_ptr(), 256, 64, 256, 64, 4)
+    args.scale = 0.1
+    call = lambda p: lib.vsk_attention_shared(h, None, cache._ref, 0, ctypes.byref(news),
+                                              ctypes.byref(args), p)
+    assert call(None) == -2
+    need = lib.vsk_attention_shared_workspace(h, cache._ref, ctypes.byref(news),
+                                              ctypes.byref(args), plan._ref)
+    assert need > 0 and call(plan._ref) == -9
+    work = torch.empty(need, dtype=torch.uint8, device=DEV)
+    args.workspace, args.workspace_bytes = work.data_ptr(), need
+    assert call(plan._ref) == 0
+    assert torch.equal(out, cache.attend(q, shared=plan, scale=0.1))
+    for field, value, status in (("n_groups", -1, -2), ("max_members", -1, -2), ("n", 1, -4),
+                                 ("groups", 0, -2), ("prefix", 0, -2)):
+        c = _lib.vsk_shared_prefix.from_buffer_copy(plan._c)
+        setattr(c, field, value)
+        assert call(ctypes.byref(c)) == status, field
+    sets = _lib.vsk_key_sets(None, None, 5, 1)
+    cross = lambda s: lib.vsk_cross_attention(h, None, cache._ref, ctypes.byref(news),
+                                              ctypes.byref(args), s)
+    assert cross(None) == -2
+    assert cross(ctypes.byref(sets)) == -8  # (pages)
+    k = normal(g, 10, 2, 64, dtype=BF)
+    kv = _lib.vsk_kv()
+    kv.k = kv.v = k.data_ptr()
+    kv.k_row = kv.v_row = 128
+    kv.k_head = kv.v_head = 64
+    kv.dtype, kv.layers, kv.pages, kv.kv_heads, kv.head_dim = 2, 1, 5, 2, 64
+    dense = lambda s: lib.vsk_cross_attention(h, None, ctypes.byref(kv), ctypes.byref(news),
+                                              ctypes.byref(args), ctypes.byref(s))
+    assert dense(sets) == -2  # two sequences, one set
+    sets.n = 2
+    args.window = 3
+    assert dense(sets) == -8
+    args.window = 0
+    assert dense(sets) == 0
+    torch.cuda.synchronize()

@@ -35,7 +35,7 @@ from .quantization import (  # noqa: F401,E402
 # the cache, its attention and the linear layers work on torch tensors; torch is
 # imported with them
 _QUEUED = {"PagedKVCache": "kvcache", "RotaryEmbedding": "kvcache", "window_attention": "kvcache",
-           "Int8Linear": "linear"}
+           "cross_attention": "kvcache", "SharedPrefix": "kvcache", "Int8Linear": "linear"}
 
 
 def __getattr__(name):

@@ -110,6 +110,16 @@ class vsk_attention_args(ctypes.Structure):
                 ("window", c_int32), ("sinks", c_int32), ("max_length", c_int32)]
 
 
+class vsk_key_sets(ctypes.Structure):
+    _fields_ = [("starts", c_void_p), ("lengths", c_void_p), ("set_rows", c_int64),
+                ("n", c_int32)]
+
+
+class vsk_shared_prefix(ctypes.Structure):
+    _fields_ = [("groups", c_void_p), ("prefix", c_void_p), ("n_groups", c_int32),
+                ("n", c_int32), ("max_members", c_int32), ("max_prefix", c_int32)]
+
+
 class vsk_int8_weight(ctypes.Structure):
     _fields_ = [("packed", c_void_p), ("scales", c_void_p), ("bias", c_void_p),
                 ("outputs", c_int32), ("inputs", c_int32)]
@@ -215,6 +225,11 @@ SIGNATURES = {
     "vsk_kv_append": (c_int32, [P, P, P, c_int32, P, P, P, P, P]),
     "vsk_attention_workspace": (c_int64, [P, P, P, P]),
     "vsk_attention": (c_int32, [P, P, P, c_int32, P, P]),
+    "vsk_cross_attention_workspace": (c_int64, [P, P, P, P]),
+    "vsk_cross_attention": (c_int32, [P, P, P, P, P, P]),
+    "vsk_kv_share": (c_int32, [P, P, P, P, P]),
+    "vsk_attention_shared_workspace": (c_int64, [P, P, P, P, P]),
+    "vsk_attention_shared": (c_int32, [P, P, P, c_int32, P, P, P]),
     "vsk_int8_packed_bytes": (c_int64, [c_int64, c_int32]),
     "vsk_int8_pack": (c_int32, [P, P, c_int32, P, c_int64, P]),
     "vsk_int8_linear_workspace": (c_int64, [P, c_int64]),

@@ -1,5 +1,6 @@
-// attention.hip -- the attention entry points: checks, the division of the
-// work, and the choice of kernel.
+// attention.hip -- the attention entry points (of a sequence's new tokens over
+// its keys, over keys of another length, over prefixes that sequences share):
+// checks, the division of the work, and the choice of kernel.
 #include <cmath>
 
 #include "attn.hpp"
@@ -33,20 +34,35 @@ bool aligned_operands(const vsk_kv *kv, const vsk_attention_args *args) {
   return ok;
 }
 
-Plan plan_of(const vsk_ctx *ctx, const vsk_kv *kv, const vsk_new_tokens *news,
-             const vsk_attention_args *args) {
+// What a plan divides: n sequences of at most max_new new tokens and keys keys.
+// all: every token sees every key; joined: its parts are joined with another
+// plan's.
+struct Span {
+  int64_t n, max_new, keys;
+  bool all, joined;
+};
+
+int64_t most_new(const vsk_new_tokens *news) { return news->starts ? news->max_new : 1; }
+
+// keys of a sequence at most, of a bound that the caller gives (0: none)
+int64_t most_keys(const vsk_kv *kv, int64_t bound) {
+  const int64_t keys = kv->table ? (int64_t)kv->width * kv->page_size : kv->pages;
+  return bound > 0 && bound < keys ? bound : keys;
+}
+
+Plan plan_of(const vsk_ctx *ctx, const vsk_kv *kv, const vsk_attention_args *args,
+             const Span &span) {
   Plan p;
   const int64_t group = args->q.heads / kv->kv_heads;
-  const int64_t max_new = news->starts ? news->max_new : 1;
-  const int64_t rows = max_new * group, pairs = (int64_t)news->n * kv->kv_heads;
+  const int64_t max_new = span.max_new;
+  const int64_t rows = max_new * group, pairs = span.n * kv->kv_heads;
   p.splits = 1;
   p.chunk = 1 << 30;
   p.tile = false;
   p.share = 4;
   const int64_t cus = ctx->cu_count;
   int64_t row_tile = 16, key_tile = kv->dtype == VSK_DTYPE_F32 ? 16 : 32;
-  int64_t keys = kv->table ? (int64_t)kv->width * kv->page_size : kv->pages;
-  if (args->max_length > 0 && args->max_length < keys) keys = args->max_length;
+  int64_t keys = span.keys;
   // Row tiles of 128 where there are rows to fill them and work for the
   // device.  Under 64 rows of a key head most of a tile would be empty; with
   // few rows in all, and few products, tiles of 16 spread over more waves and
@@ -56,7 +72,7 @@ Plan plan_of(const vsk_ctx *ctx, const vsk_kv *kv, const vsk_new_tokens *news,
   // 4 heads of 128 on one 41 / 27; of 333, 32 heads of 128 on 8, 16 / 22; 64
   // new tokens of 8 heads of 64 after 4,000 keys 23 / 15, after 30,000 25 / 33;
   // of one head after 30,000 24 / 16.
-  int64_t seen = keys - (max_new < keys ? max_new : keys) / 2;
+  int64_t seen = span.all ? keys : keys - (max_new < keys ? max_new : keys) / 2;
   if (args->window > 0 && args->window + (int64_t)args->sinks < seen)
     seen = args->window + (int64_t)args->sinks;
   const int64_t unit = (kv->head_dim <= 64 ? 64 : 32) * cus;
@@ -81,7 +97,7 @@ Plan plan_of(const vsk_ctx *ctx, const vsk_kv *kv, const vsk_new_tokens *news,
     // of 1,000, 32 heads of 128 on 8, window 100 (16,000 row tiles) 160 / 263;
     // one of 4,000, 8 heads of 64, window 64 (2,000) 18 / 88; 8 f16 prompts of
     // 500, 10 heads of 100 (2,560) 357 / 297.
-    if (p.tiles >= 4 && (blocks >= 16 * cus || (blocks >= 4 * cus && keys <= 384) ||
+    if (!span.joined && p.tiles >= 4 && (blocks >= 16 * cus || (blocks >= 4 * cus && keys <= 384) ||
                          (blocks >= 2 * cus && keys <= 128))) {
       p.share = 1;
       return p;
@@ -130,10 +146,36 @@ Plan plan_of(const vsk_ctx *ctx, const vsk_kv *kv, const vsk_new_tokens *news,
   return p;
 }
 
-int64_t workspace_of(const Plan &p, const vsk_kv *kv, const vsk_new_tokens *news,
+// The plans of a call: its own, and before it one over the groups' prefixes.
+struct Plans {
+  Plan own, prefix;
+  int64_t group_tokens = 0;  // new tokens of a group at most; 0: no prefixes
+  int32_t parts() const { return own.splits + (group_tokens ? prefix.splits : 0); }
+};
+
+Plans plans_of(const vsk_ctx *ctx, const vsk_kv *kv, const vsk_new_tokens *news,
+               const vsk_attention_args *args, bool all, const vsk_shared_prefix *shared) {
+  Plans p;
+  const int64_t keys = most_keys(kv, args->max_length);
+  // (a window leaves little of a prefix: each sequence reads its own)
+  if (shared && shared->n_groups > 0 && shared->max_members > 1 && args->window <= 0) {
+    p.group_tokens = (int64_t)shared->max_members * most_new(news);
+    if (p.group_tokens > news->tokens) p.group_tokens = news->tokens;
+    const int64_t first = most_keys(kv, shared->max_prefix > 0 ? shared->max_prefix : keys);
+    p.prefix = plan_of(ctx, kv, args, Span{shared->n_groups, p.group_tokens, first, true, true});
+    const int64_t rest = shared->max_prefix > 0 && shared->max_prefix < keys
+                             ? keys - shared->max_prefix : keys;
+    p.own = plan_of(ctx, kv, args, Span{news->n, most_new(news), rest, false, true});
+  } else {
+    p.own = plan_of(ctx, kv, args, Span{news->n, most_new(news), keys, all, false});
+  }
+  return p;
+}
+
+int64_t workspace_of(const Plans &p, const vsk_kv *kv, const vsk_new_tokens *news,
                      const vsk_attention_args *args) {
-  if (p.splits == 1) return 0;
-  return (int64_t)sizeof(float) * p.splits * news->tokens * args->q.heads *
+  if (p.parts() == 1) return 0;
+  return (int64_t)sizeof(float) * p.parts() * news->tokens * args->q.heads *
          (padded_head(kv->head_dim) + 2);
 }
 
@@ -156,35 +198,31 @@ template <class P> bool aligned_to(const P *p, int64_t bytes) {
   return ((uintptr_t)p % bytes) == 0;
 }
 
-}  // namespace
+bool optional_device(const void *p) { return !p || is_device_ptr(p); }
 
-}  // namespace vsk
-
-using namespace vsk;
-
-extern "C" {
-
-int64_t vsk_attention_workspace(vsk_ctx *ctx, const vsk_kv *kv, const vsk_new_tokens *news,
-                                const vsk_attention_args *args) {
+// sets: cross attention to them; shared: the groups' prefixes
+int64_t workspace_call(vsk_ctx *ctx, const vsk_kv *kv, const vsk_new_tokens *news,
+                       const vsk_attention_args *args, bool all,
+                       const vsk_shared_prefix *shared) {
   if (!ctx) return 0;
   try {
     check_shapes(kv, news, args);
   } catch (...) {
-    return 0;  // (vsk_attention says why)
+    return 0;  // (the call itself says why)
   }
   // (no rows: nothing to divide)
   if (news->n == 0 || news->tokens == 0 || news->max_new == 0) return 0;
-  return workspace_of(plan_of(ctx, kv, news, args), kv, news, args);
+  return workspace_of(plans_of(ctx, kv, news, args, all, shared), kv, news, args);
 }
 
-vsk_status vsk_attention(vsk_ctx *ctx, void *stream, const vsk_kv *kv, int32_t layer,
-                         const vsk_new_tokens *news, const vsk_attention_args *args) {
-  QUEUED_API_BEGIN(ctx);
+void attend(vsk_ctx *ctx, void *stream, const vsk_kv *kv, int32_t layer,
+            const vsk_new_tokens *news, const vsk_attention_args *args, const vsk_key_sets *sets,
+            const vsk_shared_prefix *shared) {
   check_shapes(kv, news, args);
   VSK_REQUIRE(std::isfinite(args->scale) && args->scale > 0, VSK_ERR_INVALID_ARGUMENT,
               "scale must be positive and finite");
   check_news(news);
-  if (news->n == 0 || news->tokens == 0 || news->max_new == 0) return VSK_OK;
+  if (news->n == 0 || news->tokens == 0 || news->max_new == 0) return;
   const bool paged = kv->table != nullptr;
   if (paged) {
     check_kv(kv);
@@ -196,20 +234,43 @@ vsk_status vsk_attention(vsk_ctx *ctx, void *stream, const vsk_kv *kv, int32_t l
                 "dense keys have no pages or layers");
     // (positions a few thousand past a sequence's end are formed in 32 bits)
     VSK_REQUIRE(kv->pages <= (1 << 30), VSK_ERR_INVALID_BUFFER_SIZE, "at most 2^30 keys");
-    VSK_REQUIRE(args->k_starts && is_device_ptr(args->k_starts), VSK_ERR_INVALID_ARGUMENT,
-                "dense keys need k_starts in device memory");
+    VSK_REQUIRE(sets || (args->k_starts && is_device_ptr(args->k_starts)),
+                VSK_ERR_INVALID_ARGUMENT, "dense keys need k_starts in device memory");
     VSK_REQUIRE(kv->k_row >= 0 && kv->v_row >= 0 && kv->k_row <= (1 << 26) &&
                     kv->v_row <= (1 << 26),
                 VSK_ERR_INVALID_BUFFER_SIZE, "a row stride of more than 2^26 elements");
     VSK_REQUIRE(kv->k && kv->v && is_device_ptr(kv->k) && is_device_ptr(kv->v),
                 VSK_ERR_INVALID_ARGUMENT, "keys and values must be device memory");
   }
+  if (sets) {
+    VSK_REQUIRE(!paged && args->window == 0 && args->sinks == 0, VSK_ERR_UNSUPPORTED,
+                "cross attention is to dense keys, without a window");
+    VSK_REQUIRE(sets->n >= 1 && sets->set_rows >= 0, VSK_ERR_INVALID_ARGUMENT,
+                "no sets of keys");
+    VSK_REQUIRE(news->seqs || news->n <= sets->n, VSK_ERR_INVALID_ARGUMENT,
+                "more sequences than sets of keys");
+    VSK_REQUIRE(optional_device(sets->starts) && optional_device(sets->lengths),
+                VSK_ERR_INVALID_ARGUMENT, "offsets and lengths must be device memory");
+  }
+  if (shared) {
+    VSK_REQUIRE(paged, VSK_ERR_UNSUPPORTED, "only pages are shared");
+    VSK_REQUIRE(shared->n_groups >= 0 && shared->max_members >= 0 && shared->max_prefix >= 0,
+                VSK_ERR_INVALID_ARGUMENT, "negative counts");
+    VSK_REQUIRE(news->n <= shared->n, VSK_ERR_DIMENSION_MISMATCH,
+                "more sequences than the prefixes are known of");
+    VSK_REQUIRE(shared->n_groups == 0 ||
+                    (shared->groups && shared->prefix && is_device_ptr(shared->groups) &&
+                     is_device_ptr(shared->prefix)),
+                VSK_ERR_INVALID_ARGUMENT, "groups and prefixes must be device memory");
+  }
   VSK_REQUIRE(news->starts || news->tokens >= news->n, VSK_ERR_DIMENSION_MISMATCH,
               "fewer rows than sequences");
   VSK_REQUIRE(args->q.src && args->q.dst && is_device_ptr(args->q.src) &&
-                  is_device_ptr(args->q.dst) && (!args->lse || is_device_ptr(args->lse)),
+                  is_device_ptr(args->q.dst) && optional_device(args->lse),
               VSK_ERR_INVALID_ARGUMENT, "queries and outputs must be device memory");
-  const Plan p = plan_of(ctx, kv, news, args);
+  const Plans p = plans_of(ctx, kv, news, args, sets != nullptr, shared);
+  VSK_REQUIRE(p.group_tokens * args->q.heads <= 0x3FFFFFFFll, VSK_ERR_INVALID_BUFFER_SIZE,
+              "too many query rows in one group");
   const int64_t need = workspace_of(p, kv, news, args);
   VSK_REQUIRE(need == 0 || (args->workspace && args->workspace_bytes >= need &&
                             aligned_to(args->workspace, 16) && is_device_ptr(args->workspace)),
@@ -232,6 +293,11 @@ vsk_status vsk_attention(vsk_ctx *ctx, void *stream, const vsk_kv *kv, int32_t l
     a.table = kv->table, a.lengths = kv->lengths, a.table_stride = kv->table_stride;
     a.pages = kv->pages, a.slots = kv->slots, a.width = kv->width;
     a.page_shift = __builtin_ctz((unsigned)kv->page_size);
+  } else if (sets) {
+    a.cross = 1;
+    a.k_starts = sets->starts, a.k_lengths = sets->lengths;
+    a.sets = sets->n, a.set_rows = sets->set_rows;
+    a.k_rows = kv->pages;
   } else {
     a.k_starts = args->k_starts;
     a.k_rows = kv->pages;
@@ -244,21 +310,87 @@ vsk_status vsk_attention(vsk_ctx *ctx, void *stream, const vsk_kv *kv, int32_t l
   a.d = kv->head_dim;
   a.window = args->window;
   a.sinks = args->sinks;
-  a.max_new = news->starts ? news->max_new : 1;
-  a.tiles = p.tiles, a.splits = p.splits, a.chunk = p.chunk;
+  a.max_new = (int32_t)most_new(news);
   a.scale_log2 = args->scale * 1.4426950408889634f;
   if (need) {
     a.part_o = static_cast<float *>(args->workspace);
-    a.part_ml = a.part_o + (int64_t)p.splits * a.tokens * a.heads * padded_head(a.d);
+    a.part_ml = a.part_o + (int64_t)p.parts() * a.tokens * a.heads * padded_head(a.d);
   }
   const bool al = aligned_operands(kv, args);
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (p.tile)
-    launch_attn_tile(ctx, st, a, kv->dtype);
-  else
-    launch_attn_rows(ctx, st, a, kv->dtype, al, p.share);
-  launch_attn_join(ctx, st, a, kv->dtype, al, p.tile ? ATTN_TILE_ROWS : 16);
+  const AttnForm form = sets || p.group_tokens ? ATTN_FORMS : ATTN_OWN;
+  auto launch = [&](const Plan &plan, AttnArgs x) {
+    x.tiles = plan.tiles, x.splits = plan.splits, x.chunk = plan.chunk;
+    if (plan.tile)
+      launch_attn_tile(ctx, st, x, kv->dtype, form);
+    else if (form == ATTN_OWN)
+      launch_attn_rows(ctx, st, x, kv->dtype, al, plan.share);
+    else
+      launch_attn_rows_forms(ctx, st, x, kv->dtype, al, plan.share);
+  };
+  if (p.group_tokens) {
+    a.prefix = shared->prefix;
+    a.joined = 1;
+    AttnArgs g = a;
+    g.groups = shared->groups;
+    g.members = a.n;
+    g.n = shared->n_groups;
+    g.max_new = (int32_t)p.group_tokens;
+    launch(p.prefix, g);
+    a.part0 = p.prefix.splits;
+  }
+  launch(p.own, a);
+  a.splits = p.parts(), a.chunk = p.own.chunk;
+  launch_attn_join(ctx, st, a, kv->dtype, al, p.own.tile ? ATTN_TILE_ROWS : 16, form);
   finish_queued(ctx, st);
+}
+
+}  // namespace
+
+}  // namespace vsk
+
+using namespace vsk;
+
+extern "C" {
+
+int64_t vsk_attention_workspace(vsk_ctx *ctx, const vsk_kv *kv, const vsk_new_tokens *news,
+                                const vsk_attention_args *args) {
+  return workspace_call(ctx, kv, news, args, false, nullptr);
+}
+
+vsk_status vsk_attention(vsk_ctx *ctx, void *stream, const vsk_kv *kv, int32_t layer,
+                         const vsk_new_tokens *news, const vsk_attention_args *args) {
+  QUEUED_API_BEGIN(ctx);
+  attend(ctx, stream, kv, layer, news, args, nullptr, nullptr);
+  VSK_API_END(ctx);
+}
+
+int64_t vsk_cross_attention_workspace(vsk_ctx *ctx, const vsk_kv *kv, const vsk_new_tokens *news,
+                                      const vsk_attention_args *args) {
+  return workspace_call(ctx, kv, news, args, true, nullptr);
+}
+
+vsk_status vsk_cross_attention(vsk_ctx *ctx, void *stream, const vsk_kv *kv,
+                               const vsk_new_tokens *news, const vsk_attention_args *args,
+                               const vsk_key_sets *sets) {
+  QUEUED_API_BEGIN(ctx);
+  VSK_REQUIRE(sets, VSK_ERR_INVALID_ARGUMENT, "null argument");
+  attend(ctx, stream, kv, 0, news, args, sets, nullptr);
+  VSK_API_END(ctx);
+}
+
+int64_t vsk_attention_shared_workspace(vsk_ctx *ctx, const vsk_kv *kv, const vsk_new_tokens *news,
+                                       const vsk_attention_args *args,
+                                       const vsk_shared_prefix *shared) {
+  return workspace_call(ctx, kv, news, args, false, shared);
+}
+
+vsk_status vsk_attention_shared(vsk_ctx *ctx, void *stream, const vsk_kv *kv, int32_t layer,
+                                const vsk_new_tokens *news, const vsk_attention_args *args,
+                                const vsk_shared_prefix *shared) {
+  QUEUED_API_BEGIN(ctx);
+  VSK_REQUIRE(shared, VSK_ERR_INVALID_ARGUMENT, "null argument");
+  attend(ctx, stream, kv, layer, news, args, nullptr, shared);
   VSK_API_END(ctx);
 }
 

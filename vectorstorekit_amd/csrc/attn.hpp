@@ -7,6 +7,11 @@
 // j < sinks).  The query heads of one key head are packed into rows, row =
 // token * group + head within the group, so that keys and values are read
 // once for all of them.
+//
+// Cross attention: every new token stands at the last key and sees them all.
+// A shared prefix is two such calls whose sums are joined: the new tokens of a
+// group of sequences, as if of one, over the keys that they share, and each
+// sequence over its keys from there on.
 #pragma once
 
 #include "device_scope.hpp"
@@ -27,6 +32,11 @@ typedef __attribute__((ext_vector_type(4))) float f32x4;
 typedef __attribute__((ext_vector_type(16))) float f32x16;
 typedef __attribute__((ext_vector_type(4))) uint32_t u32x4;
 
+// Kernels of the plain form (a sequence's own keys, causal) and of the others,
+// whose arguments say which.  Apart at compile time: what a block asks of its
+// arguments before its first key costs one short context (11.1 us) 0.5 us.
+enum AttnForm { ATTN_OWN, ATTN_FORMS };
+
 // The operands of a call, by value to every kernel.  Strides in elements.
 struct AttnArgs {
   const void *q, *k, *v;
@@ -37,14 +47,24 @@ struct AttnArgs {
   const int32_t *table;    // slots x width page ids; null: dense rows
   const int32_t *lengths;  // per slot (paged)
   const int32_t *starts;   // n + 1 offsets of the sequences' tokens, or null: one each
+  const int32_t *seqs;     // slot (cross: set of keys) of each sequence, or null
+  const int32_t *prefix;   // per sequence: keys that its group shares, or null
+  const int32_t *groups;   // n + 1 offsets of the groups' sequences: a call over prefixes
   const int32_t *k_starts; // n + 1 offsets of the sequences' keys (dense)
-  const int32_t *seqs;     // slot of each sequence, or null
+  const int32_t *k_lengths;  // (cross, no k_starts) keys of each set, or null: all its rows
   int64_t table_stride;
   int64_t tokens, k_rows;
   int32_t n, heads, kv_heads, group, d;
   int32_t pages, page_shift, slots, width;
   int32_t window, sinks;  // window <= 0: none
   int32_t max_new;
+  // ATTN_FORMS
+  int32_t cross;        // every token sees every key
+  int32_t sets;         // sets of keys (cross)
+  int64_t set_rows;     // rows from a set to the next where there are no k_starts
+  int32_t members;      // sequences that the groups' offsets may name
+  int32_t joined;       // parts are written also where there is one, absent ones marked
+  int32_t part0;        // the call's first part
   int32_t tiles;        // row tiles of a sequence's max_new tokens
   int32_t splits;       // parts a tile's keys may be split into
   int32_t chunk;        // key tiles of a part
@@ -53,45 +73,106 @@ struct AttnArgs {
   float *part_ml;       // splits x tokens x heads x 2: reference (a score), sum
 };
 
-// One sequence of the call.
+// One sequence of the call (or one group of them, over its prefix).
 struct AttnSeq {
   int64_t token0, key0;  // its first row in q; its first dense key
-  int32_t slot, T, L;    // new tokens, keys
+  int64_t row;           // its first entry of the table
+  int32_t T, L;          // new tokens, keys
+  int32_t p0, each;      // token t stands at p0 + (t & each)
+  int32_t first, end;    // (a group) its sequences
 };
 
-__device__ inline AttnSeq attn_seq(const AttnArgs &a, int32_t b) {
+__device__ inline int32_t attn_length(const AttnArgs &a, int32_t slot) {
+  const int64_t most = (int64_t)a.width << a.page_shift;
+  const int32_t l = a.lengths[slot];
+  return l < 0 ? 0 : l > most ? (int32_t)most : l;
+}
+
+// Every index below is taken from device memory, so each is held to its
+// buffer here: a slot, length or offset out of range reads no foreign memory.
+template <AttnForm F> __device__ inline AttnSeq attn_seq(const AttnArgs &a, int32_t b) {
   AttnSeq s;
-  s.slot = a.seqs ? a.seqs[b] : b;
+  s.first = b, s.end = b + 1;
+  if (F && a.groups) {
+    s.first = a.groups[b], s.end = a.groups[b + 1];
+    s.first = s.first < 0 ? 0 : s.first > a.members ? a.members : s.first;
+    s.end = s.end < s.first ? s.first : s.end > a.members ? a.members : s.end;
+    b = s.first < a.members ? s.first : 0;  // (whose keys; of an empty group none are read)
+  }
   if (a.starts) {
-    int32_t t0 = a.starts[b], t1 = a.starts[b + 1];
+    int32_t t0 = a.starts[s.first], t1 = a.starts[s.end];
     t0 = t0 < 0 ? 0 : t0;
     if (t1 > a.tokens) t1 = (int32_t)a.tokens;
     s.token0 = t0;
     s.T = t1 > t0 ? t1 - t0 : 0;
   } else {
-    s.token0 = b;
-    s.T = 1;
+    s.token0 = s.first;
+    s.T = s.end - s.first;
   }
+  const int32_t slot = a.seqs ? a.seqs[b] : b;
   s.key0 = 0;
-  // every index below is taken from device memory, so each is held to its
-  // buffer here: a slot, length or offset out of range reads no foreign memory
+  s.row = 0;
+  s.L = 0;
   if (a.table) {
-    if ((uint32_t)s.slot >= (uint32_t)a.slots) {
-      s.slot = 0;
-      s.L = 0;
-    } else {
-      const int64_t most = (int64_t)a.width << a.page_shift;
-      const int32_t l = a.lengths[s.slot];
-      s.L = l < 0 ? 0 : l > most ? (int32_t)most : l;
+    if ((uint32_t)slot < (uint32_t)a.slots) {
+      s.row = slot * a.table_stride;
+      s.L = attn_length(a, slot);
+      if (F && a.prefix) {
+        // whole pages: the keys that a group shares, or a sequence's others
+        int32_t pages = a.prefix[b] >> a.page_shift;
+        pages = pages < 0 ? 0 : pages > a.width ? a.width : pages;
+        const int32_t keys = pages << a.page_shift;
+        if (a.groups) {
+          s.L = s.L < keys ? s.L : keys;
+        } else {
+          s.row += pages;
+          s.L = s.L > keys ? s.L - keys : 0;
+        }
+      }
     }
-  } else {
-    int64_t k0 = a.k_starts[b], k1 = a.k_starts[b + 1];
-    k0 = k0 < 0 ? 0 : k0;
-    if (k1 > a.k_rows) k1 = a.k_rows;
-    s.key0 = k0;
-    s.L = k1 > k0 ? (int32_t)(k1 - k0) : 0;
+  } else if (!F || a.k_starts) {
+    const int32_t set = F ? slot : b;
+    if (!F || (uint32_t)set < (uint32_t)a.sets) {
+      int64_t k0 = a.k_starts[set], k1 = a.k_starts[set + 1];
+      k0 = k0 < 0 ? 0 : k0;
+      if (k1 > a.k_rows) k1 = a.k_rows;
+      s.key0 = k0;
+      s.L = k1 > k0 ? (int32_t)(k1 - k0) : 0;
+    }
+  } else if ((uint32_t)slot < (uint32_t)a.sets) {
+    s.key0 = slot * a.set_rows;
+    const int32_t l = a.k_lengths ? a.k_lengths[slot] : (int32_t)a.k_rows;
+    s.L = l < 0 ? 0 : l > a.k_rows ? (int32_t)a.k_rows : l;
   }
+  s.p0 = F && a.cross ? s.L - 1 : s.L - s.T;
+  s.each = F && a.cross ? 0 : -1;
   return s;
+}
+
+// Position of the sequence's new token t among its keys.  Of a group's, it is
+// the position in the token's own sequence, found among the group's, or the
+// prefix's last.
+template <AttnForm F>
+__device__ inline int32_t attn_position(const AttnArgs &a, const AttnSeq &s, int32_t t) {
+  if (!F || !a.groups) return s.p0 + (t & s.each);
+  int32_t b = s.first + t, at = 0, count = 1;
+  if (a.starts) {
+    const int32_t token = (int32_t)s.token0 + t;
+    b = s.first;
+    for (int32_t end = s.end; end - b > 1;) {
+      const int32_t mid = b + (end - b) / 2;
+      if (a.starts[mid] <= token)
+        b = mid;
+      else
+        end = mid;
+    }
+    at = token - a.starts[b];
+    count = a.starts[b + 1] - a.starts[b];
+  }
+  const int32_t slot = a.seqs ? a.seqs[b] : b;
+  if ((uint32_t)slot >= (uint32_t)a.slots) return -1;
+  const int64_t pos = (int64_t)attn_length(a, slot) - count + at;
+  return pos >= s.L ? s.L - 1 : pos < -1 ? -1 : (int32_t)pos;
 }
 
 // The keys that query positions q0 .. q1 see between them, in groups of G keys
@@ -133,6 +214,15 @@ __device__ inline int32_t attn_parts(const AttnArgs &a, int32_t tiles) {
   return p < 1 ? 1 : p > a.splits ? a.splits : p;
 }
 
+// A part that is not there, of query row r of key head h: the sums of no keys.
+__device__ inline void attn_empty_part(const AttnArgs &a, const AttnSeq &s, int32_t h, int32_t r,
+                                       int32_t part) {
+  const int64_t row = (s.token0 + r / a.group) * a.heads + h * a.group + r % a.group;
+  const int64_t x = (int64_t)(a.part0 + part) * a.tokens * a.heads + row;
+  a.part_ml[2 * x] = -INFINITY;
+  a.part_ml[2 * x + 1] = 0.f;
+}
+
 __device__ inline bool attn_sees(const AttnArgs &a, int32_t pos, int32_t j) {
   return j <= pos && (a.window <= 0 || pos - j < a.window || j < a.sinks);
 }
@@ -156,7 +246,7 @@ __device__ inline int32_t attn_page(const AttnArgs &a, const AttnSeq &s, int32_t
   if (!a.table) return 0;
   int32_t i = attn_row16(s, j16) >> a.page_shift;
   asm volatile("" : "+v"(i));
-  return a.table[s.slot * a.table_stride + i];
+  return a.table[s.row + i];
 }
 __device__ inline AttnRows attn_rows(const AttnArgs &a, const AttnSeq &s, int32_t h, int32_t j16,
                                      int32_t page) {
@@ -258,15 +348,19 @@ void finish_queued(vsk_ctx *ctx, hipStream_t stream);
 // to 64), 4, or 1
 void launch_attn_rows(vsk_ctx *ctx, hipStream_t stream, const AttnArgs &a, int32_t t,
                       bool aligned, int32_t share);
+// attn_forms.hip: the same of ATTN_FORMS
+void launch_attn_rows_forms(vsk_ctx *ctx, hipStream_t stream, const AttnArgs &a, int32_t t,
+                            bool aligned, int32_t share);
 // keys of a tile of attn_tile.hip, by the (padded) head
 constexpr int attn_tile_keys(int d) { return d > 128 ? 32 : 64; }
 // attn_tile.hip: 16-bit types, aligned, row tiles of ATTN_TILE_ROWS
 constexpr int ATTN_TILE_ROWS = 128;
 constexpr int ATTN_TILE_GROUP = 16;  // keys that lie together in a tile
-void launch_attn_tile(vsk_ctx *ctx, hipStream_t stream, const AttnArgs &a, int32_t t);
+void launch_attn_tile(vsk_ctx *ctx, hipStream_t stream, const AttnArgs &a, int32_t t,
+                      AttnForm form);
 // joins the parts that row tiles of `rows` rows left: 16 (launch_attn_rows) or
 // ATTN_TILE_ROWS
 void launch_attn_join(vsk_ctx *ctx, hipStream_t stream, const AttnArgs &a, int32_t t,
-                      bool aligned, int32_t rows);
+                      bool aligned, int32_t rows, AttnForm form);
 
 }  // namespace vsk

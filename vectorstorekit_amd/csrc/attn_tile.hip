@@ -79,7 +79,7 @@ __device__ inline float max3(float a, float b, float c) {
 // compute unit, so that one's start and end hide behind the other's products
 // (one of eight waves over twice the rows: 340 us where these take 308, 8
 // ragged prompts to 4,096 of 32 heads of 128, window 1,024).
-template <class T, int DP>
+template <class T, int DP, AttnForm F>
 __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void k_attn_tile(const AttnArgs a) {
   typedef typename Mm<T>::V8 V8;
   typedef __attribute__((ext_vector_type(4))) T V4;
@@ -108,31 +108,55 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void k_attn_tile(const 
   const int32_t tile = a.tiles - 1 - (int32_t)(at % a.tiles);
   at /= a.tiles;
   const int32_t part = at % a.splits;
-  const AttnSeq s = attn_seq(a, at / a.splits);
+  const AttnSeq s = attn_seq<F>(a, at / a.splits);
   const int32_t row0 = tile * ROWS;
   const int32_t T_used = s.T < a.max_new ? s.T : a.max_new;
   const int32_t rows_all = T_used * a.group;
   if (row0 >= rows_all) return;
   const int32_t last = row0 + ROWS < rows_all ? row0 + ROWS - 1 : rows_all - 1;
-  const int32_t p0 = s.L - s.T;
-  const auto span = attn_span<KT, G>(a, p0 + row0 / a.group, p0 + last / a.group);
+  // this lane's row, and the positions between which the block's and this
+  // wave's rows stand
+  const int32_t w0 = row0 + 32 * w, w1 = w0 + 31 < last ? w0 + 31 : last;
+  const bool have = w0 <= last;
+  const int32_t my_row = w0 + n, my_t = my_row / a.group;
+  const int32_t my_head = h * a.group + my_row - my_t * a.group;
+  const bool real = my_row <= last;
+  int32_t b_lo = s.p0 + (row0 / a.group & s.each), b_hi = s.p0 + (last / a.group & s.each);
+  int32_t q_lo = s.p0 + (w0 / a.group & s.each), q_hi = have ? s.p0 + (w1 / a.group & s.each) : -1;
+  int32_t pos = real ? s.p0 + (my_t & s.each) : -1;
+  if (F && a.groups) {
+    // rows of several sequences (through the keys' LDS: with any more of its
+    // own, two workgroups would not fit a compute unit)
+    int32_t(*ends)[NW] = reinterpret_cast<int32_t(*)[NW]>(keys_lds);
+    pos = real ? attn_position<F>(a, s, my_t) : -1;
+    q_lo = real ? pos : 0x7FFFFFFF, q_hi = pos;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      q_lo = min(q_lo, __shfl_xor(q_lo, o));
+      q_hi = max(q_hi, __shfl_xor(q_hi, o));
+    }
+    if (lane == 0) ends[0][w] = q_lo, ends[1][w] = q_hi;
+    __syncthreads();
+    b_lo = ends[0][0], b_hi = ends[1][0];
+#pragma unroll
+    for (int i = 1; i < NW; ++i) b_lo = min(b_lo, ends[0][i]), b_hi = max(b_hi, ends[1][i]);
+    __syncthreads();
+    q_lo = __builtin_amdgcn_readfirstlane(q_lo), q_hi = __builtin_amdgcn_readfirstlane(q_hi);
+    b_lo = __builtin_amdgcn_readfirstlane(b_lo), b_hi = __builtin_amdgcn_readfirstlane(b_hi);
+  }
+  const auto span = attn_span<KT, G>(a, b_lo, b_hi);
   const int32_t parts = attn_parts(a, span.tiles);
-  if (part >= parts) return;
+  if (part >= parts) {
+    if (F && a.joined && real && h2 == 0) attn_empty_part(a, s, h, my_row, part);
+    return;
+  }
   const int32_t first = part * a.chunk;
   const int32_t end = part == parts - 1 ? span.tiles : first + a.chunk;
 
-  // this wave's rows and what they see
-  const int32_t w0 = row0 + 32 * w, w1 = w0 + 31 < last ? w0 + 31 : last;
-  const bool have = w0 <= last;
-  const int32_t q_lo = p0 + w0 / a.group, q_hi = have ? p0 + w1 / a.group : -1;
   // (a head of 256 leaves no registers for the queries: each lane's wait in LDS)
   constexpr bool QLDS = DP == 256;
   __shared__ __attribute__((aligned(1024))) char queries_lds[QLDS ? NW * KS * 1024 : 16];
   lds_char *const qbuf = (lds_char *)queries_lds + 16 * lane;
-  const int32_t my_row = w0 + n, my_t = my_row / a.group;
-  const int32_t my_head = h * a.group + my_row - my_t * a.group;
-  const bool real = my_row <= last;
-  const int32_t pos = real ? p0 + my_t : -1;
   V8 q[QLDS ? 1 : KS];
   auto query = [&](int x) -> V8 {
     if constexpr (QLDS) return *(const lds_as V8 *)(qbuf + (w * KS + x) * 1024);
@@ -179,7 +203,7 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void k_attn_tile(const 
     const int32_t j = attn_row16(s, span.group(KT / G * (i + lane) + MINE * w / G));
     int64_t page = 0, in = s.key0 + j;
     if (a.table) {
-      int32_t x = a.table[s.slot * a.table_stride + (j >> a.page_shift)];
+      int32_t x = a.table[s.row + (j >> a.page_shift)];
       page = x < 0 ? 0 : x >= a.pages ? a.pages - 1 : x;
       in = j & ((1 << a.page_shift) - 1);
     }
@@ -389,7 +413,7 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void k_attn_tile(const 
   // of the last row to the first row's diagonal
   int32_t hot0 = first, hot1 = first;
   {
-    const int32_t lo = p0 + row0 / a.group, hi = p0 + last / a.group;
+    const int32_t lo = b_lo, hi = b_hi;
     int32_t x0 = G * span.sink_groups;
     const int32_t x1 = lo + 1 > span.lo ? (x0 + lo + 1 - span.lo) / KT : 0;
     if (a.window > 0 && hi - span.lo >= a.window) x0 += hi - a.window - span.lo + 1;
@@ -553,7 +577,7 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void k_attn_tile(const 
     m = ref * a.scale_log2;
   }
   const int64_t out_row = (s.token0 + my_t) * a.heads + my_head;
-  if (parts > 1) {
+  if (parts > 1 || (F && a.joined)) {
     if (!real) return;
     // a part's reference is a score: the one that m was made of, or near it
     if (!by_key && m != -INFINITY) {
@@ -563,7 +587,7 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void k_attn_tile(const 
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) acc[dt] *= f;
     }
-    const int64_t x = (int64_t)part * a.tokens * a.heads + out_row;
+    const int64_t x = (int64_t)(F ? a.part0 + part : part) * a.tokens * a.heads + out_row;
     float *dst = a.part_o + x * PITCH;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
@@ -604,27 +628,29 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void k_attn_tile(const 
     a.lse[out_row] = attn_lse(m, sum);
 }
 
-template <class T> void tile_of(hipStream_t st, const AttnArgs &a, unsigned g) {
+template <class T, AttnForm F> void tile_of(hipStream_t st, const AttnArgs &a, unsigned g) {
   if (a.d <= 64)
-    k_attn_tile<T, 64><<<g, 64 * NW, 0, st>>>(a);
+    k_attn_tile<T, 64, F><<<g, 64 * NW, 0, st>>>(a);
   else if (a.d <= 96)
-    k_attn_tile<T, 96><<<g, 64 * NW, 0, st>>>(a);
+    k_attn_tile<T, 96, F><<<g, 64 * NW, 0, st>>>(a);
   else if (a.d <= 128)
-    k_attn_tile<T, 128><<<g, 64 * NW, 0, st>>>(a);
+    k_attn_tile<T, 128, F><<<g, 64 * NW, 0, st>>>(a);
   else
-    k_attn_tile<T, 256><<<g, 64 * NW, 0, st>>>(a);
+    k_attn_tile<T, 256, F><<<g, 64 * NW, 0, st>>>(a);
 }
 
 }  // namespace
 
-void launch_attn_tile(vsk_ctx *ctx, hipStream_t st, const AttnArgs &a, int32_t t) {
+void launch_attn_tile(vsk_ctx *ctx, hipStream_t st, const AttnArgs &a, int32_t t, AttnForm form) {
   const int64_t grid = (int64_t)a.n * a.splits * a.tiles * a.kv_heads;
   VSK_REQUIRE(grid <= 0x7FFFFFFFll, VSK_ERR_INVALID_BUFFER_SIZE, "too many query rows in one call");
   KernelTimer kt(ctx, "attn_tile", (double)a.tokens * a.heads, st);
-  if (t == VSK_DTYPE_F16)
-    tile_of<_Float16>(st, a, (unsigned)grid);
+  const unsigned g = (unsigned)grid;
+  if (form == ATTN_OWN)
+    t == VSK_DTYPE_F16 ? tile_of<_Float16, ATTN_OWN>(st, a, g) : tile_of<__bf16, ATTN_OWN>(st, a, g);
   else
-    tile_of<__bf16>(st, a, (unsigned)grid);
+    t == VSK_DTYPE_F16 ? tile_of<_Float16, ATTN_FORMS>(st, a, g)
+                       : tile_of<__bf16, ATTN_FORMS>(st, a, g);
   check_launch("attn_tile");
 }
 

@@ -482,6 +482,59 @@ void launch_move(vsk_ctx *ctx, hipStream_t st, const vsk_kv *kv, const Pool &p, 
   check_launch("kv_move");
 }
 
+// A workgroup a group: the first page in which a member differs from the first
+// member ends the prefix.  Members' tables are read 256 pages at a time; the
+// end found so far bounds what is read of the others (64 branches of 32,768
+// tokens in pages of 64: 9 us).
+__global__ __launch_bounds__(256) void k_kv_share(const int32_t *table, const int32_t *lengths,
+                                                  int64_t stride, int32_t slots, int32_t width,
+                                                  int32_t shift, const int32_t *seqs,
+                                                  const int32_t *groups, int32_t n_groups,
+                                                  int32_t n, int32_t *prefix) {
+  __shared__ int32_t pages;
+  auto offset = [&](int32_t g) -> int32_t {
+    const int32_t x = groups[g];
+    return x < 0 ? 0 : x > n ? n : x;
+  };
+  const int32_t g = blockIdx.x;
+  const int32_t first = offset(g), end = offset(g + 1);
+  // (sequences before the first group and behind the last are in none)
+  if (g == 0)
+    for (int32_t b = threadIdx.x; b < first; b += 256) prefix[b] = 0;
+  if (g == n_groups - 1)
+    for (int32_t b = (end > first ? end : first) + threadIdx.x; b < n; b += 256) prefix[b] = 0;
+  if (end <= first) return;
+  auto slot_of = [&](int32_t b) -> int32_t { return seqs ? seqs[b] : b; };
+  if (threadIdx.x == 0) pages = end - first > 1 ? width : 0;
+  __syncthreads();
+  const int32_t head = slot_of(first);
+  for (int32_t b = first + threadIdx.x; b < end; b += 256) {
+    const int32_t slot = slot_of(b);
+    int32_t whole = 0;
+    if ((uint32_t)slot < (uint32_t)slots && (uint32_t)head < (uint32_t)slots) {
+      const int32_t l = lengths[slot];
+      whole = l < 0 ? 0 : l >> shift;
+    }
+    if (whole < width) atomicMin(&pages, whole);
+  }
+  __syncthreads();
+  int32_t most = pages;
+  for (int32_t b = first + 1; b < end && most > 0; ++b) {
+    const int32_t *x = table + head * stride, *y = table + slot_of(b) * stride;
+    int32_t at = most;
+    for (int32_t i = threadIdx.x; i < most; i += 256)
+      if (x[i] != y[i] || x[i] < 0) {
+        at = i;
+        break;
+      }
+    if (at < most) atomicMin(&pages, at);
+    __syncthreads();
+    most = pages;
+    __syncthreads();
+  }
+  for (int32_t b = first + threadIdx.x; b < end; b += 256) prefix[b] = most << shift;
+}
+
 void check_list(const int32_t *x, int32_t n) {
   VSK_REQUIRE(n >= 0, VSK_ERR_INVALID_ARGUMENT, "negative counts");
   VSK_REQUIRE(n == 0 || (x && is_device_ptr(x)), VSK_ERR_INVALID_ARGUMENT,
@@ -581,6 +634,34 @@ vsk_status vsk_kv_compact(vsk_ctx *ctx, void *stream, const vsk_kv *kv) {
   m.src = p.scratch + p.pages;
   m.count = p.status + 2;
   launch_move(ctx, st, kv, p, m, p.pages / 2, p.scratch + 2 * (int64_t)p.pages);
+  finish_queued(ctx, st);
+  VSK_API_END(ctx);
+}
+
+vsk_status vsk_kv_share(vsk_ctx *ctx, void *stream, const vsk_kv *kv, const int32_t *seqs,
+                        const vsk_shared_prefix *shared) {
+  QUEUED_API_BEGIN(ctx);
+  VSK_REQUIRE(kv && shared, VSK_ERR_INVALID_ARGUMENT, "null argument");
+  check_kv(kv);
+  VSK_REQUIRE(shared->n_groups >= 0 && shared->n >= 0, VSK_ERR_INVALID_ARGUMENT,
+              "negative counts");
+  VSK_REQUIRE(shared->n_groups <= (1 << 30) && shared->n <= (1 << 30),
+              VSK_ERR_INVALID_BUFFER_SIZE, "at most 2^30 sequences and groups");
+  VSK_REQUIRE(seqs || shared->n <= kv->slots, VSK_ERR_INVALID_ARGUMENT,
+              "more sequences than the cache has slots");
+  if (shared->n_groups == 0 || shared->n == 0) return VSK_OK;
+  VSK_REQUIRE(shared->groups && shared->prefix && is_device_ptr(shared->groups) &&
+                  is_device_ptr(shared->prefix) && (!seqs || is_device_ptr(seqs)),
+              VSK_ERR_INVALID_ARGUMENT, "groups, prefixes and slots must be device memory");
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  {
+    KernelTimer kt(ctx, "kv_share", shared->n, st);
+    k_kv_share<<<(unsigned)shared->n_groups, 256, 0, st>>>(
+        kv->table, kv->lengths, kv->table_stride, kv->slots, kv->width,
+        __builtin_ctz((unsigned)kv->page_size), seqs, shared->groups, shared->n_groups, shared->n,
+        shared->prefix);
+    check_launch("kv_share");
+  }
   finish_queued(ctx, st);
   VSK_API_END(ctx);
 }

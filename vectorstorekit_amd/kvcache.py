@@ -5,9 +5,12 @@ answers over retrieved vectors calls next to the search.
   the head, scaled for longer contexts);
 * ``PagedKVCache`` -- pages of keys and values resident in HBM, their tables
   and reference counts; ``append``, ``attend``, ``reserve``, ``fork``,
-  ``free``, ``compact``, ``copy_pages``;
+  ``free``, ``compact``, ``copy_pages``; ``share`` finds the prefixes that
+  branches share, which ``attend`` then reads once for all of them;
 * ``window_attention`` -- causal attention over keys and values as the
-  projections left them, through a sliding window with sinks.
+  projections left them, through a sliding window with sinks;
+* ``cross_attention`` -- attention to keys and values of another length, an
+  encoder's states of the documents found.
 
 Tensors are torch tensors on the context's GPU.  Unlike the search calls,
 these are queued on torch's current stream and do not wait: a decoder makes
@@ -38,12 +41,14 @@ _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 
 # The call's structures as bytes: a decoder makes these calls dozens of times a
 # token, and setting a ctypes structure's fields takes several times as long.
-# Layouts: vsk_kv, vsk_head_rows, vsk_new_tokens and vsk_attention_args of
-# vsk_hip.h.
+# Layouts: vsk_kv, vsk_head_rows, vsk_new_tokens, vsk_attention_args and
+# vsk_key_sets of vsk_hip.h.
 _KV = struct.Struct("@QQqqqqqqqqQQQQQqiiiiiiii")
 _ROWS = struct.Struct("@QQqqqqixxxx")
 _NEWS = struct.Struct("@QQiiq")
 _ATTEND = struct.Struct("@QQqqqqixxxxQQQqfiii")
+_SETS = struct.Struct("@QQqixxxx")
+assert _SETS.size == ctypes.sizeof(_lib.vsk_key_sets)
 assert _ATTEND.size == ctypes.sizeof(_lib.vsk_attention_args)
 assert _KV.size == ctypes.sizeof(_lib.vsk_kv)
 assert _ROWS.size == ctypes.sizeof(_lib.vsk_head_rows)
@@ -255,8 +260,10 @@ class RotaryEmbedding:
         return n
 
 
-def _attend(ctx, kv, layer, q, news, k_starts, scale, window, sinks, max_length, return_lse):
-    """The checked call of vsk_attention."""
+def _attend(ctx, kv, layer, q, news, k_starts, scale, window, sinks, max_length, return_lse,
+            sets=None, shared=None):
+    """The checked call of vsk_attention (``sets``: vsk_cross_attention,
+    ``shared``: vsk_attention_shared)."""
     if window is not None and window < 1:
         raise VSKError(-2, "window must be at least 1 (None: no window)")
     if sinks < 0:
@@ -276,11 +283,22 @@ def _attend(ctx, kv, layer, q, news, k_starts, scale, window, sinks, max_length,
                          scale, window, sinks, max_length)
         if need:
             break
-        need = lib.vsk_attention_workspace(handle, kv, news, a)
+        if sets is not None:
+            need = lib.vsk_cross_attention_workspace(handle, kv, news, a)
+        elif shared is not None:
+            need = lib.vsk_attention_shared_workspace(handle, kv, news, a, shared)
+        else:
+            need = lib.vsk_attention_workspace(handle, kv, news, a)
         if not need:
             break
         work = torch.empty(need, dtype=torch.uint8, device=q.device)
-    status = lib.vsk_attention(handle, _stream(ctx.device), kv, layer, news, a)
+    stream = _stream(ctx.device)
+    if sets is not None:
+        status = lib.vsk_cross_attention(handle, stream, kv, news, a, sets)
+    elif shared is not None:
+        status = lib.vsk_attention_shared(handle, stream, kv, layer, news, a, shared)
+    else:
+        status = lib.vsk_attention(handle, stream, kv, layer, news, a)
     if status:
         ctx.check(status)
     return (out, lse) if return_lse else out
@@ -444,7 +462,8 @@ class PagedKVCache:
 
     def attend(self, q, *, starts=None, seqs=None, max_new=None, layer: int = 0,
                scale: float | None = None, window: int | None = None, sinks: int = 0,
-               max_length: int | None = None, return_lse: bool = False):
+               max_length: int | None = None, return_lse: bool = False,
+               shared: "SharedPrefix | None" = None):
         """Attention of the new tokens' queries (tokens x heads x head_dim;
         consecutive heads share a key head) over their sequences in the
         cache, laid out as in ``append``.  A token sees the keys up to its own
@@ -458,14 +477,44 @@ class PagedKVCache:
         Scores, sums and outputs are computed in 32 bits.  In 16 bits a weight
         is rounded before it multiplies a value: for few rows to two 16-bit
         parts, for many (prompts) once to the values' type, which is off by as
-        much as the output's own rounding."""
+        much as the output's own rounding.
+
+        ``shared``, of ``share``: the same attention, in which the keys that a
+        group of sequences shares are read once for all of them.  Its
+        sequences are the call's (``seqs`` is not given again).  With a window
+        each sequence reads its own keys."""
         self._layer(layer)
         q = self._heads(q, "q")
+        if shared is not None:
+            if not isinstance(shared, SharedPrefix) or shared.cache is not self:
+                raise VSKError(-2, "shared must be what this cache's share() returned")
+            if seqs is not None:
+                raise VSKError(-2, "the slots are those that share() was called with")
+            seqs = shared.seqs
         if q.shape[1] % self.kv_heads or not q.shape[1]:
             raise VSKError(-4, f"{q.shape[1]} query heads over {self.kv_heads} key heads")
         news, keep = self._news(q, starts, seqs, max_new)
+        if shared is not None:
+            n = q.shape[0] if starts is None else keep[0].shape[0] - 1
+            if n > shared.n:
+                raise VSKError(-4, f"{n} sequences, share() knows {shared.n}")
+            shared = shared._ref
         return _attend(self.ctx, self._ref, layer, q, news, 0, scale, window, sinks, max_length,
-                       return_lse)
+                       return_lse, None, shared)
+
+    def share(self, groups, *, seqs=None, members: int | None = None,
+              prefix: int | None = None) -> "SharedPrefix":
+        """Finds the pages that groups of sequences share, for ``attend``:
+        group g are the sequences ``groups[g] .. groups[g + 1]`` (ascending
+        offsets) of those in slots ``seqs`` (default: slot i is sequence i).
+        Nothing is assumed of them: a group's prefix is the leading whole pages
+        that all its members' tables agree on.  What is found stays true while
+        the sequences grow and the pool is compacted; after a ``fork`` into, or
+        a ``free`` of, one of these slots call ``update`` of what is returned.
+        ``members`` bounds a group's sequences (default: known of a host
+        sequence, all of them otherwise), ``prefix`` says about how many keys
+        the longest prefix has, to divide the work by."""
+        return SharedPrefix(self, groups, seqs, members, prefix)
 
     # -- pages ------------------------------------------------------------------
     def _keeping(self):
@@ -544,6 +593,142 @@ class PagedKVCache:
         for the stream)."""
         self._keeping()
         return int(self.status[0])
+
+
+class SharedPrefix:
+    """What ``PagedKVCache.share`` found: ``prefix``, the keys that each
+    sequence's group shares (int32, on the GPU)."""
+
+    def __init__(self, cache: PagedKVCache, groups, seqs, members, prefix):
+        gpu = cache.gpu
+        self.cache = cache
+        self.seqs = None if seqs is None else _ints(gpu, seqs, "seqs")
+        if seqs is not None:
+            cache._known(seqs, "seqs")
+        self.n = cache.slots if seqs is None else self.seqs.shape[0]
+        if not isinstance(groups, torch.Tensor):
+            a = np.asarray(groups)
+            if a.ndim != 1 or a.size < 1 or a.dtype.kind not in "iu":
+                raise VSKError(-2, "groups holds an offset a group and the end")
+            if a.min() < 0 or a.max() > self.n or (np.diff(a) < 0).any():
+                raise VSKError(-2, f"groups must ascend from 0 to at most {self.n}")
+            if members is None:
+                members = int(np.diff(a).max()) if a.size > 1 else 0
+        self.groups = _ints(gpu, groups, "groups")
+        if self.groups.shape[0] < 1:
+            raise VSKError(-2, "groups holds an offset a group and the end")
+        members = self.n if members is None else min(int(members), self.n)
+        most = 0 if prefix is None else int(prefix)
+        if members < 0 or not 0 <= most < 1 << 31:
+            raise VSKError(-2, "members and prefix are counts")
+        self.prefix = torch.zeros(self.n, dtype=torch.int32, device=cache.device)
+        self._c = _lib.vsk_shared_prefix(self.groups.data_ptr(), self.prefix.data_ptr(),
+                                         self.groups.shape[0] - 1, self.n, members, most)
+        self._ref = ctypes.byref(self._c)
+        self.update()
+
+    def update(self):
+        """Finds the prefixes anew, in the same tensors."""
+        c = self.cache
+        c.ctx.check(c.ctx.lib.vsk_kv_share(c.ctx.handle, _stream(c.gpu), c._ref,
+                                           self.seqs.data_ptr() if self.seqs is not None else None,
+                                           self._ref))
+
+
+def cross_attention(ctx: Context, q, k, v, *, starts=None, k_starts=None, k_lengths=None,
+                    sets=None, max_length: int | None = None, max_keys: int | None = None,
+                    scale: float | None = None, return_lse: bool = False):
+    """Attention to keys and values of another length, all of which every query
+    sees: a decoder's tokens to an encoder's states of the documents found.
+
+    q is tokens x heads x head_dim; sequence i its rows ``starts[i] ..
+    starts[i + 1]`` (default: row i alone, a decoding step's).  k and v are
+    rows x kv_heads x head_dim with ``k_starts``, the offsets of the sets of
+    keys (and the end), or a padded batch, sets x length x kv_heads x head_dim,
+    with ``k_lengths`` (default: all of them are keys).  Sequence i sees set
+    ``sets[i]`` (default: i); several may see one, and one that is not there
+    (-1) is empty.  A query that sees no key gets zeros (and -inf).
+    ``max_length`` bounds a sequence's queries, ``max_keys`` a set's keys, to
+    divide the work by (default: all rows, or the padded length).  scale,
+    return_lse, the rounding of weights and the rows that are not treated as
+    in ``PagedKVCache.attend``; keys past a set's length may hold anything."""
+    gpu = ctx.device
+    dtype = _tensor(gpu, q, "q", None, 3).dtype
+    _tensor(gpu, k, "k", dtype), _tensor(gpu, v, "v", dtype)
+    if dtype not in _TYPES:
+        raise VSKError(-8, f"{dtype} is not supported")
+    if k.shape != v.shape or k.dim() not in (3, 4) or q.shape[2] != k.shape[-1]:
+        raise VSKError(-4, f"q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}")
+    tokens, heads, d = q.shape
+    kv_heads = k.shape[-2]
+    if not heads or not kv_heads or heads % kv_heads:
+        raise VSKError(-4, f"{heads} query heads over {kv_heads} key heads")
+    q, k, v = _dense_heads(q), _dense_heads(k), _dense_heads(v)
+    at = lengths = None
+    step = 0
+    if k.dim() == 3:
+        if k_starts is None or k_lengths is not None:
+            raise VSKError(-2, "rows of keys take k_starts, a padded batch k_lengths")
+        at = _ints(gpu, k_starts, "k_starts")
+        if at.shape[0] < 1:
+            raise VSKError(-4, "k_starts holds an offset a set and the end")
+        n_sets, rows = at.shape[0] - 1, k.shape[0]
+        x, y = k.stride(), v.stride()
+    else:
+        if k_starts is not None:
+            raise VSKError(-2, "rows of keys take k_starts, a padded batch k_lengths")
+        n_sets, rows = k.shape[:2]
+        if k_lengths is not None:
+            lengths = _ints(gpu, k_lengths, "k_lengths")
+            if lengths.shape[0] != n_sets:
+                raise VSKError(-4, f"{lengths.shape[0]} lengths for {n_sets} sets")
+        (k, x, step), (v, y, other) = _padded(k), _padded(v)
+        if step != other:
+            (k, x, step), (v, y, _) = _padded(k.contiguous()), _padded(v.contiguous())
+    if max(rows, kv_heads, heads, step) > 1 << 30 or n_sets >= 1 << 31:
+        raise VSKError(-9, f"{rows} keys of {kv_heads} heads: at most 2^30")
+    n, most, s = tokens, 1, None
+    if starts is not None:
+        s = _ints(gpu, starts, "starts")
+        n = s.shape[0] - 1
+        if n < 0:
+            raise VSKError(-4, "starts holds an offset a sequence and the end")
+        most = tokens if max_length is None else min(int(max_length), tokens)
+        if most < 0:
+            raise VSKError(-2, "max_length must not be negative")
+    which = None
+    if sets is not None:
+        which = _ints(gpu, sets, "sets")
+        if which.shape[0] != n:
+            raise VSKError(-4, f"{which.shape[0]} sets for {n} sequences")
+    elif n > n_sets:
+        raise VSKError(-4, f"{n} sequences, {n_sets} sets of keys")
+    if not rows or not n_sets:
+        # (no memory that could be read: one empty set)
+        k, v, x, y, step, rows = q, q, (q.stride(0), 0), (q.stride(0), 0), 0, 0
+        at, lengths, n_sets, which = None, None, 1, torch.zeros_like(
+            which) if which is not None else torch.zeros(n, dtype=torch.int32, device=q.device)
+    kv = _KV.pack(k.data_ptr(), v.data_ptr(), 0, 0, x[0], x[1], 0, 0, y[0], y[1], 0, 0, 0, 0, 0,
+                  0, _TYPES[dtype], 1, rows, 0, kv_heads, d, 0, 0)
+    news = _NEWS.pack(s.data_ptr() if s is not None else 0,
+                      which.data_ptr() if which is not None else 0, n, most, tokens)
+    key_sets = _SETS.pack(at.data_ptr() if at is not None else 0,
+                          lengths.data_ptr() if lengths is not None else 0, step, n_sets)
+    return _attend(ctx, kv, 0, q, news, 0, scale, None, 0, max_keys, return_lse, key_sets)
+
+
+def _padded(x):
+    """x, sets x length x heads x d, its row and head strides, and the rows
+    from a set to the next (x, or a copy where that is no whole number)."""
+    a, b, c = x.stride()[:3]
+    if x.shape[1] <= 1:
+        return x, (max(a, 1), c), 1
+    if x.shape[0] <= 1:
+        return x, (b, c), x.shape[1]
+    if b <= 0 or a < 0 or a % b:
+        x = x.contiguous()
+        a, b, c = x.stride()[:3]
+    return x, (b, c), a // b
 
 
 def window_attention(ctx: Context, q, k, v, *, starts, k_starts=None, max_length: int | None = None,
