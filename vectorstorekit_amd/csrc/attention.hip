@@ -14,7 +14,7 @@ int32_t padded_head(int32_t d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
 
 // How a call's work is divided.
 struct Plan {
-  int32_t tiles, splits, chunk;
+  int32_t tiles, splits, chunk, key_tile;
   int32_t share;  // attn_rows: waves that take a row tile's keys in turn
   bool tile;      // attn_tile
 };
@@ -83,7 +83,14 @@ Plan plan_of(const vsk_ctx *ctx, const vsk_kv *kv, const vsk_attention_args *arg
     row_tile = ATTN_TILE_ROWS;
     key_tile = attn_tile_keys(kv->head_dim);
   }
+  if (kv->dtype == VSK_DTYPE_F32 && (span.all || span.joined) && rows >= (getenv("R32") ? atoi(getenv("R32")) : 96) &&
+      kv->head_dim <= 128 && aligned_operands(kv, args)) {
+    p.tile = true;
+    row_tile = ATTN_TILE_ROWS;
+    key_tile = ATTN_TILE32_KEYS;
+  }
   p.tiles = (int32_t)ceil_div(rows, row_tile);
+  p.key_tile = (int32_t)key_tile;
   const int64_t blocks = pairs * p.tiles;
   if (args->window > 0) {
     const int64_t reach = (int64_t)args->window + args->sinks + ceil_div(row_tile, group) +
@@ -123,6 +130,7 @@ Plan plan_of(const vsk_ctx *ctx, const vsk_kv *kv, const vsk_attention_args *arg
     // 128 on 8 (us): 512 tokens (128 blocks) 519 / 284, 2,000 (504) 893 / 998.
     per = 16;
     want = 2 * blocks > cus ? 1 : 2 * cus;
+    if (kv->dtype == VSK_DTYPE_F32) want = getenv("W32") ? atoi(getenv("W32")) * cus : 12 * cus;
   } else {
     // A tile for each of the four waves that share a part at least.  Contexts
     // differ in length, so several rounds of blocks share the work more evenly
@@ -321,7 +329,9 @@ void attend(vsk_ctx *ctx, void *stream, const vsk_kv *kv, int32_t layer,
   const AttnForm form = sets || p.group_tokens ? ATTN_FORMS : ATTN_OWN;
   auto launch = [&](const Plan &plan, AttnArgs x) {
     x.tiles = plan.tiles, x.splits = plan.splits, x.chunk = plan.chunk;
-    if (plan.tile)
+    if (plan.tile && kv->dtype == VSK_DTYPE_F32)
+      launch_attn_tile32(ctx, st, x);
+    else if (plan.tile)
       launch_attn_tile(ctx, st, x, kv->dtype, form);
     else if (form == ATTN_OWN)
       launch_attn_rows(ctx, st, x, kv->dtype, al, plan.share);
@@ -341,7 +351,10 @@ void attend(vsk_ctx *ctx, void *stream, const vsk_kv *kv, int32_t layer,
   }
   launch(p.own, a);
   a.splits = p.parts(), a.chunk = p.own.chunk;
-  launch_attn_join(ctx, st, a, kv->dtype, al, p.own.tile ? ATTN_TILE_ROWS : 16, form);
+  if (form == ATTN_OWN)
+    launch_attn_join(ctx, st, a, kv->dtype, al, p.own.tile ? ATTN_TILE_ROWS : 16);
+  else
+    launch_attn_join_forms(ctx, st, a, kv->dtype, al, p.own.key_tile);
   finish_queued(ctx, st);
 }
 

@@ -296,6 +296,14 @@ template <int CH> __device__ inline int k_swizzle(int row) {
   return CH >= 16 ? row & 15 : (row & 7) ^ ((row >> 3) & 1);
 }
 
+// (fmaxf would first quiet each product, an instruction a value: the maximum
+// here passes over NaN without it)
+__device__ inline float max3(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+
 __device__ inline float attn_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 // log of a row's sum, whose weights are 2^(score * scale_log2 - ref)
 __device__ inline float attn_lse(float ref, float sum) {
@@ -358,9 +366,15 @@ constexpr int ATTN_TILE_ROWS = 128;
 constexpr int ATTN_TILE_GROUP = 16;  // keys that lie together in a tile
 void launch_attn_tile(vsk_ctx *ctx, hipStream_t stream, const AttnArgs &a, int32_t t,
                       AttnForm form);
+// attn_tile32.hip: 32 bits, aligned, ATTN_FORMS, the same row tiles
+constexpr int ATTN_TILE32_KEYS = 32;
+void launch_attn_tile32(vsk_ctx *ctx, hipStream_t stream, const AttnArgs &a);
 // joins the parts that row tiles of `rows` rows left: 16 (launch_attn_rows) or
 // ATTN_TILE_ROWS
 void launch_attn_join(vsk_ctx *ctx, hipStream_t stream, const AttnArgs &a, int32_t t,
-                      bool aligned, int32_t rows, AttnForm form);
+                      bool aligned, int32_t rows);
+// attn_forms.hip: the same of ATTN_FORMS; key_tile: keys of a tile of the parts
+void launch_attn_join_forms(vsk_ctx *ctx, hipStream_t stream, const AttnArgs &a, int32_t t,
+                            bool aligned, int32_t key_tile);
 
 }  // namespace vsk

@@ -31,9 +31,6 @@
 // without 16-byte alignment are loaded a value at a time: 32 contexts of 4,000,
 // 10 f16 heads of 100, 595 us where heads of 104 take 125.
 #include "attn_rows.hpp"
-
-#include <type_traits>
-
 #include "vsk_api.hpp"
 
 namespace vsk {
@@ -45,7 +42,7 @@ namespace {
 // of one; the threads take four values each of several parts at a time.  Its
 // bytes are few: it is bound by the chain count, maximum, parts, each a trip to
 // memory (5 us behind 64 parts of 192 rows of 128).
-template <class T, int DV, int SL, int KTILE, int G, bool ALIGNED, AttnForm F>
+template <class T, int DV, int SL, int KTILE, int G, bool ALIGNED>
 __global__ __launch_bounds__(256) void k_attn_join(const AttnArgs a, const int32_t RT) {
   constexpr int LANES = SL / 4, WAYS = 256 / LANES;
   __shared__ __attribute__((aligned(16))) float so[WAYS][SL];
@@ -54,7 +51,7 @@ __global__ __launch_bounds__(256) void k_attn_join(const AttnArgs a, const int32
   const uint32_t block = blockIdx.x / (DV / SL);
   const int e0 = blockIdx.x % (DV / SL) * SL;
   if (e0 >= a.d) return;
-  const AttnSeq s = attn_seq<F>(a, block / per);
+  const AttnSeq s = attn_seq<ATTN_OWN>(a, block / per);
   const int32_t x = block % per, t = x / a.heads, head = x % a.heads;
   if (t >= s.T) return;
   const int64_t stride = a.tokens * a.heads;
@@ -73,26 +70,19 @@ __global__ __launch_bounds__(256) void k_attn_join(const AttnArgs a, const int32
   const int32_t row0 = row / RT * RT;
   const int32_t all = (s.T < a.max_new ? s.T : a.max_new) * a.group;
   const int32_t last = row0 + RT < all ? row0 + RT - 1 : all - 1;
-  const auto span = attn_span<KTILE, G>(a, s.p0 + (row0 / a.group & s.each),
-                                        s.p0 + (last / a.group & s.each));
-  int32_t parts = attn_parts(a, span.tiles), from = 0;
-  if (F && a.joined) {
-    // the prefix's parts, where the sequence has one, and its own
-    parts = a.splits;
-    from = a.prefix[block / per] >> a.page_shift > 0 ? 0 : a.part0;
-  } else if (parts == 1) {
-    return;  // written by the row tile itself
-  }
-  float top = (!F || i0 >= from) && i0 < parts ? m0 : -INFINITY;
+  const int32_t p0 = s.L - s.T;
+  const auto span = attn_span<KTILE, G>(a, p0 + row0 / a.group, p0 + last / a.group);
+  const int32_t parts = attn_parts(a, span.tiles);
+  if (parts == 1) return;  // written by the row tile itself
+  float top = i0 < parts ? m0 : -INFINITY;
   for (int32_t i = i0 + 64; i < parts; i += 64)
-    if (!F || i >= from) top = fmaxf(top, a.part_ml[2 * (i * stride + at)]);
+    top = fmaxf(top, a.part_ml[2 * (i * stride + at)]);
   for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
   top = xor16_32_max(top);
   const float use = top == -INFINITY ? 0.f : top;
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
   float sum = 0.f;
-  // (a part that is not there holds no values)
-  if (way < parts && (!F || (way >= from && !(a.joined && fm0 == -INFINITY)))) {
+  if (way < parts) {
     const float f = attn_exp2((fm0 - use) * a.scale_log2);
     sum = f * fl0;
     o = f * o0;
@@ -100,9 +90,7 @@ __global__ __launch_bounds__(256) void k_attn_join(const AttnArgs a, const int32
 #pragma unroll 4
   for (int32_t i = way + WAYS; i < parts; i += WAYS) {
     const int64_t r = i * stride + at;
-    const float ref = a.part_ml[2 * r];
-    if (F && (i < from || (a.joined && ref == -INFINITY))) continue;
-    const float f = attn_exp2((ref - use) * a.scale_log2);
+    const float f = attn_exp2((a.part_ml[2 * r] - use) * a.scale_log2);
     sum += f * a.part_ml[2 * r + 1];
     if (e < a.d) o += f * *reinterpret_cast<const f32x4 *>(a.part_o + r * DV + e);
   }
@@ -191,19 +179,19 @@ void launch_attn_rows(vsk_ctx *ctx, hipStream_t st, const AttnArgs &a, int32_t t
 }
 
 namespace {
-template <class T, int DV, int SL, AttnForm F>
+template <class T, int DV, int SL>
 void join_slice(hipStream_t st, const AttnArgs &a, bool aligned, int32_t rows, unsigned g) {
   constexpr int KR = 16 * SUBS<T>, KB = attn_tile_keys(DV);
   if (rows == ROWS) {
     if (aligned)
-      k_attn_join<T, DV, SL, KR, KR, true, F><<<g, 256, 0, st>>>(a, rows);
+      k_attn_join<T, DV, SL, KR, KR, true><<<g, 256, 0, st>>>(a, rows);
     else
-      k_attn_join<T, DV, SL, KR, KR, false, F><<<g, 256, 0, st>>>(a, rows);
+      k_attn_join<T, DV, SL, KR, KR, false><<<g, 256, 0, st>>>(a, rows);
   } else if constexpr (sizeof(T) == 2) {  // (tiles are for 16-bit, aligned operands)
-    k_attn_join<T, DV, SL, KB, ATTN_TILE_GROUP, true, F><<<g, 256, 0, st>>>(a, rows);
+    k_attn_join<T, DV, SL, KB, ATTN_TILE_GROUP, true><<<g, 256, 0, st>>>(a, rows);
   }
 }
-template <class T, int DV, AttnForm F>
+template <class T, int DV>
 void join_head(hipStream_t st, const AttnArgs &a, bool aligned, int32_t rows, uint64_t g,
                uint64_t cus) {
   // slices of 16 values where all of them find a compute unit each: one context
@@ -212,43 +200,36 @@ void join_head(hipStream_t st, const AttnArgs &a, bool aligned, int32_t rows, ui
   // slices of 64: 4 f32 contexts to 30,000, 8 heads of 256 on one, 44 us, 49
   // without them; 3 f16 to 200,003, 64 of 128 on 8, 209 / 212.
   if (g * (DV / 16) <= cus)
-    join_slice<T, DV, 16, F>(st, a, aligned, rows, g * (DV / 16));
+    join_slice<T, DV, 16>(st, a, aligned, rows, g * (DV / 16));
   else if (DV > 64 && g <= cus)
-    join_slice<T, DV, 64, F>(st, a, aligned, rows, g * (DV / 64));
+    join_slice<T, DV, 64>(st, a, aligned, rows, g * (DV / 64));
   else
-    join_slice<T, DV, DV, F>(st, a, aligned, rows, g);
+    join_slice<T, DV, DV>(st, a, aligned, rows, g);
 }
-template <class T, AttnForm F>
+template <class T>
 void join_of(hipStream_t st, const AttnArgs &a, bool aligned, int32_t rows, uint64_t g,
              uint64_t cus) {
   if (a.d <= 64)
-    join_head<T, 64, F>(st, a, aligned, rows, g, cus);
+    join_head<T, 64>(st, a, aligned, rows, g, cus);
   else if (a.d <= 128)
-    join_head<T, 128, F>(st, a, aligned, rows, g, cus);
+    join_head<T, 128>(st, a, aligned, rows, g, cus);
   else
-    join_head<T, 256, F>(st, a, aligned, rows, g, cus);
+    join_head<T, 256>(st, a, aligned, rows, g, cus);
 }
 }  // namespace
 
 void launch_attn_join(vsk_ctx *ctx, hipStream_t st, const AttnArgs &a, int32_t t, bool aligned,
-                      int32_t rows, AttnForm form) {
+                      int32_t rows) {
   if (a.splits == 1) return;
   const int64_t grid = (int64_t)a.n * a.max_new * a.heads;
   VSK_REQUIRE(grid <= 0x7FFFFFFFll, VSK_ERR_INVALID_BUFFER_SIZE, "too many query rows in one call");
   KernelTimer kt(ctx, "attn_join", (double)grid, st);
-  auto of = [&](auto form) {
-    constexpr AttnForm F = decltype(form)::value;
-    if (t == VSK_DTYPE_F32)
-      join_of<float, F>(st, a, aligned, rows, grid, ctx->cu_count);
-    else if (t == VSK_DTYPE_F16)
-      join_of<_Float16, F>(st, a, aligned, rows, grid, ctx->cu_count);
-    else
-      join_of<__bf16, F>(st, a, aligned, rows, grid, ctx->cu_count);
-  };
-  if (form == ATTN_OWN)
-    of(std::integral_constant<AttnForm, ATTN_OWN>());
+  if (t == VSK_DTYPE_F32)
+    join_of<float>(st, a, aligned, rows, grid, ctx->cu_count);
+  else if (t == VSK_DTYPE_F16)
+    join_of<_Float16>(st, a, aligned, rows, grid, ctx->cu_count);
   else
-    of(std::integral_constant<AttnForm, ATTN_FORMS>());
+    join_of<__bf16>(st, a, aligned, rows, grid, ctx->cu_count);
   check_launch("attn_join");
 }
 

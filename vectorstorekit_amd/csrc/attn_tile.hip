@@ -67,14 +67,6 @@ template <int CH> __device__ inline int v_swizzle(int row) {
   return CH >= 16 ? 4 * x + 2 * (x >> 1) : 2 * x;
 }
 
-// (fmaxf would first quiet each product, an instruction a value: the maximum
-// here passes over NaN without it)
-__device__ inline float max3(float a, float b, float c) {
-  float r;
-  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
-  return r;
-}
-
 // DP: the head, padded to products.  Two workgroups of four waves share a
 // compute unit, so that one's start and end hide behind the other's products
 // (one of eight waves over twice the rows: 340 us where these take 308, 8

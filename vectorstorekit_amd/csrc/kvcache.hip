@@ -482,15 +482,16 @@ void launch_move(vsk_ctx *ctx, hipStream_t st, const vsk_kv *kv, const Pool &p, 
   check_launch("kv_move");
 }
 
-// A workgroup a group: the first page in which a member differs from the first
-// member ends the prefix.  Members' tables are read 256 pages at a time; the
-// end found so far bounds what is read of the others (64 branches of 32,768
-// tokens in pages of 64: 9 us).
-__global__ __launch_bounds__(256) void k_kv_share(const int32_t *table, const int32_t *lengths,
-                                                  int64_t stride, int32_t slots, int32_t width,
-                                                  int32_t shift, const int32_t *seqs,
-                                                  const int32_t *groups, int32_t n_groups,
-                                                  int32_t n, int32_t *prefix) {
+// A workgroup a group: the first page in which a member's table differs from
+// the first member's ends the prefix.  A wave takes a member at a time, 256
+// pages a step, up to the end that any wave has found so far (64 branches of
+// 32,768 tokens in pages of 64: SHARE_US us).
+constexpr int SHARE_WAVES = 16;
+__global__ __launch_bounds__(64 * SHARE_WAVES) void k_kv_share(
+    const int32_t *table, const int32_t *lengths, int64_t stride, int32_t slots, int32_t width,
+    int32_t shift, const int32_t *seqs, const int32_t *groups, int32_t n_groups, int32_t n,
+    int32_t *prefix) {
+  constexpr int NT = 64 * SHARE_WAVES;
   __shared__ int32_t pages;
   auto offset = [&](int32_t g) -> int32_t {
     const int32_t x = groups[g];
@@ -500,39 +501,48 @@ __global__ __launch_bounds__(256) void k_kv_share(const int32_t *table, const in
   const int32_t first = offset(g), end = offset(g + 1);
   // (sequences before the first group and behind the last are in none)
   if (g == 0)
-    for (int32_t b = threadIdx.x; b < first; b += 256) prefix[b] = 0;
+    for (int32_t b = threadIdx.x; b < first; b += NT) prefix[b] = 0;
   if (g == n_groups - 1)
-    for (int32_t b = (end > first ? end : first) + threadIdx.x; b < n; b += 256) prefix[b] = 0;
+    for (int32_t b = (end > first ? end : first) + threadIdx.x; b < n; b += NT) prefix[b] = 0;
   if (end <= first) return;
-  auto slot_of = [&](int32_t b) -> int32_t { return seqs ? seqs[b] : b; };
+  auto slot_of = [&](int32_t b) -> int32_t {
+    const int32_t x = seqs ? seqs[b] : b;
+    return (uint32_t)x < (uint32_t)slots ? x : -1;
+  };
+  // the whole pages of the shortest member
   if (threadIdx.x == 0) pages = end - first > 1 ? width : 0;
   __syncthreads();
-  const int32_t head = slot_of(first);
-  for (int32_t b = first + threadIdx.x; b < end; b += 256) {
+  for (int32_t b = first + threadIdx.x; b < end; b += NT) {
     const int32_t slot = slot_of(b);
-    int32_t whole = 0;
-    if ((uint32_t)slot < (uint32_t)slots && (uint32_t)head < (uint32_t)slots) {
-      const int32_t l = lengths[slot];
-      whole = l < 0 ? 0 : l >> shift;
-    }
+    const int32_t l = slot < 0 ? 0 : lengths[slot], whole = l < 0 ? 0 : l >> shift;
     if (whole < width) atomicMin(&pages, whole);
   }
   __syncthreads();
-  int32_t most = pages;
-  for (int32_t b = first + 1; b < end && most > 0; ++b) {
-    const int32_t *x = table + head * stride, *y = table + slot_of(b) * stride;
-    int32_t at = most;
-    for (int32_t i = threadIdx.x; i < most; i += 256)
-      if (x[i] != y[i] || x[i] < 0) {
-        at = i;
-        break;
+  const int32_t head = slot_of(first);
+  const int32_t lane = threadIdx.x & 63;
+  for (int32_t b = first + 1 + (threadIdx.x >> 6); b < end; b += SHARE_WAVES) {
+    const int32_t slot = slot_of(b);
+    if (slot < 0 || head < 0) break;  // (no pages are left to compare)
+    const int32_t *x = table + head * stride, *y = table + slot * stride;
+    for (int32_t i = lane;; i += 256) {
+      const int32_t most = *(volatile int32_t *)&pages;
+      if (i - lane >= most) break;
+      int32_t u[4], v[4];
+#pragma unroll
+      for (int z = 0; z < 4; ++z) {
+        const int32_t j = i + 64 * z < most ? i + 64 * z : most - 1;
+        u[z] = x[j], v[z] = y[j];
       }
-    if (at < most) atomicMin(&pages, at);
-    __syncthreads();
-    most = pages;
-    __syncthreads();
+      int32_t at = most;
+#pragma unroll
+      for (int z = 3; z >= 0; --z)
+        if (i + 64 * z < most && (u[z] != v[z] || u[z] < 0)) at = i + 64 * z;
+      if (at < most) atomicMin(&pages, at);
+    }
   }
-  for (int32_t b = first + threadIdx.x; b < end; b += 256) prefix[b] = most << shift;
+  __syncthreads();
+  const int32_t shared = pages << shift;
+  for (int32_t b = first + threadIdx.x; b < end; b += NT) prefix[b] = shared;
 }
 
 void check_list(const int32_t *x, int32_t n) {
@@ -656,7 +666,7 @@ vsk_status vsk_kv_share(vsk_ctx *ctx, void *stream, const vsk_kv *kv, const int3
   hipStream_t st = static_cast<hipStream_t>(stream);
   {
     KernelTimer kt(ctx, "kv_share", shared->n, st);
-    k_kv_share<<<(unsigned)shared->n_groups, 256, 0, st>>>(
+    k_kv_share<<<(unsigned)shared->n_groups, 64 * SHARE_WAVES, 0, st>>>(
         kv->table, kv->lengths, kv->table_stride, kv->slots, kv->width,
         __builtin_ctz((unsigned)kv->page_size), seqs, shared->groups, shared->n_groups, shared->n,
         shared->prefix);
