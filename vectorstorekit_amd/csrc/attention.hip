@@ -116,7 +116,7 @@ Plan plan_of(const vsk_ctx *ctx, const vsk_kv *kv, const vsk_attention_args *arg
     // heads of 64 45 / 65; 64 of up to 300 in 32 bits 27 / 22, heads of 64 14 / 22.
     const bool many = kv->head_dim <= 64 || (kv->head_dim <= 128 && kv->dtype != VSK_DTYPE_F32 &&
                                              blocks <= 6 * cus);
-    if (many && tiles <= (blocks < cus ? 32 : 64)) {
+    if (!span.joined && many && tiles <= (blocks < cus ? 32 : 64)) {
       p.share = 8;
       return p;
     }
@@ -143,7 +143,7 @@ Plan plan_of(const vsk_ctx *ctx, const vsk_kv *kv, const vsk_attention_args *arg
     // 2 contexts of 100,000 of 8 heads of 128 121 us, in 96 parts 129.
     per = 4;
     const int64_t most = kv->head_dim <= 64 ? 16 : kv->head_dim > 128 ? 1
-                         : kv->dtype == VSK_DTYPE_F32 ? 2 : 6;
+                         : kv->dtype != VSK_DTYPE_F32 ? 6 : span.joined ? 8 : 2;
     want = most * cus < 64 * blocks ? most * cus : 64 * blocks;
     if (want < cus) want = cus;
   }
@@ -341,15 +341,35 @@ void attend(vsk_ctx *ctx, void *stream, const vsk_kv *kv, int32_t layer,
   if (p.group_tokens) {
     a.prefix = shared->prefix;
     a.joined = 1;
-    AttnArgs g = a;
-    g.groups = shared->groups;
-    g.members = a.n;
-    g.n = shared->n_groups;
-    g.max_new = (int32_t)p.group_tokens;
-    launch(p.prefix, g);
     a.part0 = p.prefix.splits;
+    a.groups = shared->groups;
+    a.members = a.n;
+    a.pre.n = shared->n_groups, a.pre.max_new = (int32_t)p.group_tokens;
+    a.pre.tiles = p.prefix.tiles, a.pre.splits = p.prefix.splits, a.pre.chunk = p.prefix.chunk;
+    const int64_t blocks = (int64_t)a.pre.n * a.pre.splits * a.pre.tiles * a.kv_heads;
+    VSK_REQUIRE(blocks <= 0x7FFFFFFFll, VSK_ERR_INVALID_BUFFER_SIZE,
+                "too many query rows in one call");
+    // one launch for both where one kernel has both
+    const bool mixed = p.prefix.tile && !p.own.tile && kv->dtype != VSK_DTYPE_F32 &&
+                       kv->head_dim <= 128;
+    if (mixed || p.prefix.tile == p.own.tile) {
+      a.pre_blocks = (uint32_t)blocks;
+    } else {
+      AttnArgs g = a;
+      g.part0 = 0;
+      g.n = a.pre.n, g.max_new = a.pre.max_new;
+      launch(p.prefix, g);
+      a.groups = nullptr;
+    }
+    if (mixed) {
+      a.tiles = p.own.tiles, a.splits = p.own.splits, a.chunk = p.own.chunk;
+      launch_attn_shared(ctx, st, a, kv->dtype);
+    } else {
+      launch(p.own, a);
+    }
+  } else {
+    launch(p.own, a);
   }
-  launch(p.own, a);
   a.splits = p.parts(), a.chunk = p.own.chunk;
   if (form == ATTN_OWN)
     launch_attn_join(ctx, st, a, kv->dtype, al, p.own.tile ? ATTN_TILE_ROWS : 16);

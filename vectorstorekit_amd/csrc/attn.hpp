@@ -65,6 +65,12 @@ struct AttnArgs {
   int32_t members;      // sequences that the groups' offsets may name
   int32_t joined;       // parts are written also where there is one, absent ones marked
   int32_t part0;        // the call's first part
+  // two calls in one launch: the first pre_blocks blocks are those of a call
+  // over prefixes, which differs in these
+  uint32_t pre_blocks;
+  struct {
+    int32_t n, max_new, tiles, splits, chunk;
+  } pre;
   int32_t tiles;        // row tiles of a sequence's max_new tokens
   int32_t splits;       // parts a tile's keys may be split into
   int32_t chunk;        // key tiles of a part
@@ -173,6 +179,23 @@ __device__ inline int32_t attn_position(const AttnArgs &a, const AttnSeq &s, int
   if ((uint32_t)slot >= (uint32_t)a.slots) return -1;
   const int64_t pos = (int64_t)attn_length(a, slot) - count + at;
   return pos >= s.L ? s.L - 1 : pos < -1 ? -1 : (int32_t)pos;
+}
+
+// the call over prefixes of the two
+__device__ inline void attn_prefix_call(AttnArgs &a) {
+  a.n = a.pre.n, a.max_new = a.pre.max_new;
+  a.tiles = a.pre.tiles, a.splits = a.pre.splits, a.chunk = a.pre.chunk;
+  a.part0 = 0;
+}
+// The call that a block belongs to, and its number there.
+__device__ inline uint32_t attn_call(AttnArgs &a, uint32_t block) {
+  if (a.pre_blocks == 0) return block;
+  if (block >= a.pre_blocks) {
+    a.groups = nullptr;
+    return block - a.pre_blocks;
+  }
+  attn_prefix_call(a);
+  return block;
 }
 
 // The keys that query positions q0 .. q1 see between them, in groups of G keys
@@ -356,7 +379,7 @@ void finish_queued(vsk_ctx *ctx, hipStream_t stream);
 // to 64), 4, or 1
 void launch_attn_rows(vsk_ctx *ctx, hipStream_t stream, const AttnArgs &a, int32_t t,
                       bool aligned, int32_t share);
-// attn_forms.hip: the same of ATTN_FORMS
+// attn_forms.hip: the same of ATTN_FORMS (with a.pre: both of its calls)
 void launch_attn_rows_forms(vsk_ctx *ctx, hipStream_t stream, const AttnArgs &a, int32_t t,
                             bool aligned, int32_t share);
 // keys of a tile of attn_tile.hip, by the (padded) head
@@ -369,6 +392,9 @@ void launch_attn_tile(vsk_ctx *ctx, hipStream_t stream, const AttnArgs &a, int32
 // attn_tile32.hip: 32 bits, aligned, ATTN_FORMS, the same row tiles
 constexpr int ATTN_TILE32_KEYS = 32;
 void launch_attn_tile32(vsk_ctx *ctx, hipStream_t stream, const AttnArgs &a);
+// attn_shared.hip: 16 bits, aligned, heads to 128: a.pre by row tiles of ATTN_TILE_ROWS, the
+// call itself by those of 16, four waves each
+void launch_attn_shared(vsk_ctx *ctx, hipStream_t stream, const AttnArgs &a, int32_t t);
 // joins the parts that row tiles of `rows` rows left: 16 (launch_attn_rows) or
 // ATTN_TILE_ROWS
 void launch_attn_join(vsk_ctx *ctx, hipStream_t stream, const AttnArgs &a, int32_t t,

@@ -10,8 +10,11 @@ namespace {
 
 template <class T, int VW, int NB, int SHARE, bool ALIGNED>
 __global__ __launch_bounds__(rows_threads(SHARE), rows_waves<T>(SHARE, VW * NB)) void
-k_attn_forms(const AttnArgs a) {
-  attn_rows_block<T, VW, NB, SHARE, ALIGNED, ATTN_FORMS>(a);
+k_attn_forms(const AttnArgs args) {
+  __shared__ __attribute__((aligned(1024))) char pool[RowsLds<T, VW, NB, SHARE, ALIGNED>::BYTES];
+  AttnArgs a = args;
+  const uint32_t block = attn_call(a, blockIdx.x);
+  attn_rows_block<T, VW, NB, SHARE, ALIGNED, ATTN_FORMS>(a, block, pool);
 }
 
 // Joins the parts of output rows: a row for DV / 4 lanes, times WAYS that share
@@ -122,7 +125,7 @@ void rows_of(hipStream_t st, const AttnArgs &a, bool aligned, int32_t share, uns
 void launch_attn_rows_forms(vsk_ctx *ctx, hipStream_t st, const AttnArgs &a, int32_t t,
                             bool aligned, int32_t share) {
   const int64_t groups = share > 1 ? a.tiles : (a.tiles + 3) / 4;
-  const int64_t grid = (int64_t)a.n * a.splits * groups * a.kv_heads;
+  const int64_t grid = a.pre_blocks + (int64_t)a.n * a.splits * groups * a.kv_heads;
   VSK_REQUIRE(grid <= 0x7FFFFFFFll, VSK_ERR_INVALID_BUFFER_SIZE, "too many query rows in one call");
   const unsigned g = (unsigned)grid;
   KernelTimer kt(ctx, "attn_forms", (double)a.tokens * a.heads, st);

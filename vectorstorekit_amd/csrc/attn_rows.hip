@@ -119,7 +119,8 @@ __global__ __launch_bounds__(256) void k_attn_join(const AttnArgs a, const int32
 template <class T, int VW, int NB, int SHARE, bool ALIGNED>
 __global__ __launch_bounds__(rows_threads(SHARE), rows_waves<T>(SHARE, VW * NB)) void
 k_attn_rows(const AttnArgs a) {
-  attn_rows_block<T, VW, NB, SHARE, ALIGNED, ATTN_OWN>(a);
+  __shared__ __attribute__((aligned(1024))) char pool[RowsLds<T, VW, NB, SHARE, ALIGNED>::BYTES];
+  attn_rows_block<T, VW, NB, SHARE, ALIGNED, ATTN_OWN>(a, blockIdx.x, pool);
 }
 
 template <class T, int VW, int NB>

@@ -493,17 +493,28 @@ template <class T> __device__ inline void store4(T *dst, const float (&x)[4], in
   }
 }
 
+// LDS of a block: the waves' keys and, after them, their sums (four waves' at a
+// time), then each row's largest scores and sums of weights.
+template <class T, int VW, int NB, int SHARE, bool ALIGNED> struct RowsLds {
+  static constexpr int DV = 16 * VW * NB, SLOTS = 4;
+  static constexpr int SUMB = SHARE > 1 ? SLOTS * ROWS * (DV + 4) * 4 : 0;
+  static constexpr int KEYB =
+      ALIGNED ? (SHARE > 4 ? SHARE : 4) * 16 * SUBS<T> * DV * (int)sizeof(T) : 16;
+  static constexpr int POOL = KEYB > SUMB ? KEYB : SUMB;
+  static constexpr int BYTES = POOL + (SHARE > 1 ? 2 * SHARE * ROWS * 4 : 0);
+};
+
 // One block: a row tile of one sequence and key head, over one part of its
 // keys that the block's SHARE waves take in turn, or (SHARE 1) four row tiles,
 // a wave each.
 template <class T, int VW, int NB, int SHARE, bool ALIGNED, AttnForm F>
-__device__ __forceinline__ void attn_rows_block(const AttnArgs &a) {
+__device__ __forceinline__ void attn_rows_block(const AttnArgs &a, uint32_t at, char *pool) {
   typedef RowTile<T, VW, NB, ALIGNED, F> Tile;
-  constexpr int DV = Tile::DV;
+  typedef RowsLds<T, VW, NB, SHARE, ALIGNED> Lds;
+  constexpr int DV = Tile::DV, SLOTS = Lds::SLOTS;
   const int lane = threadIdx.x & 63;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   // key heads fastest: neighbouring blocks read neighbouring parts of a page
-  uint32_t at = blockIdx.x;
   const int32_t h = at % a.kv_heads;
   at /= a.kv_heads;
   const int32_t groups = SHARE > 1 ? a.tiles : (a.tiles + 3) / 4;
@@ -542,10 +553,6 @@ __device__ __forceinline__ void attn_rows_block(const AttnArgs &a) {
   const int32_t first = part * a.chunk + (SHARE > 1 ? w : 0);
   const int32_t end = part == parts - 1 ? span.tiles : (part + 1) * a.chunk;
 
-  // the waves' keys and, after them, their sums: four waves' at a time
-  constexpr int SLOTS = 4, SUMB = SHARE > 1 ? SLOTS * ROWS * (DV + 4) * 4 : 0;
-  constexpr int KEYB = ALIGNED ? (SHARE > 4 ? SHARE : 4) * Tile::KT * Tile::ROWB : 16;
-  __shared__ __attribute__((aligned(1024))) char pool[KEYB > SUMB ? KEYB : SUMB];
   Tile tl(a, s, h, lane, (lds_char *)pool + (ALIGNED ? w * Tile::KT * Tile::ROWB : 0));
   tl.begin(have ? row0 + tl.n : 0x3fffffff);
   const auto base = [&](int32_t x) { return span.base(first + SHARE * x); };
@@ -594,8 +601,9 @@ __device__ __forceinline__ void attn_rows_block(const AttnArgs &a) {
     }
   } else {
     typedef float Sums[ROWS][DV + 4];
+    typedef float Ends[ROWS];
     Sums *so = reinterpret_cast<Sums *>(pool);
-    __shared__ float sm[SHARE][ROWS], sl[SHARE][ROWS];
+    Ends *sm = reinterpret_cast<Ends *>(pool + Lds::POOL), *sl = sm + SHARE;
     if (tl.g == 0) sm[w][tl.n] = tl.m, sl[w][tl.n] = tl.l;
     __syncthreads();
     float top = -INFINITY, sum = 0.f;

@@ -1,0 +1,55 @@
+// attn_shared.hip -- attention over shared prefixes in one launch: row tiles of
+// 128 over the prefixes (attn_tile.hpp), whose bound is the products, and
+// beside them row tiles of 16 over each sequence's own keys (attn_rows.hpp),
+// whose bound is their bytes.
+#include "attn_rows.hpp"
+#include "attn_tile.hpp"
+#include "vsk_api.hpp"
+
+namespace vsk {
+
+namespace {
+
+template <class T, int DP, int VW, int NB>
+__global__ __launch_bounds__(64 * TILE_WAVES, 2) void k_attn_shared(
+    const AttnArgs args) {
+  typedef TileLds<DP> Lds;
+  typedef RowsLds<T, VW, NB, 4, true> Rows;
+  constexpr int TILES = 5 * Lds::TILEB;
+  __shared__ __attribute__((aligned(1024))) char pool[TILES > Rows::BYTES ? TILES : Rows::BYTES];
+  // (each with a copy of its own: one that both changed would hold its values
+  // in scalars that neither has left)
+  if (blockIdx.x < args.pre_blocks) {
+    AttnArgs a = args;
+    attn_prefix_call(a);
+    attn_tile_block<T, DP, ATTN_FORMS>(a, blockIdx.x, pool, pool + 3 * Lds::TILEB, pool);
+  } else {
+    AttnArgs a = args;
+    a.groups = nullptr;
+    attn_rows_block<T, VW, NB, 4, true, ATTN_FORMS>(a, blockIdx.x - args.pre_blocks, pool);
+  }
+}
+
+template <class T> void shared_of(hipStream_t st, const AttnArgs &a, unsigned g) {
+  if (a.d <= 64)
+    k_attn_shared<T, 64, 4, 1><<<g, 64 * TILE_WAVES, 0, st>>>(a);
+  else if (a.d <= 96)
+    k_attn_shared<T, 96, 8, 1><<<g, 64 * TILE_WAVES, 0, st>>>(a);
+  else
+    k_attn_shared<T, 128, 8, 1><<<g, 64 * TILE_WAVES, 0, st>>>(a);
+}
+
+}  // namespace
+
+void launch_attn_shared(vsk_ctx *ctx, hipStream_t st, const AttnArgs &a, int32_t t) {
+  const int64_t grid = a.pre_blocks + (int64_t)a.n * a.splits * a.tiles * a.kv_heads;
+  VSK_REQUIRE(grid <= 0x7FFFFFFFll, VSK_ERR_INVALID_BUFFER_SIZE, "too many query rows in one call");
+  KernelTimer kt(ctx, "attn_shared", (double)a.tokens * a.heads, st);
+  if (t == VSK_DTYPE_F16)
+    shared_of<_Float16>(st, a, (unsigned)grid);
+  else
+    shared_of<__bf16>(st, a, (unsigned)grid);
+  check_launch("attn_shared");
+}
+
+}  // namespace vsk

@@ -34,7 +34,9 @@ typedef __attribute__((ext_vector_type(4))) float f4;
 // DT: dimensions in blocks of 32 (the queries of more than 128 would not fit
 // the registers), padded to PITCH in LDS
 template <int DT>
-__global__ __launch_bounds__(64 * NW, 2) void k_attn_tile32(const AttnArgs a) {
+__global__ __launch_bounds__(64 * NW, 2) void k_attn_tile32(const AttnArgs args) {
+  AttnArgs a = args;
+  uint32_t at = attn_call(a, blockIdx.x);
   constexpr int PITCH = DT <= 2 ? 64 : 128;
   constexpr int CH = PITCH / 4;              // 16-byte pieces of a row
   constexpr int ROWB = 4 * PITCH;
@@ -50,7 +52,6 @@ __global__ __launch_bounds__(64 * NW, 2) void k_attn_tile32(const AttnArgs a) {
 
   const int lane = threadIdx.x & 63, h2 = lane >> 5, n = lane & 31;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  uint32_t at = blockIdx.x;
   const int32_t h = at % a.kv_heads;
   at /= a.kv_heads;
   const int32_t tile = a.tiles - 1 - (int32_t)(at % a.tiles);
@@ -350,7 +351,7 @@ __global__ __launch_bounds__(64 * NW, 2) void k_attn_tile32(const AttnArgs a) {
 }  // namespace
 
 void launch_attn_tile32(vsk_ctx *ctx, hipStream_t st, const AttnArgs &a) {
-  const int64_t grid = (int64_t)a.n * a.splits * a.tiles * a.kv_heads;
+  const int64_t grid = a.pre_blocks + (int64_t)a.n * a.splits * a.tiles * a.kv_heads;
   VSK_REQUIRE(grid <= 0x7FFFFFFFll, VSK_ERR_INVALID_BUFFER_SIZE, "too many query rows in one call");
   KernelTimer kt(ctx, "attn_tile32", (double)a.tokens * a.heads, st);
   const unsigned g = (unsigned)grid;
