@@ -130,6 +130,7 @@ Plan plan_of(const vsk_ctx *ctx, const vsk_kv *kv, const vsk_attention_args *arg
     // 128 on 8 (us): 512 tokens (128 blocks) 519 / 284, 2,000 (504) 893 / 998.
     per = 16;
     want = 2 * blocks > cus ? 1 : 2 * cus;
+    if (span.joined && span.all) { const char *e = getenv("WA"); if (e) want = atoi(e) * cus / 2; }
     if (kv->dtype == VSK_DTYPE_F32) want = getenv("W32") ? atoi(getenv("W32")) * cus : 12 * cus;
   } else {
     // A tile for each of the four waves that share a part at least.  Contexts

@@ -67,7 +67,7 @@ struct AttnArgs {
   int32_t part0;        // the call's first part
   // two calls in one launch: the first pre_blocks blocks are those of a call
   // over prefixes, which differs in these
-  uint32_t pre_blocks;
+  uint32_t pre_blocks, own_blocks;
   struct {
     int32_t n, max_new, tiles, splits, chunk;
   } pre;
@@ -394,7 +394,7 @@ constexpr int ATTN_TILE32_KEYS = 32;
 void launch_attn_tile32(vsk_ctx *ctx, hipStream_t stream, const AttnArgs &a);
 // attn_shared.hip: 16 bits, aligned, heads to 128: a.pre by row tiles of ATTN_TILE_ROWS, the
 // call itself by those of 16, four waves each
-void launch_attn_shared(vsk_ctx *ctx, hipStream_t stream, const AttnArgs &a, int32_t t);
+void launch_attn_shared(vsk_ctx *ctx, hipStream_t stream, AttnArgs a, int32_t t);
 // joins the parts that row tiles of `rows` rows left: 16 (launch_attn_rows) or
 // ATTN_TILE_ROWS
 void launch_attn_join(vsk_ctx *ctx, hipStream_t stream, const AttnArgs &a, int32_t t,

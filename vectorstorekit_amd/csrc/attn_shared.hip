@@ -17,16 +17,25 @@ __global__ __launch_bounds__(64 * TILE_WAVES, 2) void k_attn_shared(
   typedef RowsLds<T, VW, NB, 4, true> Rows;
   constexpr int TILES = 5 * Lds::TILEB;
   __shared__ __attribute__((aligned(1024))) char pool[TILES > Rows::BYTES ? TILES : Rows::BYTES];
+  // Eight blocks (one an XCD) of the one, eight of the other, in turn, and the
+  // other way round from 32 such on, so that a compute unit (an XCD has 32, which
+  // get their second block when each has its first) has one of each.
+  const uint32_t pre = (args.pre_blocks + 7) / 8, own = (args.own_blocks + 7) / 8;
+  const uint32_t both = pre < own ? pre : own, g = blockIdx.x / 8;
+  const bool paired = g < 2 * both;
+  const bool prefix = paired ? (g ^ g >> 5) & 1 : pre > own;
+  const uint32_t block = 8 * (paired ? g / 2 : g - both) + blockIdx.x % 8;
+  if (block >= (prefix ? args.pre_blocks : args.own_blocks)) return;
   // (each with a copy of its own: one that both changed would hold its values
   // in scalars that neither has left)
-  if (blockIdx.x < args.pre_blocks) {
+  if (prefix) {
     AttnArgs a = args;
     attn_prefix_call(a);
-    attn_tile_block<T, DP, ATTN_FORMS>(a, blockIdx.x, pool, pool + 3 * Lds::TILEB, pool);
+    attn_tile_block<T, DP, ATTN_FORMS>(a, block, pool, pool + 3 * Lds::TILEB, pool);
   } else {
     AttnArgs a = args;
     a.groups = nullptr;
-    attn_rows_block<T, VW, NB, 4, true, ATTN_FORMS>(a, blockIdx.x - args.pre_blocks, pool);
+    attn_rows_block<T, VW, NB, 4, true, ATTN_FORMS>(a, block, pool);
   }
 }
 
@@ -41,8 +50,10 @@ template <class T> void shared_of(hipStream_t st, const AttnArgs &a, unsigned g)
 
 }  // namespace
 
-void launch_attn_shared(vsk_ctx *ctx, hipStream_t st, const AttnArgs &a, int32_t t) {
-  const int64_t grid = a.pre_blocks + (int64_t)a.n * a.splits * a.tiles * a.kv_heads;
+void launch_attn_shared(vsk_ctx *ctx, hipStream_t st, AttnArgs a, int32_t t) {
+  const int64_t own = (int64_t)a.n * a.splits * a.tiles * a.kv_heads;
+  const int64_t grid = 8 * (ceil_div(a.pre_blocks, 8) + ceil_div(own, 8));
+  a.own_blocks = (uint32_t)own;
   VSK_REQUIRE(grid <= 0x7FFFFFFFll, VSK_ERR_INVALID_BUFFER_SIZE, "too many query rows in one call");
   KernelTimer kt(ctx, "attn_shared", (double)a.tokens * a.heads, st);
   if (t == VSK_DTYPE_F16)
