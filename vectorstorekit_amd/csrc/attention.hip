@@ -83,7 +83,9 @@ Plan plan_of(const vsk_ctx *ctx, const vsk_kv *kv, const vsk_attention_args *arg
     row_tile = ATTN_TILE_ROWS;
     key_tile = attn_tile_keys(kv->head_dim);
   }
-  if (kv->dtype == VSK_DTYPE_F32 && (span.all || span.joined) && rows >= (getenv("R32") ? atoi(getenv("R32")) : 96) &&
+  // In 32 bits such tiles are for rows that share their keys (two thirds of a
+  // tile at least: 6 groups of up to 90 rows 160 us, in tiles of 16 110).
+  if (kv->dtype == VSK_DTYPE_F32 && (span.all || span.joined) && rows >= 96 &&
       kv->head_dim <= 128 && aligned_operands(kv, args)) {
     p.tile = true;
     row_tile = ATTN_TILE_ROWS;
@@ -129,9 +131,13 @@ Plan plan_of(const vsk_ctx *ctx, const vsk_kv *kv, const vsk_attention_args *arg
     // fit or less would work.  Unsplit / split after 30,000 keys, 32 heads of
     // 128 on 8 (us): 512 tokens (128 blocks) 519 / 284, 2,000 (504) 893 / 998.
     per = 16;
-    want = 2 * blocks > cus ? 1 : 2 * cus;
-    if (span.joined && span.all) { const char *e = getenv("WA"); if (e) want = atoi(e) * cus / 2; }
-    if (kv->dtype == VSK_DTYPE_F32) want = getenv("W32") ? atoi(getenv("W32")) * cus : 12 * cus;
+    // A prefix's tiles have the other half of each compute unit's room to the
+    // sequences' own keys (64 branches of 32,768, want of 1, 2 and 4 halves: 99,
+    // 70 and 81 us).
+    want = 2 * blocks > cus ? 1 : span.joined && span.all ? cus : 2 * cus;
+    // In 32 bits a tile takes so long that ragged texts are divided for their
+    // balance (7 of up to 500 against 3,001 keys, want 2 and 12: 575 / 501 us).
+    if (kv->dtype == VSK_DTYPE_F32) want = 12 * cus;
   } else {
     // A tile for each of the four waves that share a part at least.  Contexts
     // differ in length, so several rounds of blocks share the work more evenly
@@ -141,7 +147,9 @@ Plan plan_of(const vsk_ctx *ctx, const vsk_kv *kv, const vsk_attention_args *arg
     // of 64 8 / 192, 16 / 164, 24 / 203; 17 of 16 f32 heads of 96, window
     // 2,048, 2 / 76, 6 / 86; 60 to 2,000 of 2 heads of 256 1 / 38, 4 / 47.  No
     // more than 64 parts a row, while there is a block for every compute unit:
-    // 2 contexts of 100,000 of 8 heads of 128 121 us, in 96 parts 129.
+    // 2 contexts of 100,000 of 8 heads of 128 121 us, in 96 parts 129.  Where a
+    // join follows anyway 32-bit rows, whose steps are long, take more (6 groups
+    // of drafts, 2 / 8: 216 / 138).
     per = 4;
     const int64_t most = kv->head_dim <= 64 ? 16 : kv->head_dim > 128 ? 1
                          : kv->dtype != VSK_DTYPE_F32 ? 6 : span.joined ? 8 : 2;
