@@ -233,56 +233,73 @@ __global__ __launch_bounds__(256, FN * FM >= 16 ? 1 : 2) void k_int8_tile(const 
     }
   }
   const int32_t steps = a.blocks / STEP;
-  auto bring = [&](int32_t s) {  // in order of s: the addresses go along
-    lds_char *to = lds + (s % STAGES) * STAGE + MINE * w * STEP * BLOCK;
-#pragma unroll
-    for (int i = 0; i < MINE; ++i) {
-#pragma unroll
-      for (int j = 0; j < STEP; ++j)
-        load_to_lds(base[i] + j * BLOCK, 16 * lane, to + (i * STEP + j) * BLOCK);
-      base[i] += STEP * BLOCK;
-    }
+  // one of the loads that bring step s, in order of s: the addresses go along
+  auto bring = [&](int32_t s, int x) {
+    load_to_lds(base[x / STEP] + x % STEP * BLOCK, 16 * lane,
+                lds + (s % STAGES) * STAGE + (MINE * w * STEP + x) * BLOCK);
+    if (x % STEP == STEP - 1) base[x / STEP] += STEP * BLOCK;
   };
   i32x4 f[2][FN + FM];
-  auto read = [&](i32x4 (&g)[FN + FM], int32_t s, int j) {
-    const lds_char *at = lds + (s % STAGES) * STAGE + j * BLOCK + 16 * lane;
-#pragma unroll
-    for (int i = 0; i < FN; ++i)
-      g[i] = *(const lds_as i32x4 *)(at + (FN * wn + i) * STEP * BLOCK);
-#pragma unroll
-    for (int i = 0; i < FM; ++i)
-      g[FN + i] = *(const lds_as i32x4 *)(at + (2 * FN + FM * wm + i) * STEP * BLOCK);
+  // operand x of the step's inner block j
+  auto read = [&](int32_t s, int j, int x) {
+    const int r = x < FN ? FN * wn + x : 2 * FN + FM * wm + x - FN;
+    return *(const lds_as i32x4 *)(lds + (s % STAGES) * STAGE + (r * STEP + j) * BLOCK + 16 * lane);
   };
   i32x16 acc[FN][FM];
 #pragma unroll
   for (int i = 0; i < FN; ++i)
 #pragma unroll
     for (int j = 0; j < FM; ++j) acc[i][j] = i32x16{};
-  auto multiply = [&](const i32x4 (&g)[FN + FM]) {
+  // The products of one inner block, with beside them, a piece after each
+  // product, the reads of the next block's operands and the loads of a later
+  // step (left to itself the compiler puts all of them before).
+  constexpr int PRODUCTS = FN * FM, PIECES_MAX = FN + FM > LOADS ? FN + FM : LOADS;
+  auto multiply = [&](const i32x4 (&g)[FN + FM], auto &&piece) {
+    constexpr int TURNS = PRODUCTS > PIECES_MAX ? PRODUCTS : PIECES_MAX;
 #pragma unroll
-    for (int i = 0; i < FN; ++i)
-#pragma unroll
-      for (int j = 0; j < FM; ++j)
-        acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(g[i], g[FN + j], acc[i][j], 0, 0, 0);
+    for (int x = 0; x < TURNS; ++x) {
+      if (x < PRODUCTS)
+        acc[x / FM][x % FM] = __builtin_amdgcn_mfma_i32_32x32x32_i8(
+            g[x / FM], g[FN + x % FM], acc[x / FM][x % FM], 0, 0, 0);
+      __builtin_amdgcn_sched_barrier(0);
+      piece(x);
+      __builtin_amdgcn_sched_barrier(0);
+    }
   };
 #pragma unroll
   for (int s = 0; s < STAGES - 1; ++s)
-    if (s < steps) bring(s);
+    if (s < steps)
+#pragma unroll
+      for (int x = 0; x < LOADS; ++x) bring(s, x);
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-  read(f[0], 0, 0);
+#pragma unroll
+  for (int x = 0; x < FN + FM; ++x) f[0][x] = read(0, 0, x);
+  auto first_half = [&](int32_t s) {
+    multiply(f[0], [&](int x) {
+      if (x < FN + FM) f[1][x] = read(s, 1, x);
+    });
+  };
+  // Between a step's halves the next step's blocks have arrived, for every
+  // wave, and every wave has read the last step's, whose place the step after
+  // the next two takes.
+  int32_t s = 0;
 #pragma unroll 1
-  for (int32_t s = 0; s < steps; ++s) {
-    read(f[1], s, 1);
-    multiply(f[0]);
-    // the next step's blocks have arrived, for every wave, and every wave has
-    // read the last step's, whose place the step after the next two takes
-    if (s + 2 < steps)
-      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LOADS) : "memory");
-    else
-      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    if (s + STAGES - 1 < steps) bring(s + STAGES - 1);
-    if (s + 1 < steps) read(f[0], s + 1, 0);
-    multiply(f[1]);
+  for (; s < steps - (STAGES - 1); ++s) {
+    first_half(s);
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LOADS) : "memory");
+    multiply(f[1], [&](int x) {
+      if (x < FN + FM) f[0][x] = read(s + 1, 0, x);
+      if (x < LOADS) bring(s + STAGES - 1, x);
+    });
+  }
+  // (behind the last step's reads is a step read before: its products are not made)
+#pragma unroll 1
+  for (; s < steps; ++s) {
+    first_half(s);
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    multiply(f[1], [&](int x) {
+      if (x < FN + FM) f[0][x] = read(s + 1, 0, x);
+    });
   }
   __syncthreads();
   // The sums leave by way of LDS, this wave's own part of it, so that a store
