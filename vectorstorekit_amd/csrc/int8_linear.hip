@@ -13,6 +13,14 @@
 // block is one load of a wave, contiguous in memory and in LDS, with no bank
 // met twice.  Weights are brought into that order once, activations by the
 // kernel that quantises them.
+//
+// What bounds it: few tokens, the weights' bytes and the launches (one token
+// through 4,096 x 4,096 5.7 us, 64 through 4,096 x 12,288 14.5, of which the
+// weights alone are 8.7 at 5.8 TB/s); many, the matrix cores: 16,384 tokens
+// through 4,096 x 12,288 take 43 us to quantise and 740 for the products, 2,230
+// TOPS, at which the card holds its power limit and 1.8 GHz.
+#include <type_traits>
+
 #include "attn.hpp"
 #include "vsk_api.hpp"
 
@@ -24,32 +32,35 @@ typedef __attribute__((ext_vector_type(4))) int i32x4;
 typedef __attribute__((ext_vector_type(16))) int i32x16;
 
 constexpr int BLOCK = 1024;       // bytes of a 32 x 32 block
-constexpr int STEP = 2;           // blocks of a step along the inner dimension
+constexpr int FILL = 2;           // the inner dimension is filled up to so many blocks
 constexpr int32_t MOST = 131072;  // inner places whose sums (128 * 127 each) fit 32 bits
 
-int64_t inner_blocks(int64_t k) { return ceil_div(k, 32 * STEP) * STEP; }
+int64_t inner_blocks(int64_t k) { return ceil_div(k, 32 * FILL) * FILL; }
 int64_t packed_bytes(int64_t rows, int64_t k) {
   return ceil_div(rows, 32) * inner_blocks(k) * BLOCK;
 }
 
 // ------------------------------------------------------------------ quantising
 
-// 16 values of a row from element e on, zero past the end
+// 16 values of a row, as they are in memory
+template <class T> struct Piece {
+  static constexpr int W = 16 / sizeof(T);
+  typedef __attribute__((ext_vector_type(W))) T V;
+  V v[16 / W];
+  __device__ float operator[](int i) const { return (float)v[i / W][i % W]; }
+};
+// those from element e on, zero past the end
 template <class T, bool ALIGNED>
-__device__ inline void load16(const T *row, int32_t e, int32_t k, float (&x)[16]) {
+__device__ inline void load16(const T *row, int32_t e, int32_t k, Piece<T> &x) {
+  constexpr int W = Piece<T>::W;
   if (ALIGNED && e + 16 <= k) {
-    constexpr int W = 16 / sizeof(T);
-    typedef __attribute__((ext_vector_type(W))) T V;
 #pragma unroll
-    for (int i = 0; i < 16 / W; ++i) {
-      const V v = *reinterpret_cast<const V *>(row + e + W * i);
-#pragma unroll
-      for (int j = 0; j < W; ++j) x[W * i + j] = (float)v[j];
-    }
+    for (int i = 0; i < 16 / W; ++i)
+      x.v[i] = *reinterpret_cast<const typename Piece<T>::V *>(row + e + W * i);
     return;
   }
 #pragma unroll
-  for (int i = 0; i < 16; ++i) x[i] = e + i < k ? (float)row[e + i] : 0.f;
+  for (int i = 0; i < 16; ++i) x.v[i / W][i % W] = e + i < k ? row[e + i] : (T)0.f;
 }
 
 // What a row's codes are made with.  The largest magnitude is compared as its
@@ -67,15 +78,9 @@ __device__ inline RowScale row_scale(uint32_t top) {
   r.scale = top >= 0x7F800000u ? __uint_as_float(0x7FC00000u) : t / 127.f;
   return r;
 }
-__device__ inline uint32_t code4(const float *x, const RowScale &r) {
-  uint32_t w = 0;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    // (the largest is 127 times 1 + 2^-22 at most; NaN times 0 is not taken)
-    const int c = r.inverse == 0.f ? 0 : (int)__builtin_rintf(x[i] * r.up * r.inverse);
-    w |= (uint32_t)(c & 255) << (8 * i);
-  }
-  return w;
+__device__ inline uint32_t code(float x, const RowScale &r) {
+  // (the largest is 127 times 1 + 2^-22 at most; NaN times 0 is not taken)
+  return (r.inverse == 0.f ? 0 : (int)__builtin_rintf(x * r.up * r.inverse)) & 255;
 }
 
 struct PackArgs {
@@ -86,7 +91,7 @@ struct PackArgs {
   int32_t k, blocks;  // inner places, inner blocks
 };
 
-template <class T> __device__ inline uint32_t magnitude(const float (&x)[16]) {
+template <class T> __device__ inline uint32_t magnitude(const Piece<T> &x) {
   uint32_t top = 0;
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
@@ -96,35 +101,36 @@ template <class T> __device__ inline uint32_t magnitude(const float (&x)[16]) {
   return top;
 }
 
-// WPR waves a row (4 / WPR rows a workgroup).  A lane takes pieces of 16
-// places; the first HELD of them stay in registers between the two passes.
-template <class T, int WPR, bool ALIGNED>
-__global__ __launch_bounds__(256) void k_int8_quantize(const PackArgs a) {
-  constexpr int HELD = sizeof(T) == 4 ? 4 : 8;
-  const int w = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const int64_t row = (int64_t)blockIdx.x * (4 / WPR) + w / WPR;
-  const int at = WPR > 1 ? threadIdx.x : lane;
-  const int pieces = 2 * a.blocks;
-  const bool real = row < a.rows;
-  const T *x = static_cast<const T *>(a.x) + (real ? row * a.x_row : 0);
-  const int32_t k = real ? a.k : 0;
-  float held[HELD][16];
+template <class T> __device__ inline u32x4 code16(const Piece<T> &y, const RowScale &r) {
+  u32x4 c;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    c[i] = code(y[4 * i], r) | code(y[4 * i + 1], r) << 8 | code(y[4 * i + 2], r) << 16 |
+           code(y[4 * i + 3], r) << 24;
+  return c;
+}
+
+// the largest magnitude of a row whose pieces of 16 places a lane takes `step`
+// apart from `at` on; the first HELD of them stay in registers
+template <class T, bool ALIGNED, int HELD>
+__device__ inline uint32_t largest(const T *x, int32_t k, int pieces, int at, int step,
+                                   Piece<T> (&held)[HELD]) {
   uint32_t top = 0;
 #pragma unroll
   for (int i = 0; i < HELD; ++i) {
-    const int p = at + 64 * WPR * i;
+    const int p = at + step * i;
     if (p < pieces) load16<T, ALIGNED>(x, 16 * p, k, held[i]);
   }
 #pragma unroll
   for (int i = 0; i < HELD; ++i)
-    if (at + 64 * WPR * i < pieces) {
-      const uint32_t t = magnitude<T>(held[i]);
+    if (at + step * i < pieces) {
+      const uint32_t t = magnitude(held[i]);
       top = t > top ? t : top;
     }
-  for (int p = at + 64 * WPR * HELD; p < pieces; p += 64 * WPR) {
-    float y[16];
+  for (int p = at + step * HELD; p < pieces; p += step) {
+    Piece<T> y;
     load16<T, ALIGNED>(x, 16 * p, k, y);
-    const uint32_t t = magnitude<T>(y);
+    const uint32_t t = magnitude(y);
     top = t > top ? t : top;
   }
 #pragma unroll
@@ -132,30 +138,79 @@ __global__ __launch_bounds__(256) void k_int8_quantize(const PackArgs a) {
     const uint32_t t = __shfl_xor(top, o);
     top = t > top ? t : top;
   }
-  if constexpr (WPR > 1) {
-    __shared__ uint32_t tops[4];
-    if (lane == 0) tops[w] = top;
-    __syncthreads();
+  return top;
+}
+
+template <class T> constexpr int HELD_PIECES = sizeof(T) == 4 ? 4 : 8;
+
+// Few rows: a workgroup a row.
+template <class T, bool ALIGNED>
+__global__ __launch_bounds__(256) void k_int8_quantize_row(const PackArgs a) {
+  constexpr int HELD = HELD_PIECES<T>;
+  const int64_t row = blockIdx.x;
+  const int pieces = 2 * a.blocks;
+  const T *x = static_cast<const T *>(a.x) + row * a.x_row;
+  Piece<T> held[HELD];
+  uint32_t top = largest<T, ALIGNED, HELD>(x, a.k, pieces, threadIdx.x, 256, held);
+  __shared__ uint32_t tops[4];
+  if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
+  __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 4; ++i) top = tops[i] > top ? tops[i] : top;
-  }
-  if (!real) return;
+  for (int i = 0; i < 4; ++i) top = tops[i] > top ? tops[i] : top;
   const RowScale r = row_scale(top);
-  if (at == 0) a.scales[row] = r.scale;
+  if (threadIdx.x == 0) a.scales[row] = r.scale;
   char *to = a.packed + (row >> 5) * a.blocks * BLOCK + (row & 31) * 16;
-  auto put = [&](int p, const float (&y)[16]) {
-    u32x4 c;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) c[i] = code4(y + 4 * i, r);
-    *reinterpret_cast<u32x4 *>(to + (int64_t)(p >> 1) * BLOCK + (p & 1) * 512) = c;
+  for (int i = 0; i < HELD; ++i) {
+    const int p = threadIdx.x + 256 * i;
+    if (p < pieces)
+      *reinterpret_cast<u32x4 *>(to + (int64_t)(p >> 1) * BLOCK + (p & 1) * 512) =
+          code16(held[i], r);
+  }
+  for (int p = threadIdx.x + 256 * HELD; p < pieces; p += 256) {
+    Piece<T> y;
+    load16<T, ALIGNED>(x, 16 * p, a.k, y);
+    *reinterpret_cast<u32x4 *>(to + (int64_t)(p >> 1) * BLOCK + (p & 1) * 512) = code16(y, r);
+  }
+}
+
+// Many rows: eight a workgroup, a wave each.  Their codes leave by way of LDS, so
+// that a store has whole lines.  The values wait for their row's largest in the
+// type that they came in: as 32-bit numbers they leave room for half as many
+// waves (16,384 tokens of 4,096 in bf16 58 us, so 43; read and written at a
+// copy's rate it would be 39).
+constexpr int PACK_ROWS = 8;
+template <class T, bool ALIGNED>
+__global__ __launch_bounds__(64 * PACK_ROWS) void k_int8_quantize(const PackArgs a) {
+  constexpr int HELD = HELD_PIECES<T>;
+  __shared__ __attribute__((aligned(16))) u32x4 codes[2][64 * PACK_ROWS];
+  const int w = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int64_t row0 = (int64_t)blockIdx.x * PACK_ROWS, row = row0 + w;
+  const int pieces = 2 * a.blocks;
+  const bool real = row < a.rows;
+  const T *x = static_cast<const T *>(a.x) + (real ? row * a.x_row : 0);
+  const int32_t k = real ? a.k : 0;
+  Piece<T> held[HELD];
+  const RowScale r = row_scale(largest<T, ALIGNED, HELD>(x, k, pieces, lane, 64, held));
+  if (real && lane == 0) a.scales[row] = r.scale;
+  char *to = a.packed + (row0 >> 5) * a.blocks * BLOCK + (row0 & 31) * 16;
+  // 64 pieces of the eight rows: piece p of row y is in slot y ^ (p % 8) of its eight
+  auto put = [&](int i, const Piece<T> &y) {
+    u32x4 *buf = codes[i & 1];
+    buf[lane * 8 + (w ^ (lane & 7))] = code16(y, r);
+    __syncthreads();  // (the other buffer's readers have passed the one before)
+    const int z = threadIdx.x >> 3, q = threadIdx.x & 7, p = 64 * i + z;
+    if (p < pieces && row0 + q < a.rows)
+      *reinterpret_cast<u32x4 *>(to + (int64_t)(p >> 1) * BLOCK + (p & 1) * 512 + 16 * q) =
+          buf[z * 8 + (q ^ (z & 7))];
   };
 #pragma unroll
   for (int i = 0; i < HELD; ++i)
-    if (at + 64 * WPR * i < pieces) put(at + 64 * WPR * i, held[i]);
-  for (int p = at + 64 * WPR * HELD; p < pieces; p += 64 * WPR) {
-    float y[16];
-    load16<T, ALIGNED>(x, 16 * p, k, y);
-    put(p, y);
+    if (64 * i < pieces) put(i, held[i]);
+  for (int i = HELD; 64 * i < pieces; ++i) {
+    Piece<T> y;
+    load16<T, ALIGNED>(x, 16 * (64 * i + lane), k, y);
+    put(i, y);
   }
 }
 
@@ -196,20 +251,20 @@ struct LinearArgs {
   bool wide;            // the outputs take 16-byte stores
 };
 
+// (the weights' scale first: a large token's scale alone could take a sum past f32)
 __device__ inline float scaled(int sum, float xs, float ws, float bias) {
-  return (float)sum * xs * ws + bias;
+  return (float)sum * ws * xs + bias;
 }
 
 // A tile of 64 FN channels and 64 FM tokens, four waves of FN x FM products of
 // 32 x 32: lane l has token l % 32 and, in register 4 q + i, channel
 // 8 q + 4 (l / 32) + i.
-template <class T, int FN, int FM>
+template <class T, int FN, int FM, int STEP, int STAGES>
 __global__ __launch_bounds__(256, FN * FM >= 16 ? 1 : 2) void k_int8_tile(const LinearArgs a) {
   constexpr int ROWS = 2 * (FN + FM);            // row blocks of a stage
   constexpr int STAGE = ROWS * STEP * BLOCK;     // bytes of it
-  constexpr int STAGES = 4;
-  constexpr int MINE = ROWS / 4;                 // row blocks that a wave brings
-  constexpr int LOADS = MINE * STEP;
+  constexpr int LOADS = ROWS * STEP / 4;         // blocks of it that a wave brings
+  static_assert(ROWS * STEP % 4 == 0 && STEP % 2 == 0 && FILL % STEP == 0, "");
   constexpr int PITCH = FN * 32 * 4 + 16;        // of a token's sums in LDS, in bytes
   constexpr int OUT = 4 * 32 * PITCH;
   __shared__ __attribute__((aligned(1024))) char lds_pool[STAGES * STAGE > OUT ? STAGES * STAGE : OUT];
@@ -219,25 +274,26 @@ __global__ __launch_bounds__(256, FN * FM >= 16 ? 1 : 2) void k_int8_tile(const 
   const int wn = w & 1, wm = w >> 1;
   const int32_t tn = blockIdx.x % a.tiles_n;
   const int64_t tm = blockIdx.x / a.tiles_n;
-  // the row blocks that this wave brings: the channels' first
-  uint64_t base[MINE];
+  // the blocks that this wave brings: the channels' first
+  uint64_t base[LOADS];
 #pragma unroll
-  for (int i = 0; i < MINE; ++i) {
-    const int r = MINE * w + i;
+  for (int x = 0; x < LOADS; ++x) {
+    const int r = (LOADS * w + x) / STEP, j = (LOADS * w + x) % STEP;
     if (r < 2 * FN) {
       const int32_t b = 2 * FN * tn + r;
-      base[i] = (uint64_t)(uintptr_t)a.w + (int64_t)(b < a.w_blocks ? b : a.w_blocks - 1) * a.blocks * BLOCK;
+      base[x] = (uint64_t)(uintptr_t)a.w +
+                ((int64_t)(b < a.w_blocks ? b : a.w_blocks - 1) * a.blocks + j) * BLOCK;
     } else {
       const int64_t b = 2 * FM * tm + r - 2 * FN;
-      base[i] = (uint64_t)(uintptr_t)a.x + (b < a.x_blocks ? b : a.x_blocks - 1) * a.blocks * BLOCK;
+      base[x] = (uint64_t)(uintptr_t)a.x +
+                ((b < a.x_blocks ? b : a.x_blocks - 1) * a.blocks + j) * BLOCK;
     }
   }
   const int32_t steps = a.blocks / STEP;
   // one of the loads that bring step s, in order of s: the addresses go along
   auto bring = [&](int32_t s, int x) {
-    load_to_lds(base[x / STEP] + x % STEP * BLOCK, 16 * lane,
-                lds + (s % STAGES) * STAGE + (MINE * w * STEP + x) * BLOCK);
-    if (x % STEP == STEP - 1) base[x / STEP] += STEP * BLOCK;
+    load_to_lds(base[x], 16 * lane, lds + (s % STAGES) * STAGE + (LOADS * w + x) * BLOCK);
+    base[x] += STEP * BLOCK;
   };
   i32x4 f[2][FN + FM];
   // operand x of the step's inner block j
@@ -274,19 +330,21 @@ __global__ __launch_bounds__(256, FN * FM >= 16 ? 1 : 2) void k_int8_tile(const 
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
 #pragma unroll
   for (int x = 0; x < FN + FM; ++x) f[0][x] = read(0, 0, x);
-  auto first_half = [&](int32_t s) {
-    multiply(f[0], [&](int x) {
-      if (x < FN + FM) f[1][x] = read(s, 1, x);
-    });
+  auto up_to_last = [&](int32_t s) {
+#pragma unroll
+    for (int j = 0; j < STEP - 1; ++j)
+      multiply(f[j & 1], [&](int x) {
+        if (x < FN + FM) f[(j + 1) & 1][x] = read(s, j + 1, x);
+      });
   };
-  // Between a step's halves the next step's blocks have arrived, for every
-  // wave, and every wave has read the last step's, whose place the step after
-  // the next two takes.
+  // Before a step's last block the next step's blocks have arrived, for every
+  // wave, and every wave has read the last step's, whose place the step
+  // STAGES - 1 on takes.
   int32_t s = 0;
 #pragma unroll 1
   for (; s < steps - (STAGES - 1); ++s) {
-    first_half(s);
-    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LOADS) : "memory");
+    up_to_last(s);
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((STAGES - 3) * LOADS) : "memory");
     multiply(f[1], [&](int x) {
       if (x < FN + FM) f[0][x] = read(s + 1, 0, x);
       if (x < LOADS) bring(s + STAGES - 1, x);
@@ -295,7 +353,7 @@ __global__ __launch_bounds__(256, FN * FM >= 16 ? 1 : 2) void k_int8_tile(const 
   // (behind the last step's reads is a step read before: its products are not made)
 #pragma unroll 1
   for (; s < steps; ++s) {
-    first_half(s);
+    up_to_last(s);
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
     multiply(f[1], [&](int x) {
       if (x < FN + FM) f[0][x] = read(s + 1, 0, x);
@@ -376,16 +434,43 @@ __global__ __launch_bounds__(64 * WAVES) void k_int8_few(const LinearArgs a) {
   i32x16 acc[F];
 #pragma unroll
   for (int j = 0; j < F; ++j) acc[j] = i32x16{};
-#pragma unroll 4
-  for (int32_t b = w; b < a.blocks; b += WAVES) {
-    const i32x4 y = *reinterpret_cast<const i32x4 *>(wp + (int64_t)b * BLOCK);
+  // AHEAD inner blocks in flight
+  constexpr int AHEAD = F == 1 ? 8 : 6;
+  i32x4 y[AHEAD], z[AHEAD][F];
+  auto load = [&](int i, int32_t b) {
+    y[i] = *reinterpret_cast<const i32x4 *>(wp + (int64_t)b * BLOCK);
 #pragma unroll
-    for (int j = 0; j < F; ++j) {
+    for (int j = 0; j < F; ++j)
       // (tokens that are not there: nothing is read for them)
-      i32x4 z = {0, 0, 0, 0};
-      if (have[j]) z = *reinterpret_cast<const i32x4 *>(xp[j] + (int64_t)b * BLOCK);
-      acc[j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(y, z, acc[j], 0, 0, 0);
+      if (have[j]) z[i][j] = *reinterpret_cast<const i32x4 *>(xp[j] + (int64_t)b * BLOCK);
+  };
+  auto step = [&](int i) {
+#pragma unroll
+    for (int j = 0; j < F; ++j)
+      acc[j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(y[i], z[i][j], acc[j], 0, 0, 0);
+  };
+#pragma unroll
+  for (int i = 0; i < AHEAD; ++i)
+#pragma unroll
+    for (int j = 0; j < F; ++j) z[i][j] = i32x4{0, 0, 0, 0};
+#pragma unroll
+  for (int i = 0; i < AHEAD; ++i)
+    if (w + WAVES * i < a.blocks) load(i, w + WAVES * i);
+  int32_t b = w;
+#pragma unroll 1
+  for (; b + WAVES * (2 * AHEAD - 1) < a.blocks; b += WAVES * AHEAD)
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      step(i);
+      load(i, b + WAVES * (AHEAD + i));
     }
+#pragma unroll
+  for (int i = 0; i < AHEAD; ++i)
+    if (b + WAVES * i < a.blocks) step(i);
+#pragma unroll 4
+  for (b += WAVES * AHEAD; b < a.blocks; b += WAVES) {
+    load(0, b);
+    step(0);
   }
 #pragma unroll
   for (int j = 0; j < F; ++j) {
@@ -408,22 +493,141 @@ __global__ __launch_bounds__(64 * WAVES) void k_int8_few(const LinearArgs a) {
   }
 }
 
+// A few tokens at once with their quantising: every workgroup quantises them
+// for itself, into LDS, while its first weights are on their way.  One launch,
+// whose latency is what such a call takes (one token through 4,096 x 4,096 5.7 us, in
+// two launches 10.8).
+struct TokenArgs {
+  LinearArgs l;
+  const void *x;
+  int64_t x_row;
+  int32_t k, pitch;  // bytes of a token's codes in LDS
+};
+template <class X, class T, int M, bool ALIGNED>
+__global__ __launch_bounds__(1024) void k_int8_token(const TokenArgs t) {
+  constexpr int WAVES = 16, AHEAD = 8;
+  const LinearArgs &a = t.l;
+  extern __shared__ __attribute__((aligned(16))) char token_lds[];  // codes, then sums
+  __shared__ uint32_t tops[M];
+  const int lane = threadIdx.x & 63;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int32_t nb = blockIdx.x;
+  const char *wp = a.w + (int64_t)nb * a.blocks * BLOCK + 16 * lane;
+  // this wave's inner blocks, w, w + 16, ..., AHEAD of them in flight
+  i32x4 ahead[AHEAD];
+#pragma unroll
+  for (int i = 0; i < AHEAD; ++i) {
+    const int32_t b = w + WAVES * i;
+    ahead[i] = *reinterpret_cast<const i32x4 *>(wp + (int64_t)(b < a.blocks ? b : 0) * BLOCK);
+  }
+  const int64_t token0 = (int64_t)blockIdx.y * M;
+  const int32_t tokens = (int32_t)(a.tokens - token0 < M ? a.tokens - token0 : M);
+  const int32_t pieces = 2 * a.blocks, all = tokens * pieces;
+  // the threads share the tokens' pieces of 16 places; the first stay in registers
+  Piece<X> held;
+  auto load = [&](int32_t i, Piece<X> &y) -> int32_t {
+    const int32_t m = M == 1 ? 0 : i / pieces;
+    load16<X, ALIGNED>(static_cast<const X *>(t.x) + (token0 + m) * t.x_row, 16 * (i - m * pieces),
+                       t.k, y);
+    return m;
+  };
+  if (threadIdx.x < M) tops[threadIdx.x] = 0;
+  __syncthreads();
+  for (int32_t i = threadIdx.x; i - lane < all; i += 64 * WAVES) {
+    Piece<X> y;
+    uint32_t top = 0;
+    int32_t m = -1;
+    if (i < all) {
+      m = load(i, y);
+      top = magnitude(y);
+      if (i == (int32_t)threadIdx.x)
+        held = y;
+    }
+    // (one access to LDS for a wave whose pieces are one token's)
+    const int32_t mine = __builtin_amdgcn_readfirstlane(m);
+    if (__all(m == mine || m < 0)) {
+#pragma unroll
+      for (int o = 32; o > 0; o >>= 1) {
+        const uint32_t z = __shfl_xor(top, o);
+        top = z > top ? z : top;
+      }
+      if (lane == 0) atomicMax(&tops[mine], top);
+    } else if (m >= 0) {
+      atomicMax(&tops[m], top);
+    }
+  }
+  __syncthreads();
+  for (int32_t i = threadIdx.x; i < all; i += 64 * WAVES) {
+    Piece<X> y;
+    int32_t m = M == 1 ? 0 : i / pieces;
+    if (i == (int32_t)threadIdx.x)
+      y = held;
+    else
+      m = load(i, y);
+    *reinterpret_cast<u32x4 *>(token_lds + m * t.pitch + 16 * (i - m * pieces)) =
+        code16(y, row_scale(tops[m]));
+  }
+  __syncthreads();
+  i32x16 acc = i32x16{};
+  const int m0 = lane & 31;
+  const char *codes = token_lds + (m0 < tokens ? m0 : 0) * t.pitch + 16 * (lane >> 5);
+  auto step = [&](int i, int32_t b) {
+    // (columns of tokens that are not there are not used)
+    const i32x4 z = *reinterpret_cast<const i32x4 *>(codes + 32 * b);
+    acc = __builtin_amdgcn_mfma_i32_32x32x32_i8(ahead[i], z, acc, 0, 0, 0);
+  };
+  int32_t b = w;
+#pragma unroll 1
+  for (; b + WAVES * (2 * AHEAD - 1) < a.blocks; b += WAVES * AHEAD)
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      step(i, b + WAVES * i);
+      ahead[i] = *reinterpret_cast<const i32x4 *>(wp + (int64_t)(b + WAVES * (AHEAD + i)) * BLOCK);
+    }
+#pragma unroll
+  for (int i = 0; i < AHEAD; ++i)
+    if (b + WAVES * i < a.blocks) step(i, b + WAVES * i);
+#pragma unroll 4
+  for (b += WAVES * AHEAD; b < a.blocks; b += WAVES) {
+    ahead[0] = *reinterpret_cast<const i32x4 *>(wp + (int64_t)b * BLOCK);
+    step(0, b);
+  }
+  __syncthreads();
+  // the waves' sums of the tokens there are, through the codes' LDS
+  int(*sums)[32 * M] = reinterpret_cast<int(*)[32 * M]>(token_lds);
+  if (m0 < M)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) sums[w][(2 * r + (lane >> 5)) * M + m0] = acc[r];
+  __syncthreads();
+  {
+    const int x = threadIdx.x & 31, m = threadIdx.x >> 5;
+    if (m >= tokens) return;
+    const int at = (2 * (4 * (x >> 3) + (x & 3)) + ((x >> 2) & 1)) * M + m;
+    int s = 0;
+#pragma unroll
+    for (int i = 0; i < WAVES; ++i) s += sums[i][at];
+    const int32_t n = 32 * nb + x;
+    if (n < a.outputs)
+      static_cast<T *>(a.out)[(token0 + m) * a.out_row + n] =
+          (T)scaled(s, row_scale(tops[m]).scale, a.w_scales[n], a.bias ? a.bias[n] : 0.f);
+  }
+}
+
 // -------------------------------------------------------------------- launches
 
-template <class T>
-void quantize_of(hipStream_t st, const PackArgs &a, bool aligned) {
-  // a workgroup a row while there are too few rows to fill the device with waves
-  if (a.rows < 1024) {
+template <class T> void quantize_of(hipStream_t st, const PackArgs &a, bool aligned) {
+  // (a workgroup a row until eight rows each fill the device)
+  if (a.rows < 2048) {
     if (aligned)
-      k_int8_quantize<T, 4, true><<<(unsigned)a.rows, 256, 0, st>>>(a);
+      k_int8_quantize_row<T, true><<<(unsigned)a.rows, 256, 0, st>>>(a);
     else
-      k_int8_quantize<T, 4, false><<<(unsigned)a.rows, 256, 0, st>>>(a);
+      k_int8_quantize_row<T, false><<<(unsigned)a.rows, 256, 0, st>>>(a);
   } else {
-    const unsigned g = (unsigned)ceil_div(a.rows, 4);
+    const unsigned g = (unsigned)ceil_div(a.rows, PACK_ROWS);
     if (aligned)
-      k_int8_quantize<T, 1, true><<<g, 256, 0, st>>>(a);
+      k_int8_quantize<T, true><<<g, 64 * PACK_ROWS, 0, st>>>(a);
     else
-      k_int8_quantize<T, 1, false><<<g, 256, 0, st>>>(a);
+      k_int8_quantize<T, false><<<g, 64 * PACK_ROWS, 0, st>>>(a);
   }
 }
 
@@ -440,30 +644,88 @@ void launch_quantize(vsk_ctx *ctx, hipStream_t st, const PackArgs &a, int32_t t)
   check_launch("int8_quantize");
 }
 
-template <class T, int FN, int FM> void tile_of(hipStream_t st, LinearArgs &a) {
+template <class T, int FN, int FM, int STEP, int STAGES>
+void tile_of(hipStream_t st, LinearArgs &a) {
   a.tiles_n = (int32_t)ceil_div(a.outputs, 64 * FN);
   const int64_t grid = a.tiles_n * ceil_div(a.tokens, 64 * FM);
   VSK_REQUIRE(grid <= 0x7FFFFFFFll, VSK_ERR_INVALID_BUFFER_SIZE, "too many outputs in one call");
-  k_int8_tile<T, FN, FM><<<(unsigned)grid, 256, 0, st>>>(a);
+  k_int8_tile<T, FN, FM, STEP, STAGES><<<(unsigned)grid, 256, 0, st>>>(a);
 }
 
-template <class T> void products_of(vsk_ctx *ctx, hipStream_t st, LinearArgs &a) {
-  if (a.tokens <= 32) {
-    k_int8_few<T, 1, 16><<<dim3((unsigned)a.w_blocks), 1024, 0, st>>>(a);
-    return;
-  }
-  if (a.tokens <= 64) {
-    k_int8_few<T, 2, 16><<<dim3((unsigned)a.w_blocks), 1024, 0, st>>>(a);
-    return;
-  }
-  const int64_t large = ceil_div(a.outputs, 256) * ceil_div(a.tokens, 256);
-  const int64_t middle = ceil_div(a.outputs, 128) * ceil_div(a.tokens, 128);
-  if (large >= ctx->cu_count)
-    tile_of<T, 4, 4>(st, a);
-  else if (middle >= ctx->cu_count)
-    tile_of<T, 2, 2>(st, a);
+template <class X, class T> void token_of(hipStream_t st, const TokenArgs &t, bool aligned) {
+  auto launch = [&](auto m) {
+    constexpr int M = decltype(m)::value;
+    // the tokens' codes, and the sums in their place
+    const int64_t codes = (t.l.tokens < M ? t.l.tokens : M) * t.pitch, sums = 16 * 32 * M * 4;
+    const dim3 g((unsigned)t.l.w_blocks, (unsigned)ceil_div(t.l.tokens, M));
+    const unsigned lds = (unsigned)(codes > sums ? codes : sums);
+    if (aligned)
+      k_int8_token<X, T, M, true><<<g, 1024, lds, st>>>(t);
+    else
+      k_int8_token<X, T, M, false><<<g, 1024, lds, st>>>(t);
+  };
+  if (t.l.tokens == 1)
+    launch(std::integral_constant<int, 1>());
+  else if (t.l.tokens <= 4)
+    launch(std::integral_constant<int, 4>());
   else
-    tile_of<T, 1, 1>(st, a);
+    launch(std::integral_constant<int, 8>());
+}
+template <class T> void token_to(hipStream_t st, const TokenArgs &t, int32_t x, bool aligned) {
+  if (x == VSK_DTYPE_F32)
+    token_of<float, T>(st, t, aligned);
+  else if (x == VSK_DTYPE_F16)
+    token_of<_Float16, T>(st, t, aligned);
+  else
+    token_of<__bf16, T>(st, t, aligned);
+}
+
+// The kernel and its tile, by how many workgroups each would have.  Measured over
+// weights that come from memory, us a call: under 33 tokens the few-tokens
+// kernel; to 64 tokens that or tiles of 64 (64 of 4,096 x 4,096 14.7 / 15.9, of
+// 4,096 x 12,288 24.7 / 19.0); then tiles of 64, many steps in flight, while
+// two a compute unit cover the outputs (256 of 4,096 x 4,096 17.8, tiles of
+// 128 27.4; 1,024 of them 40.7 / 33.3); tiles of 128 in the same way (256 of
+// 4,096 x 12,288 30.2, with four steps in flight 33.0; 512 of them 48.0 / 39.7)
+// until tiles of 256 reach two thirds of the device (1,024 of 4,096 x 12,288
+// 72 / 65; 2,048 of 4,096 x 4,096 50 / 60).  A tile has no more places for tokens
+// than it needs (64 of 4,096 x 65,536 in tiles of 64 47.7, of 256 69.7; 128 of
+// them in tiles of 128 55.7, of 256 70.7).
+template <class T> void products_of(vsk_ctx *ctx, hipStream_t st, LinearArgs &a) {
+  const int64_t cus = ctx->cu_count;
+  if (a.tokens <= 32) {
+    k_int8_few<T, 1, 8><<<dim3((unsigned)a.w_blocks), 512, 0, st>>>(a);
+    return;
+  }
+  if (a.tokens <= 64 && a.w_blocks <= cus) {
+    k_int8_few<T, 2, 8><<<dim3((unsigned)a.w_blocks), 512, 0, st>>>(a);
+    return;
+  }
+  auto tiles = [&](int64_t size) {
+    return ceil_div(a.outputs, size) * ceil_div(a.tokens, size);
+  };
+  if (a.tokens <= 64 || tiles(64) <= 2 * cus)
+    tile_of<T, 1, 1, 2, 8>(st, a);
+  else if (a.tokens > 128 && 3 * tiles(256) >= 2 * cus)
+    tile_of<T, 4, 4, 2, 4>(st, a);
+  else if (tiles(128) <= cus)
+    tile_of<T, 2, 2, 2, 8>(st, a);
+  else
+    tile_of<T, 2, 2, 2, 4>(st, a);
+}
+
+// Does k_int8_token take the call?  Each of its workgroups quantises up to eight
+// tokens for itself: up to 16,384 places, which take about as long as the launch
+// that they save (4 tokens of 4,096 through 4,096 outputs 8.0 us, in two launches
+// 9.8; 8 of them 10.3 / 10.0; 64 of 1,024 through 1,024 5.1 / 8.1), and no more
+// workgroups than run together (400 of 512 through 512 would take 12.6 us, 7.5
+// in two launches), or the same in all.
+constexpr int64_t GROUP = 8, PLACES = 16384, TOGETHER = 512;
+bool one_launch(int64_t tokens, const vsk_int8_weight *w) {
+  const int64_t places = (tokens < GROUP ? tokens : GROUP) * w->inputs;
+  const int64_t groups = ceil_div(tokens, GROUP), blocks = groups * ceil_div(w->outputs, 32);
+  return places <= PLACES &&
+         (blocks <= TOGETHER || (groups == 1 && blocks * places <= TOGETHER * PLACES));
 }
 
 void check_layer(const vsk_int8_weight *w) {
@@ -517,7 +779,7 @@ vsk_status vsk_int8_pack(vsk_ctx *ctx, void *stream, int32_t dtype, const void *
 
 int64_t vsk_int8_linear_workspace(const vsk_int8_weight *w, int64_t tokens) {
   if (!w || tokens < 1 || tokens > 0x7FFFFFFFll || w->inputs < 1 || w->inputs > MOST) return 0;
-  return scales_bytes(tokens) + packed_bytes(tokens, w->inputs);
+  return one_launch(tokens, w) ? 0 : scales_bytes(tokens) + packed_bytes(tokens, w->inputs);
 }
 
 vsk_status vsk_int8_linear(vsk_ctx *ctx, void *stream, const vsk_int8_weight *w,
@@ -534,22 +796,40 @@ vsk_status vsk_int8_linear(vsk_ctx *ctx, void *stream, const vsk_int8_weight *w,
   VSK_REQUIRE(r->x && r->out && is_device_ptr(r->x) && is_device_ptr(r->out),
               VSK_ERR_INVALID_ARGUMENT, "inputs and outputs must be device memory");
   const int64_t need = vsk_int8_linear_workspace(w, r->tokens);
-  VSK_REQUIRE(r->workspace && r->workspace_bytes >= need && (uintptr_t)r->workspace % 16 == 0 &&
-                  is_device_ptr(r->workspace),
+  VSK_REQUIRE(need == 0 || (r->workspace && r->workspace_bytes >= need &&
+                            (uintptr_t)r->workspace % 16 == 0 && is_device_ptr(r->workspace)),
               VSK_ERR_INVALID_BUFFER_SIZE,
               "the workspace must be " + std::to_string(need) + " bytes of device memory");
   hipStream_t st = static_cast<hipStream_t>(stream);
   float *scales = static_cast<float *>(r->workspace);
   char *codes = static_cast<char *>(r->workspace) + scales_bytes(r->tokens);
   const int32_t blocks = (int32_t)inner_blocks(w->inputs);
-  launch_quantize(ctx, st, PackArgs{r->x, r->x_row, r->tokens, codes, scales, w->inputs, blocks},
-                  r->x_dtype);
   LinearArgs a{};
   a.w = static_cast<const char *>(w->packed), a.x = codes;
   a.w_scales = w->scales, a.x_scales = scales, a.bias = w->bias;
   a.out = r->out, a.out_row = r->out_row, a.tokens = r->tokens;
   a.outputs = w->outputs, a.blocks = blocks;
   a.w_blocks = (int32_t)ceil_div(w->outputs, 32), a.x_blocks = ceil_div(r->tokens, 32);
+  const int64_t pitch = 32 * (int64_t)blocks + 16;
+  if (one_launch(r->tokens, w)) {
+    const int64_t x_size = r->x_dtype == VSK_DTYPE_F32 ? 4 : 2;
+    const bool al = (uintptr_t)r->x % 16 == 0 && r->x_row * x_size % 16 == 0;
+    const TokenArgs t{a, r->x, r->x_row, w->inputs, (int32_t)pitch};
+    {
+      KernelTimer kt(ctx, "int8_token", (double)a.tokens * a.outputs * w->inputs, st);
+      if (r->out_dtype == VSK_DTYPE_F32)
+        token_to<float>(st, t, r->x_dtype, al);
+      else if (r->out_dtype == VSK_DTYPE_F16)
+        token_to<_Float16>(st, t, r->x_dtype, al);
+      else
+        token_to<__bf16>(st, t, r->x_dtype, al);
+      check_launch("int8_token");
+    }
+    finish_queued(ctx, st);
+    return VSK_OK;
+  }
+  launch_quantize(ctx, st, PackArgs{r->x, r->x_row, r->tokens, codes, scales, w->inputs, blocks},
+                  r->x_dtype);
   const int64_t size = r->out_dtype == VSK_DTYPE_F32 ? 4 : 2;
   a.wide = (uintptr_t)r->out % 16 == 0 && r->out_row * size % 16 == 0 && w->outputs * size % 16 == 0;
   {

@@ -103,20 +103,20 @@ class Int8Linear:
         dtype = x.dtype if dtype is None else dtype
         if dtype not in _TYPES:
             raise VSKError(-8, f"{dtype} is not supported")
-        out = torch.empty(x.shape[:-1] + (self.outputs,), dtype=dtype, device=x.device)
         rows = _dense(x if x.dim() == 2 else x.reshape(-1, self.inputs))
-        tokens = rows.shape[0]
+        tokens, lib = rows.shape[0], ctx.lib
+        out = rows.new_empty((tokens, self.outputs), dtype=dtype)
+        shaped = out if x.dim() == 2 else out.view(x.shape[:-1] + (self.outputs,))
         if not tokens:
-            return out
-        lib = ctx.lib
-        need = lib.vsk_int8_linear_workspace(self._ref, tokens)
-        if not need:
+            return shaped
+        if tokens >= 1 << 31:
             raise VSKError(-9, f"{tokens} tokens: at most 2^31 - 1")
-        work = torch.empty(need, dtype=torch.uint8, device=x.device)
+        need = lib.vsk_int8_linear_workspace(self._ref, tokens)
+        work = rows.new_empty(need, dtype=torch.uint8) if need else None
         status = lib.vsk_int8_linear(
             ctx.handle, _stream(ctx.device), self._ref,
             _ROWS.pack(rows.data_ptr(), out.data_ptr(), rows.stride(0), self.outputs, tokens,
-                       work.data_ptr(), need, _TYPES[x.dtype], _TYPES[dtype]))
+                       work.data_ptr() if need else 0, need, _TYPES[x.dtype], _TYPES[dtype]))
         if status:
             ctx.check(status)
-        return out
+        return shaped
