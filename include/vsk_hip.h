@@ -661,7 +661,7 @@ vsk_status vsk_cross_attention(vsk_ctx *ctx, void *stream, const vsk_kv *kv,
 typedef struct {
   int32_t *groups, *prefix;
   int32_t n_groups, n;
-  int32_t max_members; /* sequences of a group, at most */
+  int32_t max_members; /* sequences of a group, at most (one of more shares nothing) */
   int32_t max_prefix;  /* about the longest prefix, to divide the work by (0: unknown) */
 } vsk_shared_prefix;
 vsk_status vsk_kv_share(vsk_ctx *ctx, void *stream, const vsk_kv *kv, const int32_t *seqs,

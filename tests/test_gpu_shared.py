@@ -486,6 +486,125 @@ def test_indices_out_of_range(ctx):
     torch.cuda.synchronize()
 
 
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("new", [1, 40])
+def test_shared_after_a_member_is_cut_back(ctx, dtype, new):
+    """A member that is shorter than the prefix now: the others still read it."""
+    g = gen(17)
+    cache, slots = cache_of(ctx, g, [(128, [50, 41, 60])], 16, 2, 64, dtype)
+    plan = cache.share([0, 3])
+    at = None if new == 1 else starts_of([new] * 3)
+    for short, length in ((0, 100), (1, 129), (0, new), (2, 128)):
+        cache.lengths[short] = length
+        q = normal(g, 3 * new, 4, 64, dtype=dtype)
+        out = cache.attend(q, shared=plan, starts=at, max_new=None if new == 1 else new)
+        check_shared(cache, slots, q, at, out, 0.125)
+
+
+def test_groups_of_more_than_the_bound(ctx):
+    """A bound on the members that is too small costs the sharing, no more."""
+    g = gen(18)
+    cache, slots = cache_of(ctx, g, [(64, [3, 4, 9]), (64, [5, 6])], 32, 2, 64, BF)
+    q = normal(g, 5, 4, 64, dtype=BF)
+    plan = cache.share(ints([0, 3, 5]), members=2)
+    assert plan.prefix.tolist() == [0, 0, 0, 64, 64, 0]
+    check_shared(cache, slots, q, None, cache.attend(q, shared=plan), 0.125)
+    for few in (0, 1):
+        plan = cache.share(ints([0, 3, 5]), members=few)
+        check_shared(cache, slots, q, None, cache.attend(q, shared=plan), 0.125)
+    # known of offsets on the host
+    assert cache.share([0, 3, 5], members=2).prefix.tolist() == [64] * 5 + [0]
+
+
+def test_one_slot_twice(ctx):
+    """Sequences of one slot share all its whole pages."""
+    g = gen(19)
+    cache, _ = cache_of(ctx, g, [(64, [3, 4])], 32, 2, 64, BF)
+    q = normal(g, 3, 4, 64, dtype=BF)
+    plan = cache.share([0, 3], seqs=[1, 1, 0])
+    assert plan.prefix.tolist() == [64] * 3
+    check_shared(cache, [1, 1, 0], q, None, cache.attend(q, shared=plan), 0.125)
+    plan = cache.share([0, 2], seqs=[1, 1])
+    assert plan.prefix.tolist() == [64] * 2
+    check_shared(cache, [1, 1], q[:2], None, cache.attend(q[:2], shared=plan), 0.125)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_cross_strange_strides(ctx, dtype):
+    """Sets that lie at one place, a key each, overlap, or in other orders."""
+    from vectorstorekit_amd import cross_attention
+
+    g = gen(20)
+    q = normal(g, 3, 4, 32, dtype=dtype)
+    one = normal(g, 200, 2, 32, dtype=dtype)
+    flat = normal(g, 5000, dtype=dtype)
+    for k in (one[None, :50].expand(3, -1, -1, -1), one[:1][None].expand(3, 1, 2, 32),
+              one[:1][None].expand(3, 40, 2, 32), one[:3, None], one[::7][:3, None],
+              one[:40, None].transpose(0, 1)[:, ::2].expand(3, -1, -1, -1),
+              one[:, :1][None, :9].expand(3, 9, 2, 32),
+              flat.as_strided((3, 30, 2, 32), (128, 64, 32, 1)),
+              flat.as_strided((3, 30, 2, 32), (96, 64, 32, 1)),
+              flat.as_strided((3, 1, 2, 32), (96, 7, 32, 1)),
+              flat.as_strided((3, 3, 2, 32), (64, 192, 32, 1)),
+              normal(g, 2, 20, 3, 32, dtype=dtype).permute(2, 1, 0, 3)):
+        for v in (k, k.contiguous() * 2, k.clone().transpose(1, 2).contiguous().transpose(1, 2)):
+            out = cross_attention(ctx, q, k, v)
+            for i in range(3):
+                want, _, tol = attended(q[i:i + 1], k[i], v[i], [k.shape[1]], 32 ** -0.5)
+                check(out[i:i + 1], want, tol)
+
+
+# ---------------------------------------------------------- offsets past 32 bits
+
+@pytest.mark.parametrize("new", [1, 70])
+def test_pages_past_32_bits(ctx, new):
+    """Pages at the end of a pool of more than 2^31 elements give what the same
+    pages give in a small one."""
+    from vectorstorekit_amd import PagedKVCache
+
+    g = gen(21)
+    small, slots = cache_of(ctx, g, [(512, [200, 90, 77]), (128, [100])], 64, 8, 128, BF)
+    pages, held = 2 ** 31 // (64 * 8 * 128) + 100, small.k.shape[0]
+    pool = [torch.empty(pages, 64, 8, 128, dtype=BF, device=DEV) for _ in range(2)]
+    pool[0][-held:], pool[1][-held:] = small.k, small.v
+    table = torch.where(small.table >= 0, small.table + (pages - held), -1).int()
+    large = PagedKVCache.over(ctx, *pool, table, small.lengths)
+    at = None if new == 1 else starts_of([new] * 4)
+    q = normal(g, 4 * new, 16, 128, dtype=BF)
+    outs = []
+    for cache in (small, large):
+        plan = cache.share([0, 3, 4])
+        assert plan.prefix.tolist() == [512] * 3 + [0] * 2
+        outs.append(cache.attend(q, shared=plan, starts=at, max_new=None if new == 1 else new))
+    assert torch.equal(*outs)
+    check_shared(small, slots, q, at, outs[0], 128 ** -0.5)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("new", [1, 200])
+def test_sets_past_32_bits(ctx, dtype, new):
+    from vectorstorekit_amd import cross_attention
+
+    g = gen(22)
+    rows = 2 ** 31 // 1024 + 5000
+    k = torch.empty(rows, 8, 128, dtype=dtype, device=DEV)
+    tail = normal(g, 3000, 8, 128, dtype=dtype)
+    k[-3000:] = tail
+    q = normal(g, 2 * new, 8, 128, dtype=dtype)
+    at = [0, new, 2 * new]
+    ragged = cross_attention(ctx, q, k, k, starts=at, max_length=new, max_keys=1700,
+                             k_starts=[rows - 3000, rows - 1700, rows])
+    want = cross_attention(ctx, q, tail, tail, starts=at, max_length=new, max_keys=1700,
+                           k_starts=[0, 1300, 3000])
+    assert torch.equal(ragged, want)
+    padded = k[-1500 * (rows // 1500):].view(-1, 1500, 8, 128)
+    sets = [len(padded) - 2, len(padded) - 1]
+    got = cross_attention(ctx, q, padded, padded, starts=at, max_length=new, sets=sets)
+    want = cross_attention(ctx, q, tail.view(2, 1500, 8, 128), tail.view(2, 1500, 8, 128),
+                           starts=at, max_length=new)
+    assert torch.equal(got, want)
+
+
 # ---------------------------------------------------------------------- refusals
 
 def test_refusals(ctx):

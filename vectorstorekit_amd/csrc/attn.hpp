@@ -129,7 +129,7 @@ template <AttnForm F> __device__ inline AttnSeq attn_seq(const AttnArgs &a, int3
         pages = pages < 0 ? 0 : pages > a.width ? a.width : pages;
         const int32_t keys = pages << a.page_shift;
         if (a.groups) {
-          s.L = s.L < keys ? s.L : keys;
+          s.L = keys;  // (also where the first member has been cut back since)
         } else {
           s.row += pages;
           s.L = s.L > keys ? s.L - keys : 0;

@@ -490,7 +490,7 @@ constexpr int SHARE_WAVES = 16;
 __global__ __launch_bounds__(64 * SHARE_WAVES) void k_kv_share(
     const int32_t *table, const int32_t *lengths, int64_t stride, int32_t slots, int32_t width,
     int32_t shift, const int32_t *seqs, const int32_t *groups, int32_t n_groups, int32_t n,
-    int32_t *prefix) {
+    int32_t members, int32_t *prefix) {
   constexpr int NT = 64 * SHARE_WAVES;
   __shared__ int32_t pages;
   auto offset = [&](int32_t g) -> int32_t {
@@ -509,8 +509,9 @@ __global__ __launch_bounds__(64 * SHARE_WAVES) void k_kv_share(
     const int32_t x = seqs ? seqs[b] : b;
     return (uint32_t)x < (uint32_t)slots ? x : -1;
   };
-  // the whole pages of the shortest member
-  if (threadIdx.x == 0) pages = end - first > 1 ? width : 0;
+  // the whole pages of the shortest member (a group of more than attention makes
+  // room for has none)
+  if (threadIdx.x == 0) pages = end - first > 1 && end - first <= members ? width : 0;
   __syncthreads();
   for (int32_t b = first + threadIdx.x; b < end; b += NT) {
     const int32_t slot = slot_of(b);
@@ -669,7 +670,7 @@ vsk_status vsk_kv_share(vsk_ctx *ctx, void *stream, const vsk_kv *kv, const int3
     k_kv_share<<<(unsigned)shared->n_groups, 64 * SHARE_WAVES, 0, st>>>(
         kv->table, kv->lengths, kv->table_stride, kv->slots, kv->width,
         __builtin_ctz((unsigned)kv->page_size), seqs, shared->groups, shared->n_groups, shared->n,
-        shared->prefix);
+        shared->max_members, shared->prefix);
     check_launch("kv_share");
   }
   finish_queued(ctx, st);

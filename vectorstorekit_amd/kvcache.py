@@ -481,8 +481,9 @@ class PagedKVCache:
 
         ``shared``, of ``share``: the same attention, in which the keys that a
         group of sequences shares are read once for all of them.  Its
-        sequences are the call's (``seqs`` is not given again).  With a window
-        each sequence reads its own keys."""
+        sequences are the call's (``seqs`` is not given again).  Of a group in
+        which a sequence has more than ``max_new`` tokens the rows behind are
+        not treated either.  With a window each sequence reads its own keys."""
         self._layer(layer)
         q = self._heads(q, "q")
         if shared is not None:
@@ -512,8 +513,9 @@ class PagedKVCache:
         the sequences grow and the pool is compacted; after a ``fork`` into, or
         a ``free`` of, one of these slots call ``update`` of what is returned.
         ``members`` bounds a group's sequences (default: known of a host
-        sequence, all of them otherwise), ``prefix`` says about how many keys
-        the longest prefix has, to divide the work by."""
+        sequence, all of them otherwise; a group of more shares nothing),
+        ``prefix`` says about how many keys the longest prefix has, to divide
+        the work by."""
         return SharedPrefix(self, groups, seqs, members, prefix)
 
     # -- pages ------------------------------------------------------------------
@@ -612,8 +614,8 @@ class SharedPrefix:
                 raise VSKError(-2, "groups holds an offset a group and the end")
             if a.min() < 0 or a.max() > self.n or (np.diff(a) < 0).any():
                 raise VSKError(-2, f"groups must ascend from 0 to at most {self.n}")
-            if members is None:
-                members = int(np.diff(a).max()) if a.size > 1 else 0
+            known = int(np.diff(a).max()) if a.size > 1 else 0
+            members = known if members is None or 0 <= members < known else members
         self.groups = _ints(gpu, groups, "groups")
         if self.groups.shape[0] < 1:
             raise VSKError(-2, "groups holds an offset a group and the end")
@@ -721,11 +723,11 @@ def _padded(x):
     """x, sets x length x heads x d, its row and head strides, and the rows
     from a set to the next (x, or a copy where that is no whole number)."""
     a, b, c = x.stride()[:3]
-    if x.shape[1] <= 1:
-        return x, (max(a, 1), c), 1
     if x.shape[0] <= 1:
         return x, (b, c), x.shape[1]
-    if b <= 0 or a < 0 or a % b:
+    if x.shape[1] <= 1 and 0 < a <= 1 << 26:
+        return x, (a, c), 1  # (the stride between a set's rows may be any)
+    if b <= 0 or a % b:
         x = x.contiguous()
         a, b, c = x.stride()[:3]
     return x, (b, c), a // b
