@@ -281,6 +281,21 @@ def test_graph_and_stream(ctx, tokens, inputs):
     check(here[0], *expected(x, codes, scales, b, BF))
 
 
+@pytest.mark.parametrize("tokens,inputs,outputs", [(70001, 64, 32768), (20001, 131072, 40)])
+def test_past_32_bits(ctx, tokens, inputs, outputs):
+    """More than 2^31 outputs, inputs and packed bytes: the last tokens' outputs
+    are what they are by themselves."""
+    g = gen(tokens)
+    layer, codes, scales, b = layer_of(ctx, g, outputs, inputs)
+    tail = normal(g, 50, inputs, dtype=BF)
+    x = torch.zeros(tokens, inputs, dtype=BF, device=DEV)
+    x[-50:] = tail
+    got = layer(x)
+    assert torch.equal(got[-50:], layer(tail))
+    assert torch.equal(got[0], b.to(BF)) and torch.equal(got[-51], b.to(BF))
+    check(got[-3:], *expected(tail[-3:], codes, scales, b, BF))
+
+
 def test_refusals(ctx):
     from vectorstorekit_amd import Int8Linear, VSKError
 
