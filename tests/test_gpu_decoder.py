@@ -3,6 +3,10 @@ that share their context and cross attention to an encoder's states, each call
 against 64 bits on the inputs that it had, and the whole captured and replayed.
 
 The tolerances of each call are those of its own tests."""
+import importlib.util
+import math
+import os
+
 import pytest
 import torch
 
@@ -117,3 +121,20 @@ def test_steps(ctx, dtype, branches, context):
         block.head(normal(g, 300, WIDTH, dtype=dtype))
     assert cache.missing() == 0
     assert cache.lengths.tolist() == [context] + [context + 5] * branches
+
+
+@pytest.mark.parametrize("eight_bits", [False, True])
+def test_example(capsys, eight_bits):
+    """The example with its options.  Without 8-bit codes it is held to itself
+    without a cache: sixteen roundings a layer of 2^-8 of a value, four layers,
+    added as independent errors, are 2^-8 sqrt(64) = 0.031 of a logit's size,
+    twice that for the largest of them.  (A code is a step of its row's largest
+    / 127, so that roundings before it can become whole steps.)"""
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples",
+                        "answer_over_retrieved.py")
+    spec = importlib.util.spec_from_file_location("answer_over_retrieved", path)
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    worst = example.main(branches=3, steps=6, eight_bits=eight_bits, states=True)
+    assert math.isfinite(worst) and (eight_bits or worst <= 0.0625)
+    assert "documents [123" in capsys.readouterr().out
