@@ -125,6 +125,7 @@ Plan plan_of(const vsk_ctx *ctx, const vsk_kv *kv, const vsk_attention_args *arg
   }
   // Parts as many as keep the device supplied with blocks.
   int64_t want, per;
+  bool apart = false;
   if (p.tile) {
     // A prompt's rows are many and joining them takes as long as some steps:
     // parts of at least 16 tiles, and only where a quarter of the blocks that
@@ -151,12 +152,22 @@ Plan plan_of(const vsk_ctx *ctx, const vsk_kv *kv, const vsk_attention_args *arg
     // join follows anyway 32-bit rows, whose steps are long, take more (6 groups
     // of drafts, 2 / 8: 216 / 138).
     per = 4;
-    const int64_t most = kv->head_dim <= 64 ? 16 : kv->head_dim > 128 ? 1
-                         : kv->dtype != VSK_DTYPE_F32 ? 6 : span.joined ? 8 : 2;
+    int64_t most = kv->head_dim <= 64 ? 16 : kv->head_dim > 128 ? 1
+                   : kv->dtype != VSK_DTYPE_F32 ? 6 : span.joined ? 8 : 2;
+    // Other sequences' keys of dense rows (and sets of one length) lie in step,
+    // and parts that begin powers of two apart meet the same memory channels at
+    // a time.  So those of cross attention are many, of 12 tiles at least and
+    // never of a multiple of 8: contexts to 4,096 of 16 heads of 64 119 / 111
+    // us, 64 to 8,000 of 8 key heads of 128 184 / 170, 200 to 4,000 262 / 238, 50
+    // to 4,000 of 16 f32 heads of 96 253 / 205 (parts of 32 tiles 300 instead of
+    // 262, of 4 tiles 24 us where 32 contexts to 6,000 of 3 key heads take 21).
+    apart = span.all && !span.joined && kv->head_dim <= 128;
+    if (apart) most = 32;
     want = most * cus < 64 * blocks ? most * cus : 64 * blocks;
     if (want < cus) want = cus;
   }
-  const int64_t chunk = ceil_div(ceil_div(tiles, ceil_div(want, blocks)), per) * per;
+  int64_t chunk = ceil_div(ceil_div(tiles, ceil_div(want, blocks)), per) * per;
+  if (apart) chunk = chunk < 12 ? 12 : chunk + (chunk % 8 == 0 ? 4 : 0);
   p.chunk = (int32_t)(chunk < per ? per : chunk);
   p.splits = (int32_t)ceil_div(tiles, p.chunk);
   if (p.splits < 1) p.splits = 1;
