@@ -1,6 +1,14 @@
 // attn_forms.hip -- the kernels of attn_rows.hip for the other forms of
 // attention: to keys of another length that every row sees, and over a prefix
 // that sequences share, where a row tile holds rows of several.
+//
+// What bounds them: the bytes of K and V, as in attn_rows.hip (64 contexts to
+// 4,096 of 16 heads of 64, four tokens each, 111 us: 4.3 TB/s, of which the join
+// is 5), short ones the launches (one token over 300 keys 9 us; 4 branches of
+// 512 shared keys 12, a launch for both calls and one for the join).  In 32 bits
+// heads over 64 leave registers for two waves a SIMD, whose products and vector
+// instructions, on one unit, take half of the time (6 groups of ten branches and
+// up to nine drafts, 16 heads of 96: 109 us for 232 MB).
 #include "attn_rows.hpp"
 #include "vsk_api.hpp"
 
@@ -19,7 +27,7 @@ k_attn_forms(const AttnArgs args) {
 
 // Joins the parts of output rows: a row for DV / 4 lanes, times WAYS that share
 // its parts.  Unlike k_attn_join it has the rows of one sequence side by side
-// (a block a row took 95 us for 70,000 rows of three parts, this JOIN_US).
+// (a block a row took 95 us for 70,000 rows of three parts, this 22).
 template <class E, int DV, int WAYS, bool ALIGNED>
 __global__ __launch_bounds__(256) void k_attn_join_forms(const AttnArgs a, const int32_t key_tile) {
   constexpr int LANES = DV / 4, WIDE = LANES * WAYS, R = 256 / WIDE;

@@ -485,7 +485,7 @@ void launch_move(vsk_ctx *ctx, hipStream_t st, const vsk_kv *kv, const Pool &p, 
 // A workgroup a group: the first page in which a member's table differs from
 // the first member's ends the prefix.  A wave takes a member at a time, 256
 // pages a step, up to the end that any wave has found so far (64 branches of
-// 32,768 tokens in pages of 64: SHARE_US us).
+// 32,768 tokens in pages of 64: 11 us).
 constexpr int SHARE_WAVES = 16;
 __global__ __launch_bounds__(64 * SHARE_WAVES) void k_kv_share(
     const int32_t *table, const int32_t *lengths, int64_t stride, int32_t slots, int32_t width,
