@@ -704,8 +704,8 @@ vsk_status vsk_int8_pack(vsk_ctx *ctx, void *stream, int32_t dtype, const void *
  * (code = x * (127 / largest), rounded to even) and
  * out = code . weights * token's scale * channel's scale + bias.  The sums are
  * exact; a token that holds an infinity or NaN has NaN outputs.  inputs at
- * most 131,072.  workspace: vsk_int8_linear_workspace() bytes, 16-byte
- * aligned. */
+ * most 131,072.  out must not overlap x.  workspace:
+ * vsk_int8_linear_workspace() bytes, 16-byte aligned (0 for few tokens: none). */
 typedef struct {
   const void *x;
   void *out;
