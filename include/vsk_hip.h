@@ -655,9 +655,10 @@ vsk_status vsk_cross_attention(vsk_ctx *ctx, void *stream, const vsk_kv *kv,
 /* Prefixes that sequences share.  Sequence i of n is in slot seqs[i] (NULL:
  * i); group g are the sequences groups[g] .. groups[g + 1] (n_groups + 1
  * ascending offsets).  vsk_kv_share writes, for each sequence, how many keys
- * lie in the leading whole pages that all of its group hold (prefix[n]; 0: in
- * no group, or alone).  What it wrote stays true until a sequence of a group
- * is forked anew or freed; growing, appending and compacting do not change it. */
+ * lie in the leading whole pages that all of its group hold (prefix[n]; alone
+ * in a group: all its whole pages; in no group: 0).  What it wrote stays true
+ * until a sequence of a group is forked anew or freed; growing, appending and
+ * compacting do not change it. */
 typedef struct {
   int32_t *groups, *prefix;
   int32_t n_groups, n;

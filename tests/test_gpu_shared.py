@@ -278,7 +278,8 @@ def test_shared_tokens(ctx, dtype, heads, kv, d, groups):
     q = normal(g, n, heads, d, dtype=dtype)
     offsets = starts_of([len(own) for _, own in groups])
     plan = cache.share(offsets)
-    want = [p if len(own) > 1 else 0 for p, own in groups for _ in own] + [0]
+    # (one alone has all its whole pages)
+    want = [p if len(own) > 1 else (p + own[0]) // 32 * 32 for p, own in groups for _ in own] + [0]
     assert plan.prefix.tolist() == want
     out, lse = cache.attend(q, shared=plan, return_lse=True)
     check_shared(cache, slots, q, None, out, d ** -0.5, lse)
@@ -554,6 +555,83 @@ def test_cross_strange_strides(ctx, dtype):
                 check(out[i:i + 1], want, tol)
 
 
+# ------------------------------------------- large calls in 32 bits (tiles of 128)
+
+BIG = {7: (300, 1100), 30: (129, 33), 31: (400, 64), 99: (256, 1)}
+
+
+@pytest.mark.parametrize("d", [68, 80, 96, 128])
+@pytest.mark.parametrize("padded", [False, True])
+def test_large_cross_32_bits(ctx, d, padded):
+    """A few long texts among many short ones; behind the sets' lengths memory
+    that was never written, in one tile values that are not finite."""
+    from vectorstorekit_amd import cross_attention
+
+    g = gen(d)
+    n, heads, kv = 120, 8, 2
+    new = [BIG[i][0] if i in BIG else i % 4 for i in range(n)]
+    keys = [BIG[i][1] if i in BIG else i % 6 for i in range(n)]
+    at, ks = starts_of(new), starts_of(keys)
+    q = normal(g, at[-1], heads, d)
+    k, v = (normal(g, ks[-1], kv, d) for _ in range(2))
+    hot = ks[7] + 500, ks[7] + 1099, ks[31] + 63  # (in a whole tile, and in last ones)
+    v[hot[0], 0, 5], v[hot[1], 1, d - 1], v[hot[2], 0, 0] = math.inf, -math.inf, math.inf
+    if padded:
+        pk, pv = (torch.full((n, 1100, kv, d), math.nan, device=DEV) for _ in range(2))
+        for i in range(n):
+            pk[i, :keys[i]], pv[i, :keys[i]] = k[ks[i]:ks[i + 1]], v[ks[i]:ks[i + 1]]
+        out, lse = cross_attention(ctx, q, pk, pv, starts=at, k_lengths=keys, max_length=400,
+                                   return_lse=True)
+    else:
+        out, lse = cross_attention(ctx, q, k, v, starts=at, k_starts=ks, max_length=400,
+                                   max_keys=1100, return_lse=True)
+    assert bool((out[at[7]:at[8], :4, 5] == math.inf).all())
+    assert bool((out[at[7]:at[8], 4:, d - 1] == -math.inf).all())
+    assert bool((out[at[31]:at[32], :4, 0] == math.inf).all())
+    out[at[7]:at[8], :4, 5] = out[at[7]:at[8], 4:, d - 1] = out[at[31]:at[32], :4, 0] = 0
+    clean = v.clone()
+    clean[hot[0], 0], clean[hot[1], 1], clean[hot[2], 0] = (
+        v[h, j].nan_to_num(posinf=0.0, neginf=0.0) for h, j in zip(hot, (0, 1, 0)))
+    for i in range(n):
+        a, b = slice(at[i], at[i + 1]), slice(ks[i], ks[i + 1])
+        want, sums, tol = attended(q[a], k[b], clean[b], [keys[i]] * new[i], d ** -0.5)
+        if i == 7:
+            want[:, :4, 5] = want[:, 4:, d - 1] = 0
+        if i == 31:
+            want[:, :4, 0] = 0
+        check(out[a], want, tol)
+        check_lse(lse[a], sums)
+
+
+@pytest.mark.parametrize("d", [72, 128])
+@pytest.mark.parametrize("known", [True, False])
+def test_large_prefix_32_bits(ctx, d, known):
+    """Prefixes by tiles of 128 in parts, with own keys by tiles of 128 or 16
+    (as a bound on them says), rows that reach back into the prefix, and NaN
+    behind the sequences' ends."""
+    g = gen(d)
+    new = [100, 7, 130, 64, 90, 1, 33, 128]
+    groups = [(2000 // 16 * 16, [150, 20, 140, 70]), (96, [100, 3, 50, 131])]
+    small, slots = cache_of(ctx, g, groups, 16, 2, d, F32)
+    for s in slots:
+        length = int(small.lengths[s])
+        if length % 16:
+            page = int(small.table[s, (length - 1) // 16])
+            small.k[page, length % 16:] = small.v[page, length % 16:] = math.nan
+    from vectorstorekit_amd import PagedKVCache
+
+    table = torch.full((small.slots, 1100), -1, dtype=torch.int32, device=DEV)
+    table[:, :small.width] = small.table
+    cache = PagedKVCache.over(ctx, small.k, small.v, table, small.lengths)
+    at = starts_of(new)
+    q = normal(g, at[-1], 8, d)
+    offsets = [0, 4] + [8] * 8
+    plan = cache.share(offsets, members=4, prefix=17400 if known else None)
+    assert plan.prefix.tolist() == [2000] * 4 + [96] * 4 + [0]
+    out, lse = cache.attend(q, shared=plan, starts=at, max_new=130, return_lse=True)
+    check_shared(cache, slots, q, at, out, d ** -0.5, lse)
+
+
 # ---------------------------------------------------------- offsets past 32 bits
 
 @pytest.mark.parametrize("new", [1, 70])
@@ -574,7 +652,7 @@ def test_pages_past_32_bits(ctx, new):
     outs = []
     for cache in (small, large):
         plan = cache.share([0, 3, 4])
-        assert plan.prefix.tolist() == [512] * 3 + [0] * 2
+        assert plan.prefix.tolist() == [512] * 3 + [192, 0]
         outs.append(cache.attend(q, shared=plan, starts=at, max_new=None if new == 1 else new))
     assert torch.equal(*outs)
     check_shared(small, slots, q, at, outs[0], 128 ** -0.5)

@@ -36,10 +36,11 @@ bool aligned_operands(const vsk_kv *kv, const vsk_attention_args *args) {
 
 // What a plan divides: n sequences of at most max_new new tokens and keys keys.
 // all: every token sees every key; joined: its parts are joined with another
-// plan's.
+// plan's; room: blocks a compute unit that it has (of a prefix's row tiles).
 struct Span {
   int64_t n, max_new, keys;
   bool all, joined;
+  int64_t room = 1;
 };
 
 int64_t most_new(const vsk_new_tokens *news) { return news->starts ? news->max_new : 1; }
@@ -83,10 +84,16 @@ Plan plan_of(const vsk_ctx *ctx, const vsk_kv *kv, const vsk_attention_args *arg
     row_tile = ATTN_TILE_ROWS;
     key_tile = attn_tile_keys(kv->head_dim);
   }
-  // In 32 bits such tiles are for rows that share their keys (two thirds of a
-  // tile at least: 6 groups of up to 90 rows 160 us, in tiles of 16 110).
-  if (kv->dtype == VSK_DTYPE_F32 && (span.all || span.joined) && rows >= 96 &&
-      kv->head_dim <= 128 && aligned_operands(kv, args)) {
+  // In 32 bits such tiles are for rows that share their keys, in large calls: a
+  // tile takes some 4 us, and its parts are as large as its keys.  Steps of row
+  // tiles and key tiles / us / in tiles of 16: 7 texts of 500 over 3,001 keys, 20
+  // heads of 80 on 5 52,000 / 351 / 497; 6 of 300 over 9,000, 12 of 96 61,000 /
+  // 255 / 322; 20 of 64 over 2,000, 28 of 128 on 4 20,000 / 285 / 158; 60 of 50
+  // over 4,000 (tiles mostly empty) 75,000 / 406 / 358; heads of 64, whose tiles
+  // of 16 leave registers for four waves, 8 of 1,000 over 3,000 48,000 / 221 / 180.
+  if (kv->dtype == VSK_DTYPE_F32 && (span.all || span.joined) && rows >= 256 &&
+      kv->head_dim > 64 && kv->head_dim <= 128 && aligned_operands(kv, args) &&
+      pairs * ceil_div(rows, ATTN_TILE_ROWS) * ceil_div(keys, ATTN_TILE32_KEYS) >= 40000) {
     p.tile = true;
     row_tile = ATTN_TILE_ROWS;
     key_tile = ATTN_TILE32_KEYS;
@@ -132,10 +139,16 @@ Plan plan_of(const vsk_ctx *ctx, const vsk_kv *kv, const vsk_attention_args *arg
     // fit or less would work.  Unsplit / split after 30,000 keys, 32 heads of
     // 128 on 8 (us): 512 tokens (128 blocks) 519 / 284, 2,000 (504) 893 / 998.
     per = 16;
-    // A prefix's tiles have the other half of each compute unit's room to the
-    // sequences' own keys (64 branches of 32,768, want of 1, 2 and 4 halves: 99,
-    // 70 and 81 us).
-    want = 2 * blocks > cus ? 1 : span.joined && span.all ? cus : 2 * cus;
+    want = 2 * blocks > cus ? 1 : 2 * cus;
+    if (span.joined && span.all) {
+      // A prefix's tiles have the other half of each compute unit's room to the
+      // sequences' own keys (64 branches of 32,768, want of 1, 2 and 4 halves:
+      // 99, 70 and 81 us), or, where those are few, all of it, and are joined
+      // anyway (4 groups of up to 32 branches, four tokens, 23,756 keys, 9 heads
+      // of 64 on 3 55 / 40 us; of 1,790, 28 of 128 on 4 48 / 33).
+      want = span.room * cus;
+      if (kv->head_dim <= 128) per = 8;
+    }
     // In 32 bits a tile takes so long that ragged texts are divided for their
     // balance (7 of up to 500 against 3,001 keys, want 2 and 12: 575 / 501 us).
     if (kv->dtype == VSK_DTYPE_F32) want = 12 * cus;
@@ -161,8 +174,11 @@ Plan plan_of(const vsk_ctx *ctx, const vsk_kv *kv, const vsk_attention_args *arg
     // us, 64 to 8,000 of 8 key heads of 128 184 / 170, 200 to 4,000 262 / 238, 50
     // to 4,000 of 16 f32 heads of 96 253 / 205 (parts of 32 tiles 300 instead of
     // 262, of 4 tiles 24 us where 32 contexts to 6,000 of 3 key heads take 21).
+    // Of several row tiles the parts to join are as many as the keys: a few
+    // blocks a compute unit (20 f32 texts of 128 over 1,000 keys, 8 heads of 128
+    // 80 / 61; 3 of 128 over 2,000, 28 on 4 104 / 80).
     apart = span.all && !span.joined && kv->head_dim <= 128;
-    if (apart) most = 32;
+    if (apart) most = p.tiles > 1 ? 4 : 32;
     want = most * cus < 64 * blocks ? most * cus : 64 * blocks;
     if (want < cus) want = cus;
   }
@@ -190,9 +206,11 @@ Plans plans_of(const vsk_ctx *ctx, const vsk_kv *kv, const vsk_new_tokens *news,
     p.group_tokens = (int64_t)shared->max_members * most_new(news);
     if (p.group_tokens > news->tokens) p.group_tokens = news->tokens;
     const int64_t first = most_keys(kv, shared->max_prefix > 0 ? shared->max_prefix : keys);
-    p.prefix = plan_of(ctx, kv, args, Span{shared->n_groups, p.group_tokens, first, true, true});
     const int64_t rest = shared->max_prefix > 0 && shared->max_prefix < keys
                              ? keys - shared->max_prefix : keys;
+    const int64_t room = 2 * news->n * rest < shared->n_groups * first ? 3 : 1;
+    p.prefix = plan_of(ctx, kv, args,
+                       Span{shared->n_groups, p.group_tokens, first, true, true, room});
     p.own = plan_of(ctx, kv, args, Span{news->n, most_new(news), rest, false, true});
   } else {
     p.own = plan_of(ctx, kv, args, Span{news->n, most_new(news), keys, all, false});

@@ -389,7 +389,7 @@ constexpr int ATTN_TILE_ROWS = 128;
 constexpr int ATTN_TILE_GROUP = 16;  // keys that lie together in a tile
 void launch_attn_tile(vsk_ctx *ctx, hipStream_t stream, const AttnArgs &a, int32_t t,
                       AttnForm form);
-// attn_tile32.hip: 32 bits, aligned, ATTN_FORMS, the same row tiles
+// attn_tile32.hip: 32 bits, aligned, heads of 65 to 128, ATTN_FORMS, the same row tiles
 constexpr int ATTN_TILE32_KEYS = 32;
 void launch_attn_tile32(vsk_ctx *ctx, hipStream_t stream, const AttnArgs &a);
 // attn_shared.hip: 16 bits, aligned, heads to 128: a.pre by row tiles of ATTN_TILE_ROWS, the

@@ -33,13 +33,13 @@ constexpr int KT = 32;
 
 typedef __attribute__((ext_vector_type(4))) float f4;
 
-// DT: dimensions in blocks of 32 (the queries of more than 128 would not fit
-// the registers), padded to PITCH in LDS
+// DT: dimensions in blocks of 32, 3 or 4 (the queries of more than 128 would not
+// fit the registers), padded to PITCH in LDS
 template <int DT>
 __global__ __launch_bounds__(64 * NW, 2) void k_attn_tile32(const AttnArgs args) {
   AttnArgs a = args;
   uint32_t at = attn_call(a, blockIdx.x);
-  constexpr int PITCH = DT <= 2 ? 64 : 128;
+  constexpr int PITCH = 128;
   constexpr int CH = PITCH / 4;              // 16-byte pieces of a row
   constexpr int ROWB = 4 * PITCH;
   constexpr int TILEB = KT * ROWB;
@@ -251,14 +251,9 @@ __global__ __launch_bounds__(64 * NW, 2) void k_attn_tile32(const AttnArgs args)
 #pragma unroll
         for (int t = 0; t < DT; ++t) v[t] = row[t];
       } else {
-        constexpr int W = DT < 4 ? DT : 4;
-        typedef __attribute__((ext_vector_type(W))) float V;
+        const f4 y = *(const lds_as f4 *)row;
 #pragma unroll
-        for (int t = 0; t < DT; t += W) {
-          const V y = *(const lds_as V *)(row + t);
-#pragma unroll
-          for (int z = 0; z < W; ++z) v[t + z] = y[z];
-        }
+        for (int t = 0; t < DT; ++t) v[t] = y[t];
       }
     };
     // What a masked place holds must not reach a sum, and 0 * NaN is NaN: of a
@@ -357,9 +352,7 @@ void launch_attn_tile32(vsk_ctx *ctx, hipStream_t st, const AttnArgs &a) {
   VSK_REQUIRE(grid <= 0x7FFFFFFFll, VSK_ERR_INVALID_BUFFER_SIZE, "too many query rows in one call");
   KernelTimer kt(ctx, "attn_tile32", (double)a.tokens * a.heads, st);
   const unsigned g = (unsigned)grid;
-  if (a.d <= 64)
-    k_attn_tile32<2><<<g, 64 * NW, 0, st>>>(a);
-  else if (a.d <= 96)
+  if (a.d <= 96)
     k_attn_tile32<3><<<g, 64 * NW, 0, st>>>(a);
   else
     k_attn_tile32<4><<<g, 64 * NW, 0, st>>>(a);

@@ -690,7 +690,9 @@ template <class T> void token_to(hipStream_t st, const TokenArgs &t, int32_t x, 
 // until tiles of 256 reach two thirds of the device (1,024 of 4,096 x 12,288
 // 72 / 65; 2,048 of 4,096 x 4,096 50 / 60).  A tile has no more places for tokens
 // than it needs (64 of 4,096 x 65,536 in tiles of 64 47.7, of 256 69.7; 128 of
-// them in tiles of 128 55.7, of 256 70.7).
+// them in tiles of 128 55.7, of 256 70.7), and up to 1,024 places are over so soon
+// that two blocks a compute unit, one's outputs beside the other's products, are
+// better (16,384 of 512 x 4,096 99 / 81, of 1,024 120 / 116, 4,096 of 2,048 50 / 55).
 template <class T> void products_of(vsk_ctx *ctx, hipStream_t st, LinearArgs &a) {
   const int64_t cus = ctx->cu_count;
   if (a.tokens <= 32) {
@@ -706,7 +708,7 @@ template <class T> void products_of(vsk_ctx *ctx, hipStream_t st, LinearArgs &a)
   };
   if (a.tokens <= 64 || tiles(64) <= 2 * cus)
     tile_of<T, 1, 1, 2, 8>(st, a);
-  else if (a.tokens > 128 && 3 * tiles(256) >= 2 * cus)
+  else if (a.tokens > 128 && a.blocks > 32 && 3 * tiles(256) >= 2 * cus)
     tile_of<T, 4, 4, 2, 4>(st, a);
   else if (tiles(128) <= cus)
     tile_of<T, 2, 2, 2, 8>(st, a);

@@ -509,9 +509,10 @@ __global__ __launch_bounds__(64 * SHARE_WAVES) void k_kv_share(
     const int32_t x = seqs ? seqs[b] : b;
     return (uint32_t)x < (uint32_t)slots ? x : -1;
   };
-  // the whole pages of the shortest member (a group of more than attention makes
-  // room for has none)
-  if (threadIdx.x == 0) pages = end - first > 1 && end - first <= members ? width : 0;
+  // the whole pages of the shortest member, of one alone its own: its keys are
+  // many, as the groups' are, and divided like them (a group of more than
+  // attention makes room for has none)
+  if (threadIdx.x == 0) pages = end - first <= members ? width : 0;
   __syncthreads();
   for (int32_t b = first + threadIdx.x; b < end; b += NT) {
     const int32_t slot = slot_of(b);
