@@ -17,7 +17,7 @@
 // What bounds it: few tokens, the weights' bytes and the launches (one token
 // through 4,096 x 4,096 5.7 us, 64 through 4,096 x 12,288 14.5, of which the
 // weights alone are 8.7 at 5.8 TB/s); many, the matrix cores: 16,384 tokens
-// through 4,096 x 12,288 take 43 us to quantise and 740 for the products, 2,230
+// through 4,096 x 12,288 take 43 us to quantise and 700 for the products, 2,350
 // TOPS, at which the card holds its power limit and 1.8 GHz.
 #include <type_traits>
 
@@ -370,11 +370,29 @@ __global__ __launch_bounds__(256, FN * FM >= 16 ? 1 : 2) void k_int8_tile(const 
   const int c = lane % PIECES;
   const int32_t n = n0 + V * c, left = a.outputs - n;
   float ws[V], bias[V];
-#pragma unroll
-  for (int z = 0; z < V; ++z) {
-    const int32_t at = z < left ? n + z : a.outputs - 1;
+  auto scales_of = [&](int z, int32_t channel) {
+    const int32_t at = channel < a.outputs ? channel : a.outputs - 1;
     ws[z] = a.w_scales[at];
     bias[z] = a.bias ? a.bias[at] : 0.f;
+  };
+  // Rows that take no stores of 16 bytes: a store has the same output of a row in
+  // neighbouring lanes, and a lane one or two channels (eight at a time, singly,
+  // 12,077 tokens of 846 x 9,931 took 302 us, so 250).
+  constexpr int COLUMNS = 32 * FN, EACH = COLUMNS > 64 ? COLUMNS / 64 : 1;
+  if (a.wide) {
+#pragma unroll
+    for (int z = 0; z < V; ++z) scales_of(z, n + z);
+  } else {
+#pragma unroll
+    for (int z = 0; z < EACH; ++z) scales_of(z, n0 + (64 * z + lane) % COLUMNS);
+  }
+  // the scale of token lane % 32 of each block (asked for where it is used, a trip
+  // to memory for every other store: 757 us where 16,384 tokens take 743)
+  float xs[FM];
+#pragma unroll
+  for (int j = 0; j < FM; ++j) {
+    const int64_t m = 64 * FM * tm + 32 * (FM * wm + j) + (lane & 31);
+    xs[j] = a.x_scales[m < a.tokens ? m : a.tokens - 1];
   }
 #pragma unroll
   for (int j = 0; j < FM; ++j) {
@@ -386,28 +404,36 @@ __global__ __launch_bounds__(256, FN * FM >= 16 ? 1 : 2) void k_int8_tile(const 
             i32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2],
                   acc[i][j][4 * q + 3]};
     const int64_t m0 = 64 * FM * tm + 32 * (FM * wm + j);
-#pragma unroll 2
+    if (!a.wide) {
+#pragma unroll 8
+      for (int x = 0; x < COLUMNS / 2; x += EACH) {
+#pragma unroll
+        for (int z = 0; z < EACH; ++z) {
+          const int at = 64 * (x + z) + lane, r = at / COLUMNS, o = at % COLUMNS;
+          const int64_t m = m0 + r;
+          const float scale = __shfl(xs[j], r);
+          if (m < a.tokens && n0 + o < a.outputs)
+            static_cast<T *>(a.out)[m * a.out_row + n0 + o] =
+                (T)scaled(*(const lds_as int *)(mine + r * PITCH + 4 * o), scale, ws[z], bias[z]);
+        }
+      }
+      continue;
+    }
+#pragma unroll 4
     for (int x = 0; x < PIECES / 2; ++x) {
       const int r = (64 * x + lane) / PIECES;
       const int64_t m = m0 + r;
-      const float xs = a.x_scales[m < a.tokens ? m : a.tokens - 1];
+      const float scale = __shfl(xs[j], r);
       typedef __attribute__((ext_vector_type(V))) T Out;
       Out y;
 #pragma unroll
       for (int z = 0; z < V; z += 4) {
         const i32x4 sum = *(const lds_as i32x4 *)(mine + r * PITCH + 4 * (V * c + z));
 #pragma unroll
-        for (int k = 0; k < 4; ++k) y[z + k] = (T)scaled(sum[k], xs, ws[z + k], bias[z + k]);
+        for (int k = 0; k < 4; ++k) y[z + k] = (T)scaled(sum[k], scale, ws[z + k], bias[z + k]);
       }
-      T *to = static_cast<T *>(a.out) + m * a.out_row + n;
-      const int32_t some = m < a.tokens ? left : 0;
-      if (a.wide) {
-        if (some > 0) *reinterpret_cast<Out *>(to) = y;
-      } else {
-#pragma unroll
-        for (int z = 0; z < V; ++z)
-          if (z < some) to[z] = y[z];
-      }
+      if (m < a.tokens && left > 0)
+        *reinterpret_cast<Out *>(static_cast<T *>(a.out) + m * a.out_row + n) = y;
     }
   }
 }
