@@ -126,7 +126,10 @@ Plan plan_of(const vsk_ctx *ctx, const vsk_kv *kv, const vsk_attention_args *arg
     const bool many = kv->head_dim <= 64 || (kv->head_dim <= 128 && kv->dtype != VSK_DTYPE_F32 &&
                                              blocks <= 6 * cus);
     if (!span.joined && many && tiles <= (blocks < cus ? 32 : 64)) {
-      p.share = 8;
+      // (four over other sequences' keys, which may be few, while eight of such
+      // heads take a compute unit: 52 sequences of 12 heads of 96 over 6 keys 20
+      // / 11, of 8 of 128 over 380 17 / 13)
+      if (!span.all || kv->head_dim <= 64 || blocks <= cus) p.share = 8;
       return p;
     }
   }
@@ -343,6 +346,11 @@ void attend(vsk_ctx *ctx, void *stream, const vsk_kv *kv, int32_t layer,
     a.cross = 1;
     a.k_starts = sets->starts, a.k_lengths = sets->lengths;
     a.sets = sets->n, a.set_rows = sets->set_rows;
+    // Sequences that see one set read the same part of it at a time (14 over one
+    // of 14,841 keys, 12 heads of 96 192 / 106 us); those with a set each would
+    // read places of all that may lie in step (64 padded to 4,096, 16 heads of 64
+    // 110 / 117).
+    a.parts_apart = sets->n < news->n;
     a.k_rows = kv->pages;
   } else {
     a.k_starts = args->k_starts;
@@ -379,6 +387,7 @@ void attend(vsk_ctx *ctx, void *stream, const vsk_kv *kv, int32_t layer,
   if (p.group_tokens) {
     a.prefix = shared->prefix;
     a.joined = 1;
+    a.parts_apart = 1;  // (pages lie anywhere: 12 groups of 16 92 / 88 us)
     a.part0 = p.prefix.splits;
     a.groups = shared->groups;
     a.members = a.n;

@@ -65,6 +65,7 @@ struct AttnArgs {
   int32_t members;      // sequences that the groups' offsets may name
   int32_t joined;       // parts are written also where there is one, absent ones marked
   int32_t part0;        // the call's first part
+  int32_t parts_apart;  // one part of every sequence, then the next
   // two calls in one launch: the first pre_blocks blocks are those of a call
   // over prefixes, which differs in these
   uint32_t pre_blocks, own_blocks;
@@ -153,6 +154,17 @@ template <AttnForm F> __device__ inline AttnSeq attn_seq(const AttnArgs &a, int3
   s.p0 = F && a.cross ? s.L - 1 : s.L - s.T;
   s.each = F && a.cross ? 0 : -1;
   return s;
+}
+
+// The sequence (or group) and part of a block, with heads and row tiles taken
+// out of its number.
+struct AttnTurn {
+  int32_t b, part;
+};
+template <AttnForm F> __device__ inline AttnTurn attn_turn(const AttnArgs &a, uint32_t at) {
+  if (F == ATTN_OWN || !a.parts_apart)
+    return {(int32_t)(at / a.splits), (int32_t)(at % a.splits)};
+  return {(int32_t)(at % a.n), (int32_t)(at / a.n)};
 }
 
 // Position of the sequence's new token t among its keys.  Of a group's, it is

@@ -3,7 +3,7 @@
 // that sequences share, where a row tile holds rows of several.
 //
 // What bounds them: the bytes of K and V, as in attn_rows.hip (64 contexts to
-// 4,096 of 16 heads of 64, four tokens each, 111 us: 4.3 TB/s, of which the join
+// 4,096 of 16 heads of 64, four tokens each, 110 us: 4.4 TB/s, of which the join
 // is 5), short ones the launches (one token over 300 keys 9 us; 4 branches of
 // 512 shared keys 12, a launch for both calls and one for the join).  In 32 bits
 // heads over 64 leave registers for two waves a SIMD, whose products and vector

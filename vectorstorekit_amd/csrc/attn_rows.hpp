@@ -521,8 +521,8 @@ __device__ __forceinline__ void attn_rows_block(const AttnArgs &a, uint32_t at, 
   // (the last tiles see the most keys: they go first)
   const int32_t tg = groups - 1 - (int32_t)(at % groups);
   at /= groups;
-  const int32_t part = at % a.splits;
-  const AttnSeq s = attn_seq<F>(a, at / a.splits);
+  const auto [b, part] = attn_turn<F>(a, at);
+  const AttnSeq s = attn_seq<F>(a, b);
   const int32_t tile = SHARE > 1 ? tg : 4 * tg + w;
   const int32_t row0 = tile * ROWS;
   const int32_t T_used = s.T < a.max_new ? s.T : a.max_new;

@@ -74,8 +74,8 @@ __device__ __forceinline__ void attn_tile_block(const AttnArgs &a, uint32_t at, 
   at /= a.kv_heads;
   const int32_t tile = a.tiles - 1 - (int32_t)(at % a.tiles);
   at /= a.tiles;
-  const int32_t part = at % a.splits;
-  const AttnSeq s = attn_seq<F>(a, at / a.splits);
+  const auto [b, part] = attn_turn<F>(a, at);
+  const AttnSeq s = attn_seq<F>(a, b);
   const int32_t row0 = tile * ROWS;
   const int32_t T_used = s.T < a.max_new ? s.T : a.max_new;
   const int32_t rows_all = T_used * a.group;

@@ -19,8 +19,8 @@
 // when a row's largest score has grown by 8 (in log2; weights up to 256 cost
 // fp32 nothing), and values looked at one by one only in tiles that not every
 // row sees whole.  7 texts of up to 500 against 3,001 keys, 20 heads of 80 on 5:
-// 480 us (16 rows a wave that brings its keys itself: 999), 80 of 157 TFLOP/s,
-// 88 with the places that the head leaves in a block of 32.
+// 470 us (16 rows a wave that brings its keys itself: 999), 81 of 157 TFLOP/s,
+// 89 with the places that the head leaves in a block of 32.
 #include "attn.hpp"
 #include "vsk_api.hpp"
 
@@ -58,8 +58,8 @@ __global__ __launch_bounds__(64 * NW, 2) void k_attn_tile32(const AttnArgs args)
   at /= a.kv_heads;
   const int32_t tile = a.tiles - 1 - (int32_t)(at % a.tiles);
   at /= a.tiles;
-  const int32_t part = at % a.splits;
-  const AttnSeq s = attn_seq<ATTN_FORMS>(a, at / a.splits);
+  const auto [b, part] = attn_turn<ATTN_FORMS>(a, at);
+  const AttnSeq s = attn_seq<ATTN_FORMS>(a, b);
   const int32_t row0 = tile * ROWS;
   const int32_t T_used = s.T < a.max_new ? s.T : a.max_new;
   const int32_t rows_all = T_used * a.group;
