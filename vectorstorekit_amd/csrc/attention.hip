@@ -148,10 +148,12 @@ Plan plan_of(const vsk_ctx *ctx, const vsk_kv *kv, const vsk_attention_args *arg
       // sequences' own keys (64 branches of 32,768, want of 1, 2 and 4 halves:
       // 99, 70 and 81 us), or, where those are few, all of it, and are joined
       // anyway (4 groups of up to 32 branches, four tokens, 23,756 keys, 9 heads
-      // of 64 on 3 55 / 40 us; of 1,790, 28 of 128 on 4 48 / 33).
+      // of 64 on 3 55 / 44 us; of 1,790, 28 of 128 on 4 48 / 33).
       want = span.room * cus;
-      if (kv->head_dim <= 128) per = 8;
     }
+    // (parts that are joined anyway may be shorter: 16 sequences of ten tokens
+    // over up to 742 keys, 64 heads of 128 on 8 35 / 30)
+    if (span.joined && kv->head_dim <= 128) per = 8;
     // In 32 bits a tile takes so long that ragged texts are divided for their
     // balance (7 of up to 500 against 3,001 keys, want 2 and 12: 575 / 501 us).
     if (kv->dtype == VSK_DTYPE_F32) want = 12 * cus;
@@ -182,6 +184,13 @@ Plan plan_of(const vsk_ctx *ctx, const vsk_kv *kv, const vsk_attention_args *arg
     // 80 / 61; 3 of 128 over 2,000, 28 on 4 104 / 80).
     apart = span.all && !span.joined && kv->head_dim <= 128;
     if (apart) most = p.tiles > 1 ? 4 : 32;
+    // Of a prefix's several row tiles each has a start and a join to the part: four
+    // tiles a wave, where that fills the device (23 branches of 2,653 keys, 28
+    // heads of 128 on 4 23 / 17, 31 of 4,087, 64 on 8 38 / 33; 3 of 856, four
+    // tokens, 32 on 8 13 / 16).
+    if (span.joined && span.all && p.tiles > 1 && kv->dtype != VSK_DTYPE_F32 &&
+        blocks * ceil_div(tiles, 16) >= cus)
+      per = 16;
     want = most * cus < 64 * blocks ? most * cus : 64 * blocks;
     if (want < cus) want = cus;
   }
