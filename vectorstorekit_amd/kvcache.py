@@ -515,7 +515,9 @@ class PagedKVCache:
         ``members`` bounds a group's sequences (default: known of a host
         sequence, all of them otherwise; a group of more shares nothing),
         ``prefix`` says about how many keys the longest prefix has, to divide
-        the work by."""
+        the work by: a sequence with more keys of its own than are left of
+        ``max_length`` then is better in a group, alone if need be, than in
+        none."""
         return SharedPrefix(self, groups, seqs, members, prefix)
 
     # -- pages ------------------------------------------------------------------
