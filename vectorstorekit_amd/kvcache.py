@@ -509,9 +509,10 @@ class PagedKVCache:
         group g are the sequences ``groups[g] .. groups[g + 1]`` (ascending
         offsets) of those in slots ``seqs`` (default: slot i is sequence i).
         Nothing is assumed of them: a group's prefix is the leading whole pages
-        that all its members' tables agree on (one alone has all its own).  What is found stays true while
-        the sequences grow and the pool is compacted; after a ``fork`` into, or
-        a ``free`` of, one of these slots call ``update`` of what is returned.
+        that all its members' tables agree on (one alone has all its own).
+        What is found stays true while the sequences grow and the pool is
+        compacted; after a ``fork`` into, or a ``free`` of, one of these slots
+        call ``update`` of what is returned.
         ``members`` bounds a group's sequences (default: known of a host
         sequence, all of them otherwise; a group of more shares nothing),
         ``prefix`` says about how many keys the longest prefix has, to divide
