@@ -652,11 +652,12 @@ def cross_attention(ctx: Context, q, k, v, *, starts=None, k_starts=None, k_leng
     keys (and the end), or a padded batch, sets x length x kv_heads x head_dim,
     with ``k_lengths`` (default: all of them are keys).  Sequence i sees set
     ``sets[i]`` (default: i); several may see one (tokens side by side that do
-    are fastest as one sequence), and one that is not there (-1) is empty.  A query that sees no key gets zeros (and -inf).
-    ``max_length`` bounds a sequence's queries, ``max_keys`` a set's keys, to
-    divide the work by (default: all rows, or the padded length).  scale,
-    return_lse, the rounding of weights and the rows that are not treated as
-    in ``PagedKVCache.attend``; keys past a set's length may hold anything."""
+    are fastest as one sequence), and one that is not there (-1) is empty. A
+    query that sees no key gets zeros (and -inf). ``max_length`` bounds a
+    sequence's queries, ``max_keys`` a set's keys, to divide the work by
+    (default: all rows, or the padded length). scale, return_lse, the rounding
+    of weights and the rows that are not treated as in ``PagedKVCache.attend``;
+    keys past a set's length may hold anything."""
     gpu = ctx.device
     dtype = _tensor(gpu, q, "q", None, 3).dtype
     _tensor(gpu, k, "k", dtype), _tensor(gpu, v, "v", dtype)
