@@ -657,8 +657,11 @@ vsk_status vsk_cross_attention(vsk_ctx *ctx, void *stream, const vsk_kv *kv,
  * ascending offsets).  vsk_kv_share writes, for each sequence, how many keys
  * lie in the leading whole pages that all of its group hold (prefix[n]; alone
  * in a group: all its whole pages; in no group: 0).  What it wrote stays true
- * until a sequence of a group is forked anew or freed; growing, appending and
- * compacting do not change it. */
+ * while the sequences grow, are appended to or cut back (their lengths lowered)
+ * and the pool is compacted.  It is to be written anew when a sequence of a
+ * group has been forked anew or freed, and when one that was cut back into its
+ * prefix has grown again: vsk_kv_reserve gave it pages of its own there, and
+ * attention would read them for the whole group, or the group's for it. */
 typedef struct {
   int32_t *groups, *prefix;
   int32_t n_groups, n;

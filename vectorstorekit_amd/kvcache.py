@@ -511,8 +511,11 @@ class PagedKVCache:
         Nothing is assumed of them: a group's prefix is the leading whole pages
         that all its members' tables agree on (one alone has all its own).
         What is found stays true while the sequences grow and the pool is
-        compacted; after a ``fork`` into, or a ``free`` of, one of these slots
-        call ``update`` of what is returned.
+        compacted, also where one has been cut back since (its length lowered).
+        Call ``update`` of what is returned after a ``fork`` into, or a ``free``
+        of, one of these slots, and after a sequence that was cut back into its
+        prefix has grown again (``reserve`` gives it pages of its own there: its
+        group would read pages that are not theirs).
         ``members`` bounds a group's sequences (default: known of a host
         sequence, all of them otherwise; a group of more shares nothing),
         ``prefix`` says about how many keys the longest prefix has, to divide
