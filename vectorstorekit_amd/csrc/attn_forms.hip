@@ -76,8 +76,9 @@ __global__ __launch_bounds__(256) void k_attn_join_forms(const AttnArgs a, const
     const float ref = a.part_ml[2 * r], l = a.part_ml[2 * r + 1];
     const f32x4 y = *reinterpret_cast<const f32x4 *>(a.part_o + r * DV + e);
     const float f = attn_exp2((ref - use) * a.scale_log2);
-    // (a part that is not there, or of no keys, holds no values)
-    const bool none = ref == -INFINITY;
+    // (a part that is not there, or of no keys, holds no values; one whose scores
+    // are all NaN has no largest either, and its sum is NaN)
+    const bool none = ref == -INFINITY && l == 0.f;
     sum += none ? 0.f : f * l;
 #pragma unroll
     for (int z = 0; z < 4; ++z) o[z] += none ? 0.f : f * y[z];
