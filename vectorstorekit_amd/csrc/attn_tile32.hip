@@ -14,11 +14,10 @@
 //
 // What bounds it: the products, 64 cycles each, and the vector instructions
 // beside them, which run on the same units in 32 bits and add to them: a tile
-// has 32 DT products or less (of the head's d, not the padding), and about 150
-// other instructions.  So the queries are scaled before, the sums rescaled only
-// when a row's largest score has grown by 8 (in log2; weights up to 256 cost
-// fp32 nothing), and values looked at one by one only in tiles that not every
-// row sees whole.  7 texts of up to 500 against 3,001 keys, 20 heads of 80 on 5:
+// has 32 DT products or less (of the head's d, not the padding), and about 170
+// other instructions.  So the sums are rescaled only when a row's largest score
+// has grown by 8 (in log2; weights up to 256 cost fp32 nothing), and values
+// looked at one by one only in tiles that not every row sees whole.  7 texts of up to 500 against 3,001 keys, 20 heads of 80 on 5:
 // 470 us (16 rows a wave that brings its keys itself: 999), 81 of 157 TFLOP/s,
 // 89 with the places that the head leaves in a block of 32.
 #include "attn.hpp"
@@ -109,7 +108,6 @@ __global__ __launch_bounds__(64 * NW, 2) void k_attn_tile32(const AttnArgs args)
 #pragma unroll
     for (int i = 0; i < KS; ++i) {
       if (!real || 8 * i + 4 * h2 >= a.d) q[i] = f4{0.f, 0.f, 0.f, 0.f};
-      q[i] *= a.scale_log2;
     }
   }
   if (a.d < PITCH) {
@@ -186,7 +184,7 @@ __global__ __launch_bounds__(64 * NW, 2) void k_attn_tile32(const AttnArgs args)
   f32x16 acc[DT];
 #pragma unroll
   for (int t = 0; t < DT; ++t) acc[t] = f32x16{};
-  float m = -INFINITY, l = 0.f;  // what the sums are relative to: a score, in log2
+  float m = -INFINITY, l = 0.f;  // what the sums are relative to: a score, unscaled
   const int key_at = n * ROWB;
 
   if (first < end) {
@@ -230,18 +228,21 @@ __global__ __launch_bounds__(64 * NW, 2) void k_attn_tile32(const AttnArgs args)
 #pragma unroll
     for (int x = 3; x < 15; x += 2) top = max3(top, sc[x], sc[x + 1]);
     top = xor32_max(max3(top, sc[15], sc[15]));
-    if (__any(top > m + 8.f)) {
-      const float nm = top > m + 8.f ? top : m;
-      const float fade = nm == -INFINITY ? 1.f : attn_exp2(m - nm);
+    const bool grown = (top - m) * a.scale_log2 > 8.f;
+    if (__any(grown)) {
+      const float nm = grown ? top : m;
+      const float fade = nm == -INFINITY ? 1.f : attn_exp2((m - nm) * a.scale_log2);
       m = nm;
       l *= fade;
 #pragma unroll
       for (int t = 0; t < DT; ++t) acc[t] *= fade;
     }
+    // (subtracted before the scale comes in: the product of a large score with it
+    // is rounded by more than a weight's range.  3 of 490 us)
     const float use = m == -INFINITY ? 0.f : m;
 #pragma unroll
     for (int x = 0; x < 16; ++x) {
-      sc[x] = attn_exp2(sc[x] - use);
+      sc[x] = attn_exp2((sc[x] - use) * a.scale_log2);
       l += sc[x];
     }
     auto values = [&](int x, float (&v)[DT]) {
@@ -305,10 +306,7 @@ __global__ __launch_bounds__(64 * NW, 2) void k_attn_tile32(const AttnArgs args)
 
   const float sum = xor32_sum(l);
   const bool partial = parts > 1 || a.joined;
-  // (a part's reference is an unscaled score: the one that m was made of, or near it)
-  const float ref = m == -INFINITY ? m : m / a.scale_log2;
-  const float again = m == -INFINITY ? 1.f : attn_exp2(fmaf(-ref, a.scale_log2, m));
-  const float f = partial ? again : sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+  const float f = partial ? 1.f : sum > 0.f || sum != sum ? 1.f / sum : 0.f;
   const int64_t row = (s.token0 + my_t) * a.heads + my_head;
   const int64_t x0 = (int64_t)(a.part0 + part) * a.tokens * a.heads + row;
   // The outputs leave by way of LDS (this wave's part of it, when no wave reads
@@ -337,10 +335,10 @@ __global__ __launch_bounds__(64 * NW, 2) void k_attn_tile32(const AttnArgs args)
   }
   if (h2 == 0 && real) {
     if (partial) {
-      a.part_ml[2 * x0] = ref;
-      a.part_ml[2 * x0 + 1] = sum * again;
+      a.part_ml[2 * x0] = m;
+      a.part_ml[2 * x0 + 1] = sum;
     } else if (a.lse) {
-      a.lse[row] = attn_lse(m, sum);
+      a.lse[row] = attn_lse(m * a.scale_log2, sum);
     }
   }
 }
