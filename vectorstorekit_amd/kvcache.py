@@ -481,7 +481,8 @@ class PagedKVCache:
 
         ``shared``, of ``share``: the same attention, in which the keys that a
         group of sequences shares are read once for all of them.  Its
-        sequences are the call's (``seqs`` is not given again).  Of a group in
+        sequences, or the first of them, are the call's (``seqs`` is not given
+        again).  Of a group in
         which a sequence has more than ``max_new`` tokens the rows behind are
         not treated either.  With a window each sequence reads its own keys."""
         self._layer(layer)
@@ -491,15 +492,16 @@ class PagedKVCache:
                 raise VSKError(-2, "shared must be what this cache's share() returned")
             if seqs is not None:
                 raise VSKError(-2, "the slots are those that share() was called with")
-            seqs = shared.seqs
+            if starts is not None:
+                starts = _ints(self.gpu, starts, "starts")
+            n = q.shape[0] if starts is None else max(starts.shape[0] - 1, 0)
+            if n > shared.n:
+                raise VSKError(-4, f"{n} sequences, share() knows {shared.n}")
+            seqs = shared.seqs if shared.seqs is None or n == shared.n else shared.seqs[:n]
+            shared = shared._ref
         if q.shape[1] % self.kv_heads or not q.shape[1]:
             raise VSKError(-4, f"{q.shape[1]} query heads over {self.kv_heads} key heads")
         news, keep = self._news(q, starts, seqs, max_new)
-        if shared is not None:
-            n = q.shape[0] if starts is None else keep[0].shape[0] - 1
-            if n > shared.n:
-                raise VSKError(-4, f"{n} sequences, share() knows {shared.n}")
-            shared = shared._ref
         return _attend(self.ctx, self._ref, layer, q, news, 0, scale, window, sinks, max_length,
                        return_lse, None, shared)
 
