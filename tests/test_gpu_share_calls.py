@@ -32,3 +32,16 @@ def test_fewer_sequences_than_the_plan(ctx, host):
     for starts in ([], [0] * 8, ints([0] * 8)):
         with pytest.raises(VSKError):
             cache.attend(q, shared=plan, starts=starts)
+
+
+def test_descending_groups_of_unsigned_numbers(ctx):
+    """They descend whatever their type, whose differences wrap around."""
+    import numpy as np
+
+    from vectorstorekit_amd import VSKError
+
+    cache, _ = cache_of(ctx, gen(2), [(32, [3, 4, 5])], 32, 2, 64, BF)
+    for dtype in (np.uint8, np.uint32, np.uint64, np.int64):
+        assert cache.share(np.array([0, 1, 3], dtype)).prefix.tolist() == [32, 32, 32, 0]
+        with pytest.raises(VSKError):
+            cache.share(np.array([0, 3, 1], dtype))

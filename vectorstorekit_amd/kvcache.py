@@ -620,9 +620,9 @@ class SharedPrefix:
             a = np.asarray(groups)
             if a.ndim != 1 or a.size < 1 or a.dtype.kind not in "iu":
                 raise VSKError(-2, "groups holds an offset a group and the end")
-            if a.min() < 0 or a.max() > self.n or (np.diff(a) < 0).any():
+            if a.min() < 0 or a.max() > self.n or (a[1:] < a[:-1]).any():
                 raise VSKError(-2, f"groups must ascend from 0 to at most {self.n}")
-            known = int(np.diff(a).max()) if a.size > 1 else 0
+            known = int((a[1:] - a[:-1]).max()) if a.size > 1 else 0
             members = known if members is None or 0 <= members < known else members
         self.groups = _ints(gpu, groups, "groups")
         if self.groups.shape[0] < 1:
