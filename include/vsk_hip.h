@@ -673,8 +673,10 @@ vsk_status vsk_kv_share(vsk_ctx *ctx, void *stream, const vsk_kv *kv, const int3
 /* vsk_attention, in which the keys of a group's prefix are read once for all
  * of its sequences.  news: at most `n` sequences, in the order of vsk_kv_share
  * (and with its seqs).  With a window each sequence reads its own keys, as
- * vsk_attention does.  Where a sequence has more than max_new new tokens, what
- * is computed for its group is unspecified. */
+ * vsk_attention does.  The rows of a group count together: in 16 bits the
+ * weights over a prefix that many share are rounded once, as a prompt's, also
+ * those of one new token a sequence.  Where a sequence has more than max_new
+ * new tokens, what is computed for its group is unspecified. */
 int64_t vsk_attention_shared_workspace(vsk_ctx *ctx, const vsk_kv *kv, const vsk_new_tokens *news,
                                        const vsk_attention_args *args,
                                        const vsk_shared_prefix *shared);

@@ -482,9 +482,11 @@ class PagedKVCache:
         ``shared``, of ``share``: the same attention, in which the keys that a
         group of sequences shares are read once for all of them.  Its
         sequences, or the first of them, are the call's (``seqs`` is not given
-        again).  Of a group in
-        which a sequence has more than ``max_new`` tokens the rows behind are
-        not treated either.  With a window each sequence reads its own keys."""
+        again).  Where a sequence has more than ``max_new`` tokens the results
+        of its whole group are undefined.  A group's rows count together as few
+        or many: a prefix that many branches share rounds its weights once, as
+        a prompt does, also for one token of each.  With a window each sequence
+        reads its own keys."""
         self._layer(layer)
         q = self._heads(q, "q")
         if shared is not None:
