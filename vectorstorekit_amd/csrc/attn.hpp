@@ -332,7 +332,10 @@ template <int CH> __device__ inline int k_swizzle(int row) {
 }
 
 // (fmaxf would first quiet each product, an instruction a value: the maximum
-// here passes over NaN without it)
+// here passes over NaN without it.)  Nothing waits for a matrix product before
+// assembly reads it: a chain of maxima starts from product_read() of the last
+// products, which it depends on.
+__device__ inline float product_read(float x) { return __builtin_canonicalizef(x); }
 __device__ inline float max3(float a, float b, float c) {
   float r;
   asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));

@@ -246,11 +246,11 @@ __device__ __forceinline__ void attn_tile_block(const AttnArgs &a, uint32_t at, 
     }
   };
   auto largest = [&](const f32x16 (&sc)[U]) {
-    float tm = max3(sc[0][0], sc[0][1], sc[0][2]);
+    float tm = product_read(sc[0][0]);
+    if (U == 2) tm = max3(tm, tm, product_read(sc[U - 1][0]));
 #pragma unroll
-    for (int x = 3; x < 16 * U - 1; x += 2)
-      tm = max3(tm, sc[x >> 4][x & 15], sc[(x + 1) >> 4][(x + 1) & 15]);
-    return xor32_max(max3(tm, sc[U - 1][15], sc[U - 1][15]));
+    for (int x = 0; x < 16 * U; x += 2) tm = max3(tm, sc[x >> 4][x & 15], sc[x >> 4][(x & 15) + 1]);
+    return xor32_max(tm);
   };
   // Past FAR the product of a score and the scale, and so m, is rounded by more
   // than an eighth of one in log2, further on (2^24) by more than the room that
@@ -436,7 +436,7 @@ __device__ __forceinline__ void attn_tile_block(const AttnArgs &a, uint32_t at, 
       const float use = m == -INFINITY ? 0.f : m;
       f32x16 sn[U];
       V8 f[AHEAD], p[2 * U], qf[QLDS ? AHEAD : 1];
-      float tm = -INFINITY;
+      float tm = 0.f;
 #pragma unroll
       for (int u = 0; u < U; ++u) sn[u] = f32x16{};
       auto piece_of = [&](int g) -> V8 {
@@ -472,6 +472,7 @@ __device__ __forceinline__ void attn_tile_block(const AttnArgs &a, uint32_t at, 
             weight(8 * U + e);
         } else {
           const int z = g - NS - NV / 2;
+          if (z == 0) tm = product_read(sn[U - 1][0]);  // (made last)
 #pragma unroll
           for (int e = 8 * U * z / (NV / 2); e < 8 * U * (z + 1) / (NV / 2); ++e)
             tm = max3(tm, sn[e >> 3][2 * (e & 7)], sn[e >> 3][2 * (e & 7) + 1]);

@@ -224,10 +224,10 @@ __global__ __launch_bounds__(64 * NW, 2) void k_attn_tile32(const AttnArgs args)
       for (int x = 0; x < 16; ++x)
         if (mine + 8 * (x >> 2) + (x & 3) > pos) sc[x] = -INFINITY;
     }
-    float top = max3(sc[0], sc[1], sc[2]);
+    float top = product_read(sc[0]);
 #pragma unroll
-    for (int x = 3; x < 15; x += 2) top = max3(top, sc[x], sc[x + 1]);
-    top = xor32_max(max3(top, sc[15], sc[15]));
+    for (int x = 0; x < 16; x += 2) top = max3(top, sc[x], sc[x + 1]);
+    top = xor32_max(top);
     const bool grown = (top - m) * a.scale_log2 > 8.f;
     if (__any(grown)) {
       const float nm = grown ? top : m;
