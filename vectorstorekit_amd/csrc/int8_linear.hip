@@ -719,27 +719,41 @@ template <class T> void token_to(hipStream_t st, const TokenArgs &t, int32_t x, 
 // them in tiles of 128 55.7, of 256 70.7), and up to 1,024 places are over so soon
 // that two blocks a compute unit, one's outputs beside the other's products, are
 // better (16,384 of 512 x 4,096 99 / 81, of 1,024 120 / 116, 4,096 of 2,048 50 / 55).
-template <class T> void products_of(vsk_ctx *ctx, hipStream_t st, LinearArgs &a) {
+enum Products { FEW, FEW_64, TILES_64, TILES_128_AHEAD, TILES_128, TILES_256 };
+// (what profiling calls them)
+constexpr const char *PRODUCTS_NAME[] = {"int8_few",          "int8_few64",   "int8_tile64",
+                                         "int8_tile128_ahead", "int8_tile128", "int8_tile256"};
+Products products_for(const vsk_ctx *ctx, const LinearArgs &a) {
   const int64_t cus = ctx->cu_count;
-  if (a.tokens <= 32) {
-    k_int8_few<T, 1, 8><<<dim3((unsigned)a.w_blocks), 512, 0, st>>>(a);
-    return;
-  }
-  if (a.tokens <= 64 && a.w_blocks <= cus) {
-    k_int8_few<T, 2, 8><<<dim3((unsigned)a.w_blocks), 512, 0, st>>>(a);
-    return;
-  }
+  if (a.tokens <= 32) return FEW;
+  if (a.tokens <= 64 && a.w_blocks <= cus) return FEW_64;
   auto tiles = [&](int64_t size) {
     return ceil_div(a.outputs, size) * ceil_div(a.tokens, size);
   };
-  if (a.tokens <= 64 || tiles(64) <= 2 * cus)
-    tile_of<T, 1, 1, 2, 8>(st, a);
-  else if (a.tokens > 128 && a.blocks > 32 && 3 * tiles(256) >= 2 * cus)
-    tile_of<T, 4, 4, 2, 4>(st, a);
-  else if (tiles(128) <= cus)
-    tile_of<T, 2, 2, 2, 8>(st, a);
-  else
-    tile_of<T, 2, 2, 2, 4>(st, a);
+  if (a.tokens <= 64 || tiles(64) <= 2 * cus) return TILES_64;
+  if (a.tokens > 128 && a.blocks > 32 && 3 * tiles(256) >= 2 * cus) return TILES_256;
+  return tiles(128) <= cus ? TILES_128_AHEAD : TILES_128;
+}
+template <class T> void products_of(hipStream_t st, LinearArgs &a, Products by) {
+  switch (by) {
+    case FEW:
+      k_int8_few<T, 1, 8><<<dim3((unsigned)a.w_blocks), 512, 0, st>>>(a);
+      break;
+    case FEW_64:
+      k_int8_few<T, 2, 8><<<dim3((unsigned)a.w_blocks), 512, 0, st>>>(a);
+      break;
+    case TILES_64:
+      tile_of<T, 1, 1, 2, 8>(st, a);
+      break;
+    case TILES_128_AHEAD:
+      tile_of<T, 2, 2, 2, 8>(st, a);
+      break;
+    case TILES_128:
+      tile_of<T, 2, 2, 2, 4>(st, a);
+      break;
+    case TILES_256:
+      tile_of<T, 4, 4, 2, 4>(st, a);
+  }
 }
 
 // Does k_int8_token take the call?  Each of its workgroups quantises up to eight
@@ -861,13 +875,14 @@ vsk_status vsk_int8_linear(vsk_ctx *ctx, void *stream, const vsk_int8_weight *w,
   const int64_t size = r->out_dtype == VSK_DTYPE_F32 ? 4 : 2;
   a.wide = (uintptr_t)r->out % 16 == 0 && r->out_row * size % 16 == 0 && w->outputs * size % 16 == 0;
   {
-    KernelTimer kt(ctx, "int8_linear", (double)a.tokens * a.outputs * w->inputs, st);
+    const Products by = products_for(ctx, a);
+    KernelTimer kt(ctx, PRODUCTS_NAME[by], (double)a.tokens * a.outputs * w->inputs, st);
     if (r->out_dtype == VSK_DTYPE_F32)
-      products_of<float>(ctx, st, a);
+      products_of<float>(st, a, by);
     else if (r->out_dtype == VSK_DTYPE_F16)
-      products_of<_Float16>(ctx, st, a);
+      products_of<_Float16>(st, a, by);
     else
-      products_of<__bf16>(ctx, st, a);
+      products_of<__bf16>(st, a, by);
     check_launch("int8_linear");
   }
   finish_queued(ctx, st);
