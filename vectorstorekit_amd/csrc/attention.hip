@@ -85,12 +85,14 @@ Plan plan_of(const vsk_ctx *ctx, const vsk_kv *kv, const vsk_attention_args *arg
     key_tile = attn_tile_keys(kv->head_dim);
   }
   // In 32 bits such tiles are for rows that share their keys, in large calls: a
-  // tile takes some 4 us, and its parts are as large as its keys.  Steps of row
-  // tiles and key tiles / us / in tiles of 16: 7 texts of 500 over 3,001 keys, 20
-  // heads of 80 on 5 52,000 / 351 / 497; 6 of 300 over 9,000, 12 of 96 61,000 /
-  // 255 / 322; 20 of 64 over 2,000, 28 of 128 on 4 20,000 / 285 / 158; 60 of 50
-  // over 4,000 (tiles mostly empty) 75,000 / 406 / 358; heads of 64, whose tiles
-  // of 16 leave registers for four waves, 8 of 1,000 over 3,000 48,000 / 221 / 180.
+  // tile takes some 4 us, and its parts are as large as its keys.  Texts and keys
+  // of up to so many, steps of row tiles and key tiles / us / in tiles of 16: 7 of
+  // 500 over 3,001, 20 heads of 80 on 5 52,600 / 397 / 746; 6 of 300 over 9,000,
+  // 12 of 96 60,900 / 441 / 537; 60 of 50 over 4,000, 28 of 128 on 4 90,000 / 705
+  // / 849; 10 of 300 over 1,500, the same heads 32,000 / 233 / 273; 20 of 64 over
+  // 2,000, these too 20,200 / 287 / 153; 3 of 128 5,300 / 153 / 102.  (The sides
+  // meet between 20,200 and 31,600: calls there are left to tiles of 16.)  Heads
+  // of 64, whose tiles of 16 leave registers for four waves, stay with those.
   if (kv->dtype == VSK_DTYPE_F32 && (span.all || span.joined) && rows >= 256 &&
       kv->head_dim > 64 && kv->head_dim <= 128 && aligned_operands(kv, args) &&
       pairs * ceil_div(rows, ATTN_TILE_ROWS) * ceil_div(keys, ATTN_TILE32_KEYS) >= 40000) {
@@ -155,7 +157,7 @@ Plan plan_of(const vsk_ctx *ctx, const vsk_kv *kv, const vsk_attention_args *arg
     // over up to 742 keys, 64 heads of 128 on 8 35 / 30)
     if (span.joined && kv->head_dim <= 128) per = 8;
     // In 32 bits a tile takes so long that ragged texts are divided for their
-    // balance (7 of up to 500 against 3,001 keys, want 2 and 12: 575 / 501 us).
+    // balance (7 of up to 500 over three sets of 3,001 keys, want 2 and 12: 575 / 501 us).
     if (kv->dtype == VSK_DTYPE_F32) want = 12 * cus;
   } else {
     // A tile for each of the four waves that share a part at least.  Contexts

@@ -14,12 +14,14 @@
 //
 // What bounds it: the products, 64 cycles each, and the vector instructions
 // beside them, which run on the same units in 32 bits and add to them: a tile
-// has 32 DT products or less (of the head's d, not the padding), and about 170
-// other instructions.  So the sums are rescaled only when a row's largest score
-// has grown by 8 (in log2; weights up to 256 cost fp32 nothing), and values
-// looked at one by one only in tiles that not every row sees whole.  7 texts of up to 500 against 3,001 keys, 20 heads of 80 on 5:
-// 470 us (16 rows a wave that brings its keys itself: 999), 81 of 157 TFLOP/s,
-// 89 with the places that the head leaves in a block of 32.
+// has 32 DT products or less (of the head's d, not the padding), and some 200
+// other instructions (2.3 a product counted).  So the sums are rescaled only when
+// a row's largest score has grown by 8 (in log2; weights up to 256 cost fp32
+// nothing), and values looked at one by one only in tiles that not every row sees
+// whole.  7 texts of up to 500 against three sets of up to 3,001 keys, 20 heads of 80 on 5: 482 us (16
+// rows a wave that brings its keys itself: 1,000), 79 of 157 TFLOP/s, 86 with the
+// places that the head leaves in a block of 32; the matrix cores are busy 0.62 of
+// the time.
 #include "attn.hpp"
 #include "vsk_api.hpp"
 
