@@ -754,7 +754,8 @@ int64_t vsk_kv_scratch_ints(int32_t pages, int32_t slots);
 /* Grows the n sequences in slots seqs[] (distinct) by counts[] tokens: takes
  * the lowest free pages, in the sequences' order, and sets the lengths.  With
  * too few free pages, or past the table's width, a sequence grows only as far
- * as its pages reach. */
+ * as its pages reach.  A page that a sequence held past its length (which the
+ * caller has lowered) is given back where a new one takes its place. */
 vsk_status vsk_kv_reserve(vsk_ctx *ctx, void *stream, const vsk_kv *kv, const int32_t *seqs,
                           const int32_t *counts, int32_t n);
 /* What the sequences in slots children[] (distinct, none of them a parent)

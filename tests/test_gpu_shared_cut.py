@@ -39,3 +39,28 @@ def test_cut_back_and_grown_again(ctx, dtype, cut, left, grown):
     assert plan.prefix.tolist() == [192] * len(rest)
     one, _ = view(cache, slots)
     check_shared(one, rest, q[:len(rest)], None, cache.attend(q[:len(rest)], shared=plan), 0.125)
+
+
+@pytest.mark.parametrize("left", [0, 64, 100, 176, 192, 195])
+@pytest.mark.parametrize("grown", [1, 40, 110])
+def test_pages_written_over_are_given_back(ctx, left, grown):
+    """A page's count is that of the table entries that name it, also of those
+    that new pages took the place of; freed, none is left."""
+    cache, slots, _ = forked(ctx)
+
+    def counted():
+        held = cache.table[cache.table >= 0].long()
+        assert torch.equal(torch.bincount(held, minlength=cache.pages).int(), cache.refs)
+
+    counted()
+    for _ in range(6):  # (64 pages would not last)
+        for slot in (1, 3):
+            cache.lengths[slot] = left
+        cache.reserve([1, 3], [grown, 1])
+        assert cache.missing() == 0
+        assert cache.lengths[[1, 3]].tolist() == [left + grown, left + 1]
+        counted()
+    cache.compact()
+    counted()
+    cache.free(range(7))
+    assert not cache.refs.any() and bool((cache.table == -1).all())

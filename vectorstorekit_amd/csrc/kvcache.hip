@@ -61,7 +61,8 @@ struct Pool {
   int32_t *table, *lengths, *refs, *status, *scratch;
   int64_t table_stride;
   int32_t layers, pages, page_size, shift, kv_heads, d, size, slots, width;
-  // scratch: three lists of a page each, then three of a slot each (reserve: the first)
+  // scratch: three lists of a page each, then three of a slot each (reserve: the first
+  // of both)
   __device__ int32_t *page_list(int i) const { return scratch + (int64_t)i * pages; }
   __device__ int32_t *slot_list(int i) const {
     return scratch + 3 * (int64_t)pages + (int64_t)i * slots;
@@ -162,6 +163,11 @@ __global__ __launch_bounds__(NT) void k_kv_reserve(const Pool p, const int32_t *
   // base: pages that the sequences before want, as far as 32 bits count (there
   // are fewer)
   int32_t *base = p.slot_list(0);
+  // pages that sequences which have been cut back held still, in the places of
+  // those that are taken
+  int32_t *was = p.page_list(0);
+  __shared__ int32_t given;
+  if (threadIdx.x == 0) given = 0;
   int64_t want = 0;
   const auto counted = [](int64_t x) { return x < INT32_MAX ? (int32_t)x : INT32_MAX; };
   for (int32_t c = 0; c < n; c += NT) {
@@ -191,10 +197,15 @@ __global__ __launch_bounds__(NT) void k_kv_reserve(const Pool p, const int32_t *
     }
     const int32_t slot = seqs[lo];
     const int32_t first = (held(p, slot) + p.page_size - 1) >> p.shift;
-    p.table[slot * p.table_stride + first + rank - base[lo]] = page;
+    int32_t *entry = p.table + slot * p.table_stride + first + rank - base[lo];
+    const int32_t old = *entry;
+    *entry = page;
+    if ((uint32_t)old < (uint32_t)p.pages) was[atomicAdd(&given, 1)] = old;
     p.refs[page] = 1;
   });
   __syncthreads();
+  // (given back when all are taken, so that which are free does not depend on it)
+  for (int32_t r = threadIdx.x; r < given; r += NT) atomicSub(p.refs + was[r], 1);
   __shared__ unsigned long long cut;
   if (threadIdx.x == 0) cut = 0;
   __syncthreads();

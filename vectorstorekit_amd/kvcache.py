@@ -551,7 +551,9 @@ class PagedKVCache:
     def reserve(self, seqs, counts):
         """Grows the sequences in these slots (distinct) by these numbers of
         tokens, taking the lowest free pages; ``missing()`` tells of a
-        shortage."""
+        shortage.  A sequence may be cut back first, by a lower length in
+        ``lengths`` (whole pages, where its pages are shared): new pages take
+        the place of those that it held past that."""
         self._keeping()
         self._known(seqs, "seqs", distinct=True)
         s, c = _ints(self.gpu, seqs, "seqs"), _ints(self.gpu, counts, "counts")
