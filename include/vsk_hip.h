@@ -708,7 +708,8 @@ vsk_status vsk_int8_pack(vsk_ctx *ctx, void *stream, int32_t dtype, const void *
                          int64_t row_stride, const vsk_int8_weight *w);
 /* tokens x inputs in, tokens x outputs out: each token is quantised as above
  * (code = x * (127 / largest), rounded to even) and
- * out = code . weights * token's scale * channel's scale + bias.  The sums are
+ * out = code . weights * channel's scale * token's scale + bias, in 32 bits and
+ * this order.  The sums are
  * exact; a token that holds an infinity or NaN has NaN outputs.  inputs at
  * most 131,072.  out must not overlap x.  workspace:
  * vsk_int8_linear_workspace() bytes, 16-byte aligned (0 for few tokens: none). */

@@ -521,9 +521,9 @@ class PagedKVCache:
         prefix has grown again (``reserve`` gives it pages of its own there: its
         group would read pages that are not theirs).
         Sharing pays from contexts of some thousand keys on: a second launch
-        joins the parts (4 branches of 512 keys take 13 us with it and 9
-        without, 8 of 8,192 18 and 30, 64 of 32,768 76 and 411: 32 heads of
-        128 on 8).
+        joins the parts (4 branches of 512 keys take 13 us with it and
+        10 without, 8 of 8,192 18 and 30, 64 of 32,768 76 and 411: 32 heads
+        of 128 on 8).
         ``members`` bounds a group's sequences (default: known of a host
         sequence, all of them otherwise; a group of more shares nothing),
         ``prefix`` says about how many keys the longest prefix has, to divide
